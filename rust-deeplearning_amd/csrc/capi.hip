@@ -400,6 +400,26 @@ struct CallWork {
     }
 };
 
+}  // namespace
+
+rdl_status rdl::call_scratch(hipStream_t s, size_t bytes, CallScratch* out) {
+    CallWork cw;
+    const rdl_status st = cw.get(nullptr, s, bytes, false);
+    out->p = cw.p;
+    out->graph_owned = cw.graph_owned;
+    return st;
+}
+
+rdl_status rdl::call_scratch_done(hipStream_t s, CallScratch* scratch) {
+    CallWork cw;
+    cw.p = scratch->p;
+    cw.graph_owned = scratch->graph_owned;
+    scratch->p = nullptr;
+    return cw.release(s);
+}
+
+namespace {
+
 rdl_status host_matmul(WType t, bool native, const float* x, size_t x_len, const uint8_t* w,
                        size_t w_len, size_t m, size_t k, size_t n, float* y, size_t y_len) {
     rdl_status st = check_matmul(t, x, x_len, w, w_len, m, k, n, y, y_len);

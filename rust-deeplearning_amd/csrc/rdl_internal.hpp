@@ -35,6 +35,15 @@ inline rdl_status api_shape_fail(const char* what, std::initializer_list<size_t>
 }
 rdl_status api_ok();
 rdl_status api_require_device();
+// Work memory of one call on stream `s` (capi.hip): the stream's, or memory
+// of the graph while the stream is being captured; call_scratch_done after
+// the call's last launch.  Contents are undefined.
+struct CallScratch {
+    void* p = nullptr;
+    bool graph_owned = false;
+};
+rdl_status call_scratch(hipStream_t s, size_t bytes, CallScratch* out);
+rdl_status call_scratch_done(hipStream_t s, CallScratch* scratch);
 
 // GGUF block geometry (rustml/quant/main/src/api/types.rs:1-17,
 // rustml/gguf/main/src/api/types.rs:54-76).
