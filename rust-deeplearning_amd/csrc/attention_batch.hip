@@ -4,6 +4,9 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "../../include/rdl_attention.h"
 #include "kv_pool.hpp"
 #include "rdl_device.hpp"
@@ -13,27 +16,13 @@ namespace rdl {
 namespace {
 
 // Keys and values of a launch: pages through a table, or (table NULL) the rows
-// of the step itself.
+// of the step itself.  Strides in elements.
 struct KvSource {
     const void *k, *v;
-    int64_t k_position, v_position, head, page;  // strides in elements
+    int64_t k_position, v_position, head, page;
     const int32_t* tables;
     int64_t table_stride;
     int n_pages, shift;
-    // element offsets of key j of sequence b (its first row row0) and KV head kvh; false: not in the pool
-    __device__ __forceinline__ bool at(int b, int64_t row0, int kvh, int j, int64_t* ko, int64_t* vo) const {
-        if (!tables) {
-            *ko = (row0 + j) * k_position + kvh * head;
-            *vo = (row0 + j) * v_position + kvh * head;
-            return true;
-        }
-        const int32_t pg = tables[b * table_stride + (j >> shift)];
-        const int64_t base = pg * page + kvh * head;
-        const int o = j & ((1 << shift) - 1);
-        *ko = base + o * k_position;
-        *vo = base + o * v_position;
-        return (uint32_t)pg < (uint32_t)n_pages;
-    }
 };
 
 struct BatchArgs {
@@ -42,83 +31,893 @@ struct BatchArgs {
     int64_t q_stride;
     float* out;
     int64_t out_stride;
-    int n_heads, n_kv, hd;
+    int n_heads, n_kv, hd, group;  // group: n_heads / n_kv
     int64_t m;
     const int32_t *row_start, *kv_len;  // kv_len NULL: the sequence's rows
     int n_seq;
     float scale;
+    // the launch: tile workgroups first, then few-row ones
+    int pairs;        // n_seq * n_kv, rounded up to 8 from 8 on (pair % 8 is then the XCD)
+    int tile_slots, tile_splits, few_slots, few_splits;
+    int tile_span, few_span;  // keys a split
+    int few_rows;             // sequences of at most this many (row, head of a group) pairs are few-row ones
+    float* part;              // [m][n_heads][splits][hd + 2]: normalised output, maximum, sum
+    int part_splits;
+    int* counters;            // [m][n_heads], zero between launches
 };
 
-// The rows of sequence b: [r0, r0 + n) of the step, cut to [0, m) by the
-// caller; t: its keys, cut to what the table can name.
-__device__ __forceinline__ void sequence(const BatchArgs& a, int b, int64_t* r0, int64_t* n, int64_t* t) {
-    *r0 = a.row_start[b];
-    *n = (int64_t)a.row_start[b + 1] - *r0;
-    *t = a.kv_len ? a.kv_len[b] : *n;
-    if (a.kv.tables) *t = min(*t, a.kv.table_stride << a.kv.shift);
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef __fp16 hp2 __attribute__((ext_vector_type(2)));  // v_cvt_pkrtz's type
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+// Weights are held as 2^(x - M + SHIFT), M a running maximum that moves only
+// when a score passes it by SLACK: at most 2^15, so hi and lo fit f16, and
+// f16's smallest step, 2^-24, lies 2^-32 below the largest weight.
+constexpr float SHIFT = 8.0f, SLACK = 7.0f;
+
+// a * 2^e as two f16 parts of 11 bits each (rounded toward zero, so both have
+// a's sign and hi + lo is off by less than 2^-21 of it).
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+    const hp2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const float ra = a - (float)h[0], rb = b - (float)h[1];
+    *hi = __builtin_bit_cast(uint32_t, h);
+    *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+}
+__device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    const uint32_t a = r[0], b = r[1];
+    return __builtin_bit_cast(float, threadIdx.x & 32 ? a : b);
+}
+__device__ __forceinline__ float max32(float v) { return fmaxf(v, other32(v)); }
+__device__ __forceinline__ float other16(float v) {  // the value of lane ^ 16
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    const uint32_t a = r[0], b = r[1];
+    return __builtin_bit_cast(float, threadIdx.x & 16 ? a : b);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max8_u32(v);
+    v = max(v, (uint32_t)dpp_i32<DPP_ROW_MIRROR>((int)v));
+    v = max(v, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, v))));
+    v = max(v, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, v))));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+// floor(log2(v)) of a positive finite f32 given by its bits (-127 below 2^-126)
+__device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }
+
+// LDS rows of one key: HD f16 values and a pad that spreads 16 rows' 16-byte
+// reads (K) and 4 rows' 64-byte transposed reads (V) over all 64 banks.
+template <typename KV, int HD>
+struct Geo {
+    static constexpr bool F32 = std::is_same<KV, float>::value;
+    static constexpr int PARTS = F32 ? 2 : 1;                // hi, lo
+    static constexpr int KROW = HD + 8, VROW = HD + (HD == 96 ? 0 : 32);
+    static constexpr int KEY = (KROW + VROW) * PARTS;        // f16 elements a key
+    static constexpr int TK = F32 || HD == 256 ? 32 : 64;    // keys of a tile
+    static constexpr int FW = F32 && HD == 256 ? 2 : 4;      // waves of the few-row kernel
+    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)FW * 32 * KEY * 2;
+    static constexpr size_t LDS = TILE_LDS > FEW_LDS ? TILE_LDS : FEW_LDS;
+    static_assert(LDS <= 160 * 1024 - 2048, "LDS of a CU");
+};
+
+// What a wave's slab of keys needs beside its LDS rows.
+struct Meta {
+    int valid;  // the keys' page is in the pool
+    int bad;    // values that are not finite were zeroed: wide4 brings them
+    int ke, ve; // f32 keys / values are held times 2^-ke, 2^-ve
+};
+
+// One wave's slab of SK keys on its way from memory to LDS: loads into
+// registers (issued a step ahead), then the f16 parts into LDS.  A slab of 16
+// keys or fewer lies on one page, so each load is a buffer load from a uniform
+// base; keys past the sequence and pages outside the pool read as zeros.
+template <typename KV, int HD, int SK>
+struct Slab {
+    using G = Geo<KV, HD>;
+    static constexpr bool F32 = G::F32;
+    static constexpr int E = (int)sizeof(KV);
+    static constexpr int CPR = HD / 8;              // 8-element pieces a key
+    static constexpr int NL = (SK * CPR + 63) / 64;  // pieces a lane
+    static constexpr int GK = SK < 16 ? SK : 16, NG = SK / GK, LPG = NL / NG;
+    static constexpr bool WHOLE = NL * 64 == SK * CPR;  // else the last piece of some lanes is past the slab
+    static_assert(NG == 1 || WHOLE, "whole pieces a group");
+    u32x4 k[NL][G::PARTS], v[NL][G::PARTS];
+    uint32_t koff[LPG], voff[LPG];
+    int pg[NG];  // table entries of the next slab to load
+
+    __device__ __forceinline__ void init(const KvSource& s, int hd) {
+#pragma unroll
+        for (int i = 0; i < LPG; i++) {
+            const int pc = (threadIdx.x & 63) + 64 * i, key = pc / CPR, col = pc % CPR;
+            const bool in = col * 8 < hd && (WHOLE || key < SK);
+            koff[i] = in ? (uint32_t)(key * (int)s.k_position + col * 8) * E : RSRC_OOB;
+            voff[i] = in ? (uint32_t)(key * (int)s.v_position + col * 8) * E : RSRC_OOB;
+        }
+    }
+    // the table entries of the slab at key j (of t)
+    __device__ __forceinline__ void pages(const KvSource& s, const int32_t* table, int j, int t) {
+#pragma unroll
+        for (int g = 0; g < NG; g++) pg[g] = s.tables && j + g * GK < t ? table[(j + g * GK) >> s.shift] : 0;
+    }
+    // issues the loads of the slab at key j; valid: bit g for group g's page in the pool
+    __device__ __forceinline__ int load(const KvSource& s, int64_t row0, int kvh, int j, int t) {
+        int valid = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const int jg = j + g * GK, nv = max(0, min(GK, t - jg));
+            int64_t kb, vb;
+            bool ok = true;
+            if (s.tables) {
+                const int p = __builtin_amdgcn_readfirstlane(pg[g]);
+                ok = (uint32_t)p < (uint32_t)s.n_pages;
+                const int64_t at = (ok ? p : 0) * s.page + kvh * s.head;
+                const int o = jg & ((1 << s.shift) - 1);
+                kb = at + o * s.k_position;
+                vb = at + o * s.v_position;
+            } else {
+                kb = (row0 + jg) * s.k_position + kvh * s.head;
+                vb = (row0 + jg) * s.v_position + kvh * s.head;
+            }
+            valid |= (int)ok << g;
+            const int rows = ok ? nv : 0;
+            if (rows == 0) kb = vb = 0;
+            const auto kr = make_rsrc(reinterpret_cast<const KV*>(s.k) + kb, (uint32_t)(rows * (int)s.k_position * E));
+            const auto vr = make_rsrc(reinterpret_cast<const KV*>(s.v) + vb, (uint32_t)(rows * (int)s.v_position * E));
+#pragma unroll
+            for (int i = 0; i < LPG; i++)
+#pragma unroll
+                for (int p = 0; p < G::PARTS; p++) {
+                    k[g * LPG + i][p] = buf_load_b128(kr, koff[i] + 16 * p);
+                    v[g * LPG + i][p] = buf_load_b128(vr, voff[i] + 16 * p);
+                }
+        }
+        return valid;
+    }
+    // Splits 8 f32 values times 2^-e.
+    static __device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u32x4* lo) {
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const float a = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].z : x[p].x)), -e);
+                const float b = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].w : x[p].y)), -e);
+                uint32_t h, l;
+                split2(a, b, &h, &l);
+                (*hi)[2 * p + c] = h;
+                (*lo)[2 * p + c] = l;
+            }
+    }
+    // Largest magnitude of an array of pieces, as f32 bits; finite: of the finite ones only.
+    static __device__ __forceinline__ uint32_t largest(const u32x4 (&x)[NL][G::PARTS], bool finite) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+#pragma unroll
+            for (int p = 0; p < G::PARTS; p++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t b = x[i][p][c] & 0x7FFFFFFFu;
+                    m = max(m, finite && b >= 0x7F800000u ? 0u : b);
+                }
+        return wave_max_u32(m);
+    }
+    // Registers to the slab's LDS rows (lds: its K hi rows; K lo, V hi, V lo
+    // `part` rows further on).  check: whether values that are not finite
+    // have to be found (f16; f32 finds them on the way to the exponent).
+    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int kpart, int vpart, int valid, bool check) {
+        const int lane = threadIdx.x & 63;
+        Meta mt{valid, 0, 0, 0};
+        if constexpr (F32) {
+            uint32_t km = largest(k, false), vm = largest(v, false);
+            if (km >= 0x7F800000u) km = largest(k, true);
+            if (vm >= 0x7F800000u) {
+                mt.bad = 1;
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            if ((v[i][p][c] & 0x7F800000u) == 0x7F800000u) v[i][p][c] = 0;
+                vm = largest(v, false);
+            }
+            mt.ke = exponent(km) - 14;
+            mt.ve = exponent(vm) - 14;
+        } else if (check) {
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    found |= ((((v[i][0][c] & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0);
+            if (__builtin_amdgcn_ballot_w64(found)) {
+                mt.bad = 1;
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if ((v[i][0][c] & 0x7C00u) == 0x7C00u) v[i][0][c] &= 0xFFFF0000u;
+                        if ((v[i][0][c] & 0x7C000000u) == 0x7C000000u) v[i][0][c] &= 0xFFFFu;
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int pc = lane + 64 * i, key = pc / CPR, col = pc % CPR;
+            if (!WHOLE && key >= SK) continue;
+            u32x4* kd = reinterpret_cast<u32x4*>(ks + key * G::KROW + col * 8);
+            u32x4* vd = reinterpret_cast<u32x4*>(vs + key * G::VROW + col * 8);
+            if constexpr (F32) {
+                u32x4 kh, kl, vh, vl;
+                split8(k[i], mt.ke, &kh, &kl);
+                split8(v[i], mt.ve, &vh, &vl);
+                *kd = kh;
+                *reinterpret_cast<u32x4*>(ks + kpart + key * G::KROW + col * 8) = kl;
+                *vd = vh;
+                *reinterpret_cast<u32x4*>(vs + vpart + key * G::VROW + col * 8) = vl;
+            } else {
+                *kd = k[i][0];
+                *vd = v[i][0];
+            }
+        }
+        return mt;
+    }
+};
+
+// 4 keys (consecutive LDS rows from `row`) of 16 dims, transposed: lane i of
+// each 16 gets dim i's 4 values.
+__device__ __forceinline__ h4 read_t(const _Float16* p) {
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
 
-// One workgroup a (row, head): scores of 256 keys at a time, a running
-// maximum and sum, a thread a value dim.
+// Row of V of key j (NULL: its page is not in the pool).
 template <typename KV>
-__global__ __launch_bounds__(256) void rows_kernel(BatchArgs a) {
-    __shared__ float qs[256], ws[256], red[4];
-    __shared__ int64_t vofs[256];
-    const int64_t r = blockIdx.x;  // < m
-    const int h = blockIdx.y, kvh = h / (a.n_heads / a.n_kv), tid = threadIdx.x;
-    int64_t r0 = 0, n = 0, t = 0;
-    int lo = 0;
-    for (; lo < a.n_seq; lo++) {
-        sequence(a, lo, &r0, &n, &t);
-        if (r0 >= 0 && r >= r0 && r - r0 < n) break;
+__device__ __forceinline__ const KV* value_row(const KvSource& s, int64_t row0, const int32_t* table, int kvh, int j) {
+    int64_t at;
+    if (s.tables) {
+        const int32_t p = table[j >> s.shift];
+        if ((uint32_t)p >= (uint32_t)s.n_pages) return nullptr;
+        at = p * s.page + kvh * s.head + (j & ((1 << s.shift) - 1)) * s.v_position;
+    } else {
+        at = (row0 + j) * s.v_position + kvh * s.head;
     }
-    if (lo == a.n_seq) return;
-    const int64_t limit = (a.kv_len ? a.kv_len[lo] : n) - n + (r - r0) + 1;
-    const int64_t seen = min(t, limit);
-    if (tid < a.hd) qs[tid] = a.q[r * a.q_stride + (int64_t)h * a.hd + tid];
-    float M = -__builtin_inff(), L = 0.0f, o = 0.0f;
-    for (int64_t j0 = 0; j0 < seen; j0 += 256) {
-        __syncthreads();
-        float s = -__builtin_inff();
-        int64_t ko = 0, vo = -1;
-        if (j0 + tid < seen && a.kv.at(lo, r0, kvh, (int)(j0 + tid), &ko, &vo)) {
-            const KV* k = reinterpret_cast<const KV*>(a.kv.k) + ko;
-            float acc = 0.0f;
-            for (int d = 0; d < a.hd; d++) acc += qs[d] * (float)k[d];
-            s = acc * a.scale;
-        } else {
-            vo = -1;
+    return reinterpret_cast<const KV*>(s.v) + at;
+}
+
+// Of 4 values those that are not finite, the others (and all without `on`) as 0.
+template <typename KV>
+__device__ __forceinline__ f4 wide4(const KV* v, bool on) {
+    typedef KV kv4 __attribute__((ext_vector_type(4)));
+    const kv4 x = *reinterpret_cast<const kv4*>(v);
+    f4 y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = on && abs_bits((float)x[i]) >= 0x7F800000u ? (float)x[i] : 0.0f;
+    return y;
+}
+
+// The rows of a sequence that a launch works on.
+struct Seq {
+    int64_t row0;   // its first row
+    int64_t pairs;  // (row, head of the group) pairs, rows cut to m
+    int64_t first;  // last key that row 0 sees
+    int t;          // keys
+};
+__device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
+    Seq s;
+    const int64_t r0 = a.row_start[b], n = (int64_t)a.row_start[b + 1] - r0;
+    int64_t t = a.kv_len ? (int64_t)a.kv_len[b] : n;
+    s.row0 = r0;
+    s.pairs = r0 < 0 ? 0 : max((int64_t)0, min(n, a.m - r0)) * a.group;
+    s.first = t - n;
+    // keys that the table can name, or that are rows of the step
+    t = min(t, a.kv.tables ? a.kv.table_stride << a.kv.shift : a.m - r0);
+    s.t = (int)max((int64_t)0, min(t, (int64_t)INT32_MAX - 4096));
+    return s;
+}
+// The last key that pair p sees (-1: none).
+__device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int64_t p) {
+    const int64_t l = s.first + p / a.group;
+    return (int)max((int64_t)-1, min(l, (int64_t)s.t - 1));
+}
+
+// ---- joining split key ranges ---------------------------------------------------------
+// A split's partial result of `pairs` pairs from p0 on: normalised outputs with
+// their maxima and sums.  Publication as attention.hpp describes it:
+// agent-coherent stores, each wave waits for its own, a barrier, then the
+// counter; the last split to arrive joins all of them in order (so results
+// do not depend on which it is) and leaves the counter at zero.
+__device__ __forceinline__ float* part_at(const BatchArgs& a, const Seq& s, int kvh, int64_t p, int z) {
+    const int64_t row = s.row0 + p / a.group, h = kvh * a.group + p % a.group;
+    return a.part + ((row * a.n_heads + h) * a.part_splits + z) * (a.hd + 2);
+}
+__device__ __forceinline__ float* out_at(const BatchArgs& a, const Seq& s, int kvh, int64_t p) {
+    return a.out + (s.row0 + p / a.group) * a.out_stride + (kvh * a.group + p % a.group) * a.hd;
+}
+__device__ __forceinline__ void put(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int64_t p0, int pairs, int splits,
+                                     int* flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int64_t row = s.row0 + p0 / a.group, h = kvh * a.group + p0 % a.group;
+        int* c = a.counters + row * a.n_heads + h;
+        const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = old == splits - 1;
+        if (old == splits - 1) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*flag) return;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int i = w; i < pairs; i += waves) {
+        const float* pt = part_at(a, s, kvh, p0 + i, 0);
+        float M = -__builtin_inff(), L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int z = 0; z < splits; z++) {
+            const float l = get(pt + z * (a.hd + 2) + a.hd + 1);
+            if (l != 0.0f) M = fmaxf(M, get(pt + z * (a.hd + 2) + a.hd));
         }
-        vofs[tid] = vo;
-        float mx = s;
-        for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        const float Mn = fmaxf(M, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        if (Mn > -__builtin_inff()) {
-            const float corr = expf(M - Mn);
-            L *= corr, o *= corr, M = Mn;
+        for (int z = 0; z < splits; z++) {
+            const float* pz = pt + z * (a.hd + 2);
+            const float l = get(pz + a.hd + 1);
+            const float wt = l != 0.0f ? l * __builtin_amdgcn_exp2f(get(pz + a.hd) - M) : 0.0f;
+            L += wt;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (lane + 64 * c < a.hd && wt != 0.0f) o[c] += wt * get(pz + lane + 64 * c);
         }
-        ws[tid] = vo >= 0 ? expf(s - M) : 0.0f;
+        float* out = out_at(a, s, kvh, p0 + i);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (lane + 64 * c < a.hd) out[lane + 64 * c] = L != 0.0f ? o[c] / L : 0.0f;
+    }
+}
+
+// q of one pair as f16 parts: NS steps of 8 dims, step i at dim d0 + i * step.
+// Scaled by the power of two that brings the row's largest value (over all
+// lanes of the pair: `reduce`) into [2^14, 2^15).  Returns the exponent.
+template <int NS, typename R>
+__device__ __forceinline__ int load_q(const float* q, bool live, int d0, int step, int hd, h8 (&hi)[NS], h8 (&lo)[NS],
+                                      R&& reduce) {
+    f4 x[NS][2];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        const int d = d0 + i * step;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            x[i][c] = live && d < hd ? *reinterpret_cast<const f4*>(q + d + 4 * c) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) m = max(m, abs_bits(x[i][c][e]));
+        }
+    }
+    m = reduce(m);
+    const int e = m >= 0x7F800000u ? 0 : exponent(m) - 14;
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        u32x4 h, l;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t a, b;
+            split2(__builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2], -e),
+                   __builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2 + 1], -e), &a, &b);
+            h[c] = a;
+            l[c] = b;
+        }
+        hi[i] = __builtin_bit_cast(h8, h);
+        lo[i] = __builtin_bit_cast(h8, l);
+    }
+    return e;
+}
+
+// ---- many rows: 4 waves of 32 pairs, tiles of TK keys shared through LDS -------------------
+// Each wave holds 32 pairs as the columns of both products, S^T = K Q^T and
+// O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a lane has 16 scores of one pair, so
+// the softmax needs one exchange with lane ^ 32, and its weights are already
+// the second product's B operand once the keys of a 16-key step are taken in
+// the order 4h .. 4h + 3, 8 + 4h .. (h = lane / 32), in which the transposed LDS reads of V
+// fetch them.
+template <typename KV, int HD>
+__device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int64_t p0,
+                                          int z, _Float16* lds, Meta* meta, int* flag) {
+    using G = Geo<KV, HD>;
+    constexpr int TK = G::TK, SK = TK / 4, KS = HD / 16, DT = HD / 32;
+    constexpr bool F32 = G::F32;
+    constexpr int KP = TK * G::KROW, VP = TK * G::VROW;  // a part's elements
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int h = lane >> 5, c = lane & 31;
+    // this tile's keys and the split's share of them
+    const int keys = last_key(a, s, min(p0 + 127, s.pairs - 1)) + 1;
+    const int splits = min(a.tile_splits, max(1, (keys + a.tile_span - 1) / a.tile_span));
+    if (z >= splits) return;
+    const int j_lo = z * a.tile_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.tile_span);
+    const int64_t p = p0 + 32 * w + c;
+    const bool live = p < s.pairs, work = p0 + 32 * w < s.pairs;
+    const int64_t row = s.row0 + p / a.group, head = kvh * a.group + p % a.group;
+    const int last = live ? last_key(a, s, p) : -1;
+    const int w_first = __builtin_amdgcn_readfirstlane(last_key(a, s, p0 + 32 * w));   // the wave's first pair sees
+    const int w_last = __builtin_amdgcn_readfirstlane(last_key(a, s, min(p0 + 32 * w + 31, s.pairs - 1)));
+    const int wg_first = last_key(a, s, p0);
+    h8 qh[KS], ql[KS];
+    const int qe = load_q<KS>(a.q + row * a.q_stride + head * a.hd, live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
+        return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
+    });
+    const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
+    f16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float M = -__builtin_inff(), L = 0.0f;
+    int ref = -1000;  // f32 values: o is held times 2^-ref
+
+    Slab<KV, HD, SK> slab;
+    slab.init(a.kv, a.hd);
+    slab.pages(a.kv, table, j_lo + SK * w, s.t);
+    int valid = slab.load(a.kv, s.row0, kvh, j_lo + SK * w, j_hi);
+    slab.pages(a.kv, table, j_lo + TK + SK * w, s.t);
+    int buf = 0;
+    for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
+        _Float16* ks = lds + buf * TK * G::KEY;
+        _Float16* vs = ks + KP * G::PARTS;
+        const Meta mine = slab.store(ks + SK * w * G::KROW, vs + SK * w * G::VROW, KP, VP, valid, j0 + TK - 1 > wg_first);
+        if (lane == 0) meta[buf * 4 + w] = mine;
+        if (j0 + TK < j_hi) {
+            valid = slab.load(a.kv, s.row0, kvh, j0 + TK + SK * w, j_hi);
+            slab.pages(a.kv, table, j0 + 2 * TK + SK * w, s.t);
+        }
         __syncthreads();
-        if (tid < a.hd)
-            for (int j = 0; j < 256; j++)
-                if (vofs[j] >= 0) {
-                    L += ws[j];
-                    o += ws[j] * (float)(reinterpret_cast<const KV*>(a.kv.v) + vofs[j])[tid];
+        if (!work || j0 > w_last) continue;
+        Meta mt[4];
+        bool masked = j0 + TK - 1 > w_first;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const Meta x = meta[buf * 4 + i];
+            mt[i].valid = __builtin_amdgcn_readfirstlane(x.valid);
+            mt[i].bad = __builtin_amdgcn_readfirstlane(x.bad);
+            mt[i].ke = F32 ? __builtin_amdgcn_readfirstlane(x.ke) : 0;
+            mt[i].ve = F32 ? __builtin_amdgcn_readfirstlane(x.ve) : 0;
+            masked |= !mt[i].valid;
+        }
+        if constexpr (F32) {
+            const int top = max(max(mt[0].ve, mt[1].ve), max(mt[2].ve, mt[3].ve));
+            if (top > ref) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] = __builtin_amdgcn_ldexpf(o[d][e], ref - top);
+                ref = top;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < TK / 32; b++) {
+            f16v sc;
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
+            const _Float16* kr = ks + (32 * b + c) * G::KROW + 8 * h;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const h8 kf = *reinterpret_cast<const h8*>(kr + 16 * k);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc, 0, 0, 0);
+                if constexpr (F32) {
+                    const h8 kl = *reinterpret_cast<const h8*>(kr + KP + 16 * k);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[k], sc, 0, 0, 0);
+                }
+            }
+            const int rel = last - (j0 + 32 * b);
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const Meta& g = mt[(32 * b + 8 * i) / SK];
+                const float f = F32 ? __builtin_amdgcn_ldexpf(cs, g.ke) : cs;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    float x = sc[4 * i + t] * f;
+                    if (masked) x = 8 * i + 4 * h + t <= rel && g.valid ? x : -__builtin_inff();
+                    sc[4 * i + t] = x;
+                    mx = fmaxf(mx, x);
+                }
+            }
+            mx = max32(mx);
+            if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
+                const float Mn = fmaxf(M, mx);
+                const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
+                L *= corr;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] *= corr;
+                M = Mn;
+            }
+            const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {  // 16 keys a step
+                u32x4 ph, pl;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int e = 8 * k + 2 * u;
+                    float x0 = __builtin_amdgcn_exp2f(sc[e] + off), x1 = __builtin_amdgcn_exp2f(sc[e + 1] + off);
+                    L += x0 + x1;
+                    if constexpr (F32) {
+                        const int sh = mt[(32 * b + 16 * k + (u >= 2 ? 8 : 0)) / SK].ve - ref;
+                        x0 = __builtin_amdgcn_ldexpf(x0, sh);
+                        x1 = __builtin_amdgcn_ldexpf(x1, sh);
+                    }
+                    uint32_t hi, lo;
+                    split2(x0, x1, &hi, &lo);
+                    ph[u] = hi;
+                    pl[u] = lo;
+                }
+                const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
+                const _Float16* vr = vs + (32 * b + 16 * k + 4 * h + ((lane & 15) >> 2)) * G::VROW +
+                                     16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const h4 v0 = read_t(vr + 32 * d), v1 = read_t(vr + 8 * G::VROW + 32 * d);
+                    const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p8, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q8, o[d], 0, 0, 0);
+                    if constexpr (F32) {
+                        const h4 w0 = read_t(vr + VP + 32 * d), w1 = read_t(vr + VP + 8 * G::VROW + 32 * d);
+                        const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p8, o[d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        // values that are not finite, where their key is seen
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (mt[i].bad)
+                for (int j = j0 + SK * i; j < min(j0 + SK * (i + 1), j_hi); j++) {
+                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+                    if (!v) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int dim = 32 * d + 8 * i + 4 * h;
+                            const f4 x = wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
+#pragma unroll
+                            for (int t = 0; t < 4; t++) o[d][4 * i + t] += x[t];
+                        }
                 }
     }
-    if (tid < a.hd) a.out[r * a.out_stride + (int64_t)h * a.hd + tid] = L != 0.0f ? o / L : 0.0f;
+    L += other32(L);
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    if (live) {
+        float* dst = splits == 1 ? out_at(a, s, kvh, p) : part_at(a, s, kvh, p, z);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int dim = 32 * d + 8 * i + 4 * h;
+                if (dim >= a.hd) continue;
+                f4 y;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const float x = o[d][4 * i + t] * inv;
+                    y[t] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+                }
+                if (splits == 1) {
+                    *reinterpret_cast<f4*>(dst + dim) = y;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) put(dst + dim + t, y[t]);
+                }
+            }
+        if (splits > 1 && h == 0) {
+            put(dst + a.hd, M);
+            put(dst + a.hd + 1, L);
+        }
+    }
+    if (splits > 1) join(a, s, kvh, p0, (int)min((int64_t)128, s.pairs - p0), splits, flag);
 }
 
-rdl_status run(const BatchArgs& a, bool f16, size_t max_rows, size_t max_kv, hipStream_t s) {
-    const dim3 grid((unsigned)a.m, (unsigned)a.n_heads);
-    if (f16)
-        hipLaunchKernelGGL(rows_kernel<_Float16>, grid, dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(rows_kernel<float>, grid, dim3(256), 0, s, a);
-    HIP_TRY(hipGetLastError());
-    return api_ok();
+// ---- few rows: up to 16 pairs, each wave its own keys ------------------------------------------
+// A decode step reads the cache once and computes little: the FW waves of a
+// workgroup take the split's keys 32 at a time in turn, each through LDS rows
+// of its own without a barrier, with the next 32 keys' loads in flight; at
+// the end they join through LDS.  The products as above, 16 columns wide
+// (v_mfma_f32_16x16x32_f16): a lane has the scores of keys 4g .. 4g + 3 and 16 +
+// 4g .. (g = lane / 16) of one pair.
+template <typename KV, int HD>
+__device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int64_t p0,
+                                         int z, _Float16* lds, float* wml, int* flag) {
+    using G = Geo<KV, HD>;
+    constexpr int KS = HD / 32, DT = HD / 16, FW = G::FW;
+    constexpr bool F32 = G::F32;
+    constexpr int KP = 32 * G::KROW, VP = 32 * G::VROW;
+    constexpr int OROW = HD + 4;  // f32 elements of a pair's joined output
+    static_assert(16 * OROW * 4 <= 32 * G::KEY * 2, "the output fits the wave's key rows");
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int pairs = (int)min((int64_t)16, s.pairs - p0);
+    const int keys = last_key(a, s, p0 + pairs - 1) + 1;
+    const int splits = min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
+    if (z >= splits) return;
+    const int j_lo = z * a.few_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.few_span);
+    const int64_t p = p0 + c;
+    const bool live = c < pairs;
+    const int64_t row = s.row0 + p / a.group, head = kvh * a.group + p % a.group;
+    const int last = live ? last_key(a, s, p) : -1;
+    const int first = last_key(a, s, p0);
+    _Float16* ks = lds + w * 32 * G::KEY;
+    _Float16* vs = ks + KP * G::PARTS;
+    float M = -__builtin_inff(), L = 0.0f;
+    f4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    int ref = -1000;
+    if (w < FW) {
+        Slab<KV, HD, 32> slab;
+        slab.init(a.kv, a.hd);
+        const int step = 32 * FW, j_w = j_lo + 32 * w;
+        int valid = 0;
+        if (j_w < j_hi) {
+            slab.pages(a.kv, table, j_w, s.t);
+            valid = slab.load(a.kv, s.row0, kvh, j_w, j_hi);
+            slab.pages(a.kv, table, j_w + step, s.t);
+        }
+        h8 qh[KS], ql[KS];
+        const int qe = load_q<KS>(a.q + row * a.q_stride + head * a.hd, live, 8 * g, 32, a.hd, qh, ql, [](uint32_t m) {
+            m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
+            return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
+        });
+        const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
+        for (int j0 = j_w; j0 < j_hi; j0 += step) {
+            const Meta mt = slab.store(ks, vs, KP, VP, valid, j0 + 31 > first);
+            if (j0 + step < j_hi) {
+                valid = slab.load(a.kv, s.row0, kvh, j0 + step, j_hi);
+                slab.pages(a.kv, table, j0 + 2 * step, s.t);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const bool masked = j0 + 31 > first || mt.valid != 3;
+            if constexpr (F32) {
+                if (mt.ve > ref) {
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[d][e] = __builtin_amdgcn_ldexpf(o[d][e], ref - mt.ve);
+                    ref = mt.ve;
+                }
+            }
+            f4 sc[2];
+            const float f = F32 ? __builtin_amdgcn_ldexpf(cs, mt.ke) : cs;
+            const int rel = last - j0;
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                sc[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                const _Float16* kr = ks + (16 * b + c) * G::KROW + 8 * g;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    const h8 kf = *reinterpret_cast<const h8*>(kr + 32 * k);
+                    sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[k], sc[b], 0, 0, 0);
+                    sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[k], sc[b], 0, 0, 0);
+                    if constexpr (F32) {
+                        const h8 kl = *reinterpret_cast<const h8*>(kr + KP + 32 * k);
+                        sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[k], sc[b], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    float x = sc[b][t] * f;
+                    if (masked) x = 16 * b + 4 * g + t <= rel && (mt.valid >> b & 1) ? x : -__builtin_inff();
+                    sc[b][t] = x;
+                    mx = fmaxf(mx, x);
+                }
+            }
+            mx = fmaxf(mx, other16(mx));
+            mx = max32(mx);
+            if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
+                const float Mn = fmaxf(M, mx);
+                const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
+                L *= corr;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[d][e] *= corr;
+                M = Mn;
+            }
+            const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
+            u32x4 ph, pl;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                float x0 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2] + off);
+                float x1 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2 + 1] + off);
+                L += x0 + x1;
+                if constexpr (F32) {
+                    x0 = __builtin_amdgcn_ldexpf(x0, mt.ve - ref);
+                    x1 = __builtin_amdgcn_ldexpf(x1, mt.ve - ref);
+                }
+                uint32_t hi, lo;
+                split2(x0, x1, &hi, &lo);
+                ph[u] = hi;
+                pl[u] = lo;
+            }
+            const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
+            const _Float16* vr = vs + (4 * g + ((lane & 15) >> 2)) * G::VROW + 4 * (lane & 3);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const h4 v0 = read_t(vr + 16 * d), v1 = read_t(vr + 16 * G::VROW + 16 * d);
+                const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p8, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, q8, o[d], 0, 0, 0);
+                if constexpr (F32) {
+                    const h4 w0 = read_t(vr + VP + 16 * d), w1 = read_t(vr + VP + 16 * G::VROW + 16 * d);
+                    const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p8, o[d], 0, 0, 0);
+                }
+            }
+            if (mt.bad)
+                for (int j = j0; j < min(j0 + 32, j_hi); j++) {
+                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+                    if (!v) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const int dim = 16 * d + 4 * g;
+                        o[d] += wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
+                    }
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        L += other16(L);
+        L += other32(L);
+        // the wave's normalised output over its own key rows, its maximum and sum beside
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        float* os = reinterpret_cast<float*>(ks);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            f4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = o[d][e] * inv;
+                y[e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+            }
+            *reinterpret_cast<f4*>(os + c * OROW + 16 * d + 4 * g) = y;
+        }
+        if (g == 0) {
+            wml[w * 32 + c] = M;
+            wml[w * 32 + 16 + c] = L;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs * (HD / 4); i += blockDim.x) {
+        const int pi = i / (HD / 4), dim = (i % (HD / 4)) * 4;
+        if (dim >= a.hd) continue;
+        float Mx = -__builtin_inff(), Ls = 0.0f;
+#pragma unroll
+        for (int x = 0; x < FW; x++)
+            if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < FW; x++) {
+            const float l = wml[x * 32 + 16 + pi];
+            if (l == 0.0f) continue;
+            const float wt = l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx);
+            Ls += wt;
+            y += wt * *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * 32 * G::KEY) + pi * OROW + dim);
+        }
+        const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
+        if (splits == 1) {
+            *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y * inv;
+        } else {
+            float* pt = part_at(a, s, kvh, p0 + pi, z);
+#pragma unroll
+            for (int e = 0; e < 4; e++) put(pt + dim + e, y[e] * inv);
+            if (dim == 0) {
+                put(pt + a.hd, Mx);
+                put(pt + a.hd + 1, Ls);
+            }
+        }
+    }
+    if (splits > 1) join(a, s, kvh, p0, pairs, splits, flag);
+}
+
+template <typename KV, int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ Meta meta[8];
+    __shared__ float wml[4 * 32];
+    __shared__ int flag;
+    _Float16* lds = reinterpret_cast<_Float16*>(smem);
+    const int tile_blocks = a.pairs * a.tile_slots * a.tile_splits;
+    const bool tile = (int)blockIdx.x < tile_blocks;
+    int id = tile ? (int)blockIdx.x : (int)blockIdx.x - tile_blocks;
+    const int pair = id % a.pairs;
+    id /= a.pairs;
+    const int splits = tile ? a.tile_splits : a.few_splits, slots = tile ? a.tile_slots : a.few_slots;
+    const int z = id % splits, slot = id / splits;
+    if (pair >= a.n_seq * a.n_kv) return;
+    const int b = pair / a.n_kv, kvh = pair % a.n_kv;
+    const Seq s = sequence(a, b);
+    if (s.pairs == 0 || (s.pairs > a.few_rows) != tile) return;
+    const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
+    // the last rows, which see the most keys, first
+    const int width = tile ? 128 : 16;
+    for (int64_t i = (s.pairs - 1) / width - slot; i >= 0; i -= slots) {
+        if (tile) tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta, &flag);
+        else few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml, &flag);
+        __syncthreads();  // before the next rows take the LDS
+    }
+}
+
+template <typename KV, int HD>
+hipError_t launch(const BatchArgs& a, hipStream_t s) {
+    const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<KV, HD>::LDS);
+    if (e != hipSuccess) return e;
+    const unsigned blocks = (unsigned)(a.pairs * (a.tile_slots * a.tile_splits + a.few_slots * a.few_splits));
+    hipLaunchKernelGGL((attend_kernel<KV, HD>), dim3(blocks), dim3(256), (Geo<KV, HD>::LDS), s, a);
+    return hipGetLastError();
+}
+template <typename KV>
+hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
+    return a.hd <= 64 ? launch<KV, 64>(a, s) : a.hd <= 96 ? launch<KV, 96>(a, s)
+         : a.hd <= 128 ? launch<KV, 128>(a, s) : launch<KV, 256>(a, s);
+}
+
+// Key ranges are split until the launch has about this many workgroups.
+constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512;
+constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 512;
+constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
+
+rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_t s) {
+    const int64_t m = a.m, rows = max_rows == 0 || (int64_t)max_rows > m ? m : (int64_t)max_rows;
+    int64_t keys = a.kv.tables ? a.kv.table_stride << a.kv.shift : m;
+    if (max_kv != 0 && (int64_t)max_kv < keys) keys = (int64_t)max_kv;
+    keys = std::max<int64_t>(1, std::min<int64_t>(keys, INT32_MAX / 2));
+    const int64_t pairs = (int64_t)a.n_seq * a.n_kv, G = a.group;
+    if (pairs > (int64_t)1 << 28) return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences of %d KV heads", a.n_seq, a.n_kv);
+    a.pairs = (int)(pairs < 8 ? pairs : (pairs + 7) / 8 * 8);
+    // sequences of up to 16 pairs; all of them where none is expected to have more
+    const bool only_few = rows * G <= 16;
+    a.few_rows = only_few ? INT32_MAX : 16;
+    const int64_t limit = (int64_t)1 << 30;  // workgroups of a launch
+    a.few_slots = 1;
+    a.tile_slots = only_few ? 0 : (int)std::max<int64_t>(1, std::min((rows * G + 127) / 128, limit / 4 / a.pairs));
+    auto split = [&](int64_t base, int64_t target, int unit, int64_t min_span, int* span, int* splits) {
+        int64_t sp = std::max(min_span, keys * base / target);
+        sp = (sp + unit - 1) / unit * unit;
+        int64_t n = (keys + sp - 1) / sp;
+        const int64_t cap = (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float)));
+        if (n > cap) n = std::max<int64_t>(1, cap);
+        sp = ((keys + n - 1) / n + unit - 1) / unit * unit;
+        *splits = (int)n;
+        *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
+    };
+    split(pairs, FEW_TARGET, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
+    const int64_t tiles = std::min<int64_t>((rows * G + 127) / 128 * a.n_seq, m * G / 128 + a.n_seq) * a.n_kv;
+    if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
+    else split(tiles, TILE_TARGET, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
+    a.part_splits = std::max(a.few_splits, a.tile_splits);
+    if ((int64_t)a.pairs * ((int64_t)a.tile_slots * a.tile_splits + a.few_splits) > limit)
+        return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences of %lld rows", a.n_seq, (long long)rows);
+    CallScratch work;
+    if (a.part_splits > 1) {
+        const size_t bytes = (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float);
+        const rdl_status st = call_scratch(s, bytes, (size_t)m * a.n_heads, &work);
+        if (st != RDL_OK) return st;
+        a.part = reinterpret_cast<float*>(work.p);
+        a.counters = work.counters;
+    }
+    const hipError_t e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
+    const rdl_status done = call_scratch_done(s, &work);
+    HIP_TRY(e);
+    return done == RDL_OK ? api_ok() : done;
 }
 
 // The checks that both entry points share; fills the fields of `a` that they name.
@@ -144,6 +943,7 @@ rdl_status check_attention(BatchArgs* a, const float* q, size_t q_stride, size_t
     a->n_heads = (int)n_heads;
     a->n_kv = (int)n_kv;
     a->hd = (int)hd;
+    a->group = (int)(n_heads / n_kv);
     a->m = (int64_t)m;
     a->row_start = row_start;
     a->n_seq = (int)n_seq;
@@ -197,6 +997,7 @@ rdl_status rdl_attention_packed_dev(const float* q_dev, size_t q_stride, size_t 
     const size_t elem = kv_dtype == RDL_DTYPE_F16 ? 2 : 4, width = n_kv_heads * head_dim;
     if ((st = rdl::check_rows("k", k_dev, k_stride, width, m, elem)) != RDL_OK) return st;
     if ((st = rdl::check_rows("v", v_dev, v_stride, width, m, elem)) != RDL_OK) return st;
+    if ((st = rdl::check_position_stride(k_stride > v_stride ? k_stride : v_stride)) != RDL_OK) return st;
     a.kv = {k_dev, v_dev, (int64_t)k_stride, (int64_t)v_stride, (int64_t)head_dim, 0, nullptr, 0, 0, 0};
     return rdl::run(a, kv_dtype == RDL_DTYPE_F16, max_rows, max_rows, (hipStream_t)stream);
 }

@@ -372,22 +372,24 @@ struct CallWork {
     int* counters = nullptr;
     bool graph_owned = false;
     rdl_status get(const rdl_weight* w, hipStream_t s, size_t bytes, bool want_counters) {
-        if (!bytes && !want_counters) return RDL_OK;
+        return get(s, bytes, want_counters ? rdl::gemm_counter_count(w->n, w->k) : 0);
+    }
+    rdl_status get(hipStream_t s, size_t bytes, size_t nc) {
+        if (!bytes && !nc) return RDL_OK;
         hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
         HIP_TRY(hipStreamIsCapturing(s, &cs));
         if (cs != hipStreamCaptureStatusActive) {
             void* q = nullptr;
             int* c = nullptr;
-            rdl_status st = stream_work(s, bytes, want_counters ? rdl::gemm_counter_count(w->n, w->k) : 0, &q, &c);
+            rdl_status st = stream_work(s, bytes, nc, &q, &c);
             p = q;
-            counters = want_counters ? c : nullptr;
+            counters = nc ? c : nullptr;
             return st;
         }
         const size_t data = (bytes + 255) & ~(size_t)255;
-        const size_t nc = want_counters ? rdl::gemm_counter_count(w->n, w->k) : 0;
         HIP_TRY(hipMallocAsync(&p, data + nc * sizeof(int) + 4, s));
         graph_owned = true;
-        if (want_counters) {
+        if (nc) {
             counters = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(p) + data);
             HIP_TRY(rdl::launch_zero_counters(counters, nc, s));
         }
@@ -402,10 +404,11 @@ struct CallWork {
 
 }  // namespace
 
-rdl_status rdl::call_scratch(hipStream_t s, size_t bytes, CallScratch* out) {
+rdl_status rdl::call_scratch(hipStream_t s, size_t bytes, size_t n_counters, CallScratch* out) {
     CallWork cw;
-    const rdl_status st = cw.get(nullptr, s, bytes, false);
+    const rdl_status st = cw.get(s, bytes, n_counters);
     out->p = cw.p;
+    out->counters = cw.counters;
     out->graph_owned = cw.graph_owned;
     return st;
 }

@@ -248,6 +248,7 @@ rdl_status check_pool(const rdl_kv_pool* p, PoolView* v) {
     if (p->page_stride % unit || p->head_stride % unit || p->position_stride % unit || ((uintptr_t)p->k_dev & 15) ||
         ((uintptr_t)p->v_dev & 15))
         return api_fail(RDL_ERR_INVALID_DATA, "pool strides and bases must be multiples of 16 bytes");
+    if (p->position_stride > 0 && (st = check_position_stride((size_t)p->position_stride)) != RDL_OK) return st;
     // the axes from the innermost out: each must step over all that the ones inside it span
     struct Axis {
         int64_t stride, count;
@@ -281,6 +282,11 @@ rdl_status check_page_positions(size_t n, int* shift) {
             return RDL_OK;
         }
     return api_fail(RDL_ERR_UNSUPPORTED, "%zu positions a page: a power of two, 16 .. 1024", n);
+}
+
+rdl_status check_position_stride(size_t n) {
+    if (n >= (size_t)1 << 24) return api_fail(RDL_ERR_UNSUPPORTED, "%zu elements between positions: below 2^24", n);
+    return RDL_OK;
 }
 
 rdl_status check_head_dim(size_t hd) {

@@ -25,6 +25,8 @@ struct PoolView {
 rdl_status check_pool(const rdl_kv_pool* p, PoolView* v);
 rdl_status check_page_positions(size_t n, int* shift);
 rdl_status check_head_dim(size_t hd);
+// elements between two positions: 16 of them within a 32-bit offset
+rdl_status check_position_stride(size_t n);
 // m rows of `width` elements, `stride` apart, 16-byte aligned and not NULL
 rdl_status check_rows(const char* what, const void* p, size_t stride, size_t width, size_t m, size_t elem);
 // whether two sets of m >= 1 f32 rows share an element

@@ -37,12 +37,14 @@ rdl_status api_ok();
 rdl_status api_require_device();
 // Work memory of one call on stream `s` (capi.hip): the stream's, or memory
 // of the graph while the stream is being captured; call_scratch_done after
-// the call's last launch.  Contents are undefined.
+// the call's last launch.  `bytes` at p, undefined, and n_counters ints that
+// are zero and that the call's launches have to leave at zero.
 struct CallScratch {
     void* p = nullptr;
+    int* counters = nullptr;
     bool graph_owned = false;
 };
-rdl_status call_scratch(hipStream_t s, size_t bytes, CallScratch* out);
+rdl_status call_scratch(hipStream_t s, size_t bytes, size_t n_counters, CallScratch* out);
 rdl_status call_scratch_done(hipStream_t s, CallScratch* scratch);
 
 // GGUF block geometry (rustml/quant/main/src/api/types.rs:1-17,
