@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "../../include/rdl_attention.h"
+#include "attention.hpp"
 #include "kv_pool.hpp"
 #include "rdl_device.hpp"
 #include "rdl_internal.hpp"
@@ -36,6 +37,7 @@ struct BatchArgs {
     const int32_t *row_start, *kv_len;  // kv_len NULL: the sequence's rows
     int n_seq;
     float scale;
+    uint32_t group_mul, group_shift;  // p / group = (mulhi(p, group_mul) + p) >> group_shift, p < 2^31
     // the launch: tile workgroups first, then few-row ones
     int pairs;        // n_seq * n_kv, rounded up to 8 from 8 on (pair % 8 is then the XCD)
     int tile_slots, tile_splits, few_slots, few_splits;
@@ -45,6 +47,14 @@ struct BatchArgs {
     int part_splits;
     int* counters;            // [m][n_heads], zero between launches
 };
+
+struct Pair {  // (row, head of the group) pair p of a sequence
+    int row, head;
+};
+__device__ __forceinline__ Pair pair_of(const BatchArgs& a, int p) {
+    const int row = (int)((__umulhi((uint32_t)p, a.group_mul) + (uint32_t)p) >> a.group_shift);
+    return {row, p - row * a.group};
+}
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
@@ -99,10 +109,10 @@ struct Geo {
     static constexpr int KROW = HD + 8, VROW = HD + (HD == 96 ? 0 : 32);
     static constexpr int KEY = (KROW + VROW) * PARTS;        // f16 elements a key
     static constexpr int TK = F32 || HD == 256 ? 32 : 64;    // keys of a tile
-    static constexpr int FW = F32 && HD == 256 ? 2 : 4;      // waves of the few-row kernel
-    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)FW * 32 * KEY * 2;
+    static constexpr int FK = F32 ? 16 : 32;                 // keys a wave takes at a time for few rows
+    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)4 * FK * KEY * 2;
     static constexpr size_t LDS = TILE_LDS > FEW_LDS ? TILE_LDS : FEW_LDS;
-    static_assert(LDS <= 160 * 1024 - 2048, "LDS of a CU");
+    static_assert(LDS <= 160 * 1024 - 6144, "LDS of a CU");
 };
 
 // What a wave's slab of keys needs beside its LDS rows.
@@ -304,7 +314,7 @@ __device__ __forceinline__ f4 wide4(const KV* v, bool on) {
 // The rows of a sequence that a launch works on.
 struct Seq {
     int64_t row0;   // its first row
-    int64_t pairs;  // (row, head of the group) pairs, rows cut to m
+    int pairs;      // (row, head of the group) pairs, rows cut to m
     int64_t first;  // last key that row 0 sees
     int t;          // keys
 };
@@ -313,7 +323,7 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
     const int64_t r0 = a.row_start[b], n = (int64_t)a.row_start[b + 1] - r0;
     int64_t t = a.kv_len ? (int64_t)a.kv_len[b] : n;
     s.row0 = r0;
-    s.pairs = r0 < 0 ? 0 : max((int64_t)0, min(n, a.m - r0)) * a.group;
+    s.pairs = r0 < 0 ? 0 : (int)(max((int64_t)0, min(n, a.m - r0)) * a.group);  // m * group < 2^31
     s.first = t - n;
     // keys that the table can name, or that are rows of the step
     t = min(t, a.kv.tables ? a.kv.table_stride << a.kv.shift : a.m - r0);
@@ -321,8 +331,8 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
     return s;
 }
 // The last key that pair p sees (-1: none).
-__device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int64_t p) {
-    const int64_t l = s.first + p / a.group;
+__device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int p) {
+    const int64_t l = s.first + pair_of(a, p).row;
     return (int)max((int64_t)-1, min(l, (int64_t)s.t - 1));
 }
 
@@ -332,12 +342,20 @@ __device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int64_
 // agent-coherent stores, each wave waits for its own, a barrier, then the
 // counter; the last split to arrive joins all of them in order (so results
 // do not depend on which it is) and leaves the counter at zero.
-__device__ __forceinline__ float* part_at(const BatchArgs& a, const Seq& s, int kvh, int64_t p, int z) {
-    const int64_t row = s.row0 + p / a.group, h = kvh * a.group + p % a.group;
-    return a.part + ((row * a.n_heads + h) * a.part_splits + z) * (a.hd + 2);
+__device__ __forceinline__ int64_t place(const BatchArgs& a, const Seq& s, int kvh, int p) {
+    const Pair x = pair_of(a, p);
+    return (s.row0 + x.row) * a.n_heads + kvh * a.group + x.head;
 }
-__device__ __forceinline__ float* out_at(const BatchArgs& a, const Seq& s, int kvh, int64_t p) {
-    return a.out + (s.row0 + p / a.group) * a.out_stride + (kvh * a.group + p % a.group) * a.hd;
+__device__ __forceinline__ float* part_at(const BatchArgs& a, const Seq& s, int kvh, int p, int z) {
+    return a.part + (place(a, s, kvh, p) * a.part_splits + z) * (a.hd + 2);
+}
+__device__ __forceinline__ float* out_at(const BatchArgs& a, const Seq& s, int kvh, int p) {
+    const Pair x = pair_of(a, p);
+    return a.out + (s.row0 + x.row) * a.out_stride + (kvh * a.group + x.head) * a.hd;
+}
+__device__ __forceinline__ const float* q_at(const BatchArgs& a, const Seq& s, int kvh, int p) {
+    const Pair x = pair_of(a, p);
+    return a.q + (s.row0 + x.row) * a.q_stride + (kvh * a.group + x.head) * a.hd;
 }
 __device__ __forceinline__ void put(float* p, float v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -345,40 +363,50 @@ __device__ __forceinline__ void put(float* p, float v) {
 __device__ __forceinline__ float get(const float* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int64_t p0, int pairs, int splits,
-                                     int* flag) {
+constexpr int MAX_SPLITS = 256;
+__device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
+                                     float* wts, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int64_t row = s.row0 + p0 / a.group, h = kvh * a.group + p0 % a.group;
-        int* c = a.counters + row * a.n_heads + h;
+        int* c = a.counters + place(a, s, kvh, p0);
         const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = old == splits - 1;
         if (old == splits - 1) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!*flag) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6, step = a.hd + 2;
+    float* wt = wts + w * MAX_SPLITS;
     for (int i = w; i < pairs; i += waves) {
         const float* pt = part_at(a, s, kvh, p0 + i, 0);
-        float M = -__builtin_inff(), L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int z = 0; z < splits; z++) {
-            const float l = get(pt + z * (a.hd + 2) + a.hd + 1);
-            if (l != 0.0f) M = fmaxf(M, get(pt + z * (a.hd + 2) + a.hd));
-        }
-        for (int z = 0; z < splits; z++) {
-            const float* pz = pt + z * (a.hd + 2);
-            const float l = get(pz + a.hd + 1);
-            const float wt = l != 0.0f ? l * __builtin_amdgcn_exp2f(get(pz + a.hd) - M) : 0.0f;
-            L += wt;
+        // a lane a split: weights L 2^(M - max M), and their sum
+        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], M = -__builtin_inff(), L = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 64 * c < a.hd && wt != 0.0f) o[c] += wt * get(pz + lane + 64 * c);
+        for (int c = 0; c < MAX_SPLITS / 64; c++) {
+            const int z = lane + 64 * c;
+            ll[c] = z < splits ? get(pt + z * step + a.hd + 1) : 0.0f;
+            ml[c] = z < splits ? get(pt + z * step + a.hd) : 0.0f;
         }
+#pragma unroll
+        for (int c = 0; c < MAX_SPLITS / 64; c++)
+            if (ll[c] != 0.0f) M = fmaxf(M, ml[c]);
+        M = att::wave_max(M);
+#pragma unroll
+        for (int c = 0; c < MAX_SPLITS / 64; c++) {
+            const float x = ll[c] != 0.0f ? ll[c] * __builtin_amdgcn_exp2f(ml[c] - M) : 0.0f;
+            wt[lane + 64 * c] = x;
+            L += x;
+        }
+        L = att::wave_sum(L);
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
         float* out = out_at(a, s, kvh, p0 + i);
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-            if (lane + 64 * c < a.hd) out[lane + 64 * c] = L != 0.0f ? o[c] / L : 0.0f;
+        for (int d = lane; d < a.hd; d += 64) {
+            float o = 0.0f;
+#pragma unroll 8
+            for (int z = 0; z < splits; z++) o += wt[z] * get(pt + z * step + d);
+            out[d] = o * inv;
+        }
     }
 }
 
@@ -426,9 +454,10 @@ __device__ __forceinline__ int load_q(const float* q, bool live, int d0, int ste
 // the second product's B operand once the keys of a 16-key step are taken in
 // the order 4h .. 4h + 3, 8 + 4h .. (h = lane / 32), in which the transposed LDS reads of V
 // fetch them.
+// Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
-__device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int64_t p0,
-                                          int z, _Float16* lds, Meta* meta, int* flag) {
+__device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
+                                          _Float16* lds, Meta* meta) {
     using G = Geo<KV, HD>;
     constexpr int TK = G::TK, SK = TK / 4, KS = HD / 16, DT = HD / 32;
     constexpr bool F32 = G::F32;
@@ -438,17 +467,16 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     // this tile's keys and the split's share of them
     const int keys = last_key(a, s, min(p0 + 127, s.pairs - 1)) + 1;
     const int splits = min(a.tile_splits, max(1, (keys + a.tile_span - 1) / a.tile_span));
-    if (z >= splits) return;
+    if (z >= splits) return 0;
     const int j_lo = z * a.tile_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.tile_span);
-    const int64_t p = p0 + 32 * w + c;
+    const int p = p0 + 32 * w + c;
     const bool live = p < s.pairs, work = p0 + 32 * w < s.pairs;
-    const int64_t row = s.row0 + p / a.group, head = kvh * a.group + p % a.group;
     const int last = live ? last_key(a, s, p) : -1;
     const int w_first = __builtin_amdgcn_readfirstlane(last_key(a, s, p0 + 32 * w));   // the wave's first pair sees
     const int w_last = __builtin_amdgcn_readfirstlane(last_key(a, s, min(p0 + 32 * w + 31, s.pairs - 1)));
     const int wg_first = last_key(a, s, p0);
     h8 qh[KS], ql[KS];
-    const int qe = load_q<KS>(a.q + row * a.q_stride + head * a.hd, live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
+    const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
     const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
@@ -621,48 +649,47 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
             put(dst + a.hd + 1, L);
         }
     }
-    if (splits > 1) join(a, s, kvh, p0, (int)min((int64_t)128, s.pairs - p0), splits, flag);
+    return splits;
 }
 
 // ---- few rows: up to 16 pairs, each wave its own keys ------------------------------------------
-// A decode step reads the cache once and computes little: the FW waves of a
+// A decode step reads the cache once and computes little: the 4 waves of a
 // workgroup take the split's keys 32 at a time in turn, each through LDS rows
-// of its own without a barrier, with the next 32 keys' loads in flight; at
+// of its own without a barrier, with the next keys' loads in flight; at
 // the end they join through LDS.  The products as above, 16 columns wide
 // (v_mfma_f32_16x16x32_f16): a lane has the scores of keys 4g .. 4g + 3 and 16 +
 // 4g .. (g = lane / 16) of one pair.
 template <typename KV, int HD>
-__device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int64_t p0,
-                                         int z, _Float16* lds, float* wml, int* flag) {
+__device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
+                                         _Float16* lds, float* wml) {
     using G = Geo<KV, HD>;
-    constexpr int KS = HD / 32, DT = HD / 16, FW = G::FW;
+    constexpr int KS = HD / 32, DT = HD / 16, FK = G::FK, NB = FK / 16;
     constexpr bool F32 = G::F32;
-    constexpr int KP = 32 * G::KROW, VP = 32 * G::VROW;
+    constexpr int KP = FK * G::KROW, VP = FK * G::VROW;
     constexpr int OROW = HD + 4;  // f32 elements of a pair's joined output
-    static_assert(16 * OROW * 4 <= 32 * G::KEY * 2, "the output fits the wave's key rows");
+    static_assert(16 * OROW * 4 <= FK * G::KEY * 2, "the output fits the wave's key rows");
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int pairs = (int)min((int64_t)16, s.pairs - p0);
+    const int pairs = min(16, s.pairs - p0);
     const int keys = last_key(a, s, p0 + pairs - 1) + 1;
     const int splits = min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
-    if (z >= splits) return;
+    if (z >= splits) return 0;
     const int j_lo = z * a.few_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.few_span);
-    const int64_t p = p0 + c;
+    const int p = p0 + c;
     const bool live = c < pairs;
-    const int64_t row = s.row0 + p / a.group, head = kvh * a.group + p % a.group;
     const int last = live ? last_key(a, s, p) : -1;
     const int first = last_key(a, s, p0);
-    _Float16* ks = lds + w * 32 * G::KEY;
+    _Float16* ks = lds + w * FK * G::KEY;
     _Float16* vs = ks + KP * G::PARTS;
     float M = -__builtin_inff(), L = 0.0f;
     f4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     int ref = -1000;
-    if (w < FW) {
-        Slab<KV, HD, 32> slab;
+    {
+        Slab<KV, HD, FK> slab;
         slab.init(a.kv, a.hd);
-        const int step = 32 * FW, j_w = j_lo + 32 * w;
+        const int step = 4 * FK, j_w = j_lo + FK * w;
         int valid = 0;
         if (j_w < j_hi) {
             slab.pages(a.kv, table, j_w, s.t);
@@ -670,20 +697,20 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
             slab.pages(a.kv, table, j_w + step, s.t);
         }
         h8 qh[KS], ql[KS];
-        const int qe = load_q<KS>(a.q + row * a.q_stride + head * a.hd, live, 8 * g, 32, a.hd, qh, ql, [](uint32_t m) {
+        const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * g, 32, a.hd, qh, ql, [](uint32_t m) {
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
         const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
-            const Meta mt = slab.store(ks, vs, KP, VP, valid, j0 + 31 > first);
+            const Meta mt = slab.store(ks, vs, KP, VP, valid, j0 + FK - 1 > first);
             if (j0 + step < j_hi) {
                 valid = slab.load(a.kv, s.row0, kvh, j0 + step, j_hi);
                 slab.pages(a.kv, table, j0 + 2 * step, s.t);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const bool masked = j0 + 31 > first || mt.valid != 3;
+            const bool masked = j0 + FK - 1 > first || mt.valid != (1 << NB) - 1;
             if constexpr (F32) {
                 if (mt.ve > ref) {
 #pragma unroll
@@ -693,12 +720,12 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
                     ref = mt.ve;
                 }
             }
-            f4 sc[2];
+            f4 sc[NB];
             const float f = F32 ? __builtin_amdgcn_ldexpf(cs, mt.ke) : cs;
             const int rel = last - j0;
             float mx = -__builtin_inff();
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < NB; b++) {
                 sc[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
                 const _Float16* kr = ks + (16 * b + c) * G::KROW + 8 * g;
 #pragma unroll
@@ -732,9 +759,9 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
                 M = Mn;
             }
             const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
-            u32x4 ph, pl;
+            uint32_t ph[2 * NB], pl[2 * NB];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < 2 * NB; u++) {
                 float x0 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2] + off);
                 float x1 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2 + 1] + off);
                 L += x0 + x1;
@@ -742,27 +769,30 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
                     x0 = __builtin_amdgcn_ldexpf(x0, mt.ve - ref);
                     x1 = __builtin_amdgcn_ldexpf(x1, mt.ve - ref);
                 }
-                uint32_t hi, lo;
-                split2(x0, x1, &hi, &lo);
-                ph[u] = hi;
-                pl[u] = lo;
+                split2(x0, x1, &ph[u], &pl[u]);
             }
-            const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
             const _Float16* vr = vs + (4 * g + ((lane & 15) >> 2)) * G::VROW + 4 * (lane & 3);
+            if constexpr (NB == 2) {
+                const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const h4 v0 = read_t(vr + 16 * d), v1 = read_t(vr + 16 * G::VROW + 16 * d);
-                const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p8, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, q8, o[d], 0, 0, 0);
-                if constexpr (F32) {
-                    const h4 w0 = read_t(vr + VP + 16 * d), w1 = read_t(vr + VP + 16 * G::VROW + 16 * d);
-                    const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p8, o[d], 0, 0, 0);
+                for (int d = 0; d < DT; d++) {
+                    const h4 v0 = read_t(vr + 16 * d), v1 = read_t(vr + 16 * G::VROW + 16 * d);
+                    const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p8, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, q8, o[d], 0, 0, 0);
+                }
+            } else {
+                const h4 p4 = __builtin_bit_cast(h4, ph), q4 = __builtin_bit_cast(h4, pl);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const h4 vf = read_t(vr + 16 * d), vl = read_t(vr + VP + 16 * d);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, p4, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, q4, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vl, p4, o[d], 0, 0, 0);
                 }
             }
             if (mt.bad)
-                for (int j = j0; j < min(j0 + 32, j_hi); j++) {
+                for (int j = j0; j < min(j0 + FK, j_hi); j++) {
                     const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
                     if (!v) continue;
 #pragma unroll
@@ -800,16 +830,16 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
         if (dim >= a.hd) continue;
         float Mx = -__builtin_inff(), Ls = 0.0f;
 #pragma unroll
-        for (int x = 0; x < FW; x++)
+        for (int x = 0; x < 4; x++)
             if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int x = 0; x < FW; x++) {
+        for (int x = 0; x < 4; x++) {
             const float l = wml[x * 32 + 16 + pi];
             if (l == 0.0f) continue;
             const float wt = l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx);
             Ls += wt;
-            y += wt * *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * 32 * G::KEY) + pi * OROW + dim);
+            y += wt * *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * FK * G::KEY) + pi * OROW + dim);
         }
         const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
         if (splits == 1) {
@@ -824,7 +854,7 @@ __device__ __forceinline__ void few_rows(const BatchArgs& a, const Seq& s, const
             }
         }
     }
-    if (splits > 1) join(a, s, kvh, p0, pairs, splits, flag);
+    return splits;
 }
 
 template <typename KV, int HD>
@@ -832,6 +862,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Meta meta[8];
     __shared__ float wml[4 * 32];
+    __shared__ float wts[4 * MAX_SPLITS];
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
     const int tile_blocks = a.pairs * a.tile_slots * a.tile_splits;
@@ -839,8 +870,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     int id = tile ? (int)blockIdx.x : (int)blockIdx.x - tile_blocks;
     const int pair = id % a.pairs;
     id /= a.pairs;
-    const int splits = tile ? a.tile_splits : a.few_splits, slots = tile ? a.tile_slots : a.few_slots;
-    const int z = id % splits, slot = id / splits;
+    const int most = tile ? a.tile_splits : a.few_splits, slots = tile ? a.tile_slots : a.few_slots;
+    const int z = id % most, slot = id / most;
     if (pair >= a.n_seq * a.n_kv) return;
     const int b = pair / a.n_kv, kvh = pair % a.n_kv;
     const Seq s = sequence(a, b);
@@ -848,9 +879,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
     // the last rows, which see the most keys, first
     const int width = tile ? 128 : 16;
-    for (int64_t i = (s.pairs - 1) / width - slot; i >= 0; i -= slots) {
-        if (tile) tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta, &flag);
-        else few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml, &flag);
+    for (int i = (s.pairs - 1) / width - slot; i >= 0; i -= slots) {
+        const int splits = tile ? tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta)
+                                : few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml);
+        if (splits > 1) join(a, s, kvh, i * width, min(width, s.pairs - i * width), splits, wts, &flag);
         __syncthreads();  // before the next rows take the LDS
     }
 }
@@ -882,6 +914,9 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     keys = std::max<int64_t>(1, std::min<int64_t>(keys, INT32_MAX / 2));
     const int64_t pairs = (int64_t)a.n_seq * a.n_kv, G = a.group;
     if (pairs > (int64_t)1 << 28) return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences of %d KV heads", a.n_seq, a.n_kv);
+    if (m * G > INT32_MAX) return api_fail(RDL_ERR_UNSUPPORTED, "%lld rows of %d heads a KV head", (long long)m, a.group);
+    while (((int64_t)1 << a.group_shift) < G) a.group_shift++;
+    a.group_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.group_shift) - (uint64_t)G)) / (uint64_t)G + 1);
     a.pairs = (int)(pairs < 8 ? pairs : (pairs + 7) / 8 * 8);
     // sequences of up to 16 pairs; all of them where none is expected to have more
     const bool only_few = rows * G <= 16;
@@ -895,6 +930,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
         int64_t n = (keys + sp - 1) / sp;
         const int64_t cap = (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float)));
         if (n > cap) n = std::max<int64_t>(1, cap);
+        n = std::min<int64_t>(n, MAX_SPLITS);
         sp = ((keys + n - 1) / n + unit - 1) / unit * unit;
         *splits = (int)n;
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);

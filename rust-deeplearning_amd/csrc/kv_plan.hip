@@ -16,126 +16,135 @@ namespace {
 // Two prefix sums over the sequences: rows (sum of new) and pages (sum of the
 // pages each takes beyond those it has).  Every workgroup forms them for
 // itself, PLAN_CHUNK sequences at a time, because a sum over a thousand
-// lengths (8 KB, in every L2) takes less time than a second launch would; it then
-// writes its own PLAN_ROWS rows, each finding its sequence by bisection in
-// LDS, and its own share of the sequences' new table entries.  Nothing passes
-// between workgroups: the slot of a row on a new page comes from the free
-// list, not from the table entry that another workgroup writes.
-constexpr int PLAN_NT = 256, PLAN_PER = 4, PLAN_CHUNK = PLAN_NT * PLAN_PER;
+// lengths (8 KB, in every L2) takes less time than a second launch would; it
+// then writes its own PLAN_ROWS rows and its own share of the new table
+// entries, a thread a row or an entry, each finding its sequence by bisection
+// in LDS.  Nothing passes between workgroups: the slot of a row on a new page
+// comes from the free list, not from the table entry that another workgroup
+// writes.  Sums stop at 2^31 - 1, which no row or free page number reaches.
+// Latency bounds it (one load of the lengths, the scan, a bisection and a
+// dependent load).
+constexpr int PLAN_NT = 512, PLAN_PER = 4, PLAN_CHUNK = PLAN_NT * PLAN_PER;
 constexpr int PLAN_ROWS = 1024;  // rows a workgroup
 
 struct PlanArgs {
     const int32_t *cached, *new_rows;
     int n_seq;
     const int32_t* free_pages;
-    int64_t n_free;
+    int n_free;
     int shift;  // log2(page_positions)
     int32_t* tables;
-    int64_t table_stride;
+    int table_stride;
     int32_t *row_start, *kv_len;
-    int64_t m;
+    int m;
     int32_t *row_seq, *positions, *slots, *summary;
 };
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {  // inclusive, over the 64 lanes
+__device__ __forceinline__ int add_cut(int a, int b) {  // of non-negative values
+    return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)INT32_MAX);
+}
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive, over the 64 lanes
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
+        const int o = __shfl_up(v, d);
+        if (lane >= d) v = add_cut(v, o);
     }
     return v;
 }
+// the last of n ascending values that is <= x (the first is)
+__device__ __forceinline__ int bisect(const int* v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
 
 __global__ __launch_bounds__(PLAN_NT) void plan_kernel(PlanArgs a) {
-    __shared__ int64_t start[PLAN_CHUNK + 1];  // first row of the chunk's sequences, then the chunk's end
-    __shared__ int64_t first[PLAN_CHUNK];      // their first place in the free list
-    __shared__ int32_t have[PLAN_CHUNK], need[PLAN_CHUNK], before[PLAN_CHUNK];
-    __shared__ int64_t wsum[2][PLAN_NT / 64];
-    __shared__ int32_t wflag[PLAN_NT / 64], wlong[PLAN_NT / 64];
+    // of the chunk's sequences: first row, first place in the free list, pages had, positions had
+    __shared__ int start[PLAN_CHUNK], first[PLAN_CHUNK], have[PLAN_CHUNK], before[PLAN_CHUNK];
+    __shared__ int wrows[PLAN_NT / 64], wpages[PLAN_NT / 64], wflag[PLAN_NT / 64], wlong[PLAN_NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t r_lo = (int64_t)blockIdx.x * PLAN_ROWS, r_hi = min(r_lo + PLAN_ROWS, a.m);
-    int64_t rows = 0, pages = 0;  // of the chunks before this one
-    int32_t flags = 0, longest = 0;
+    const int r_lo = min((int)blockIdx.x * PLAN_ROWS, a.m), r_hi = min(r_lo + PLAN_ROWS, a.m);
+    const int mask = (1 << a.shift) - 1;
+    int rows = 0, pages = 0;  // of the chunks before this one
+    int flags = 0, longest = 0;
     for (int c0 = 0; c0 < a.n_seq; c0 += PLAN_CHUNK) {
-        int32_t h[PLAN_PER], n[PLAN_PER], bf[PLAN_PER], nw[PLAN_PER];
-        int64_t sr = 0, sp = 0;
+        const int live = min(PLAN_CHUNK, a.n_seq - c0);
+        int c[PLAN_PER], k[PLAN_PER], h[PLAN_PER], n[PLAN_PER];
 #pragma unroll
         for (int i = 0; i < PLAN_PER; i++) {
-            const int b = c0 + tid * PLAN_PER + i;
-            h[i] = n[i] = bf[i] = nw[i] = 0;
-            if (b < a.n_seq) {
-                int32_t c = a.cached[b], k = a.new_rows[b];
-                if (c < 0 || k < 0) flags |= RDL_PLAN_BAD_LENGTH;
-                c = max(c, 0), k = max(k, 0);
-                int64_t t = (int64_t)c + k;
-                if (t > INT32_MAX) {
-                    flags |= RDL_PLAN_BAD_LENGTH;
-                    t = INT32_MAX, k = (int32_t)(t - c);
-                }
-                const int64_t mask = ((int64_t)1 << a.shift) - 1;
-                const int64_t hp = ((int64_t)c + mask) >> a.shift, tp = (t + mask) >> a.shift;
-                if (tp > a.table_stride) flags |= RDL_PLAN_TABLE_FULL;
-                h[i] = (int32_t)min(hp, a.table_stride);
-                n[i] = (int32_t)(min(tp, a.table_stride) - h[i]);
-                bf[i] = c, nw[i] = k;
-                longest = max(longest, (int32_t)t);
-                if (blockIdx.x == 0) a.kv_len[b] = (int32_t)t;
-            }
-            sr += nw[i], sp += n[i];
+            const int s = tid * PLAN_PER + i;
+            c[i] = s < live ? a.cached[c0 + s] : 0;
+            k[i] = s < live ? a.new_rows[c0 + s] : 0;
         }
-        const int64_t ir = wave_scan(sr), ip = wave_scan(sp);
+        int sr = 0, sp = 0;
+#pragma unroll
+        for (int i = 0; i < PLAN_PER; i++) {
+            const int s = tid * PLAN_PER + i;
+            if (c[i] < 0 || k[i] < 0) flags |= RDL_PLAN_BAD_LENGTH;
+            c[i] = max(c[i], 0), k[i] = max(k[i], 0);
+            const int t = add_cut(c[i], k[i]);
+            if (t - c[i] != k[i]) flags |= RDL_PLAN_BAD_LENGTH;
+            k[i] = t - c[i];
+            // ceil(x / page) of x < 2^31
+            const int hp = (c[i] >> a.shift) + ((c[i] & mask) != 0), tp = (t >> a.shift) + ((t & mask) != 0);
+            if (tp > a.table_stride) flags |= RDL_PLAN_TABLE_FULL;
+            h[i] = min(hp, a.table_stride);
+            n[i] = min(tp, a.table_stride) - h[i];
+            longest = max(longest, t);
+            if (blockIdx.x == 0 && s < live) a.kv_len[c0 + s] = t;
+            sr = add_cut(sr, k[i]), sp = add_cut(sp, n[i]);
+        }
+        const int ir = wave_scan(sr), ip = wave_scan(sp);
         __syncthreads();  // the previous chunk's LDS reads are done
-        if (lane == 63) wsum[0][w] = ir, wsum[1][w] = ip;
+        if (lane == 63) wrows[w] = ir, wpages[w] = ip;
         __syncthreads();
-        int64_t xr = rows + ir - sr, xp = pages + ip - sp;
+        const int rows0 = rows, pages0 = pages;
+        // what lies before this thread's first sequence
+        int xr = __shfl_up(ir, 1), xp = __shfl_up(ip, 1);
+        if (lane == 0) xr = xp = 0;
+        xr = add_cut(rows, xr), xp = add_cut(pages, xp);
 #pragma unroll
         for (int i = 0; i < PLAN_NT / 64; i++) {
-            if (i < w) xr += wsum[0][i], xp += wsum[1][i];
-            rows += wsum[0][i], pages += wsum[1][i];
+            if (i < w) xr = add_cut(xr, wrows[i]), xp = add_cut(xp, wpages[i]);
+            rows = add_cut(rows, wrows[i]), pages = add_cut(pages, wpages[i]);
         }
 #pragma unroll
         for (int i = 0; i < PLAN_PER; i++) {
-            const int s = tid * PLAN_PER + i, b = c0 + s;
-            start[s] = xr, first[s] = xp;
-            have[s] = h[i], need[s] = n[i], before[s] = bf[i];
-            if (blockIdx.x == 0 && b < a.n_seq) a.row_start[b] = (int32_t)min(xr, (int64_t)INT32_MAX);
-            xr += nw[i], xp += n[i];
+            const int s = tid * PLAN_PER + i;
+            start[s] = xr, first[s] = xp, have[s] = h[i], before[s] = c[i];
+            if (blockIdx.x == 0 && s < live) a.row_start[c0 + s] = xr;
+            xr = add_cut(xr, k[i]), xp = add_cut(xp, n[i]);
         }
-        if (tid == PLAN_NT - 1) start[PLAN_CHUNK] = rows;
         __syncthreads();
-        const int live = min(PLAN_CHUNK, a.n_seq - c0);
-        // new table entries: a wave a sequence
-        for (int s = (int)(blockIdx.x * (PLAN_NT / 64)) + w; s < live; s += (int)gridDim.x * (PLAN_NT / 64)) {
-            int32_t* row = a.tables + (int64_t)(c0 + s) * a.table_stride;
-            for (int i = lane; i < need[s]; i += 64) {
-                const int64_t f = first[s] + i;
-                row[have[s] + i] = f < a.n_free ? a.free_pages[f] : -1;
+        for (int r = max(r_lo, rows0) + tid; r < min(r_hi, rows); r += PLAN_NT) {
+            const int s = bisect(start, live, r);
+            const int pos = before[s] + (r - start[s]), p = pos >> a.shift;
+            int page = -1;
+            if (p < a.table_stride) {
+                if (p < have[s]) {
+                    page = a.tables[(int64_t)(c0 + s) * a.table_stride + p];
+                } else {
+                    const int f = add_cut(first[s], p - have[s]);
+                    if (f < a.n_free) page = a.free_pages[f];
+                }
             }
+            const int64_t slot = ((int64_t)page << a.shift) + (pos & mask);
+            a.row_seq[r] = c0 + s;
+            a.positions[r] = pos;
+            a.slots[r] = page < 0 || slot > INT32_MAX ? -1 : (int)slot;
         }
-        // this workgroup's rows of the chunk
-        for (int64_t r = max(r_lo, start[0]) + tid; r < min(r_hi, rows); r += PLAN_NT) {
-            int lo = 0, hi = live;  // the last sequence that starts at or before r
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= r) lo = mid;
-                else hi = mid;
-            }
-            const int64_t pos = before[lo] + (r - start[lo]), p = pos >> a.shift;
-            int32_t page = -1;
-            if (p < have[lo]) {
-                page = a.tables[(int64_t)(c0 + lo) * a.table_stride + p];
-            } else if (p - have[lo] < need[lo]) {
-                const int64_t f = first[lo] + (p - have[lo]);
-                if (f < a.n_free) page = a.free_pages[f];
-            }
-            const int64_t slot = ((int64_t)page << a.shift) + (pos & (((int64_t)1 << a.shift) - 1));
-            a.row_seq[r] = c0 + lo;
-            a.positions[r] = (int32_t)pos;
-            a.slots[r] = page < 0 || slot > INT32_MAX ? -1 : (int32_t)slot;
+        // entries of pages past the free list too: -1
+        for (int f = add_cut(pages0, (int)blockIdx.x * PLAN_NT + tid); f < pages; f = add_cut(f, (int)gridDim.x * PLAN_NT)) {
+            const int s = bisect(first, live, f);
+            a.tables[(int64_t)(c0 + s) * a.table_stride + have[s] + (f - first[s])] = f < a.n_free ? a.free_pages[f] : -1;
         }
     }
-    for (int64_t r = max(r_lo, rows) + tid; r < r_hi; r += PLAN_NT) {
+    for (int r = max(r_lo, rows) + tid; r < r_hi; r += PLAN_NT) {
         a.row_seq[r] = -1;
         a.positions[r] = 0;
         a.slots[r] = -1;
@@ -152,10 +161,9 @@ __global__ __launch_bounds__(PLAN_NT) void plan_kernel(PlanArgs a) {
         for (int i = 1; i < PLAN_NT / 64; i++) flags |= wflag[i], longest = max(longest, wlong[i]);
         if (pages > a.n_free) flags |= RDL_PLAN_NO_PAGES;
         if (rows > a.m) flags |= RDL_PLAN_NO_ROWS;
-        const int32_t total = (int32_t)min(rows, (int64_t)INT32_MAX);
-        a.row_start[a.n_seq] = total;
-        a.summary[0] = total;
-        a.summary[1] = (int32_t)min(pages, a.n_free);
+        a.row_start[a.n_seq] = rows;
+        a.summary[0] = rows;
+        a.summary[1] = min(pages, a.n_free);
         a.summary[2] = flags;
         a.summary[3] = longest;
     }
@@ -354,12 +362,12 @@ rdl_status rdl_kv_plan_dev(const int32_t* cached_dev, const int32_t* new_rows_de
     a.new_rows = new_rows_dev;
     a.n_seq = (int)n_seq;
     a.free_pages = free_pages_dev;
-    a.n_free = (int64_t)n_free;
+    a.n_free = (int)n_free;
     a.tables = tables_dev;
-    a.table_stride = (int64_t)table_stride;
+    a.table_stride = (int)table_stride;
     a.row_start = row_start_dev;
     a.kv_len = kv_len_dev;
-    a.m = (int64_t)m;
+    a.m = (int)m;
     a.row_seq = row_seq_dev;
     a.positions = positions_dev;
     a.slots = slots_dev;
