@@ -73,9 +73,20 @@ constexpr float SHIFT = 8.0f, SLACK = 7.0f;
 // a's sign and hi + lo is off by less than 2^-21 of it).
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
     const hp2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const float ra = a - (float)h[0], rb = b - (float)h[1];
+    const float ra = fmaf((float)h[0], -1.0f, a), rb = fmaf((float)h[1], -1.0f, b);
     *hi = __builtin_bit_cast(uint32_t, h);
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+}
+// What a product of a row with exponent qe is times to be a power of 2.  Not
+// below 2^-126, where it stands for scores of nothing in any case: masked
+// scores are -infinity before it.
+__device__ __forceinline__ float score_factor(float scale, int qe) {
+    return fmaxf(__builtin_amdgcn_ldexpf(scale * LOG2E, qe), 0x1p-126f);
+}
+// The weight of a score: f32 keys' scores carry the factor already.
+template <bool SCALED>
+__device__ __forceinline__ float weight(float s, float cs, float off) {
+    return __builtin_amdgcn_exp2f(SCALED ? s + off : fmaf(s, cs, off));
 }
 __device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
@@ -479,7 +490,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
-    const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
+    const float cs = score_factor(a.scale, qe);
     f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -487,6 +498,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
     float M = -__builtin_inff(), L = 0.0f;
     int ref = -1000;  // f32 values: o is held times 2^-ref
+    int wide = 0;     // some values were not finite
 
     Slab<KV, HD, SK> slab;
     slab.init(a.kv, a.hd);
@@ -515,6 +527,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
             mt[i].ke = F32 ? __builtin_amdgcn_readfirstlane(x.ke) : 0;
             mt[i].ve = F32 ? __builtin_amdgcn_readfirstlane(x.ve) : 0;
             masked |= !mt[i].valid;
+            wide |= mt[i].bad;
         }
         if constexpr (F32) {
             const int top = max(max(mt[0].ve, mt[1].ve), max(mt[2].ve, mt[3].ve));
@@ -542,20 +555,25 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[k], sc, 0, 0, 0);
                 }
             }
-            const int rel = last - (j0 + 32 * b);
-            float mx = -__builtin_inff();
+            if constexpr (F32)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const Meta& g = mt[(32 * b + 8 * i) / SK];
-                const float f = F32 ? __builtin_amdgcn_ldexpf(cs, g.ke) : cs;
+                for (int i = 0; i < 4; i++) {
+                    const float f = __builtin_amdgcn_ldexpf(cs, mt[(32 * b + 8 * i) / SK].ke);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    float x = sc[4 * i + t] * f;
-                    if (masked) x = 8 * i + 4 * h + t <= rel && g.valid ? x : -__builtin_inff();
-                    sc[4 * i + t] = x;
-                    mx = fmaxf(mx, x);
+                    for (int t = 0; t < 4; t++) sc[4 * i + t] *= f;
+                }
+            if (masked) {
+                const int rel = last - (j0 + 32 * b) - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const bool in = mt[(32 * b + 8 * (e >> 2)) / SK].valid && 8 * (e >> 2) + (e & 3) <= rel;
+                    sc[e] = in ? sc[e] : -__builtin_inff();
                 }
             }
+            float mx = sc[0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
+            if constexpr (!F32) mx *= cs;
             mx = max32(mx);
             if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
                 const float Mn = fmaxf(M, mx);
@@ -574,7 +592,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int e = 8 * k + 2 * u;
-                    float x0 = __builtin_amdgcn_exp2f(sc[e] + off), x1 = __builtin_amdgcn_exp2f(sc[e + 1] + off);
+                    float x0 = weight<F32>(sc[e], cs, off), x1 = weight<F32>(sc[e + 1], cs, off);
                     L += x0 + x1;
                     if constexpr (F32) {
                         const int sh = mt[(32 * b + 16 * k + (u >= 2 ? 8 : 0)) / SK].ve - ref;
@@ -603,26 +621,30 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                 }
             }
         }
-        // values that are not finite, where their key is seen
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (mt[i].bad)
-                for (int j = j0 + SK * i; j < min(j0 + SK * (i + 1), j_hi); j++) {
-                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
-                    if (!v) continue;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int dim = 32 * d + 8 * i + 4 * h;
-                            const f4 x = wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
-#pragma unroll
-                            for (int t = 0; t < 4; t++) o[d][4 * i + t] += x[t];
-                        }
-                }
     }
     L += other32(L);
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float x = o[d][e] * inv;
+            o[d][e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+        }
+    if (wide)  // rows that see a value that is not finite
+        for (int j = j_lo; j < min(j_hi, w_last + 1); j++) {
+            const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+            if (!v) continue;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int dim = 32 * d + 8 * i + 4 * h;
+                    const f4 x = wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
+#pragma unroll
+                    for (int t = 0; t < 4; t++) o[d][4 * i + t] += x[t];
+                }
+        }
     if (live) {
         float* dst = splits == 1 ? out_at(a, s, kvh, p) : part_at(a, s, kvh, p, z);
 #pragma unroll
@@ -633,10 +655,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                 if (dim >= a.hd) continue;
                 f4 y;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const float x = o[d][4 * i + t] * inv;
-                    y[t] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
-                }
+                for (int t = 0; t < 4; t++) y[t] = o[d][4 * i + t];
                 if (splits == 1) {
                     *reinterpret_cast<f4*>(dst + dim) = y;
                 } else {
@@ -685,7 +704,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     f4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    int ref = -1000;
+    int ref = -1000, wide = 0;
     {
         Slab<KV, HD, FK> slab;
         slab.init(a.kv, a.hd);
@@ -701,7 +720,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
-        const float cs = __builtin_amdgcn_ldexpf(a.scale * LOG2E, qe);
+        const float cs = score_factor(a.scale, qe);
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
             const Meta mt = slab.store(ks, vs, KP, VP, valid, j0 + FK - 1 > first);
             if (j0 + step < j_hi) {
@@ -711,6 +730,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             const bool masked = j0 + FK - 1 > first || mt.valid != (1 << NB) - 1;
+            wide |= mt.bad;
             if constexpr (F32) {
                 if (mt.ve > ref) {
 #pragma unroll
@@ -721,8 +741,6 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                 }
             }
             f4 sc[NB];
-            const float f = F32 ? __builtin_amdgcn_ldexpf(cs, mt.ke) : cs;
-            const int rel = last - j0;
             float mx = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -738,14 +756,21 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                         sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[k], sc[b], 0, 0, 0);
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    float x = sc[b][t] * f;
-                    if (masked) x = 16 * b + 4 * g + t <= rel && (mt.valid >> b & 1) ? x : -__builtin_inff();
-                    sc[b][t] = x;
-                    mx = fmaxf(mx, x);
-                }
+                if constexpr (F32) sc[b] *= __builtin_amdgcn_ldexpf(cs, mt.ke);
             }
+            if (masked) {
+                const int rel = last - j0 - 4 * g;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        sc[b][t] = (mt.valid >> b & 1) && 16 * b + t <= rel ? sc[b][t] : -__builtin_inff();
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) mx = fmaxf(mx, sc[b][t]);
+            if constexpr (!F32) mx *= cs;
             mx = fmaxf(mx, other16(mx));
             mx = max32(mx);
             if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
@@ -762,8 +787,8 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             uint32_t ph[2 * NB], pl[2 * NB];
 #pragma unroll
             for (int u = 0; u < 2 * NB; u++) {
-                float x0 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2] + off);
-                float x1 = __builtin_amdgcn_exp2f(sc[u >> 1][(u & 1) * 2 + 1] + off);
+                float x0 = weight<F32>(sc[u >> 1][(u & 1) * 2], cs, off);
+                float x1 = weight<F32>(sc[u >> 1][(u & 1) * 2 + 1], cs, off);
                 L += x0 + x1;
                 if constexpr (F32) {
                     x0 = __builtin_amdgcn_ldexpf(x0, mt.ve - ref);
@@ -791,16 +816,6 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vl, p4, o[d], 0, 0, 0);
                 }
             }
-            if (mt.bad)
-                for (int j = j0; j < min(j0 + FK, j_hi); j++) {
-                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
-                    if (!v) continue;
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const int dim = 16 * d + 4 * g;
-                        o[d] += wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
-                    }
-                }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -810,15 +825,25 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
         float* os = reinterpret_cast<float*>(ks);
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            f4 y;
+        for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float x = o[d][e] * inv;
-                y[e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+                o[d][e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
             }
-            *reinterpret_cast<f4*>(os + c * OROW + 16 * d + 4 * g) = y;
-        }
+        if (wide)  // rows that see a value that is not finite
+            for (int j0 = j_w; j0 < j_hi; j0 += step)
+                for (int j = j0; j < min(j0 + FK, j_hi); j++) {
+                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+                    if (!v) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const int dim = 16 * d + 4 * g;
+                        o[d] += wide4(v + (dim < a.hd ? dim : 0), j <= last && dim < a.hd);
+                    }
+                }
+#pragma unroll
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f4*>(os + c * OROW + 16 * d + 4 * g) = o[d];
         if (g == 0) {
             wml[w * 32 + c] = M;
             wml[w * 32 + 16 + c] = L;
