@@ -882,7 +882,10 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     return splits;
 }
 
-template <typename KV, int HD>
+// KIND: which workgroups a launch has.  The two bodies in one kernel keep more
+// registers than either needs, so launches that need one of them have it alone.
+constexpr int TILE = 1, FEW = 2;
+template <typename KV, int HD, int KIND>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Meta meta[8];
@@ -891,7 +894,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
     const int tile_blocks = a.pairs * a.tile_slots * a.tile_splits;
-    const bool tile = (int)blockIdx.x < tile_blocks;
+    const bool tile = KIND == TILE || (KIND != FEW && (int)blockIdx.x < tile_blocks);
     int id = tile ? (int)blockIdx.x : (int)blockIdx.x - tile_blocks;
     const int pair = id % a.pairs;
     id /= a.pairs;
@@ -905,26 +908,36 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     // the last rows, which see the most keys, first
     const int width = tile ? 128 : 16;
     for (int i = (s.pairs - 1) / width - slot; i >= 0; i -= slots) {
-        const int splits = tile ? tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta)
-                                : few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml);
+        int splits = 0;
+        if constexpr (KIND & TILE)
+            if (tile) splits = tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta);
+        if constexpr (KIND & FEW)
+            if (!tile) splits = few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml);
         if (splits > 1) join(a, s, kvh, i * width, min(width, s.pairs - i * width), splits, wts, &flag);
         __syncthreads();  // before the next rows take the LDS
     }
 }
 
-template <typename KV, int HD>
+template <typename KV, int HD, int KIND>
 hipError_t launch(const BatchArgs& a, hipStream_t s) {
-    const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<KV, HD>::LDS);
+    using G = Geo<KV, HD>;
+    constexpr size_t lds = KIND == TILE ? G::TILE_LDS : KIND == FEW ? G::FEW_LDS : G::LDS;
+    const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD, KIND>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     const unsigned blocks = (unsigned)(a.pairs * (a.tile_slots * a.tile_splits + a.few_slots * a.few_splits));
-    hipLaunchKernelGGL((attend_kernel<KV, HD>), dim3(blocks), dim3(256), (Geo<KV, HD>::LDS), s, a);
+    hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(256), lds, s, a);
     return hipGetLastError();
+}
+template <typename KV, int HD>
+hipError_t launch_kind(const BatchArgs& a, hipStream_t s) {
+    return !a.few_slots ? launch<KV, HD, TILE>(a, s) : !a.tile_slots ? launch<KV, HD, FEW>(a, s)
+                                                                     : launch<KV, HD, TILE | FEW>(a, s);
 }
 template <typename KV>
 hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
-    return a.hd <= 64 ? launch<KV, 64>(a, s) : a.hd <= 96 ? launch<KV, 96>(a, s)
-         : a.hd <= 128 ? launch<KV, 128>(a, s) : launch<KV, 256>(a, s);
+    return a.hd <= 64 ? launch_kind<KV, 64>(a, s) : a.hd <= 96 ? launch_kind<KV, 96>(a, s)
+         : a.hd <= 128 ? launch_kind<KV, 128>(a, s) : launch_kind<KV, 256>(a, s);
 }
 
 // Key ranges are split until the launch has about this many workgroups.
@@ -944,10 +957,10 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     a.group_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.group_shift) - (uint64_t)G)) / (uint64_t)G + 1);
     a.pairs = (int)(pairs < 8 ? pairs : (pairs + 7) / 8 * 8);
     // sequences of up to 16 pairs; all of them where none is expected to have more
-    const bool only_few = rows * G <= 16;
-    a.few_rows = only_few ? INT32_MAX : 16;
+    const bool only_few = rows * G <= 16, only_tile = !only_few && a.n_seq == 1;
+    a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : 16;
     const int64_t limit = (int64_t)1 << 30;  // workgroups of a launch
-    a.few_slots = 1;
+    a.few_slots = only_tile ? 0 : 1;
     a.tile_slots = only_few ? 0 : (int)std::max<int64_t>(1, std::min((rows * G + 127) / 128, limit / 4 / a.pairs));
     auto split = [&](int64_t base, int64_t target, int unit, int64_t min_span, int* span, int* splits) {
         int64_t sp = std::max(min_span, keys * base / target);
@@ -960,7 +973,8 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
         *splits = (int)n;
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
     };
-    split(pairs, FEW_TARGET, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
+    if (only_tile) a.few_span = INT32_MAX / 2, a.few_splits = 1;
+    else split(pairs, FEW_TARGET, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
     const int64_t tiles = std::min<int64_t>((rows * G + 127) / 128 * a.n_seq, m * G / 128 + a.n_seq) * a.n_kv;
     if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
     else split(tiles, TILE_TARGET, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
