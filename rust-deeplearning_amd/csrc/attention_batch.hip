@@ -38,12 +38,13 @@ struct BatchArgs {
     int n_seq;
     float scale;
     uint32_t group_mul, group_shift;  // p / group = (mulhi(p, group_mul) + p) >> group_shift, p < 2^31
-    // the launch: tile workgroups first, then few-row ones
-    int pairs;        // n_seq * n_kv, rounded up to 8 from 8 on (pair % 8 is then the XCD)
-    int tile_slots, tile_splits, few_slots, few_splits;
+    // The launch: tile workgroups first, then few-row ones, KV heads fastest
+    // (of 8 KV heads each has an XCD and its L2 to itself).
+    int tiles, tile_splits, few_splits;
     int tile_span, few_span;  // keys a split
     int few_rows;             // sequences of at most this many (row, head of a group) pairs are few-row ones
-    float* part;              // [m][n_heads][splits][hd + 2]: normalised output, maximum, sum
+    float* part;              // [m][n_heads][part_splits][hd]
+    float* part_ml;           // [m][n_heads][part_splits][2]
     int part_splits;
     int* counters;            // [m][n_heads], zero between launches
 };
@@ -297,6 +298,12 @@ __device__ __forceinline__ h4 read_t(const _Float16* p) {
     return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
 
+// Orders a wave's LDS accesses between its lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Row of V of key j (NULL: its page is not in the pool).
 template <typename KV>
 __device__ __forceinline__ const KV* value_row(const KvSource& s, int64_t row0, const int32_t* table, int kvh, int j) {
@@ -341,6 +348,39 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
     s.t = (int)max((int64_t)0, min(t, (int64_t)INT32_MAX - 4096));
     return s;
 }
+// Tiles are numbered so that a sequence is found from row_start alone:
+// sequence b's are TILE_PAIRS pairs each and numbered from row_start[b] group
+// / TILE_PAIRS + b on, which leaves at least as many numbers as it has tiles before
+// those of b + 1.
+constexpr int TILE_PAIRS = 128, FEW_PAIRS = 16;
+__device__ __forceinline__ int tiles_of(int pairs) { return (pairs + TILE_PAIRS - 1) / TILE_PAIRS; }
+__device__ __forceinline__ int first_tile(const BatchArgs& a, int64_t row0, int b) {
+    return (int)(row0 * a.group / TILE_PAIRS) + b;  // rows of sequences with pairs lie below m
+}
+// The sequence of tile number t, or -1 (the same in every lane): 64 samples of
+// row_start a step narrow it down, the last step looks at 64 sequences.
+__device__ __forceinline__ int sequence_of(const BatchArgs& a, int t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.n_seq;
+    while (n > 64) {
+        const int step = (n + 63) / 64, b = lo + lane * step;
+        const bool in = lane * step < n && first_tile(a, min((int64_t)a.row_start[min(b, a.n_seq)], a.m), b) <= t;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+        if (mask == 0) return -1;
+        const int k = (63 - __builtin_clzll(mask)) * step;
+        lo += k;
+        n = min(step, n - k);
+    }
+    const int b = lo + lane;
+    bool hit = false;
+    if (lane < n) {
+        const Seq s = sequence(a, b);
+        const int f = s.pairs ? first_tile(a, s.row0, b) : 0;
+        hit = s.pairs && t >= f && t - f < tiles_of(s.pairs);
+    }
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(hit);
+    return mask ? __builtin_amdgcn_readfirstlane(lo + __builtin_ctzll(mask)) : -1;
+}
 // The last key that pair p sees (-1: none).
 __device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int p) {
     const int64_t l = s.first + pair_of(a, p).row;
@@ -348,17 +388,14 @@ __device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int p)
 }
 
 // ---- joining split key ranges ---------------------------------------------------------
-// A split's partial result of `pairs` pairs from p0 on: normalised outputs with
-// their maxima and sums.  Publication as attention.hpp describes it:
+// A split's partial result: each pair's normalised outputs (part) with their
+// maximum and sum (part_ml).  Publication as attention.hpp describes it:
 // agent-coherent stores, each wave waits for its own, a barrier, then the
 // counter; the last split to arrive joins all of them in order (so results
 // do not depend on which it is) and leaves the counter at zero.
 __device__ __forceinline__ int64_t place(const BatchArgs& a, const Seq& s, int kvh, int p) {
     const Pair x = pair_of(a, p);
     return (s.row0 + x.row) * a.n_heads + kvh * a.group + x.head;
-}
-__device__ __forceinline__ float* part_at(const BatchArgs& a, const Seq& s, int kvh, int p, int z) {
-    return a.part + (place(a, s, kvh, p) * a.part_splits + z) * (a.hd + 2);
 }
 __device__ __forceinline__ float* out_at(const BatchArgs& a, const Seq& s, int kvh, int p) {
     const Pair x = pair_of(a, p);
@@ -368,18 +405,26 @@ __device__ __forceinline__ const float* q_at(const BatchArgs& a, const Seq& s, i
     const Pair x = pair_of(a, p);
     return a.q + (s.row0 + x.row) * a.q_stride + (kvh * a.group + x.head) * a.hd;
 }
-__device__ __forceinline__ void put(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+typedef float f2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void put2(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, f2{x, y}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float get(const float* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ f2 get2(const float* p) {
+    return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_AGENT));
 }
-constexpr int MAX_SPLITS = 256;
+// Pair p's partial of split z: outputs, maximum and sum.
+__device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, float M, float L) {
+    put2(a.part_ml + (at * a.part_splits + z) * 2, M, L);
+}
+constexpr int JOIN_NT = 256, JOIN_WEIGHTS = 4096;  // pairs * splits of a join, at most
 __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
-                                     float* wts, int* flag) {
+                                     float* wt, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) {
+    const int tid = threadIdx.x;
+    if (tid == 0) {
         int* c = a.counters + place(a, s, kvh, p0);
         const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = old == splits - 1;
@@ -387,37 +432,40 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     }
     __syncthreads();
     if (!*flag) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6, step = a.hd + 2;
-    float* wt = wts + w * MAX_SPLITS;
-    for (int i = w; i < pairs; i += waves) {
-        const float* pt = part_at(a, s, kvh, p0 + i, 0);
-        // a lane a split: weights L 2^(M - max M), and their sum
-        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], M = -__builtin_inff(), L = 0.0f;
-#pragma unroll
-        for (int c = 0; c < MAX_SPLITS / 64; c++) {
-            const int z = lane + 64 * c;
-            ll[c] = z < splits ? get(pt + z * step + a.hd + 1) : 0.0f;
-            ml[c] = z < splits ? get(pt + z * step + a.hd) : 0.0f;
-        }
-#pragma unroll
-        for (int c = 0; c < MAX_SPLITS / 64; c++)
-            if (ll[c] != 0.0f) M = fmaxf(M, ml[c]);
-        M = att::wave_max(M);
-#pragma unroll
-        for (int c = 0; c < MAX_SPLITS / 64; c++) {
-            const float x = ll[c] != 0.0f ? ll[c] * __builtin_amdgcn_exp2f(ml[c] - M) : 0.0f;
-            wt[lane + 64 * c] = x;
+    // maxima and sums to LDS, then a thread a pair: weights L 2^(M - max M) / their sum
+    float* mx = wt + JOIN_WEIGHTS;
+    for (int i = tid; i < pairs * splits; i += JOIN_NT) {
+        const int pi = i / splits, z = i - pi * splits;
+        const f2 ml = get2(a.part_ml + (place(a, s, kvh, p0 + pi) * a.part_splits + z) * 2);
+        mx[i] = ml[0];
+        wt[i] = ml[1];
+    }
+    __syncthreads();
+    if (tid < pairs) {
+        float M = -__builtin_inff(), L = 0.0f;
+        for (int i = tid * splits; i < (tid + 1) * splits; i++)
+            if (wt[i] != 0.0f) M = fmaxf(M, mx[i]);
+        for (int i = tid * splits; i < (tid + 1) * splits; i++) {
+            const float x = wt[i] != 0.0f ? wt[i] * __builtin_amdgcn_exp2f(mx[i] - M) : 0.0f;
+            wt[i] = x;
             L += x;
         }
-        L = att::wave_sum(L);
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        float* out = out_at(a, s, kvh, p0 + i);
-        for (int d = lane; d < a.hd; d += 64) {
-            float o = 0.0f;
-#pragma unroll 8
-            for (int z = 0; z < splits; z++) o += wt[z] * get(pt + z * step + d);
-            out[d] = o * inv;
+        for (int i = tid * splits; i < (tid + 1) * splits; i++) wt[i] *= inv;
+    }
+    __syncthreads();
+    const int quads = a.hd >> 2;
+    for (int i = tid; i < pairs * quads; i += JOIN_NT) {
+        const int pi = i / quads, d = (i - pi * quads) * 4;
+        const float* o = a.part + place(a, s, kvh, p0 + pi) * a.part_splits * a.hd + d;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int z = 0; z < splits; z++) {
+            const f2 u = get2(o + z * a.hd), v = get2(o + z * a.hd + 2);
+            const float w = wt[pi * splits + z];
+            y += w * f4{u[0], u[1], v[0], v[1]};
         }
+        *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + d) = y;
     }
 }
 
@@ -476,7 +524,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
     // this tile's keys and the split's share of them
-    const int keys = last_key(a, s, min(p0 + 127, s.pairs - 1)) + 1;
+    const int keys = last_key(a, s, min(p0 + TILE_PAIRS - 1, s.pairs - 1)) + 1;
     const int splits = min(a.tile_splits, max(1, (keys + a.tile_span - 1) / a.tile_span));
     if (z >= splits) return 0;
     const int j_lo = z * a.tile_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.tile_span);
@@ -645,29 +693,42 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                     for (int t = 0; t < 4; t++) o[d][4 * i + t] += x[t];
                 }
         }
-    if (live) {
-        float* dst = splits == 1 ? out_at(a, s, kvh, p) : part_at(a, s, kvh, p, z);
+    // the wave's rows through LDS of its own, OD dims at a time, so that each
+    // store covers whole rows: a lane's own values lie 16 bytes apart in 32 rows,
+    // and as write-through stores those took longer than the keys of a split
+    __syncthreads();
+    constexpr int OD = HD < 128 ? HD : 128, OROW = OD + 4;
+    static_assert((size_t)4 * 32 * OROW * 4 <= G::TILE_LDS, "outputs fit the tiles' LDS");
+    float* os = reinterpret_cast<float*>(lds) + w * 32 * OROW;
+    const int rows = min(32, s.pairs - p0 - 32 * w);
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+    for (int d0 = 0; d0 < HD; d0 += OD) {
+#pragma unroll
+        for (int d = 0; d < OD / 32; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int dim = 32 * d + 8 * i + 4 * h;
-                if (dim >= a.hd) continue;
-                f4 y;
-#pragma unroll
-                for (int t = 0; t < 4; t++) y[t] = o[d][4 * i + t];
-                if (splits == 1) {
-                    *reinterpret_cast<f4*>(dst + dim) = y;
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 4; t++) put(dst + dim + t, y[t]);
-                }
+                const f16v& x = o[d0 / 32 + d];
+                *reinterpret_cast<f4*>(os + c * OROW + 32 * d + 8 * i + 4 * h) =
+                    f4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
             }
-        if (splits > 1 && h == 0) {
-            put(dst + a.hd, M);
-            put(dst + a.hd + 1, L);
+        wave_sync();
+        constexpr int QR = OD / 4;  // float4 a row
+        for (int i = lane; i < rows * QR; i += 64) {
+            const int r = i / QR, d = d0 + i % QR * 4;
+            if (d >= a.hd) continue;
+            const f4 y = *reinterpret_cast<const f4*>(os + r * OROW + d - d0);
+            const int pr = p0 + 32 * w + r;
+            if (splits == 1) {
+                *reinterpret_cast<f4*>(out_at(a, s, kvh, pr) + d) = y;
+            } else {
+                float* dst = a.part + (place(a, s, kvh, pr) * a.part_splits + z) * a.hd + d;
+                put2(dst, y[0], y[1]);
+                put2(dst + 2, y[2], y[3]);
+            }
         }
+        wave_sync();
     }
+    if (splits > 1 && live && h == 0) put_ml(a, place(a, s, kvh, p), z, M, L);
     return splits;
 }
 
@@ -689,7 +750,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     static_assert(16 * OROW * 4 <= FK * G::KEY * 2, "the output fits the wave's key rows");
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int pairs = min(16, s.pairs - p0);
+    const int pairs = min(FEW_PAIRS, s.pairs - p0);
     const int keys = last_key(a, s, p0 + pairs - 1) + 1;
     const int splits = min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
     if (z >= splits) return 0;
@@ -727,8 +788,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                 valid = slab.load(a.kv, s.row0, kvh, j0 + step, j_hi);
                 slab.pages(a.kv, table, j0 + 2 * step, s.t);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
             const bool masked = j0 + FK - 1 > first || mt.valid != (1 << NB) - 1;
             wide |= mt.bad;
             if constexpr (F32) {
@@ -816,8 +876,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vl, p4, o[d], 0, 0, 0);
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
         }
         L += other16(L);
         L += other32(L);
@@ -870,13 +929,11 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         if (splits == 1) {
             *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y * inv;
         } else {
-            float* pt = part_at(a, s, kvh, p0 + pi, z);
-#pragma unroll
-            for (int e = 0; e < 4; e++) put(pt + dim + e, y[e] * inv);
-            if (dim == 0) {
-                put(pt + a.hd, Mx);
-                put(pt + a.hd + 1, Ls);
-            }
+            const int64_t at = place(a, s, kvh, p0 + pi);
+            float* pt = a.part + (at * a.part_splits + z) * a.hd + dim;
+            put2(pt, y[0] * inv, y[1] * inv);
+            put2(pt + 2, y[2] * inv, y[3] * inv);
+            if (dim == 0) put_ml(a, at, z, Mx, Ls);
         }
     }
     return splits;
@@ -890,31 +947,37 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Meta meta[8];
     __shared__ float wml[4 * 32];
-    __shared__ float wts[4 * MAX_SPLITS];
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
-    const int tile_blocks = a.pairs * a.tile_slots * a.tile_splits;
+    const int tile_blocks = a.n_kv * a.tiles * a.tile_splits;
     const bool tile = KIND == TILE || (KIND != FEW && (int)blockIdx.x < tile_blocks);
     int id = tile ? (int)blockIdx.x : (int)blockIdx.x - tile_blocks;
-    const int pair = id % a.pairs;
-    id /= a.pairs;
-    const int most = tile ? a.tile_splits : a.few_splits, slots = tile ? a.tile_slots : a.few_slots;
+    const int kvh = id % a.n_kv;
+    id /= a.n_kv;
+    const int most = tile ? a.tile_splits : a.few_splits;
     const int z = id % most, slot = id / most;
-    if (pair >= a.n_seq * a.n_kv) return;
-    const int b = pair / a.n_kv, kvh = pair % a.n_kv;
+    const int b = tile ? sequence_of(a, slot) : slot;
+    if (b < 0) return;
     const Seq s = sequence(a, b);
     if (s.pairs == 0 || (s.pairs > a.few_rows) != tile) return;
     const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
-    // the last rows, which see the most keys, first
-    const int width = tile ? 128 : 16;
-    for (int i = (s.pairs - 1) / width - slot; i >= 0; i -= slots) {
-        int splits = 0;
-        if constexpr (KIND & TILE)
-            if (tile) splits = tile_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, meta);
+    if (tile) {
+        if constexpr (KIND & TILE) {
+            // the last rows, which see the most keys, first
+            const int p0 = (tiles_of(s.pairs) - 1 - (slot - first_tile(a, s.row0, b))) * TILE_PAIRS;
+            const int splits = tile_rows<KV, HD>(a, s, table, kvh, p0, z, lds, meta);
+            // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
+            if (splits > 1)
+                join(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+        }
+    } else {
         if constexpr (KIND & FEW)
-            if (!tile) splits = few_rows<KV, HD>(a, s, table, kvh, i * width, z, lds, wml);
-        if (splits > 1) join(a, s, kvh, i * width, min(width, s.pairs - i * width), splits, wts, &flag);
-        __syncthreads();  // before the next rows take the LDS
+            for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once only where max_rows was too small
+                const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml);
+                if (splits > 1)
+                    join(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                __syncthreads();  // before the next rows take the LDS
+            }
     }
 }
 
@@ -925,14 +988,14 @@ hipError_t launch(const BatchArgs& a, hipStream_t s) {
     const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD, KIND>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
-    const unsigned blocks = (unsigned)(a.pairs * (a.tile_slots * a.tile_splits + a.few_slots * a.few_splits));
+    const unsigned blocks = (unsigned)(a.n_kv * (a.tiles * a.tile_splits + (KIND & FEW ? a.n_seq * a.few_splits : 0)));
     hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(256), lds, s, a);
     return hipGetLastError();
 }
 template <typename KV, int HD>
 hipError_t launch_kind(const BatchArgs& a, hipStream_t s) {
-    return !a.few_slots ? launch<KV, HD, TILE>(a, s) : !a.tile_slots ? launch<KV, HD, FEW>(a, s)
-                                                                     : launch<KV, HD, TILE | FEW>(a, s);
+    return a.few_rows == 0 ? launch<KV, HD, TILE>(a, s) : a.tiles == 0 ? launch<KV, HD, FEW>(a, s)
+                                                                       : launch<KV, HD, TILE | FEW>(a, s);
 }
 template <typename KV>
 hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
@@ -942,7 +1005,7 @@ hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
 
 // Key ranges are split until the launch has about this many workgroups.
 constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512;
-constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 512;
+constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 256;
 constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
 
 rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_t s) {
@@ -955,38 +1018,35 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     if (m * G > INT32_MAX) return api_fail(RDL_ERR_UNSUPPORTED, "%lld rows of %d heads a KV head", (long long)m, a.group);
     while (((int64_t)1 << a.group_shift) < G) a.group_shift++;
     a.group_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.group_shift) - (uint64_t)G)) / (uint64_t)G + 1);
-    a.pairs = (int)(pairs < 8 ? pairs : (pairs + 7) / 8 * 8);
     // sequences of up to 16 pairs; all of them where none is expected to have more
-    const bool only_few = rows * G <= 16, only_tile = !only_few && a.n_seq == 1;
-    a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : 16;
-    const int64_t limit = (int64_t)1 << 30;  // workgroups of a launch
-    a.few_slots = only_tile ? 0 : 1;
-    a.tile_slots = only_few ? 0 : (int)std::max<int64_t>(1, std::min((rows * G + 127) / 128, limit / 4 / a.pairs));
-    auto split = [&](int64_t base, int64_t target, int unit, int64_t min_span, int* span, int* splits) {
+    const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && a.n_seq == 1;
+    a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
+    a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
+    auto split = [&](int64_t base, int64_t target, int width, int unit, int64_t min_span, int* span, int* splits) {
         int64_t sp = std::max(min_span, keys * base / target);
         sp = (sp + unit - 1) / unit * unit;
         int64_t n = (keys + sp - 1) / sp;
         const int64_t cap = (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float)));
         if (n > cap) n = std::max<int64_t>(1, cap);
-        n = std::min<int64_t>(n, MAX_SPLITS);
+        n = std::min<int64_t>(n, JOIN_WEIGHTS / width);
         sp = ((keys + n - 1) / n + unit - 1) / unit * unit;
         *splits = (int)n;
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
     };
     if (only_tile) a.few_span = INT32_MAX / 2, a.few_splits = 1;
-    else split(pairs, FEW_TARGET, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
-    const int64_t tiles = std::min<int64_t>((rows * G + 127) / 128 * a.n_seq, m * G / 128 + a.n_seq) * a.n_kv;
+    else split(pairs, FEW_TARGET, FEW_PAIRS, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
     if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
-    else split(tiles, TILE_TARGET, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
+    else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, TILE_PAIRS, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
     a.part_splits = std::max(a.few_splits, a.tile_splits);
-    if ((int64_t)a.pairs * ((int64_t)a.tile_slots * a.tile_splits + a.few_splits) > limit)
-        return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences of %lld rows", a.n_seq, (long long)rows);
+    if (((int64_t)a.tiles * a.tile_splits + (int64_t)a.n_seq * a.few_splits) * a.n_kv > (int64_t)1 << 30)
+        return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows", a.n_seq, (long long)m);
     CallScratch work;
     if (a.part_splits > 1) {
         const size_t bytes = (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float);
         const rdl_status st = call_scratch(s, bytes, (size_t)m * a.n_heads, &work);
         if (st != RDL_OK) return st;
         a.part = reinterpret_cast<float*>(work.p);
+        a.part_ml = a.part + (size_t)m * a.n_heads * a.part_splits * a.hd;
         a.counters = work.counters;
     }
     const hipError_t e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
