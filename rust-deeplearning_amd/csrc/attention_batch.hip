@@ -47,6 +47,10 @@ struct BatchArgs {
     float* part_ml;           // [m][n_heads][part_splits][2]
     int part_splits;
     int* counters;            // [m][n_heads], zero between launches
+    // Split sources: tiles of TK keys as LDS holds them, numbered as row tiles
+    // are (tile of TK rows * n_kv + KV head), and their exponents and flags
+    const _Float16* images;
+    const int4* notes;
 };
 
 struct Pair {  // (row, head of the group) pair p of a sequence
@@ -78,17 +82,13 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
     *hi = __builtin_bit_cast(uint32_t, h);
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
 }
-// What a product of a row with exponent qe is times to be a power of 2.  Not
+// x 2^e, the factor from a product of scaled parts to a power of 2.  Not
 // below 2^-126, where it stands for scores of nothing in any case: masked
 // scores are -infinity before it.
-__device__ __forceinline__ float score_factor(float scale, int qe) {
-    return fmaxf(__builtin_amdgcn_ldexpf(scale * LOG2E, qe), 0x1p-126f);
+__device__ __forceinline__ float score_factor(float x, int e) {
+    return fmaxf(__builtin_amdgcn_ldexpf(x, e), 0x1p-126f);
 }
-// The weight of a score: f32 keys' scores carry the factor already.
-template <bool SCALED>
-__device__ __forceinline__ float weight(float s, float cs, float off) {
-    return __builtin_amdgcn_exp2f(SCALED ? s + off : fmaf(s, cs, off));
-}
+__device__ __forceinline__ float weight(float s, float f, float off) { return __builtin_amdgcn_exp2f(fmaf(s, f, off)); }
 __device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
                                                     false, false);
@@ -109,22 +109,77 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     v = max(v, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, v))));
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
+// Maximum over the first N lanes of each N (4 or 8), uniform.
+template <int N>
+__device__ __forceinline__ int lanes_max(int v) {
+    v = max(v, dpp_i32<DPP_QUAD_XOR1>(v));
+    v = max(v, dpp_i32<DPP_QUAD_XOR2>(v));
+    if constexpr (N == 8) v = max(v, dpp_i32<DPP_ROW_HALF_MIRROR>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
 // floor(log2(v)) of a positive finite f32 given by its bits (-127 below 2^-126)
 __device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }
 
-// LDS rows of one key: HD f16 values and a pad that spreads 16 rows' 16-byte
-// reads (K) and 4 rows' 64-byte transposed reads (V) over all 64 banks.
+// Splits 8 f32 values times 2^-e.
+__device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u32x4* lo) {
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float a = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].z : x[p].x)), -e);
+            const float b = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].w : x[p].y)), -e);
+            uint32_t h, l;
+            split2(a, b, &h, &l);
+            (*hi)[2 * p + c] = h;
+            (*lo)[2 * p + c] = l;
+        }
+}
+// Largest magnitude over a wave's pieces, as f32 bits; finite: of the finite
+// ones only.  As integers, the largest signed value is the largest positive
+// f32 (NaN above infinity) and the largest unsigned one, where its sign is
+// set, the negative f32 of the largest magnitude.
+template <int N, int P>
+__device__ __forceinline__ uint32_t largest_bits(const u32x4 (&x)[N][P], bool finite) {
+    int32_t pos = 0;
+    uint32_t neg = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t b = x[i][p][c];
+                if (finite && (b & 0x7F800000u) == 0x7F800000u) b = 0;
+                pos = max(pos, (int32_t)b);
+                neg = max(neg, b);
+            }
+    return wave_max_u32(max((uint32_t)pos, neg & 0x80000000u ? neg & 0x7FFFFFFFu : 0u));
+}
+
+// Where a launch's keys and values come from: _Float16 and float as they
+// are, Split as f32 rows that split_kernel has made f16 parts of before.
+struct Split {};
+
+// LDS rows of one key, HDP f16 values without a pad (direct loads fill them
+// 16 bytes a lane in order).  The 16-byte pieces of a row stand in the order
+// piece ^ k_swap (K) or ^ v_swap (V) of the row, so that 16 rows' reads of one
+// piece (K) and the transposed reads of 4 rows' 64 bytes (V) fall on all 64 banks.
 template <typename KV, int HD>
 struct Geo {
-    static constexpr bool F32 = std::is_same<KV, float>::value;
-    static constexpr int PARTS = F32 ? 2 : 1;                // hi, lo
-    static constexpr int KROW = HD + 8, VROW = HD + (HD == 96 ? 0 : 32);
-    static constexpr int KEY = (KROW + VROW) * PARTS;        // f16 elements a key
-    static constexpr int TK = F32 || HD == 256 ? 32 : 64;    // keys of a tile
-    static constexpr int FK = F32 ? 16 : 32;                 // keys a wave takes at a time for few rows
-    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)4 * FK * KEY * 2;
+    static constexpr bool TWO = !std::is_same<KV, _Float16>::value;  // hi, lo parts
+    static constexpr int PARTS = TWO ? 2 : 1;
+    static constexpr int HDP = HD == 96 ? 128 : HD;
+    static constexpr int KEY = 2 * HDP * PARTS;              // f16 elements a key
+    static constexpr int W = 4;                              // waves of a workgroup, 32 pairs each of a tile
+    static constexpr int TK = HD == 64 ? 64 : TWO || HD == 256 ? 32 : 64;  // keys of a tile
+    static constexpr int FK = TWO ? 16 : 32;                 // keys a wave takes at a time for few rows
+    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)W * FK * KEY * 2;
     static constexpr size_t LDS = TILE_LDS > FEW_LDS ? TILE_LDS : FEW_LDS;
     static_assert(LDS <= 160 * 1024 - 6144, "LDS of a CU");
+    static __device__ __forceinline__ int k_swap(int row) { return HDP == 64 ? (row >> 1) & 7 : row & 15; }
+    static __device__ __forceinline__ int v_swap(int row) {
+        return (HDP == 64 ? (row & 2) << 1 : (row & 3) << 2) | (row & 4) >> 1;
+    }
 };
 
 // What a wave's slab of keys needs beside its LDS rows.
@@ -141,7 +196,7 @@ struct Meta {
 template <typename KV, int HD, int SK>
 struct Slab {
     using G = Geo<KV, HD>;
-    static constexpr bool F32 = G::F32;
+    static constexpr bool F32 = G::TWO;
     static constexpr int E = (int)sizeof(KV);
     static constexpr int CPR = HD / 8;              // 8-element pieces a key
     static constexpr int NL = (SK * CPR + 63) / 64;  // pieces a lane
@@ -200,43 +255,24 @@ struct Slab {
         }
         return valid;
     }
-    // Splits 8 f32 values times 2^-e.
-    static __device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u32x4* lo) {
-#pragma unroll
-        for (int p = 0; p < 2; p++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const float a = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].z : x[p].x)), -e);
-                const float b = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].w : x[p].y)), -e);
-                uint32_t h, l;
-                split2(a, b, &h, &l);
-                (*hi)[2 * p + c] = h;
-                (*lo)[2 * p + c] = l;
-            }
+    // The exponent to hold a slab of largest magnitude `bits` with: the one in
+    // use, `ref`, where that keeps 22 bits of its values (f16 parts of
+    // values that begin 2^12 below 2^15 still end 2^-27 of them further down),
+    // so that slabs seldom differ; else its own.
+    static __device__ __forceinline__ int hold(uint32_t bits, int ref) {
+        const int e = exponent(bits) - 14;
+        return e <= ref && e >= ref - 12 ? ref : e;
     }
-    // Largest magnitude of an array of pieces, as f32 bits; finite: of the finite ones only.
-    static __device__ __forceinline__ uint32_t largest(const u32x4 (&x)[NL][G::PARTS], bool finite) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < NL; i++)
-#pragma unroll
-            for (int p = 0; p < G::PARTS; p++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t b = x[i][p][c] & 0x7FFFFFFFu;
-                    m = max(m, finite && b >= 0x7F800000u ? 0u : b);
-                }
-        return wave_max_u32(m);
-    }
-    // Registers to the slab's LDS rows (lds: its K hi rows; K lo, V hi, V lo
-    // `part` rows further on).  check: whether values that are not finite
+    // Registers to LDS rows row0 .. of ks and vs (the lo parts `part` elements
+    // further on).  check: whether values that are not finite
     // have to be found (f16; f32 finds them on the way to the exponent).
-    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int kpart, int vpart, int valid, bool check) {
+    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int row0, int part, int valid, bool check, int kref,
+                                          int vref) {
         const int lane = threadIdx.x & 63;
         Meta mt{valid, 0, 0, 0};
         if constexpr (F32) {
-            uint32_t km = largest(k, false), vm = largest(v, false);
-            if (km >= 0x7F800000u) km = largest(k, true);
+            uint32_t km = largest_bits(k, false), vm = largest_bits(v, false);
+            if (km >= 0x7F800000u) km = largest_bits(k, true);
             if (vm >= 0x7F800000u) {
                 mt.bad = 1;
 #pragma unroll
@@ -246,10 +282,10 @@ struct Slab {
 #pragma unroll
                         for (int c = 0; c < 4; c++)
                             if ((v[i][p][c] & 0x7F800000u) == 0x7F800000u) v[i][p][c] = 0;
-                vm = largest(v, false);
+                vm = largest_bits(v, false);
             }
-            mt.ke = exponent(km) - 14;
-            mt.ve = exponent(vm) - 14;
+            mt.ke = hold(km, kref);
+            mt.ve = hold(vm, vref);
         } else if (check) {
             bool found = false;
 #pragma unroll
@@ -272,16 +308,17 @@ struct Slab {
         for (int i = 0; i < NL; i++) {
             const int pc = lane + 64 * i, key = pc / CPR, col = pc % CPR;
             if (!WHOLE && key >= SK) continue;
-            u32x4* kd = reinterpret_cast<u32x4*>(ks + key * G::KROW + col * 8);
-            u32x4* vd = reinterpret_cast<u32x4*>(vs + key * G::VROW + col * 8);
+            const int row = row0 + key;
+            u32x4* kd = reinterpret_cast<u32x4*>(ks + row * G::HDP + (col ^ G::k_swap(row)) * 8);
+            u32x4* vd = reinterpret_cast<u32x4*>(vs + row * G::HDP + (col ^ G::v_swap(row)) * 8);
             if constexpr (F32) {
                 u32x4 kh, kl, vh, vl;
                 split8(k[i], mt.ke, &kh, &kl);
                 split8(v[i], mt.ve, &vh, &vl);
                 *kd = kh;
-                *reinterpret_cast<u32x4*>(ks + kpart + key * G::KROW + col * 8) = kl;
+                kd[part / 8] = kl;
                 *vd = vh;
-                *reinterpret_cast<u32x4*>(vs + vpart + key * G::VROW + col * 8) = vl;
+                vd[part / 8] = vl;
             } else {
                 *kd = k[i][0];
                 *vd = v[i][0];
@@ -291,9 +328,99 @@ struct Slab {
     }
 };
 
+// One load of 16 bytes a lane from a buffer straight to LDS (lane l's at lds + 16
+// l; an offset past the buffer writes zeros).  In asm, because the compiler
+// makes every LDS read wait for all such loads that it knows of, the next
+// tile's among them; they have no output register, and loads_done() stands
+// before the barrier that precedes the reads.
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
+                 : "memory");
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ i32x4 uniform_rsrc(const void* base, int bytes) {
+    const uint64_t b = (uint64_t)base;
+    return {__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xFFFF),
+            __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// A wave's slab of SK f16 keys straight to its LDS rows.
+template <int HD, int SK>
+struct DirectSlab {
+    using G = Geo<_Float16, HD>;
+    static constexpr int C = G::HDP / 8, KI = 64 / C, NL = SK / KI;  // pieces a row, rows a load, loads
+    static_assert(SK <= 16 && NL * KI == SK, "whole loads of one page");
+    uint32_t koff[NL], voff[NL];
+    int pg;
+    __device__ __forceinline__ void init(const KvSource& s, int hd, int row0) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int key = KI * i + (threadIdx.x & 63) / C, piece = (threadIdx.x & 63) % C;
+            const int kc = piece ^ G::k_swap(row0 + key), vc = piece ^ G::v_swap(row0 + key);
+            koff[i] = kc * 8 < hd ? (uint32_t)(key * (int)s.k_position + kc * 8) * 2 : RSRC_OOB;
+            voff[i] = vc * 8 < hd ? (uint32_t)(key * (int)s.v_position + vc * 8) * 2 : RSRC_OOB;
+        }
+    }
+    __device__ __forceinline__ void pages(const KvSource& s, const int32_t* table, int j, int t) {
+        pg = s.tables && j < t ? table[j >> s.shift] : 0;
+    }
+    // issues the loads of the slab at key j to LDS rows at byte addresses ks, vs; whether its page is in the pool
+    __device__ __forceinline__ int load(const KvSource& s, int64_t row0, int kvh, int j, int t, uint32_t ks, uint32_t vs) {
+        int64_t kb, vb;
+        bool ok = true;
+        if (s.tables) {
+            const int p = __builtin_amdgcn_readfirstlane(pg);
+            ok = (uint32_t)p < (uint32_t)s.n_pages;
+            const int64_t at = (ok ? p : 0) * s.page + kvh * s.head;
+            const int o = j & ((1 << s.shift) - 1);
+            kb = at + o * s.k_position;
+            vb = at + o * s.v_position;
+        } else {
+            kb = (row0 + j) * s.k_position + kvh * s.head;
+            vb = (row0 + j) * s.v_position + kvh * s.head;
+        }
+        const int rows = ok ? max(0, min(SK, t - j)) : 0;
+        if (rows == 0) kb = vb = 0;
+        const i32x4 kr = uniform_rsrc(reinterpret_cast<const _Float16*>(s.k) + kb, rows * (int)s.k_position * 2);
+        const i32x4 vr = uniform_rsrc(reinterpret_cast<const _Float16*>(s.v) + vb, rows * (int)s.v_position * 2);
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            load_to_lds(kr, koff[i], ks + 1024 * i);
+            load_to_lds(vr, voff[i], vs + 1024 * i);
+        }
+        return ok;
+    }
+    // Zeroes the values of the slab's LDS rows that are not finite; whether there were any.
+    static __device__ __forceinline__ int clean(_Float16* vs) {
+        u32x4* v = reinterpret_cast<u32x4*>(vs) + (threadIdx.x & 63);
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const u32x4 x = v[64 * i];
+#pragma unroll
+            for (int c = 0; c < 4; c++) found |= ((((x[c] & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0);
+        }
+        if (!__builtin_amdgcn_ballot_w64(found)) return 0;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            u32x4 x = v[64 * i];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if ((x[c] & 0x7C00u) == 0x7C00u) x[c] &= 0xFFFF0000u;
+                if ((x[c] & 0x7C000000u) == 0x7C000000u) x[c] &= 0xFFFFu;
+            }
+            v[64 * i] = x;
+        }
+        return 1;
+    }
+};
+
 // 4 keys (consecutive LDS rows from `row`) of 16 dims, transposed: lane i of
 // each 16 gets dim i's 4 values.
-__device__ __forceinline__ h4 read_t(const _Float16* p) {
+__device__ __forceinline__ h4 read_t(const void* p) {
     typedef __attribute__((address_space(3))) s4 lds_s4;
     return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
@@ -353,18 +480,22 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
 // / TILE_PAIRS + b on, which leaves at least as many numbers as it has tiles before
 // those of b + 1.
 constexpr int TILE_PAIRS = 128, FEW_PAIRS = 16;
-__device__ __forceinline__ int tiles_of(int pairs) { return (pairs + TILE_PAIRS - 1) / TILE_PAIRS; }
-__device__ __forceinline__ int first_tile(const BatchArgs& a, int64_t row0, int b) {
-    return (int)(row0 * a.group / TILE_PAIRS) + b;  // rows of sequences with pairs lie below m
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int n) { return (int)(((uint32_t)n + TILE - 1) / TILE); }
+template <int TILE>
+__device__ __forceinline__ int first_tile(int64_t row0, int unit, int b) {
+    return (int)((uint64_t)max((int64_t)0, row0 * unit) / TILE) + b;  // row0 * unit < 2^31: rows lie below m
 }
-// The sequence of tile number t, or -1 (the same in every lane): 64 samples of
-// row_start a step narrow it down, the last step looks at 64 sequences.
-__device__ __forceinline__ int sequence_of(const BatchArgs& a, int t) {
+// The sequence of number t among tiles of TILE units, `unit` units a row, or -1
+// (the same in every lane): 64 samples of row_start a step narrow it down, the last
+// step looks at 64 sequences.
+template <int TILE>
+__device__ __forceinline__ int sequence_of(const BatchArgs& a, int t, int unit) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = a.n_seq;
     while (n > 64) {
         const int step = (n + 63) / 64, b = lo + lane * step;
-        const bool in = lane * step < n && first_tile(a, min((int64_t)a.row_start[min(b, a.n_seq)], a.m), b) <= t;
+        const bool in = lane * step < n && first_tile<TILE>(min((int64_t)a.row_start[min(b, a.n_seq)], a.m), unit, b) <= t;
         const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
         if (mask == 0) return -1;
         const int k = (63 - __builtin_clzll(mask)) * step;
@@ -375,8 +506,9 @@ __device__ __forceinline__ int sequence_of(const BatchArgs& a, int t) {
     bool hit = false;
     if (lane < n) {
         const Seq s = sequence(a, b);
-        const int f = s.pairs ? first_tile(a, s.row0, b) : 0;
-        hit = s.pairs && t >= f && t - f < tiles_of(s.pairs);
+        const int rows = unit == 1 ? pair_of(a, s.pairs).row : s.pairs;  // units: rows, or pairs
+        const int f = rows ? first_tile<TILE>(s.row0, unit, b) : 0;
+        hit = rows && t >= f && t - f < tiles_of<TILE>(rows);
     }
     const uint64_t mask = __builtin_amdgcn_ballot_w64(hit);
     return mask ? __builtin_amdgcn_readfirstlane(lo + __builtin_ctzll(mask)) : -1;
@@ -418,7 +550,8 @@ __device__ __forceinline__ f2 get2(const float* p) {
 __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, float M, float L) {
     put2(a.part_ml + (at * a.part_splits + z) * 2, M, L);
 }
-constexpr int JOIN_NT = 256, JOIN_WEIGHTS = 4096;  // pairs * splits of a join, at most
+constexpr int JOIN_WEIGHTS = 4096;  // pairs * splits of a join, at most
+template <int NT>
 __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
                                      float* wt, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -434,7 +567,7 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     if (!*flag) return;
     // maxima and sums to LDS, then a thread a pair: weights L 2^(M - max M) / their sum
     float* mx = wt + JOIN_WEIGHTS;
-    for (int i = tid; i < pairs * splits; i += JOIN_NT) {
+    for (int i = tid; i < pairs * splits; i += NT) {
         const int pi = i / splits, z = i - pi * splits;
         const f2 ml = get2(a.part_ml + (place(a, s, kvh, p0 + pi) * a.part_splits + z) * 2);
         mx[i] = ml[0];
@@ -455,7 +588,7 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     }
     __syncthreads();
     const int quads = a.hd >> 2;
-    for (int i = tid; i < pairs * quads; i += JOIN_NT) {
+    for (int i = tid; i < pairs * quads; i += NT) {
         const int pi = i / quads, d = (i - pi * quads) * 4;
         const float* o = a.part + place(a, s, kvh, p0 + pi) * a.part_splits * a.hd + d;
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -506,7 +639,7 @@ __device__ __forceinline__ int load_q(const float* q, bool live, int d0, int ste
     return e;
 }
 
-// ---- many rows: 4 waves of 32 pairs, tiles of TK keys shared through LDS -------------------
+// ---- many rows: waves of 32 pairs, tiles of TK keys shared through LDS -------------------
 // Each wave holds 32 pairs as the columns of both products, S^T = K Q^T and
 // O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a lane has 16 scores of one pair, so
 // the softmax needs one exchange with lane ^ 32, and its weights are already
@@ -515,16 +648,19 @@ __device__ __forceinline__ int load_q(const float* q, bool live, int d0, int ste
 // fetch them.
 // Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
-__device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
-                                          _Float16* lds, Meta* meta) {
+__device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
+                                         int p0, int z, _Float16* lds, Meta* meta) {
     using G = Geo<KV, HD>;
-    constexpr int TK = G::TK, SK = TK / 4, KS = HD / 16, DT = HD / 32;
-    constexpr bool F32 = G::F32;
-    constexpr int KP = TK * G::KROW, VP = TK * G::VROW;  // a part's elements
+    typedef typename std::conditional<std::is_same<KV, Split>::value, float, KV>::type Elem;
+    constexpr int TK = G::TK, W = G::W, SK = TK / W, KS = HD / 16, DT = HD / 32, HDP = G::HDP;
+    constexpr bool TWO = G::TWO, RAW32 = std::is_same<KV, float>::value, PRE = std::is_same<KV, Split>::value;
+    // blocks of 32 keys that take one softmax step together: two where registers hold their scores
+    constexpr int NB = TWO || HD == 256 ? 1 : 2;
+    constexpr int PART = TK * HDP;  // a part's elements
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
     // this tile's keys and the split's share of them
-    const int keys = last_key(a, s, min(p0 + TILE_PAIRS - 1, s.pairs - 1)) + 1;
+    const int keys = last_key(a, s, min(p0 + 32 * G::W - 1, s.pairs - 1)) + 1;
     const int splits = min(a.tile_splits, max(1, (keys + a.tile_span - 1) / a.tile_span));
     if (z >= splits) return 0;
     const int j_lo = z * a.tile_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.tile_span);
@@ -538,7 +674,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
-    const float cs = score_factor(a.scale, qe);
+    const float cs = score_factor(a.scale * LOG2E, qe);
     f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -546,39 +682,82 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
     float M = -__builtin_inff(), L = 0.0f;
     int ref = -1000;  // f32 values: o is held times 2^-ref
+    int kref = -1000; // f32 keys: the exponent last used
     int wide = 0;     // some values were not finite
 
-    Slab<KV, HD, SK> slab;
-    slab.init(a.kv, a.hd);
-    slab.pages(a.kv, table, j_lo + SK * w, s.t);
-    int valid = slab.load(a.kv, s.row0, kvh, j_lo + SK * w, j_hi);
-    slab.pages(a.kv, table, j_lo + TK + SK * w, s.t);
+    // LDS addresses of this lane's operands; a step further along a row is an
+    // exclusive or, because the pieces' order is one
+    const uint32_t k_off = (c * HDP + (h ^ G::k_swap(c)) * 8) * 2;
+    const int v_row = 4 * h + ((lane & 15) >> 2);
+    const uint32_t v_off = (PART * G::PARTS + v_row * HDP +
+                            ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ G::v_swap(v_row)) * 8 + 4 * (lane & 1)) * 2;
+    typedef typename std::conditional<RAW32, Slab<float, HD, SK>, DirectSlab<HD, (SK < 16 ? SK : 16)>>::type Stage;
+    Stage slab;
+    int valid = 1;
+    [[maybe_unused]] int4 note_next = {0, 0, 0, 0};
+    const uint32_t lds0 = lds_address(lds);
+    [[maybe_unused]] const int64_t image = PRE ? ((int64_t)(s.row0 / TK) + b) * a.n_kv + kvh : 0;  // of the sequence's first tile
+    auto fetch = [&](int j, int to) {  // a wave's share of the tile at key j, to buffer `to`
+        if constexpr (PRE) {
+            const int64_t im = image + (int64_t)(j / TK) * a.n_kv;
+            note_next = a.notes[im];
+            constexpr int SHARE = TK * G::KEY * 2 / W;  // bytes
+            const i32x4 r = uniform_rsrc(a.images + im * (TK * G::KEY) + w * (SHARE / 2), SHARE);
+#pragma unroll
+            for (int i = 0; i < SHARE / 1024; i++)
+                load_to_lds(r, 1024 * i + 16 * lane, lds0 + to * TK * G::KEY * 2 + w * SHARE + 1024 * i);
+        } else if constexpr (RAW32) {
+            valid = slab.load(a.kv, s.row0, kvh, j + SK * w, j_hi);
+            slab.pages(a.kv, table, j + TK + SK * w, s.t);
+        } else {
+            const uint32_t at = lds0 + (to * TK * G::KEY + SK * w * HDP) * 2;
+            valid = slab.load(a.kv, s.row0, kvh, j + SK * w, j_hi, at, at + PART * 2);
+            slab.pages(a.kv, table, j + TK + SK * w, s.t);
+        }
+    };
+    if (j_lo < j_hi) {
+        if constexpr (RAW32) slab.init(a.kv, a.hd);
+        else if constexpr (!PRE) slab.init(a.kv, a.hd, SK * w);
+        if constexpr (!PRE) slab.pages(a.kv, table, j_lo + SK * w, s.t);
+        fetch(j_lo, 0);
+    }
     int buf = 0;
     for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
-        _Float16* ks = lds + buf * TK * G::KEY;
-        _Float16* vs = ks + KP * G::PARTS;
-        const Meta mine = slab.store(ks + SK * w * G::KROW, vs + SK * w * G::VROW, KP, VP, valid, j0 + TK - 1 > wg_first);
-        if (lane == 0) meta[buf * 4 + w] = mine;
-        if (j0 + TK < j_hi) {
-            valid = slab.load(a.kv, s.row0, kvh, j0 + TK + SK * w, j_hi);
-            slab.pages(a.kv, table, j0 + 2 * TK + SK * w, s.t);
+        const int at = buf * TK * G::KEY;  // elements
+        Meta note;
+        if constexpr (RAW32) {
+            const Meta mine = slab.store(lds + at, lds + at + PART * 2, SK * w, PART, valid, true, kref, ref);
+            if (lane == 0) meta[buf * W + w] = mine;
+            if (j0 + TK < j_hi) fetch(j0 + TK, 0);
+            __syncthreads();
+            note = meta[buf * W + (lane & (W - 1))];
+        } else if constexpr (PRE) {
+            note = Meta{1, note_next.z, note_next.x, note_next.y};
+            loads_done();
+            __syncthreads();
+            if (j0 + TK < j_hi) fetch(j0 + TK, buf ^ 1);
+        } else {
+            if (lane == 0) meta[buf * W + w] = Meta{valid, 0, 0, 0};
+            loads_done();
+            __syncthreads();
+            if (j0 + TK - 1 > wg_first) {  // some of its values are masked
+                if (Stage::clean(lds + at + PART + SK * w * HDP) && lane == 0) meta[buf * W + w].bad = 1;
+                __syncthreads();
+            }
+            if (j0 + TK < j_hi) fetch(j0 + TK, buf ^ 1);
+            note = meta[buf * W + (lane & (W - 1))];
         }
-        __syncthreads();
         if (!work || j0 > w_last) continue;
-        Meta mt[4];
-        bool masked = j0 + TK - 1 > w_first;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const Meta x = meta[buf * 4 + i];
-            mt[i].valid = __builtin_amdgcn_readfirstlane(x.valid);
-            mt[i].bad = __builtin_amdgcn_readfirstlane(x.bad);
-            mt[i].ke = F32 ? __builtin_amdgcn_readfirstlane(x.ke) : 0;
-            mt[i].ve = F32 ? __builtin_amdgcn_readfirstlane(x.ve) : 0;
-            masked |= !mt[i].valid;
-            wide |= mt[i].bad;
-        }
-        if constexpr (F32) {
-            const int top = max(max(mt[0].ve, mt[1].ve), max(mt[2].ve, mt[3].ve));
+        // the slabs' notes, a lane a slab
+        [[maybe_unused]] const Meta* notes = meta + buf * W;
+        const bool masked = j0 + TK - 1 > w_first || __builtin_amdgcn_ballot_w64(!note.valid);
+        wide |= __builtin_amdgcn_ballot_w64(note.bad) != 0;
+        float f = cs;
+        bool other_k = false, other_v = false;  // f32: slabs held with other exponents than the rest
+        [[maybe_unused]] int pre_ve = 0;
+        if constexpr (TWO) {
+            kref = lanes_max<W>(note.ke);
+            const int top = lanes_max<W>(note.ve);
             if (top > ref) {
 #pragma unroll
                 for (int d = 0; d < DT; d++)
@@ -586,43 +765,53 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                     for (int e = 0; e < 16; e++) o[d][e] = __builtin_amdgcn_ldexpf(o[d][e], ref - top);
                 ref = top;
             }
+            f = score_factor(cs, kref);
+            other_k = __builtin_amdgcn_ballot_w64(note.ke != kref);
+            other_v = __builtin_amdgcn_ballot_w64(note.ve != ref);
+            pre_ve = top;
         }
 #pragma unroll
-        for (int b = 0; b < TK / 32; b++) {
-            f16v sc;
+        for (int b0 = 0; b0 < TK / 32; b0 += NB) {
+            f16v sc[NB];
 #pragma unroll
-            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-            const _Float16* kr = ks + (32 * b + c) * G::KROW + 8 * h;
+            for (int b = 0; b < NB; b++) {
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const h8 kf = *reinterpret_cast<const h8*>(kr + 16 * k);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc, 0, 0, 0);
-                if constexpr (F32) {
-                    const h8 kl = *reinterpret_cast<const h8*>(kr + KP + 16 * k);
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[k], sc, 0, 0, 0);
+                for (int e = 0; e < 16; e++) sc[b][e] = 0.0f;
+                const char* kr = reinterpret_cast<const char*>(lds) + (size_t)(at + 32 * (b0 + b) * HDP) * 2;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    const uint32_t ko = k_off ^ (32 * k);
+                    const h8 kf = *reinterpret_cast<const h8*>(kr + ko);
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc[b], 0, 0, 0);
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[b], 0, 0, 0);
+                    if constexpr (TWO) {
+                        const h8 kl = *reinterpret_cast<const h8*>(kr + ko + PART * 2);
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[k], sc[b], 0, 0, 0);
+                    }
                 }
             }
-            if constexpr (F32)
+            if (RAW32 && other_k)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float f = __builtin_amdgcn_ldexpf(cs, mt[(32 * b + 8 * i) / SK].ke);
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++) sc[4 * i + t] *= f;
+                    for (int e = 0; e < 16; e++)
+                        sc[b][e] = __builtin_amdgcn_ldexpf(sc[b][e], notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ke - kref);
+            if (masked)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const int rel = last - (j0 + 32 * (b0 + b)) - 4 * h;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const bool in = (PRE || notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].valid) && 8 * (e >> 2) + (e & 3) <= rel;
+                        sc[b][e] = in ? sc[b][e] : -__builtin_inff();
+                    }
                 }
-            if (masked) {
-                const int rel = last - (j0 + 32 * b) - 4 * h;
+            float mx = sc[0][0];
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const bool in = mt[(32 * b + 8 * (e >> 2)) / SK].valid && 8 * (e >> 2) + (e & 3) <= rel;
-                    sc[e] = in ? sc[e] : -__builtin_inff();
-                }
-            }
-            float mx = sc[0];
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
-            if constexpr (!F32) mx *= cs;
-            mx = max32(mx);
+                for (int e = b == 0; e < 16; e++) mx = fmaxf(mx, sc[b][e]);
+            mx = max32(mx) * f;
             if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
                 const float Mn = fmaxf(M, mx);
                 const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
@@ -634,40 +823,46 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                 M = Mn;
             }
             const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
+            auto values = [&](auto shifted) {
 #pragma unroll
-            for (int k = 0; k < 2; k++) {  // 16 keys a step
-                u32x4 ph, pl;
+                for (int b = 0; b < NB; b++) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int e = 8 * k + 2 * u;
-                    float x0 = weight<F32>(sc[e], cs, off), x1 = weight<F32>(sc[e + 1], cs, off);
-                    L += x0 + x1;
-                    if constexpr (F32) {
-                        const int sh = mt[(32 * b + 16 * k + (u >= 2 ? 8 : 0)) / SK].ve - ref;
-                        x0 = __builtin_amdgcn_ldexpf(x0, sh);
-                        x1 = __builtin_amdgcn_ldexpf(x1, sh);
+                    for (int e = 0; e < 16; e++) {
+                        sc[b][e] = weight(sc[b][e], f, off);
+                        L += sc[b][e];
+                        if constexpr (decltype(shifted)::value)
+                            sc[b][e] = __builtin_amdgcn_ldexpf(sc[b][e], (PRE ? pre_ve : notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ve) - ref);
                     }
-                    uint32_t hi, lo;
-                    split2(x0, x1, &hi, &lo);
-                    ph[u] = hi;
-                    pl[u] = lo;
-                }
-                const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
-                const _Float16* vr = vs + (32 * b + 16 * k + 4 * h + ((lane & 15) >> 2)) * G::VROW +
-                                     16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const h4 v0 = read_t(vr + 32 * d), v1 = read_t(vr + 8 * G::VROW + 32 * d);
-                    const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p8, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q8, o[d], 0, 0, 0);
-                    if constexpr (F32) {
-                        const h4 w0 = read_t(vr + VP + 32 * d), w1 = read_t(vr + VP + 8 * G::VROW + 32 * d);
-                        const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p8, o[d], 0, 0, 0);
+                    for (int k = 0; k < 2; k++) {  // 16 keys a step
+                        u32x4 ph, pl;
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            uint32_t hi, lo;
+                            split2(sc[b][8 * k + 2 * u], sc[b][8 * k + 2 * u + 1], &hi, &lo);
+                            ph[u] = hi;
+                            pl[u] = lo;
+                        }
+                        const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
+                        const char* vr = reinterpret_cast<const char*>(lds) + (size_t)(at + (32 * (b0 + b) + 16 * k) * HDP) * 2;
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            const char* vd = vr + (v_off ^ (64 * d));
+                            const h4 v0 = read_t(vd), v1 = read_t(vd + 16 * HDP);
+                            const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p8, o[d], 0, 0, 0);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q8, o[d], 0, 0, 0);
+                            if constexpr (TWO) {
+                                const h4 w0 = read_t(vd + PART * 2), w1 = read_t(vd + PART * 2 + 16 * HDP);
+                                const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p8, o[d], 0, 0, 0);
+                            }
+                        }
                     }
                 }
-            }
+            };
+            if (TWO && other_v) values(std::true_type{});
+            else values(std::false_type{});
         }
     }
     L += other32(L);
@@ -677,11 +872,11 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const float x = o[d][e] * inv;
-            o[d][e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+            o[d][e] = TWO ? __builtin_amdgcn_ldexpf(x, ref) : x;
         }
     if (wide)  // rows that see a value that is not finite
         for (int j = j_lo; j < min(j_hi, w_last + 1); j++) {
-            const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+            const Elem* v = value_row<Elem>(a.kv, s.row0, table, kvh, j);
             if (!v) continue;
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -697,8 +892,8 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     // store covers whole rows: a lane's own values lie 16 bytes apart in 32 rows,
     // and as write-through stores those took longer than the keys of a split
     __syncthreads();
-    constexpr int OD = HD < 128 ? HD : 128, OROW = OD + 4;
-    static_assert((size_t)4 * 32 * OROW * 4 <= G::TILE_LDS, "outputs fit the tiles' LDS");
+    constexpr int OD = HD < 128 ? HD : 128, OROW = HDP < 128 ? HDP : 128;
+    static_assert((size_t)W * 32 * OROW * 4 <= G::TILE_LDS, "outputs fit the tiles' LDS");
     float* os = reinterpret_cast<float*>(lds) + w * 32 * OROW;
     const int rows = min(32, s.pairs - p0 - 32 * w);
 #pragma unroll
@@ -708,7 +903,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const f16v& x = o[d0 / 32 + d];
-                *reinterpret_cast<f4*>(os + c * OROW + 32 * d + 8 * i + 4 * h) =
+                *reinterpret_cast<f4*>(os + c * OROW + ((8 * d + 2 * i + h) ^ (c & 15)) * 4) =
                     f4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
             }
         wave_sync();
@@ -716,7 +911,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
         for (int i = lane; i < rows * QR; i += 64) {
             const int r = i / QR, d = d0 + i % QR * 4;
             if (d >= a.hd) continue;
-            const f4 y = *reinterpret_cast<const f4*>(os + r * OROW + d - d0);
+            const f4 y = *reinterpret_cast<const f4*>(os + r * OROW + ((i % QR) ^ (r & 15)) * 4);
             const int pr = p0 + 32 * w + r;
             if (splits == 1) {
                 *reinterpret_cast<f4*>(out_at(a, s, kvh, pr) + d) = y;
@@ -733,7 +928,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 }
 
 // ---- few rows: up to 16 pairs, each wave its own keys ------------------------------------------
-// A decode step reads the cache once and computes little: the 4 waves of a
+// A decode step reads the cache once and computes little: the waves of a
 // workgroup take the split's keys 32 at a time in turn, each through LDS rows
 // of its own without a barrier, with the next keys' loads in flight; at
 // the end they join through LDS.  The products as above, 16 columns wide
@@ -743,9 +938,9 @@ template <typename KV, int HD>
 __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
                                          _Float16* lds, float* wml) {
     using G = Geo<KV, HD>;
-    constexpr int KS = HD / 32, DT = HD / 16, FK = G::FK, NB = FK / 16;
-    constexpr bool F32 = G::F32;
-    constexpr int KP = FK * G::KROW, VP = FK * G::VROW;
+    constexpr int KS = HD / 32, DT = HD / 16, FK = G::FK, NB = FK / 16, W = G::W, HDP = G::HDP;
+    constexpr bool F32 = G::TWO;
+    constexpr int PART = FK * HDP;
     constexpr int OROW = HD + 4;  // f32 elements of a pair's joined output
     static_assert(16 * OROW * 4 <= FK * G::KEY * 2, "the output fits the wave's key rows");
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -760,7 +955,10 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     const int last = live ? last_key(a, s, p) : -1;
     const int first = last_key(a, s, p0);
     _Float16* ks = lds + w * FK * G::KEY;
-    _Float16* vs = ks + KP * G::PARTS;
+    _Float16* vs = ks + PART * G::PARTS;
+    const int v_row = 4 * g + ((lane & 15) >> 2);
+    const uint32_t k_off = (c * HDP + (g ^ G::k_swap(c)) * 8) * 2;
+    const uint32_t v_off = (v_row * HDP + (((lane & 3) >> 1) ^ G::v_swap(v_row)) * 8 + 4 * (lane & 1)) * 2;
     float M = -__builtin_inff(), L = 0.0f;
     f4 o[DT];
 #pragma unroll
@@ -769,7 +967,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     {
         Slab<KV, HD, FK> slab;
         slab.init(a.kv, a.hd);
-        const int step = 4 * FK, j_w = j_lo + FK * w;
+        const int step = W * FK, j_w = j_lo + FK * w;
         int valid = 0;
         if (j_w < j_hi) {
             slab.pages(a.kv, table, j_w, s.t);
@@ -781,9 +979,9 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
-        const float cs = score_factor(a.scale, qe);
+        const float cs = score_factor(a.scale * LOG2E, qe);
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
-            const Meta mt = slab.store(ks, vs, KP, VP, valid, j0 + FK - 1 > first);
+            const Meta mt = slab.store(ks, vs, 0, PART, valid, j0 + FK - 1 > first, 0, -1000);
             if (j0 + step < j_hi) {
                 valid = slab.load(a.kv, s.row0, kvh, j0 + step, j_hi);
                 slab.pages(a.kv, table, j0 + 2 * step, s.t);
@@ -805,18 +1003,17 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 sc[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                const _Float16* kr = ks + (16 * b + c) * G::KROW + 8 * g;
+                const char* kr = reinterpret_cast<const char*>(ks + 16 * b * HDP);
 #pragma unroll
                 for (int k = 0; k < KS; k++) {
-                    const h8 kf = *reinterpret_cast<const h8*>(kr + 32 * k);
+                    const h8 kf = *reinterpret_cast<const h8*>(kr + (k_off ^ (64 * k)));
                     sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[k], sc[b], 0, 0, 0);
                     sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[k], sc[b], 0, 0, 0);
                     if constexpr (F32) {
-                        const h8 kl = *reinterpret_cast<const h8*>(kr + KP + 32 * k);
+                        const h8 kl = *reinterpret_cast<const h8*>(kr + (k_off ^ (64 * k)) + PART * 2);
                         sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[k], sc[b], 0, 0, 0);
                     }
                 }
-                if constexpr (F32) sc[b] *= __builtin_amdgcn_ldexpf(cs, mt.ke);
             }
             if (masked) {
                 const int rel = last - j0 - 4 * g;
@@ -830,7 +1027,8 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) mx = fmaxf(mx, sc[b][t]);
-            if constexpr (!F32) mx *= cs;
+            const float f = F32 ? score_factor(cs, mt.ke) : cs;
+            mx *= f;
             mx = fmaxf(mx, other16(mx));
             mx = max32(mx);
             if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
@@ -847,8 +1045,8 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             uint32_t ph[2 * NB], pl[2 * NB];
 #pragma unroll
             for (int u = 0; u < 2 * NB; u++) {
-                float x0 = weight<F32>(sc[u >> 1][(u & 1) * 2], cs, off);
-                float x1 = weight<F32>(sc[u >> 1][(u & 1) * 2 + 1], cs, off);
+                float x0 = weight(sc[u >> 1][(u & 1) * 2], f, off);
+                float x1 = weight(sc[u >> 1][(u & 1) * 2 + 1], f, off);
                 L += x0 + x1;
                 if constexpr (F32) {
                     x0 = __builtin_amdgcn_ldexpf(x0, mt.ve - ref);
@@ -856,12 +1054,13 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                 }
                 split2(x0, x1, &ph[u], &pl[u]);
             }
-            const _Float16* vr = vs + (4 * g + ((lane & 15) >> 2)) * G::VROW + 4 * (lane & 3);
+            const char* vr = reinterpret_cast<const char*>(vs);
             if constexpr (NB == 2) {
                 const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    const h4 v0 = read_t(vr + 16 * d), v1 = read_t(vr + 16 * G::VROW + 16 * d);
+                    const char* vd = vr + (v_off ^ (32 * d));
+                    const h4 v0 = read_t(vd), v1 = read_t(vd + 32 * HDP);
                     const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p8, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, q8, o[d], 0, 0, 0);
@@ -870,7 +1069,8 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                 const h4 p4 = __builtin_bit_cast(h4, ph), q4 = __builtin_bit_cast(h4, pl);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    const h4 vf = read_t(vr + 16 * d), vl = read_t(vr + VP + 16 * d);
+                    const char* vd = vr + (v_off ^ (32 * d));
+                    const h4 vf = read_t(vd), vl = read_t(vd + PART * 2);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, p4, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, q4, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vl, p4, o[d], 0, 0, 0);
@@ -909,16 +1109,16 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < pairs * (HD / 4); i += blockDim.x) {
+    for (int i = threadIdx.x; i < pairs * (HD / 4); i += W * 64) {
         const int pi = i / (HD / 4), dim = (i % (HD / 4)) * 4;
         if (dim >= a.hd) continue;
         float Mx = -__builtin_inff(), Ls = 0.0f;
 #pragma unroll
-        for (int x = 0; x < 4; x++)
+        for (int x = 0; x < W; x++)
             if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
+        for (int x = 0; x < W; x++) {
             const float l = wml[x * 32 + 16 + pi];
             if (l == 0.0f) continue;
             const float wt = l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx);
@@ -943,10 +1143,11 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
 // registers than either needs, so launches that need one of them have it alone.
 constexpr int TILE = 1, FEW = 2;
 template <typename KV, int HD, int KIND>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArgs a) {
+__global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void attend_kernel(BatchArgs a) {
+    constexpr int W = Geo<KV, HD>::W, NT = W * 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    __shared__ Meta meta[8];
-    __shared__ float wml[4 * 32];
+    __shared__ Meta meta[2 * W];
+    __shared__ float wml[W * 32];
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
     const int tile_blocks = a.n_kv * a.tiles * a.tile_splits;
@@ -956,7 +1157,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     id /= a.n_kv;
     const int most = tile ? a.tile_splits : a.few_splits;
     const int z = id % most, slot = id / most;
-    const int b = tile ? sequence_of(a, slot) : slot;
+    const int b = tile ? sequence_of<TILE_PAIRS>(a, slot, a.group) : slot;
     if (b < 0) return;
     const Seq s = sequence(a, b);
     if (s.pairs == 0 || (s.pairs > a.few_rows) != tile) return;
@@ -964,20 +1165,89 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void attend_kernel(BatchArg
     if (tile) {
         if constexpr (KIND & TILE) {
             // the last rows, which see the most keys, first
-            const int p0 = (tiles_of(s.pairs) - 1 - (slot - first_tile(a, s.row0, b))) * TILE_PAIRS;
-            const int splits = tile_rows<KV, HD>(a, s, table, kvh, p0, z, lds, meta);
+            const int p0 = (tiles_of<TILE_PAIRS>(s.pairs) - 1 - (slot - first_tile<TILE_PAIRS>(s.row0, a.group, b))) * TILE_PAIRS;
+            const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta);
             // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
             if (splits > 1)
-                join(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                join<NT>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
         }
     } else {
-        if constexpr (KIND & FEW)
+        if constexpr ((KIND & FEW) != 0)
             for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once only where max_rows was too small
                 const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml);
                 if (splits > 1)
-                    join(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                    join<NT>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
                 __syncthreads();  // before the next rows take the LDS
             }
+    }
+}
+
+// ---- f32 rows as f16 parts, once a launch ---------------------------------------------
+// Where many tiles of rows read the same f32 keys, splitting them in every
+// tile (5 operations a value) cost more than the products' own work on them:
+// here a workgroup splits one tile of TK keys of a KV head and writes it as LDS will
+// hold it.  Keys get the tile's own exponent, values one rounded up to a multiple
+// of 4 (3 of the 17 bits that f16 parts have to spare), so that tiles seldom
+// differ in it.
+template <int HD>
+__global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* images, int4* notes) {
+    using G = Geo<Split, HD>;
+    constexpr int TK = G::TK, HDP = G::HDP, CPR = HDP / 8, NP = TK * CPR / 256, PART = TK * HDP;
+    static_assert(NP * 256 == TK * CPR, "whole pieces a thread");
+    __shared__ uint32_t red[2][4];
+    const int kvh = (int)(blockIdx.x % a.n_kv), t = (int)(blockIdx.x / a.n_kv), tid = threadIdx.x;
+    const int b = sequence_of<TK>(a, t, 1);
+    if (b < 0) return;
+    const Seq s = sequence(a, b);
+    const int j0 = (t - (int)(s.row0 / TK) - b) * TK;
+    u32x4 k[NP][2], v[NP][2];
+    const float* ks = reinterpret_cast<const float*>(a.kv.k) + (s.row0 + j0) * a.kv.k_position + kvh * a.kv.head;
+    const float* vs = reinterpret_cast<const float*>(a.kv.v) + (s.row0 + j0) * a.kv.v_position + kvh * a.kv.head;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const int pc = tid + 256 * i, key = pc / CPR, col = pc % CPR;
+        const bool in = j0 + key < s.t && col * 8 < a.hd;
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            k[i][p] = in ? *reinterpret_cast<const u32x4*>(ks + key * a.kv.k_position + col * 8 + 4 * p) : u32x4{0, 0, 0, 0};
+            v[i][p] = in ? *reinterpret_cast<const u32x4*>(vs + key * a.kv.v_position + col * 8 + 4 * p) : u32x4{0, 0, 0, 0};
+        }
+    }
+    auto block_max = [&](uint32_t km, uint32_t vm) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[0][tid >> 6] = km, red[1][tid >> 6] = vm;
+        __syncthreads();
+        return uint2{max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3])),
+                     max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]))};
+    };
+    uint2 m = block_max(largest_bits(k, false), largest_bits(v, false));
+    const int bad = m.y >= 0x7F800000u;
+    if (m.x >= 0x7F800000u || bad) {  // the exponents go by the finite ones; values that are not are zeroed
+#pragma unroll
+        for (int i = 0; i < NP; i++)
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if ((v[i][p][c] & 0x7F800000u) == 0x7F800000u) v[i][p][c] = 0;
+        m = block_max(largest_bits(k, true), largest_bits(v, false));
+    }
+    const int ke = exponent(m.x) - 14, ve = (exponent(m.y) - 14 + 3) & ~3;
+    const int64_t im = (int64_t)t * a.n_kv + kvh;
+    if (tid == 0) notes[im] = int4{ke, ve, bad, 0};
+    _Float16* out = images + im * (TK * G::KEY);
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const int pc = tid + 256 * i, key = pc / CPR, col = pc % CPR;
+        u32x4 kh, kl, vh, vl;
+        split8(k[i], ke, &kh, &kl);
+        split8(v[i], ve, &vh, &vl);
+        u32x4* kd = reinterpret_cast<u32x4*>(out + key * HDP + (col ^ G::k_swap(key)) * 8);
+        u32x4* vd = reinterpret_cast<u32x4*>(out + 2 * PART + key * HDP + (col ^ G::v_swap(key)) * 8);
+        *kd = kh;
+        kd[PART / 8] = kl;
+        *vd = vh;
+        vd[PART / 8] = vl;
     }
 }
 
@@ -989,13 +1259,19 @@ hipError_t launch(const BatchArgs& a, hipStream_t s) {
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     const unsigned blocks = (unsigned)(a.n_kv * (a.tiles * a.tile_splits + (KIND & FEW ? a.n_seq * a.few_splits : 0)));
-    hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(G::W * 64), lds, s, a);
     return hipGetLastError();
 }
 template <typename KV, int HD>
 hipError_t launch_kind(const BatchArgs& a, hipStream_t s) {
     return a.few_rows == 0 ? launch<KV, HD, TILE>(a, s) : a.tiles == 0 ? launch<KV, HD, FEW>(a, s)
                                                                        : launch<KV, HD, TILE | FEW>(a, s);
+}
+template <int HD>
+hipError_t launch_split(const BatchArgs& a, _Float16* images, int4* notes, int tiles, hipStream_t s) {
+    hipLaunchKernelGGL(split_kernel<HD>, dim3((unsigned)(tiles * a.n_kv)), dim3(256), 0, s, a, images, notes);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? launch<Split, HD, TILE>(a, s) : e;
 }
 template <typename KV>
 hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
@@ -1007,6 +1283,10 @@ hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
 constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512;
 constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 256;
 constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
+// f32 prompts are split beforehand from this many tiles a sequence on, as far
+// as this much memory holds them.
+constexpr int64_t SPLIT_MIN_TILES = 4;
+constexpr size_t SPLIT_BYTES = (size_t)1 << 30;
 
 rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_t s) {
     const int64_t m = a.m, rows = max_rows == 0 || (int64_t)max_rows > m ? m : (int64_t)max_rows;
@@ -1019,7 +1299,8 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     while (((int64_t)1 << a.group_shift) < G) a.group_shift++;
     a.group_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.group_shift) - (uint64_t)G)) / (uint64_t)G + 1);
     // sequences of up to 16 pairs; all of them where none is expected to have more
-    const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && a.n_seq == 1;
+    // (packed prompts of few rows have few keys: tiles serve them too)
+    const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && (a.n_seq == 1 || !a.kv.tables);
     a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
     a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
     auto split = [&](int64_t base, int64_t target, int width, int unit, int64_t min_span, int* span, int* splits) {
@@ -1040,16 +1321,34 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     a.part_splits = std::max(a.few_splits, a.tile_splits);
     if (((int64_t)a.tiles * a.tile_splits + (int64_t)a.n_seq * a.few_splits) * a.n_kv > (int64_t)1 << 30)
         return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows", a.n_seq, (long long)m);
+    // f32 prompts whose keys several tiles read: split once
+    const int hdp = a.hd <= 64 ? 64 : a.hd <= 128 ? 128 : 256, tk = a.hd <= 64 ? 64 : 32;  // Geo<Split, HD>
+    const int64_t tiles = m / tk + a.n_seq;
+    const size_t image_bytes = (size_t)tiles * a.n_kv * tk * hdp * 8, note_bytes = (size_t)tiles * a.n_kv * sizeof(int4);
+    const bool pre = !f16 && !a.kv.tables && only_tile && m * G >= SPLIT_MIN_TILES * TILE_PAIRS * a.n_seq &&
+                     image_bytes <= SPLIT_BYTES;
+    const size_t part_bytes = a.part_splits > 1 ? (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float) : 0;
+    const size_t part_room = (part_bytes + 255) & ~(size_t)255;
     CallScratch work;
-    if (a.part_splits > 1) {
-        const size_t bytes = (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float);
-        const rdl_status st = call_scratch(s, bytes, (size_t)m * a.n_heads, &work);
+    if (part_bytes || pre) {
+        const rdl_status st = call_scratch(s, part_room + (pre ? image_bytes + note_bytes : 0),
+                                           part_bytes ? (size_t)m * a.n_heads : 0, &work);
         if (st != RDL_OK) return st;
         a.part = reinterpret_cast<float*>(work.p);
         a.part_ml = a.part + (size_t)m * a.n_heads * a.part_splits * a.hd;
         a.counters = work.counters;
     }
-    const hipError_t e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
+    hipError_t e;
+    if (pre) {
+        _Float16* images = reinterpret_cast<_Float16*>(reinterpret_cast<uint8_t*>(work.p) + part_room);
+        int4* notes = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(images) + image_bytes);
+        a.images = images;
+        a.notes = notes;
+        auto go = a.hd <= 64 ? launch_split<64> : a.hd <= 96 ? launch_split<96> : a.hd <= 128 ? launch_split<128> : launch_split<256>;
+        e = go(a, images, notes, (int)tiles, s);
+    } else {
+        e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
+    }
     const rdl_status done = call_scratch_done(s, &work);
     HIP_TRY(e);
     return done == RDL_OK ? api_ok() : done;
