@@ -823,46 +823,45 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                 M = Mn;
             }
             const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
-            auto values = [&](auto shifted) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
+            for (int b = 0; b < NB; b++) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        sc[b][e] = weight(sc[b][e], f, off);
-                        L += sc[b][e];
-                        if constexpr (decltype(shifted)::value)
-                            sc[b][e] = __builtin_amdgcn_ldexpf(sc[b][e], (PRE ? pre_ve : notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ve) - ref);
+                for (int e = 0; e < 16; e++) {
+                    sc[b][e] = weight(sc[b][e], f, off);
+                    L += sc[b][e];
+                }
+                if (TWO && other_v)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        sc[b][e] = __builtin_amdgcn_ldexpf(
+                            sc[b][e], (PRE ? pre_ve : notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ve) - ref);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {  // 16 keys a step
+                    u32x4 ph, pl;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        uint32_t hi, lo;
+                        split2(sc[b][8 * k + 2 * u], sc[b][8 * k + 2 * u + 1], &hi, &lo);
+                        ph[u] = hi;
+                        pl[u] = lo;
                     }
+                    const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
+                    const char* vr = reinterpret_cast<const char*>(lds) + (size_t)(at + (32 * (b0 + b) + 16 * k) * HDP) * 2;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {  // 16 keys a step
-                        u32x4 ph, pl;
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            uint32_t hi, lo;
-                            split2(sc[b][8 * k + 2 * u], sc[b][8 * k + 2 * u + 1], &hi, &lo);
-                            ph[u] = hi;
-                            pl[u] = lo;
-                        }
-                        const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
-                        const char* vr = reinterpret_cast<const char*>(lds) + (size_t)(at + (32 * (b0 + b) + 16 * k) * HDP) * 2;
-#pragma unroll
-                        for (int d = 0; d < DT; d++) {
-                            const char* vd = vr + (v_off ^ (64 * d));
-                            const h4 v0 = read_t(vd), v1 = read_t(vd + 16 * HDP);
-                            const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p8, o[d], 0, 0, 0);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q8, o[d], 0, 0, 0);
-                            if constexpr (TWO) {
-                                const h4 w0 = read_t(vd + PART * 2), w1 = read_t(vd + PART * 2 + 16 * HDP);
-                                const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
-                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p8, o[d], 0, 0, 0);
-                            }
+                    for (int d = 0; d < DT; d++) {
+                        const char* vd = vr + (v_off ^ (64 * d));
+                        const h4 v0 = read_t(vd), v1 = read_t(vd + 16 * HDP);
+                        const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p8, o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, q8, o[d], 0, 0, 0);
+                        if constexpr (TWO) {
+                            const h4 w0 = read_t(vd + PART * 2), w1 = read_t(vd + PART * 2 + 16 * HDP);
+                            const h8 vl = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p8, o[d], 0, 0, 0);
                         }
                     }
                 }
-            };
-            if (TWO && other_v) values(std::true_type{});
-            else values(std::false_type{});
+            }
         }
     }
     L += other32(L);
