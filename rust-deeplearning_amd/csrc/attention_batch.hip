@@ -550,8 +550,13 @@ __device__ __forceinline__ f2 get2(const float* p) {
 __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, float M, float L) {
     put2(a.part_ml + (at * a.part_splits + z) * 2, M, L);
 }
-constexpr int JOIN_WEIGHTS = 4096;  // pairs * splits of a join, at most
-template <int NT>
+// A join of up to PAIRS pairs: NT / PAIRS lanes a pair form the splits' weights,
+// while the first outputs are on their way; then a thread takes four dims of a
+// pair at a time.  Its latency is what it costs.
+constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4;  // splits a lane, at most; splits whose outputs are read ahead
+template <int NT, int PAIRS>
+constexpr int JOIN_SPLITS = NT / PAIRS * JOIN_DEEP;
+template <int NT, int PAIRS>
 __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
                                      float* wt, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -565,61 +570,89 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     }
     __syncthreads();
     if (!*flag) return;
-    // maxima and sums to LDS, then a thread a pair: weights L 2^(M - max M) / their sum
-    float* mx = wt + JOIN_WEIGHTS;
-    for (int i = tid; i < pairs * splits; i += NT) {
-        const int pi = i / splits, z = i - pi * splits;
-        const f2 ml = get2(a.part_ml + (place(a, s, kvh, p0 + pi) * a.part_splits + z) * 2);
-        mx[i] = ml[0];
-        wt[i] = ml[1];
-    }
-    __syncthreads();
-    if (tid < pairs) {
-        float M = -__builtin_inff(), L = 0.0f;
-        for (int i = tid * splits; i < (tid + 1) * splits; i++)
-            if (wt[i] != 0.0f) M = fmaxf(M, mx[i]);
-        for (int i = tid * splits; i < (tid + 1) * splits; i++) {
-            const float x = wt[i] != 0.0f ? wt[i] * __builtin_amdgcn_exp2f(mx[i] - M) : 0.0f;
-            wt[i] = x;
-            L += x;
-        }
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        for (int i = tid * splits; i < (tid + 1) * splits; i++) wt[i] *= inv;
-    }
-    __syncthreads();
+    constexpr int LP = NT / PAIRS;
     const int quads = a.hd >> 2;
-    for (int i = tid; i < pairs * quads; i += NT) {
-        const int pi = i / quads, d = (i - pi * quads) * 4;
-        const float* o = a.part + place(a, s, kvh, p0 + pi) * a.part_splits * a.hd + d;
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto outputs = [&](int i) {  // item i's first split
+        const int pi = i / quads;
+        return a.part + place(a, s, kvh, p0 + pi) * a.part_splits * a.hd + (i - pi * quads) * 4;
+    };
+    const int pi = tid / LP, l = tid % LP;
+    const float* ml_at = a.part_ml + place(a, s, kvh, p0 + min(pi, pairs - 1)) * a.part_splits * 2;
+    auto ml = [&](int z) { return get2(ml_at + z * 2); };
+    const f2 own = ml(min(l, splits - 1));  // the lane's first split; more of them are read twice
+    const float* o0 = outputs(min(tid, pairs * quads - 1));
+    f2 ahead[JOIN_AHEAD][2];
+#pragma unroll
+    for (int z = 0; z < JOIN_AHEAD; z++) {
+        ahead[z][0] = get2(o0 + min(z, splits - 1) * a.hd);
+        ahead[z][1] = get2(o0 + min(z, splits - 1) * a.hd + 2);
+    }
+    auto top = [](f2 x, float M) { return x[1] != 0.0f ? fmaxf(M, x[0]) : M; };
+    auto weigh = [](f2 x, float M) { return x[1] != 0.0f ? x[1] * __builtin_amdgcn_exp2f(x[0] - M) : 0.0f; };
+    float M = l < splits ? top(own, -__builtin_inff()) : -__builtin_inff();
 #pragma unroll 4
-        for (int z = 0; z < splits; z++) {
-            const f2 u = get2(o + z * a.hd), v = get2(o + z * a.hd + 2);
-            const float w = wt[pi * splits + z];
-            y += w * f4{u[0], u[1], v[0], v[1]};
+    for (int z = l + LP; z < splits; z += LP) M = top(ml(z), M);
+#pragma unroll
+    for (int d = 1; d < LP; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+    float L = l < splits ? weigh(own, M) : 0.0f;
+    if (l < splits && pi < pairs) wt[pi * splits + l] = L;
+#pragma unroll 4
+    for (int z = l + LP; z < splits; z += LP) {
+        const float x = weigh(ml(z), M);
+        if (pi < pairs) wt[pi * splits + z] = x;
+        L += x;
+    }
+#pragma unroll
+    for (int d = 1; d < LP; d <<= 1) L += __shfl_xor(L, d);
+    float* inv = wt + PAIRS * JOIN_SPLITS<NT, PAIRS>;
+    if (l == 0 && pi < pairs) inv[pi] = L != 0.0f ? 1.0f / L : 0.0f;
+    __syncthreads();
+    for (int i = tid; i < pairs * quads; i += NT) {
+        const int pr = i / quads;
+        const float *o = outputs(i), *w = wt + pr * splits;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        int z0 = 0;
+        if (i == tid) {
+#pragma unroll
+            for (int z = 0; z < JOIN_AHEAD; z++)
+                if (z < splits) y += w[z] * f4{ahead[z][0][0], ahead[z][0][1], ahead[z][1][0], ahead[z][1][1]};
+            z0 = min(JOIN_AHEAD, splits);
         }
-        *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + d) = y;
+#pragma unroll 4
+        for (int z = z0; z < splits; z++) {
+            const f2 u = get2(o + z * a.hd), v = get2(o + z * a.hd + 2);
+            y += w[z] * f4{u[0], u[1], v[0], v[1]};
+        }
+        *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y * inv[pr];
     }
 }
 
 // q of one pair as f16 parts: NS steps of 8 dims, step i at dim d0 + i * step.
 // Scaled by the power of two that brings the row's largest value (over all
 // lanes of the pair: `reduce`) into [2^14, 2^15).  Returns the exponent.
-template <int NS, typename R>
-__device__ __forceinline__ int load_q(const float* q, bool live, int d0, int step, int hd, h8 (&hi)[NS], h8 (&lo)[NS],
-                                      R&& reduce) {
+template <int NS>
+struct QRow {
     f4 x[NS][2];
-    uint32_t m = 0;
+    __device__ __forceinline__ void load(const float* q, bool live, int d0, int step, int hd) {
 #pragma unroll
-    for (int i = 0; i < NS; i++) {
-        const int d = d0 + i * step;
+        for (int i = 0; i < NS; i++) {
+            const int d = d0 + i * step;
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            x[i][c] = live && d < hd ? *reinterpret_cast<const f4*>(q + d + 4 * c) : f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < 4; e++) m = max(m, abs_bits(x[i][c][e]));
+            for (int c = 0; c < 2; c++)
+                x[i][c] = live && d < hd ? *reinterpret_cast<const f4*>(q + d + 4 * c) : f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+};
+template <int NS, typename R>
+__device__ __forceinline__ int split_q(const QRow<NS>& row, h8 (&hi)[NS], h8 (&lo)[NS], R&& reduce) {
+    const f4 (&x)[NS][2] = row.x;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NS; i++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) m = max(m, abs_bits(x[i][c][e]));
     m = reduce(m);
     const int e = m >= 0x7F800000u ? 0 : exponent(m) - 14;
 #pragma unroll
@@ -670,11 +703,6 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     const int w_first = __builtin_amdgcn_readfirstlane(last_key(a, s, p0 + 32 * w));   // the wave's first pair sees
     const int w_last = __builtin_amdgcn_readfirstlane(last_key(a, s, min(p0 + 32 * w + 31, s.pairs - 1)));
     const int wg_first = last_key(a, s, p0);
-    h8 qh[KS], ql[KS];
-    const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd, qh, ql, [](uint32_t m) {
-        return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
-    });
-    const float cs = score_factor(a.scale * LOG2E, qe);
     f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -719,8 +747,16 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
         if constexpr (RAW32) slab.init(a.kv, a.hd);
         else if constexpr (!PRE) slab.init(a.kv, a.hd, SK * w);
         if constexpr (!PRE) slab.pages(a.kv, table, j_lo + SK * w, s.t);
-        fetch(j_lo, 0);
     }
+    // the rows of q on their way while the page numbers are
+    QRow<KS> q;
+    q.load(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd);
+    if (j_lo < j_hi) fetch(j_lo, 0);
+    h8 qh[KS], ql[KS];
+    const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
+        return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
+    });
+    const float cs = score_factor(a.scale * LOG2E, qe);
     int buf = 0;
     for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
         const int at = buf * TK * G::KEY;  // elements
@@ -967,14 +1003,17 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         Slab<KV, HD, FK> slab;
         slab.init(a.kv, a.hd);
         const int step = W * FK, j_w = j_lo + FK * w;
+        // the row of q on its way while the page numbers are
         int valid = 0;
+        if (j_w < j_hi) slab.pages(a.kv, table, j_w, s.t);
+        QRow<KS> q;
+        q.load(q_at(a, s, kvh, p), live, 8 * g, 32, a.hd);
         if (j_w < j_hi) {
-            slab.pages(a.kv, table, j_w, s.t);
             valid = slab.load(a.kv, s.row0, kvh, j_w, j_hi);
             slab.pages(a.kv, table, j_w + step, s.t);
         }
         h8 qh[KS], ql[KS];
-        const int qe = load_q<KS>(q_at(a, s, kvh, p), live, 8 * g, 32, a.hd, qh, ql, [](uint32_t m) {
+        const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
@@ -1168,14 +1207,14 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
             const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta);
             // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
             if (splits > 1)
-                join<NT>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                join<NT, TILE_PAIRS>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
         }
     } else {
         if constexpr ((KIND & FEW) != 0)
             for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once only where max_rows was too small
                 const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml);
                 if (splits > 1)
-                    join<NT>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                    join<NT, FEW_PAIRS>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
                 __syncthreads();  // before the next rows take the LDS
             }
     }
@@ -1302,21 +1341,21 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && (a.n_seq == 1 || !a.kv.tables);
     a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
     a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
-    auto split = [&](int64_t base, int64_t target, int width, int unit, int64_t min_span, int* span, int* splits) {
+    auto split = [&](int64_t base, int64_t target, int most, int unit, int64_t min_span, int* span, int* splits) {
         int64_t sp = std::max(min_span, keys * base / target);
         sp = (sp + unit - 1) / unit * unit;
         int64_t n = (keys + sp - 1) / sp;
         const int64_t cap = (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float)));
         if (n > cap) n = std::max<int64_t>(1, cap);
-        n = std::min<int64_t>(n, JOIN_WEIGHTS / width);
+        n = std::min<int64_t>(n, most);
         sp = ((keys + n - 1) / n + unit - 1) / unit * unit;
         *splits = (int)n;
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
     };
     if (only_tile) a.few_span = INT32_MAX / 2, a.few_splits = 1;
-    else split(pairs, FEW_TARGET, FEW_PAIRS, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
+    else split(pairs, FEW_TARGET, JOIN_SPLITS<256, FEW_PAIRS>, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
     if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
-    else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, TILE_PAIRS, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
+    else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, JOIN_SPLITS<256, TILE_PAIRS>, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
     a.part_splits = std::max(a.few_splits, a.tile_splits);
     if (((int64_t)a.tiles * a.tile_splits + (int64_t)a.n_seq * a.few_splits) * a.n_kv > (int64_t)1 << 30)
         return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows", a.n_seq, (long long)m);
