@@ -51,6 +51,7 @@ struct BatchArgs {
     // are (tile of TK rows * n_kv + KV head), and their exponents and flags
     const _Float16* images;
     const int4* notes;
+    const int2* exps;  // [image][TK]
 };
 
 struct Pair {  // (row, head of the group) pair p of a sequence
@@ -71,8 +72,9 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr float LOG2E = 1.44269504088896340736f;
 // Weights are held as 2^(x - M + SHIFT), M a running maximum that moves only
 // when a score passes it by SLACK: at most 2^15, so hi and lo fit f16, and
-// f16's smallest step, 2^-24, lies 2^-32 below the largest weight.
-constexpr float SHIFT = 8.0f, SLACK = 7.0f;
+// f16's smallest step, 2^-24, lies 2^-35 below the largest weight.  (8 and 7
+// instead take the same time: M seldom moves after a sequence's first tiles.)
+constexpr float SHIFT = 11.0f, SLACK = 4.0f;
 
 // a * 2^e as two f16 parts of 11 bits each (rounded toward zero, so both have
 // a's sign and hi + lo is off by less than 2^-21 of it).
@@ -134,28 +136,6 @@ __device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u3
             (*lo)[2 * p + c] = l;
         }
 }
-// Largest magnitude over a wave's pieces, as f32 bits; finite: of the finite
-// ones only.  As integers, the largest signed value is the largest positive
-// f32 (NaN above infinity) and the largest unsigned one, where its sign is
-// set, the negative f32 of the largest magnitude.
-template <int N, int P>
-__device__ __forceinline__ uint32_t largest_bits(const u32x4 (&x)[N][P], bool finite) {
-    int32_t pos = 0;
-    uint32_t neg = 0;
-#pragma unroll
-    for (int i = 0; i < N; i++)
-#pragma unroll
-        for (int p = 0; p < P; p++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t b = x[i][p][c];
-                if (finite && (b & 0x7F800000u) == 0x7F800000u) b = 0;
-                pos = max(pos, (int32_t)b);
-                neg = max(neg, b);
-            }
-    return wave_max_u32(max((uint32_t)pos, neg & 0x80000000u ? neg & 0x7FFFFFFFu : 0u));
-}
-
 // Where a launch's keys and values come from: _Float16 and float as they
 // are, Split as f32 rows that split_kernel has made f16 parts of before.
 struct Split {};
@@ -182,12 +162,103 @@ struct Geo {
     }
 };
 
-// What a wave's slab of keys needs beside its LDS rows.
+// What a wave's slab of keys needs beside its LDS rows.  f32 keys and values
+// are held times 2^-ke and 2^-ve, except the rows of a flagged slab that are
+// too small for that: each row's own exponents (x: key, y: value) stand beside
+// the LDS rows.
 struct Meta {
-    int valid;  // the keys' page is in the pool
-    int bad;    // values that are not finite were zeroed: wide4 brings them
-    int ke, ve; // f32 keys / values are held times 2^-ke, 2^-ve
+    int valid;   // the keys' page is in the pool
+    int flags;
+    int ke, ve;
 };
+constexpr int SLAB_WIDE = 1;     // values that are not finite were zeroed: wide4 brings them
+constexpr int SLAB_OTHER_K = 2;  // some keys have an exponent of their own
+constexpr int SLAB_OTHER_V = 4;  // some values have one
+
+// The exponent to hold a row of largest magnitude `bits` with: the one in use,
+// `ref`, where the row begins at most 2^HOLD below it or is all zero, so that
+// rows seldom differ; else its own.  Held below 2^15 a row's f16 parts end at
+// 2^-24, 2^-33 of its largest.  For values the 2^HOLD also come off the weights,
+// which are held for the largest exponent (weigh_two).
+constexpr int HOLD = 5, NO_EXPONENT = -1000;
+__device__ __forceinline__ int hold(uint32_t bits, int ref) {
+    const int e = exponent(bits) - 14;
+    return (e <= ref && e >= ref - HOLD) || bits == 0 ? ref : e;
+}
+// The same for a slab or tile as a whole, whose own exponent is rounded up to
+// an even one: those of one size then mostly agree from the first on.
+__device__ __forceinline__ int hold_all(uint32_t bits, int ref) {
+    const int e = hold(bits, ref);
+    return e == ref ? ref : (e + 1) & ~1;
+}
+// Largest magnitude of 8 values as f32 bits (finite: of the finite ones).  As
+// integers, the largest signed value is the largest positive f32 (NaN above
+// infinity) and the largest unsigned one, where its sign is set, the
+// negative f32 of the largest magnitude.
+__device__ __forceinline__ uint32_t largest8(const u32x4 (&x)[2], bool finite) {
+    int32_t pos = 0;
+    uint32_t neg = 0;
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t b = x[p][c];
+            if (finite && (b & 0x7F800000u) == 0x7F800000u) b = 0;
+            pos = max(pos, (int32_t)b);
+            neg = max(neg, b);
+        }
+    return max((uint32_t)pos, neg & 0x80000000u ? neg & 0x7FFFFFFFu : 0u);
+}
+// Maximum over each aligned group of C = 8, 16 or 32 lanes: a row's pieces.
+template <int C>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max8_u32(v);
+    if constexpr (C >= 16) v = max(v, (uint32_t)dpp_i32<DPP_ROW_MIRROR>((int)v));
+    if constexpr (C == 32) v = max(v, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, v))));
+    return v;
+}
+// Of N pieces a lane, C lanes a row: their largest magnitudes (as largest8).
+// Those that are not finite count as zero; zero: and become zero.  Returns
+// whether there were any in the wave.
+template <int N>
+__device__ __forceinline__ bool piece_sizes(u32x4 (&x)[N][2], uint32_t (&m)[N], bool zero) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) t = max(t, m[i] = largest8(x[i], false));
+    if (!__builtin_amdgcn_ballot_w64(t >= 0x7F800000u)) return false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        m[i] = largest8(x[i], true);
+        if (zero)
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if ((x[i][p][c] & 0x7F800000u) == 0x7F800000u) x[i][p][c] = 0;
+    }
+    return true;
+}
+// The rows' exponents where the wave's or tile's is E, at least the largest
+// row's: e; whether any differs from E.  Two ballots a piece find that none
+// does, without the rows' maxima.
+template <int C, int N>
+__device__ __forceinline__ bool row_exponents(const uint32_t (&m)[N], int E, int (&e)[N]) {
+    const uint32_t low = (uint32_t)max(E + 14 - HOLD + 127, 0) << 23;  // what begins at most 2^HOLD below
+    constexpr uint64_t STARTS = C == 8 ? 0x0101010101010101u : C == 16 ? 0x0001000100010001u : 0x0000000100000001u;
+    uint64_t other = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint64_t some = __builtin_amdgcn_ballot_w64(m[i] != 0), enough = __builtin_amdgcn_ballot_w64(m[i] >= low);
+#pragma unroll
+        for (int k = 1; k < C; k *= 2) some |= some >> k, enough |= enough >> k;  // at a row's first lane: any of it
+        other |= some & ~enough & STARTS;
+        e[i] = E;
+    }
+    if (!other) return false;
+#pragma unroll
+    for (int i = 0; i < N; i++) e[i] = hold(row_max<C>(m[i]), E);
+    return true;
+}
 
 // One wave's slab of SK keys on its way from memory to LDS: loads into
 // registers (issued a step ahead), then the f16 parts into LDS.  A slab of 16
@@ -198,11 +269,10 @@ struct Slab {
     using G = Geo<KV, HD>;
     static constexpr bool F32 = G::TWO;
     static constexpr int E = (int)sizeof(KV);
-    static constexpr int CPR = HD / 8;              // 8-element pieces a key
-    static constexpr int NL = (SK * CPR + 63) / 64;  // pieces a lane
+    static constexpr int CPR = G::HDP / 8;          // 8-element pieces a key
+    static constexpr int NL = SK * CPR / 64;        // pieces a lane
     static constexpr int GK = SK < 16 ? SK : 16, NG = SK / GK, LPG = NL / NG;
-    static constexpr bool WHOLE = NL * 64 == SK * CPR;  // else the last piece of some lanes is past the slab
-    static_assert(NG == 1 || WHOLE, "whole pieces a group");
+    static_assert(NL * 64 == SK * CPR && LPG * NG == NL, "whole pieces");
     u32x4 k[NL][G::PARTS], v[NL][G::PARTS];
     uint32_t koff[LPG], voff[LPG];
     int pg[NG];  // table entries of the next slab to load
@@ -211,7 +281,7 @@ struct Slab {
 #pragma unroll
         for (int i = 0; i < LPG; i++) {
             const int pc = (threadIdx.x & 63) + 64 * i, key = pc / CPR, col = pc % CPR;
-            const bool in = col * 8 < hd && (WHOLE || key < SK);
+            const bool in = col * 8 < hd;
             koff[i] = in ? (uint32_t)(key * (int)s.k_position + col * 8) * E : RSRC_OOB;
             voff[i] = in ? (uint32_t)(key * (int)s.v_position + col * 8) * E : RSRC_OOB;
         }
@@ -255,37 +325,31 @@ struct Slab {
         }
         return valid;
     }
-    // The exponent to hold a slab of largest magnitude `bits` with: the one in
-    // use, `ref`, where that keeps 22 bits of its values (f16 parts of
-    // values that begin 2^12 below 2^15 still end 2^-27 of them further down),
-    // so that slabs seldom differ; else its own.
-    static __device__ __forceinline__ int hold(uint32_t bits, int ref) {
-        const int e = exponent(bits) - 14;
-        return e <= ref && e >= ref - 12 ? ref : e;
-    }
     // Registers to LDS rows row0 .. of ks and vs (the lo parts `part` elements
-    // further on).  check: whether values that are not finite
+    // further on) and, f32, the rows' exponents to exps.  check: whether values that are not finite
     // have to be found (f16; f32 finds them on the way to the exponent).
-    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int row0, int part, int valid, bool check, int kref,
-                                          int vref) {
+    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int2* exps, int row0, int part, int valid, bool check,
+                                          int kref, int vref) {
         const int lane = threadIdx.x & 63;
         Meta mt{valid, 0, 0, 0};
+        [[maybe_unused]] int ek[NL], ev[NL];
         if constexpr (F32) {
-            uint32_t km = largest_bits(k, false), vm = largest_bits(v, false);
-            if (km >= 0x7F800000u) km = largest_bits(k, true);
-            if (vm >= 0x7F800000u) {
-                mt.bad = 1;
+            uint32_t km[NL], vm[NL], kt = 0, vt = 0;
+            piece_sizes(k, km, false);
+            if (piece_sizes(v, vm, true)) mt.flags |= SLAB_WIDE;
+#pragma unroll
+            for (int i = 0; i < NL; i++) kt = max(kt, km[i]), vt = max(vt, vm[i]);
+            mt.ke = hold_all(wave_max_u32(kt), kref);
+            mt.ve = hold_all(wave_max_u32(vt), vref);
+            if (row_exponents<CPR>(km, mt.ke, ek)) mt.flags |= SLAB_OTHER_K;
+            if (row_exponents<CPR>(vm, mt.ve, ev)) mt.flags |= SLAB_OTHER_V;
+            if (mt.flags & (SLAB_OTHER_K | SLAB_OTHER_V)) {
 #pragma unroll
                 for (int i = 0; i < NL; i++)
-#pragma unroll
-                    for (int p = 0; p < 2; p++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            if ((v[i][p][c] & 0x7F800000u) == 0x7F800000u) v[i][p][c] = 0;
-                vm = largest_bits(v, false);
+                    if (lane % CPR == 0) exps[row0 + (lane + 64 * i) / CPR] = int2{ek[i], ev[i]};
+            } else if (lane < SK) {
+                exps[row0 + lane] = int2{mt.ke, mt.ve};
             }
-            mt.ke = hold(km, kref);
-            mt.ve = hold(vm, vref);
         } else if (check) {
             bool found = false;
 #pragma unroll
@@ -294,7 +358,7 @@ struct Slab {
                 for (int c = 0; c < 4; c++)
                     found |= ((((v[i][0][c] & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0);
             if (__builtin_amdgcn_ballot_w64(found)) {
-                mt.bad = 1;
+                mt.flags = SLAB_WIDE;
 #pragma unroll
                 for (int i = 0; i < NL; i++)
 #pragma unroll
@@ -307,14 +371,13 @@ struct Slab {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             const int pc = lane + 64 * i, key = pc / CPR, col = pc % CPR;
-            if (!WHOLE && key >= SK) continue;
             const int row = row0 + key;
             u32x4* kd = reinterpret_cast<u32x4*>(ks + row * G::HDP + (col ^ G::k_swap(row)) * 8);
             u32x4* vd = reinterpret_cast<u32x4*>(vs + row * G::HDP + (col ^ G::v_swap(row)) * 8);
             if constexpr (F32) {
                 u32x4 kh, kl, vh, vl;
-                split8(k[i], mt.ke, &kh, &kl);
-                split8(v[i], mt.ve, &vh, &vl);
+                split8(k[i], ek[i], &kh, &kl);
+                split8(v[i], ev[i], &vh, &vl);
                 *kd = kh;
                 kd[part / 8] = kl;
                 *vd = vh;
@@ -672,6 +735,73 @@ __device__ __forceinline__ int split_q(const QRow<NS>& row, h8 (&hi)[NS], h8 (&l
     return e;
 }
 
+// 2^ref as a factor, where it is below f32's normal numbers too.
+struct Power {
+    float part;
+    int whole;
+    __device__ __forceinline__ explicit Power(float ref) {
+        const float w = floorf(fmaxf(ref, (float)NO_EXPONENT));
+        part = ref < w ? 1.0f : __builtin_amdgcn_exp2f(ref - w);
+        whole = (int)w;
+    }
+    __device__ __forceinline__ float times(float x) const { return __builtin_amdgcn_ldexpf(x * part, whole); }
+};
+
+// The softmax step of f32 values.  A value is held times 2^-ve, so the weight
+// that enters the product with it is 2^(x - M + SHIFT + ve - ref): ref, a pair's
+// own, follows the largest x - M + ve of the keys that it sees, as M follows x.
+// (By the largest ve alone, values that a pair does not see or hardly weighs
+// would push its own below f16's smallest step.)  A weight's step of 2^-24 times a
+// value's 2^15 is so 2^-28 of the largest weighted row's size at most, 2^HOLD
+// of it for rows held with a larger one's exponent.  L sums 2^(x - M + SHIFT).
+// Where all keys have one exponent E the two differ by a factor only.
+// N scores of a lane: get(i), put(i, weight); value(i): key i's exponent;
+// rescale(c): o *= c; reduce: the maximum over a pair's lanes; mx: the pair's largest x.
+template <int N, typename Get, typename Put, typename Value, typename Rescale, typename Reduce>
+__device__ __forceinline__ void weigh_two(Get&& get, Put&& put, Value&& value, Rescale&& rescale, Reduce&& reduce, float f,
+                                          float mx, int E, bool other, float& M, float& L, float& ref) {
+    if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
+        const float Mn = fmaxf(M, mx);
+        if (Mn != M) {
+            L *= __builtin_amdgcn_exp2f(M - Mn);
+            ref += M - Mn;
+            M = Mn;
+        }
+    }
+    const float Mu = M == -__builtin_inff() ? 0.0f : M;
+    float top = mx - Mu + (float)E;
+    if (other) {
+        top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < N; i++) top = fmaxf(top, fmaf(get(i), f, -Mu) + (float)value(i));
+        top = reduce(top);
+    }
+    if (__builtin_amdgcn_ballot_w64(top > ref + SLACK)) {
+        const float rn = fmaxf(ref, ceilf(top));
+        rescale(rn == ref ? 1.0f : __builtin_amdgcn_exp2f(ref - rn));
+        ref = rn;
+    }
+    const float r = ref == -__builtin_inff() ? (float)E : ref;
+    if (!other && !__builtin_amdgcn_ballot_w64(r - (float)E > 60.0f)) {
+        const float off = SHIFT - Mu + ((float)E - r);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float w = weight(get(i), f, off);
+            sum += w;
+            put(i, w);
+        }
+        L += sum * __builtin_amdgcn_exp2f(r - (float)E);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float x = fmaf(get(i), f, SHIFT - Mu);
+            L += __builtin_amdgcn_exp2f(x);
+            put(i, __builtin_amdgcn_exp2f(x + ((other ? (float)value(i) : (float)E) - r)));
+        }
+    }
+}
+
 // ---- many rows: waves of 32 pairs, tiles of TK keys shared through LDS -------------------
 // Each wave holds 32 pairs as the columns of both products, S^T = K Q^T and
 // O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a lane has 16 scores of one pair, so
@@ -682,7 +812,7 @@ __device__ __forceinline__ int split_q(const QRow<NS>& row, h8 (&hi)[NS], h8 (&l
 // Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
 __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
-                                         int p0, int z, _Float16* lds, Meta* meta) {
+                                         int p0, int z, _Float16* lds, Meta* meta, int2* exps) {
     using G = Geo<KV, HD>;
     typedef typename std::conditional<std::is_same<KV, Split>::value, float, KV>::type Elem;
     constexpr int TK = G::TK, W = G::W, SK = TK / W, KS = HD / 16, DT = HD / 32, HDP = G::HDP;
@@ -709,8 +839,8 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
     float M = -__builtin_inff(), L = 0.0f;
-    int ref = -1000;  // f32 values: o is held times 2^-ref
-    int kref = -1000; // f32 keys: the exponent last used
+    [[maybe_unused]] float ref = -__builtin_inff();      // f32 values: o is held times 2^-ref
+    [[maybe_unused]] int kref = NO_EXPONENT, vref = NO_EXPONENT;  // f32: the exponents last used
     int wide = 0;     // some values were not finite
 
     // LDS addresses of this lane's operands; a step further along a row is an
@@ -761,14 +891,16 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
         const int at = buf * TK * G::KEY;  // elements
         Meta note;
+        [[maybe_unused]] const int2* key_exps = exps + buf * TK;
         if constexpr (RAW32) {
-            const Meta mine = slab.store(lds + at, lds + at + PART * 2, SK * w, PART, valid, true, kref, ref);
+            const Meta mine = slab.store(lds + at, lds + at + PART * 2, exps + buf * TK, SK * w, PART, valid, true, kref, vref);
             if (lane == 0) meta[buf * W + w] = mine;
             if (j0 + TK < j_hi) fetch(j0 + TK, 0);
             __syncthreads();
             note = meta[buf * W + (lane & (W - 1))];
         } else if constexpr (PRE) {
             note = Meta{1, note_next.z, note_next.x, note_next.y};
+            key_exps = a.exps + (image + (int64_t)(j0 / TK) * a.n_kv) * TK;
             loads_done();
             __syncthreads();
             if (j0 + TK < j_hi) fetch(j0 + TK, buf ^ 1);
@@ -777,7 +909,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
             loads_done();
             __syncthreads();
             if (j0 + TK - 1 > wg_first) {  // some of its values are masked
-                if (Stage::clean(lds + at + PART + SK * w * HDP) && lane == 0) meta[buf * W + w].bad = 1;
+                if (Stage::clean(lds + at + PART + SK * w * HDP) && lane == 0) meta[buf * W + w].flags = SLAB_WIDE;
                 __syncthreads();
             }
             if (j0 + TK < j_hi) fetch(j0 + TK, buf ^ 1);
@@ -787,24 +919,15 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
         // the slabs' notes, a lane a slab
         [[maybe_unused]] const Meta* notes = meta + buf * W;
         const bool masked = j0 + TK - 1 > w_first || __builtin_amdgcn_ballot_w64(!note.valid);
-        wide |= __builtin_amdgcn_ballot_w64(note.bad) != 0;
+        wide |= __builtin_amdgcn_ballot_w64(note.flags & SLAB_WIDE) != 0;
         float f = cs;
-        bool other_k = false, other_v = false;  // f32: slabs held with other exponents than the rest
-        [[maybe_unused]] int pre_ve = 0;
+        bool other_k = false, other_v = false;  // f32: keys held with other exponents than the rest
         if constexpr (TWO) {
             kref = lanes_max<W>(note.ke);
-            const int top = lanes_max<W>(note.ve);
-            if (top > ref) {
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] = __builtin_amdgcn_ldexpf(o[d][e], ref - top);
-                ref = top;
-            }
+            vref = lanes_max<W>(note.ve);
             f = score_factor(cs, kref);
-            other_k = __builtin_amdgcn_ballot_w64(note.ke != kref);
-            other_v = __builtin_amdgcn_ballot_w64(note.ve != ref);
-            pre_ve = top;
+            other_k = __builtin_amdgcn_ballot_w64((note.ke != kref && note.ke != NO_EXPONENT) || (note.flags & SLAB_OTHER_K));
+            other_v = __builtin_amdgcn_ballot_w64((note.ve != vref && note.ve != NO_EXPONENT) || (note.flags & SLAB_OTHER_V));
         }
 #pragma unroll
         for (int b0 = 0; b0 < TK / 32; b0 += NB) {
@@ -826,12 +949,13 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
                     }
                 }
             }
-            if (RAW32 && other_k)
+            if (TWO && other_k)
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        sc[b][e] = __builtin_amdgcn_ldexpf(sc[b][e], notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ke - kref);
+                        sc[b][e] = __builtin_amdgcn_ldexpf(
+                            sc[b][e], key_exps[32 * (b0 + b) + 8 * (e >> 2) + 4 * h + (e & 3)].x - kref);
             if (masked)
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
@@ -848,29 +972,35 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 #pragma unroll
                 for (int e = b == 0; e < 16; e++) mx = fmaxf(mx, sc[b][e]);
             mx = max32(mx) * f;
-            if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
-                const float Mn = fmaxf(M, mx);
-                const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
-                L *= corr;
+            auto rescale = [&](float corr) {
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) o[d][e] *= corr;
-                M = Mn;
+            };
+            [[maybe_unused]] float off = 0.0f;
+            if constexpr (TWO) {
+                weigh_two<16>([&](int e) { return sc[0][e]; }, [&](int e, float v) { sc[0][e] = v; },
+                              [&](int e) { return key_exps[32 * b0 + 8 * (e >> 2) + 4 * h + (e & 3)].y; }, rescale,
+                              [](float v) { return max32(v); }, f, mx, vref, other_v, M, L, ref);
+            } else {
+                if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
+                    const float Mn = fmaxf(M, mx);
+                    const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
+                    L *= corr;
+                    rescale(corr);
+                    M = Mn;
+                }
+                off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
             }
-            const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
+                if constexpr (!TWO)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    sc[b][e] = weight(sc[b][e], f, off);
-                    L += sc[b][e];
-                }
-                if (TWO && other_v)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        sc[b][e] = __builtin_amdgcn_ldexpf(
-                            sc[b][e], (PRE ? pre_ve : notes[(32 * (b0 + b) + 8 * (e >> 2)) / SK].ve) - ref);
+                    for (int e = 0; e < 16; e++) {
+                        sc[b][e] = weight(sc[b][e], f, off);
+                        L += sc[b][e];
+                    }
 #pragma unroll
                 for (int k = 0; k < 2; k++) {  // 16 keys a step
                     u32x4 ph, pl;
@@ -902,12 +1032,13 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     }
     L += other32(L);
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    [[maybe_unused]] const Power unit(ref);
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const float x = o[d][e] * inv;
-            o[d][e] = TWO ? __builtin_amdgcn_ldexpf(x, ref) : x;
+            o[d][e] = TWO ? unit.times(x) : x;
         }
     if (wide)  // rows that see a value that is not finite
         for (int j = j_lo; j < min(j_hi, w_last + 1); j++) {
@@ -971,7 +1102,7 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
 // 4g .. (g = lane / 16) of one pair.
 template <typename KV, int HD>
 __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
-                                         _Float16* lds, float* wml) {
+                                        _Float16* lds, float* wml, int2* exps) {
     using G = Geo<KV, HD>;
     constexpr int KS = HD / 32, DT = HD / 16, FK = G::FK, NB = FK / 16, W = G::W, HDP = G::HDP;
     constexpr bool F32 = G::TWO;
@@ -998,7 +1129,8 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     f4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    int ref = -1000, wide = 0;
+    int wide = 0;
+    [[maybe_unused]] float ref = -__builtin_inff();  // f32 values: o is held times 2^-ref
     {
         Slab<KV, HD, FK> slab;
         slab.init(a.kv, a.hd);
@@ -1019,23 +1151,14 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         });
         const float cs = score_factor(a.scale * LOG2E, qe);
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
-            const Meta mt = slab.store(ks, vs, 0, PART, valid, j0 + FK - 1 > first, 0, -1000);
+            const Meta mt = slab.store(ks, vs, exps + FK * w, 0, PART, valid, j0 + FK - 1 > first, NO_EXPONENT, NO_EXPONENT);
             if (j0 + step < j_hi) {
                 valid = slab.load(a.kv, s.row0, kvh, j0 + step, j_hi);
                 slab.pages(a.kv, table, j0 + 2 * step, s.t);
             }
             wave_sync();
             const bool masked = j0 + FK - 1 > first || mt.valid != (1 << NB) - 1;
-            wide |= mt.bad;
-            if constexpr (F32) {
-                if (mt.ve > ref) {
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[d][e] = __builtin_amdgcn_ldexpf(o[d][e], ref - mt.ve);
-                    ref = mt.ve;
-                }
-            }
+            wide |= mt.flags & SLAB_WIDE;
             f4 sc[NB];
             float mx = -__builtin_inff();
 #pragma unroll
@@ -1053,6 +1176,12 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                     }
                 }
             }
+            if (F32 && (mt.flags & SLAB_OTHER_K))
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        sc[b][t] = __builtin_amdgcn_ldexpf(sc[b][t], exps[FK * w + 16 * b + 4 * g + t].x - mt.ke);
             if (masked) {
                 const int rel = last - j0 - 4 * g;
 #pragma unroll
@@ -1069,29 +1198,36 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             mx *= f;
             mx = fmaxf(mx, other16(mx));
             mx = max32(mx);
-            if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
-                const float Mn = fmaxf(M, mx);
-                const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
-                L *= corr;
+            auto rescale = [&](float corr) {
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++) o[d] *= corr;
+            };
+            if constexpr (F32) {
+                weigh_two<4 * NB>([&](int i) { return sc[i >> 2][i & 3]; }, [&](int i, float v) { sc[i >> 2][i & 3] = v; },
+                                  [&](int i) { return exps[FK * w + 16 * (i >> 2) + 4 * g + (i & 3)].y; }, rescale,
+                                  [](float v) { return max32(fmaxf(v, other16(v))); }, f, mx, mt.ve,
+                                  (mt.flags & SLAB_OTHER_V) != 0, M, L, ref);
+            } else {
+                if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {
+                    const float Mn = fmaxf(M, mx);
+                    const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
+                    L *= corr;
+                    rescale(corr);
+                    M = Mn;
+                }
+                const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[d][e] *= corr;
-                M = Mn;
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        sc[b][t] = weight(sc[b][t], f, off);
+                        L += sc[b][t];
+                    }
             }
-            const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
             uint32_t ph[2 * NB], pl[2 * NB];
 #pragma unroll
-            for (int u = 0; u < 2 * NB; u++) {
-                float x0 = weight(sc[u >> 1][(u & 1) * 2], f, off);
-                float x1 = weight(sc[u >> 1][(u & 1) * 2 + 1], f, off);
-                L += x0 + x1;
-                if constexpr (F32) {
-                    x0 = __builtin_amdgcn_ldexpf(x0, mt.ve - ref);
-                    x1 = __builtin_amdgcn_ldexpf(x1, mt.ve - ref);
-                }
-                split2(x0, x1, &ph[u], &pl[u]);
-            }
+            for (int u = 0; u < 2 * NB; u++)
+                split2(sc[u >> 1][(u & 1) * 2], sc[u >> 1][(u & 1) * 2 + 1], &ph[u], &pl[u]);
             const char* vr = reinterpret_cast<const char*>(vs);
             if constexpr (NB == 2) {
                 const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);
@@ -1120,13 +1256,14 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         L += other32(L);
         // the wave's normalised output over its own key rows, its maximum and sum beside
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        [[maybe_unused]] const Power unit(ref);
         float* os = reinterpret_cast<float*>(ks);
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float x = o[d][e] * inv;
-                o[d][e] = F32 ? __builtin_amdgcn_ldexpf(x, ref) : x;
+                o[d][e] = F32 ? unit.times(x) : x;
             }
         if (wide)  // rows that see a value that is not finite
             for (int j0 = j_w; j0 < j_hi; j0 += step)
@@ -1185,6 +1322,7 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
     constexpr int W = Geo<KV, HD>::W, NT = W * 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Meta meta[2 * W];
+    __shared__ int2 exps[2 * 64];  // of a tile's keys, twice, or of each wave's
     __shared__ float wml[W * 32];
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
@@ -1204,7 +1342,7 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
         if constexpr (KIND & TILE) {
             // the last rows, which see the most keys, first
             const int p0 = (tiles_of<TILE_PAIRS>(s.pairs) - 1 - (slot - first_tile<TILE_PAIRS>(s.row0, a.group, b))) * TILE_PAIRS;
-            const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta);
+            const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta, exps);
             // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
             if (splits > 1)
                 join<NT, TILE_PAIRS>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
@@ -1212,7 +1350,7 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
     } else {
         if constexpr ((KIND & FEW) != 0)
             for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once only where max_rows was too small
-                const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml);
+                const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml, exps);
                 if (splits > 1)
                     join<NT, FEW_PAIRS>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
                 __syncthreads();  // before the next rows take the LDS
@@ -1224,15 +1362,13 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
 // Where many tiles of rows read the same f32 keys, splitting them in every
 // tile (5 operations a value) cost more than the products' own work on them:
 // here a workgroup splits one tile of TK keys of a KV head and writes it as LDS will
-// hold it.  Keys get the tile's own exponent, values one rounded up to a multiple
-// of 4 (3 of the 17 bits that f16 parts have to spare), so that tiles seldom
-// differ in it.
+// hold it.
 template <int HD>
-__global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* images, int4* notes) {
+__global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* images, int4* notes, int2* exps) {
     using G = Geo<Split, HD>;
     constexpr int TK = G::TK, HDP = G::HDP, CPR = HDP / 8, NP = TK * CPR / 256, PART = TK * HDP;
     static_assert(NP * 256 == TK * CPR, "whole pieces a thread");
-    __shared__ uint32_t red[2][4];
+    __shared__ uint32_t red[3][4];
     const int kvh = (int)(blockIdx.x % a.n_kv), t = (int)(blockIdx.x / a.n_kv), tid = threadIdx.x;
     const int b = sequence_of<TK>(a, t, 1);
     if (b < 0) return;
@@ -1251,35 +1387,34 @@ __global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* image
             v[i][p] = in ? *reinterpret_cast<const u32x4*>(vs + key * a.kv.v_position + col * 8 + 4 * p) : u32x4{0, 0, 0, 0};
         }
     }
-    auto block_max = [&](uint32_t km, uint32_t vm) {
-        __syncthreads();
-        if ((tid & 63) == 0) red[0][tid >> 6] = km, red[1][tid >> 6] = vm;
-        __syncthreads();
-        return uint2{max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3])),
-                     max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]))};
-    };
-    uint2 m = block_max(largest_bits(k, false), largest_bits(v, false));
-    const int bad = m.y >= 0x7F800000u;
-    if (m.x >= 0x7F800000u || bad) {  // the exponents go by the finite ones; values that are not are zeroed
+    uint32_t km[NP], vm[NP], kt = 0, vt = 0;
+    piece_sizes(k, km, false);
+    const bool wide = piece_sizes(v, vm, true);
 #pragma unroll
-        for (int i = 0; i < NP; i++)
-#pragma unroll
-            for (int p = 0; p < 2; p++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if ((v[i][p][c] & 0x7F800000u) == 0x7F800000u) v[i][p][c] = 0;
-        m = block_max(largest_bits(k, true), largest_bits(v, false));
-    }
-    const int ke = exponent(m.x) - 14, ve = (exponent(m.y) - 14 + 3) & ~3;
+    for (int i = 0; i < NP; i++) kt = max(kt, km[i]), vt = max(vt, vm[i]);
+    kt = wave_max_u32(kt);
+    vt = wave_max_u32(vt);
+    if ((tid & 63) == 0) red[0][tid >> 6] = kt, red[1][tid >> 6] = vt, red[2][tid >> 6] = wide ? SLAB_WIDE : 0;
+    __syncthreads();
+    const int ke = hold_all(max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3])), NO_EXPONENT);
+    const int ve = hold_all(max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3])), NO_EXPONENT);
     const int64_t im = (int64_t)t * a.n_kv + kvh;
-    if (tid == 0) notes[im] = int4{ke, ve, bad, 0};
+    int ek[NP], ev[NP], flags = 0;
+    if (row_exponents<CPR>(km, ke, ek)) flags |= SLAB_OTHER_K;
+    if (row_exponents<CPR>(vm, ve, ev)) flags |= SLAB_OTHER_V;
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+        if (tid % CPR == 0) exps[im * TK + (tid + 256 * i) / CPR] = int2{ek[i], ev[i]};
+    if (flags && (tid & 63) == 0) atomicOr(&red[2][0], flags);
+    __syncthreads();
+    if (tid == 0) notes[im] = int4{ke, ve, (int)(red[2][0] | red[2][1] | red[2][2] | red[2][3]), 0};
     _Float16* out = images + im * (TK * G::KEY);
 #pragma unroll
     for (int i = 0; i < NP; i++) {
         const int pc = tid + 256 * i, key = pc / CPR, col = pc % CPR;
         u32x4 kh, kl, vh, vl;
-        split8(k[i], ke, &kh, &kl);
-        split8(v[i], ve, &vh, &vl);
+        split8(k[i], ek[i], &kh, &kl);
+        split8(v[i], ev[i], &vh, &vl);
         u32x4* kd = reinterpret_cast<u32x4*>(out + key * HDP + (col ^ G::k_swap(key)) * 8);
         u32x4* vd = reinterpret_cast<u32x4*>(out + 2 * PART + key * HDP + (col ^ G::v_swap(key)) * 8);
         *kd = kh;
@@ -1306,8 +1441,8 @@ hipError_t launch_kind(const BatchArgs& a, hipStream_t s) {
                                                                        : launch<KV, HD, TILE | FEW>(a, s);
 }
 template <int HD>
-hipError_t launch_split(const BatchArgs& a, _Float16* images, int4* notes, int tiles, hipStream_t s) {
-    hipLaunchKernelGGL(split_kernel<HD>, dim3((unsigned)(tiles * a.n_kv)), dim3(256), 0, s, a, images, notes);
+hipError_t launch_split(const BatchArgs& a, _Float16* images, int4* notes, int2* exps, int tiles, hipStream_t s) {
+    hipLaunchKernelGGL(split_kernel<HD>, dim3((unsigned)(tiles * a.n_kv)), dim3(256), 0, s, a, images, notes, exps);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? launch<Split, HD, TILE>(a, s) : e;
 }
@@ -1362,7 +1497,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     // f32 prompts whose keys several tiles read: split once
     const int hdp = a.hd <= 64 ? 64 : a.hd <= 128 ? 128 : 256, tk = a.hd <= 64 ? 64 : 32;  // Geo<Split, HD>
     const int64_t tiles = m / tk + a.n_seq;
-    const size_t image_bytes = (size_t)tiles * a.n_kv * tk * hdp * 8, note_bytes = (size_t)tiles * a.n_kv * sizeof(int4);
+    const size_t image_bytes = (size_t)tiles * a.n_kv * tk * hdp * 8, note_bytes = (size_t)tiles * a.n_kv * (sizeof(int4) + tk * sizeof(int2));
     const bool pre = !f16 && !a.kv.tables && only_tile && m * G >= SPLIT_MIN_TILES * TILE_PAIRS * a.n_seq &&
                      image_bytes <= SPLIT_BYTES;
     const size_t part_bytes = a.part_splits > 1 ? (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float) : 0;
@@ -1382,8 +1517,10 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
         int4* notes = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(images) + image_bytes);
         a.images = images;
         a.notes = notes;
+        int2* exps = reinterpret_cast<int2*>(notes + tiles * a.n_kv);
+        a.exps = exps;
         auto go = a.hd <= 64 ? launch_split<64> : a.hd <= 96 ? launch_split<96> : a.hd <= 128 ? launch_split<128> : launch_split<256>;
-        e = go(a, images, notes, (int)tiles, s);
+        e = go(a, images, notes, exps, (int)tiles, s);
     } else {
         e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
     }

@@ -508,6 +508,109 @@ def test_packed_long(rq, gpu, kv):
             close(out[a:z], *ref.attention(q[a:z], k[a:z], v[a:z], 0, 0.09))
 
 
+@pytest.mark.parametrize("heads,kvh,hd", SHAPES)
+def test_packed_prompts_split_beforehand(rq, gpu, heads, kvh, hd):
+    # f32 prompts long enough that their keys are made f16 parts once a call; sizes around its tiles
+    torch.manual_seed(hd)
+    lens = [700, 1, 64, 65, 129, 900]
+    rows = sum(lens) + 3
+    qkv = torch.randn(rows, heads + 2 * kvh, hd, device="cuda")
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    out = run_packed(q, k, v, ints(starts), 1 / math.sqrt(hd), max(lens))
+    for a, z in zip(starts, starts[1:]):
+        close(out[a:z], *ref.attention(q[a:z], k[a:z], v[a:z], 0, 1 / math.sqrt(hd)))
+    assert (out[starts[-1]:] == -7.0).all()
+    first = out.clone()
+    assert torch.equal(run_packed(q, k, v, ints(starts), 1 / math.sqrt(hd), max(lens)), first)
+
+
+def test_packed_split_beforehand_wide_and_not_finite(rq, gpu):
+    torch.manual_seed(4)
+    n, hd = 1500, 64
+    q, k, v = torch.randn(3, n, 4, hd, device="cuda")
+    # values of very different sizes from tile to tile, tiles of zeros among them
+    size = torch.logspace(-12, 12, n, device="cuda")[torch.randperm(n, device="cuda")][:, None, None]
+    v = v * size
+    k = k * torch.logspace(-8, 0, n, device="cuda")[torch.randperm(n, device="cuda")][:, None, None]
+    k[64:192], v[128:256] = 0.0, 0.0
+    close(run_packed(q, k, v, ints([0, n]), 0.1), *ref.attention(q, k, v, 0, 0.1))
+    # values that are not finite reach the rows that see them and no others
+    want, bound = ref.attention(q, k, v, 0, 0.1)
+    k[1000, 1], v[1100, 2, 7], v[1200, :, 3] = float("nan"), float("inf"), float("nan")
+    out = run_packed(q, k, v, ints([0, n]), 0.1)
+    close(out[:1000], want[:1000], bound[:1000])
+    close(out[1000:1100, 0], want[1000:1100, 0], bound[1000:1100, 0])
+    assert out[1000:, 1].isnan().all()
+    assert (out[1100:, 2, 7] == float("inf")).all()
+    assert out[1200:, :, 3].isnan().all()
+    close(out[1100:, 0, 8:], want[1100:, 0, 8:], bound[1100:, 0, 8:])
+
+
+@pytest.mark.parametrize("n", [3, 40, 1500])
+@pytest.mark.parametrize("power", [-118, -60, 60, 110])
+def test_f32_values_of_extreme_size(rq, gpu, n, power):
+    """Values by a power of two: the outputs by the same one, but for f32's last step near zero."""
+    torch.manual_seed(n)
+    q, k, v = torch.randn(3, n, 4, 64, device="cuda")
+    v = v.sign() * v.abs().clamp(0.01, 4.0)
+    a = run_packed(q, k, v, ints([0, n]), 0.1)
+    b = run_packed(q, k, v * 2.0**power, ints([0, n]), 0.1)
+    want, bound = ref.attention(q, k, v, 0, 0.1)
+    close(a, want, bound)
+    close(b.double() * 2.0**-power, want, bound + 2.0 ** (-149 - power))
+
+
+def test_packed_split_beforehand_captured(rq, gpu):
+    torch.manual_seed(6)
+    q, k, v = torch.randn(3, 1200, 4, 64, device="cuda")
+    starts = ints([0, 1200])
+    out = torch.zeros_like(q)
+    run_packed(q, k, v, starts, 0.1, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run_packed(q, k, v, starts, 0.1, out=out)
+    for lens in ([0, 1200], [0, 500], [3, 1100]):
+        for t in (q, k, v):
+            t.normal_()
+        starts.copy_(ints(lens))
+        out.fill_(-7.0)
+        g.replay()
+        a, z = lens
+        got = out.clone()
+        torch.randn(1000, device="cuda").sum().item()
+        assert torch.equal(run_packed(q, k, v, starts, 0.1), got)
+        close(got[a:z], *ref.attention(q[a:z], k[a:z], v[a:z], 0, 0.1))
+
+
+@pytest.mark.parametrize("n_seq", [65, 200, 4097])
+def test_many_sequences(rq, gpu, n_seq):
+    # more than one step of the search for a tile's sequence; sequences without rows among them
+    r = random.Random(n_seq)
+    lens = [r.choice([0, 1, 1, 2, 5, 70]) if n_seq < 1000 or i % 97 == 0 else r.choice([0, 1, 6]) for i in range(n_seq)]
+    torch.manual_seed(n_seq)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    q, k, v = torch.randn(3, starts[-1] + 1, 2, 64, device="cuda")
+    out = run_packed(q, k.half(), v.half(), ints(starts), 0.1, max(lens))
+    seq = torch.repeat_interleave(torch.arange(n_seq), torch.tensor(lens)).cuda()
+    i = torch.arange(starts[-1], device="cuda")
+    for h in range(2):
+        kk, vv = k[:-1, h].half().double(), v[:-1, h].half().double()
+        s = (q[:-1, h].double() @ kk.T.contiguous()) * 0.1
+        s = s.masked_fill((seq[:, None] != seq) | (i > i[:, None]), -math.inf)
+        want = torch.softmax(s, -1) @ vv
+        # |scores| below 8: weights off by 2^-17 at most (ref.attention), sums of at most 70 values below 6
+        assert (out[:-1, h].double() - want).abs().max() <= 2.0**-17 * 6 * 4
+    assert (out[-1] == -7.0).all()
+    # the same as a step over a cache: every row its own sequence's tail
+    b = Batch([(r.choice([0, 3, 64]), n) for n in lens[:200]], 4, 2, 64, page=16)
+    b.check()
+
+
 def test_packed_rows_before_the_first_and_bad_starts(rq, gpu):
     q, k, v = torch.randn(3, 20, 2, 64, device="cuda")
     out = run_packed(q, k, v, ints([4, 10]), 0.1)  # rows 0 .. 3 belong to nobody
