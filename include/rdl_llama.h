@@ -175,6 +175,30 @@ rdl_status rdl_llama_get_path_counts(const rdl_llama* model, rdl_llama_path_coun
 rdl_status rdl_llama_forward(rdl_llama* model, const int32_t* tokens, size_t n, float* logits,
                              size_t logits_len);
 
+/* Several sequences over the model's pages, one call a step (the reference
+ * runs one sequence: LlmModel::forward_with_cache_pass, model.rs:890-937).
+ * rdl_llama_batch_begin makes n_seq (1 .. 4096) empty sequences, on an empty
+ * cache (position 0); until rdl_llama_reset the cache is theirs, and
+ * rdl_llama_forward and _generate_greedy are RDL_ERR_INVALID_DATA.  They
+ * share the max_seq positions of the pool by pages of 64, each up to max_seq long.
+ * head_dim % 8 == 0, dim % 4 == 0 (RDL_ERR_UNSUPPORTED). */
+rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq);
+/* A step: sequence b takes counts[b] >= 0 tokens, the next of the n tokens
+ * (all sequences', one behind the other; n = the counts' sum, 1 .. max_batch),
+ * behind those it has.  logits[b * vocab ..]: its last row's logits; those of
+ * a sequence without tokens are left as they were.  Single tokens and prompt
+ * chunks may share a step.  A step that needs more pages than are free or passes
+ * max_seq is RDL_ERR_INVALID_DATA and changes nothing.  Synchronous; after
+ * RDL_ERR_HIP the cache contents are undefined.  The rows run as a prompt chunk's do, the
+ * cache through rdl_kv_plan_dev, rdl_kv_store_dev and rdl_attention_paged_dev
+ * (rdl_attention.h). */
+rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
+                                   size_t n, float* logits, size_t logits_len);
+/* Positions that each of the n (= n_seq) sequences has. */
+rdl_status rdl_llama_batch_positions(const rdl_llama* model, size_t* out, size_t n);
+/* Empties one sequence; its pages are free for the others. */
+rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq);
+
 /* Greedy generation (Generator::generate with argmax sampling): prefill of
  * the prompt (in chunks of max_batch), then n_gen - 1 decode steps, each one
  * replay of a captured graph; out_tokens receives the n_gen sampled ids.

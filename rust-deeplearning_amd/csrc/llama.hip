@@ -31,6 +31,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "../../include/rdl_attention.h"
 #include "../../include/rdl_gguf.h"
 #include "../../include/rdl_llama.h"
 #include "attention.hpp"
@@ -571,6 +572,14 @@ __global__ void advance_kernel(int* pos, int by) {
 __global__ void set_int_kernel(int* p, int v) {
     if (threadIdx.x == 0) *p = v;
 }
+// out[i] = x[rows[i]], rows of d floats (d % 4 == 0)
+__global__ __launch_bounds__(NT) void gather_rows_kernel(const float* __restrict__ x, const int* __restrict__ rows, int d,
+                                                         float* __restrict__ out) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const f4* src = reinterpret_cast<const f4*>(x + (size_t)rows[blockIdx.x] * d);
+    f4* dst = reinterpret_cast<f4*>(out + (size_t)blockIdx.x * d);
+    for (int c = threadIdx.x; c < d / 4; c += NT) dst[c] = src[c];
+}
 
 // ---- synthetic weights --------------------------------------------------------------
 __device__ __forceinline__ uint64_t splitmix64(uint64_t& s) {
@@ -678,7 +687,22 @@ struct LlamaModel {
     size_t host_pos = 0;  // mirror of *pos
     std::vector<void*> allocs;
 
+    // Several sequences over the pool's pages (rdl_llama_batch_*): their page
+    // tables, the pages none of them holds, and the current step's lengths,
+    // rows and slots (rdl_kv_plan_dev).
+    struct Batch {
+        bool on = false;
+        size_t n_seq = 0, cap = 0;  // sequences; sequences the memory below is for
+        int *table = nullptr, *cached = nullptr, *count = nullptr, *free_pages = nullptr, *row_start = nullptr,
+            *kv_len = nullptr, *row_seq = nullptr, *positions = nullptr, *slots = nullptr, *summary = nullptr,
+            *last_rows = nullptr;
+        float *x = nullptr, *logits = nullptr;  // [cap][dim], [cap][vocab]
+        size_t max_rows = 0, max_kv = 0;        // of the step
+        std::vector<int> len, free_host;
+    } batch;
+
     ~LlamaModel() {
+        if (batch.cap) (void)rdl_release_stream_work(stream);  // the attention's
         if (decode_exec) (void)hipGraphExecDestroy(decode_exec);
         if (decode_graph) (void)hipGraphDestroy(decode_graph);
         for (hipEvent_t e : ev)
@@ -781,9 +805,26 @@ struct LlamaModel {
         return reinterpret_cast<uint8_t*>(base) + (size_t)l * kv_layer_elems() * kv_elem();
     }
 
+    // The same for a step of several sequences.
+    hipError_t batch_attention(int l, size_t m) {
+        const int hd = cfg.head_dim;
+        const rdl_kv_pool pool = {kv_layer(kc, l), kv_layer(vc, l), cfg.kv_f16 ? RDL_DTYPE_F16 : RDL_DTYPE_F32, n_pages,
+                                  KV_PAGE, cfg.n_kv_heads, hd, (int64_t)cfg.n_kv_heads * KV_PAGE * hd,
+                                  (int64_t)KV_PAGE * hd, hd};
+        rdl_status st = rdl_kv_store_dev(&pool, m, qkv, qkv_dim, qkv, qkv_dim, cfg.n_heads, qkv + q_dim, qkv_dim,
+                                         qkv + q_dim + kv_dim, qkv_dim, batch.positions, batch.slots, cos_t, sin_t,
+                                         cfg.max_seq, stream);
+        if (st == RDL_OK)
+            st = rdl_attention_paged_dev(&pool, qkv, qkv_dim, cfg.n_heads, m, batch.row_start, batch.kv_len, batch.n_seq,
+                                         batch.table, n_pages, 1.0f / sqrtf((float)hd), att, q_dim, batch.max_rows,
+                                         batch.max_kv, stream);
+        return st == RDL_OK ? hipSuccess : hipErrorUnknown;
+    }
+
     // RoPE + cache write (unless the qkv launch did it), then attention.
     template <typename KV>
     hipError_t layer_attention(int l, size_t m, bool rope = true) {
+        if (batch.on) return batch_attention(l, m);
         KV* kcl = reinterpret_cast<KV*>(kv_layer(kc, l));
         KV* vcl = reinterpret_cast<KV*>(kv_layer(vc, l));
         const int hd = cfg.head_dim;
@@ -1026,7 +1067,7 @@ struct LlamaModel {
         if (want_xn && !qkv_done) rmsnorm(L.attn_norm);
         // a K-quant [Wq; Wk; Wv] (or K-quant [Wq; Wk] and Wv, two launches)
         // also applies RoPE and writes the cache
-        const bool rope_fused = !qkv_done && ((np == 1 && kfold_m(L.qkv)) ||
+        const bool rope_fused = !qkv_done && !batch.on && ((np == 1 && kfold_m(L.qkv)) ||
                                               (np == 2 && kfold_m(L.qk) && kfold_m(L.v)));
         for (size_t r = 0; rope_fused && r < m; r += 4) {
             const size_t mr = (m - r < 4) ? m - r : 4;
@@ -1157,6 +1198,23 @@ struct LlamaModel {
         if (e != hipSuccess) return e;
         if (advance) hipLaunchKernelGGL(advance_kernel, dim3(1), dim3(64), 0, stream, pos, (int)m);
         return hipGetLastError();
+    }
+
+    // forward_with_cache_pass over the m rows of a step of several sequences
+    // (tokens, lengths and last_rows on the device): the logits of the n_last
+    // sequences' last rows into batch.logits.
+    hipError_t forward_batch(size_t m, size_t n_last) {
+        const int d = cfg.dim;
+        hipError_t e = launch_dequant_rows(emb.type, emb.dev, emb.n, emb.k, tokens, m, x, stream);
+        for (int l = 0; l < cfg.n_layers && e == hipSuccess; l++) e = layer_plain(l, m);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)n_last), dim3(NT), 0, stream, x, batch.last_rows, d, batch.x);
+        hipLaunchKernelGGL(rmsnorm_kernel, dim3((unsigned)n_last), dim3(NT), 0, stream, batch.x, final_norm, d,
+                           cfg.norm_eps, xn);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        for (size_t r = 0; r < n_last && e == hipSuccess; r += 4)  // four rows a launch: the GEMVs need no scratch
+            e = linear(out, xn + r * d, std::min<size_t>(4, n_last - r), batch.logits + r * cfg.vocab);
+        return e;
     }
 
     // argmax of `logits` -> token, out_tokens, step; position += advance; the
@@ -1557,6 +1615,7 @@ rdl_status rdl_llama_reset(rdl_llama* model) {
     HIP_TRY(hipMemset(M.att_xch, 0, (size_t)M.cfg.n_layers * M.xch_stride() * sizeof(uint64_t)));
     HIP_TRY(hipMemset(M.att_err, 0, sizeof(int)));
     M.host_pos = 0;
+    M.batch.on = false;
     return api_ok();
 }
 
@@ -1592,10 +1651,135 @@ rdl_status rdl_llama_set_kv_page_table(rdl_llama* model, const int32_t* table, s
     return api_ok();
 }
 
+rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
+    if (!model) return api_fail(RDL_ERR_NULL_POINTER, "NULL model");
+    rdl::LlamaModel& M = model->m;
+    const rdl_llama_config& c = M.cfg;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (n_seq == 0 || n_seq > 4096) return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences: 1 .. 4096", n_seq);
+    if (c.head_dim % 8 || c.dim % 4)
+        return api_fail(RDL_ERR_UNSUPPORTED, "several sequences need head_dim %% 8 == 0 (%d), dim %% 4 == 0 (%d)", c.head_dim,
+                        c.dim);
+    if (M.host_pos != 0 || B.on)
+        return api_fail(RDL_ERR_INVALID_DATA, "sequences can begin only on an empty cache (rdl_llama_reset first)");
+    auto fail_free = [&](hipError_t e) { return api_fail(RDL_ERR_HIP, "allocation failed: %s", hipGetErrorString(e)); };
+    try {
+        B.len.assign(n_seq, 0);
+        B.free_host.resize((size_t)M.n_pages);
+    } catch (const std::exception&) {
+        return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
+    }
+    for (int p = 0; p < M.n_pages; p++) B.free_host[p] = p;
+    hipError_t e;
+    if (n_seq > B.cap) {  // (memory of an earlier, smaller batch stays until the model is freed)
+        const size_t mb = c.max_batch, pg = M.n_pages;
+        for (auto& a : {std::make_pair(&B.table, n_seq * pg), {&B.cached, n_seq}, {&B.count, n_seq}, {&B.free_pages, pg},
+                        {&B.row_start, n_seq + 1}, {&B.kv_len, n_seq}, {&B.row_seq, mb}, {&B.positions, mb},
+                        {&B.slots, mb}, {&B.summary, (size_t)4}, {&B.last_rows, n_seq}})
+            if ((e = M.alloc_t(a.first, a.second)) != hipSuccess) return fail_free(e);
+        if ((e = M.alloc_t(&B.x, n_seq * c.dim)) != hipSuccess) return fail_free(e);
+        if ((e = M.alloc_t(&B.logits, n_seq * c.vocab)) != hipSuccess) return fail_free(e);
+        B.cap = n_seq;
+    }
+    B.n_seq = n_seq;
+    B.on = true;
+    return api_ok();
+}
+
+rdl_status rdl_llama_batch_positions(const rdl_llama* model, size_t* out, size_t n) {
+    if (!model || !out) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
+    const rdl::LlamaModel::Batch& B = model->m.batch;
+    if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
+    if (n != B.n_seq) return rdl::api_shape_fail("sequences", {B.n_seq}, {n});
+    for (size_t b = 0; b < n; b++) out[b] = (size_t)B.len[b];
+    return api_ok();
+}
+
+rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq) {
+    if (!model) return api_fail(RDL_ERR_NULL_POINTER, "NULL model");
+    rdl::LlamaModel& M = model->m;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
+    if (seq >= B.n_seq) return api_fail(RDL_ERR_INVALID_DATA, "sequence %zu of %zu", seq, B.n_seq);
+    const size_t held = ((size_t)B.len[seq] + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
+    const size_t had = B.free_host.size();
+    B.free_host.resize(had + held);  // within the capacity it began with
+    if (held) {
+        const hipError_t e = hipMemcpy(B.free_host.data() + had, B.table + seq * M.n_pages, held * sizeof(int),
+                                       hipMemcpyDeviceToHost);
+        if (e != hipSuccess) {
+            B.free_host.resize(had);
+            return api_fail(RDL_ERR_HIP, "page table read failed: %s", hipGetErrorString(e));
+        }
+    }
+    B.len[seq] = 0;
+    return api_ok();
+}
+
+rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
+                                   size_t n, float* logits, size_t logits_len) {
+    if (!model || !counts || !tokens || !logits) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
+    rdl::LlamaModel& M = model->m;
+    const rdl_llama_config& c = M.cfg;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
+    if (n_seq != B.n_seq) return rdl::api_shape_fail("sequences", {B.n_seq}, {n_seq});
+    if (n == 0 || n > (size_t)c.max_batch)
+        return api_fail(RDL_ERR_SHAPE_MISMATCH, "%zu tokens: 1 .. max_batch (%d) per call", n, c.max_batch);
+    if (logits_len < n_seq * (size_t)c.vocab) return rdl::api_shape_fail("logits length", {n_seq * (size_t)c.vocab}, {logits_len});
+    size_t rows = 0, pages = 0;
+    B.max_rows = B.max_kv = 0;
+    for (size_t b = 0; b < n_seq; b++) {
+        if (counts[b] < 0) return api_fail(RDL_ERR_INVALID_DATA, "sequence %zu: %d tokens", b, counts[b]);
+        const size_t len = (size_t)B.len[b], t = len + (size_t)counts[b];
+        if (t > (size_t)c.max_seq)
+            return api_fail(RDL_ERR_INVALID_DATA, "sequence length %zu exceeds maximum %d (start_pos=%zu)", t, c.max_seq, len);
+        rows += (size_t)counts[b];
+        pages += (t + rdl::KV_PAGE - 1) / rdl::KV_PAGE - (len + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
+        B.max_rows = std::max(B.max_rows, (size_t)counts[b]);
+        if (counts[b]) B.max_kv = std::max(B.max_kv, t);
+    }
+    if (rows != n) return rdl::api_shape_fail("tokens", {rows}, {n});
+    if (pages > B.free_host.size())
+        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.free_host.size());
+    for (size_t i = 0; i < n; i++)
+        if (tokens[i] < 0 || tokens[i] >= c.vocab)
+            return api_fail(RDL_ERR_INVALID_DATA, "token %d out of bounds for embedding with %d entries", tokens[i], c.vocab);
+    std::vector<int> last;
+    try {
+        for (size_t b = 0, r = 0; b < n_seq; b++)
+            if (r += (size_t)counts[b]; counts[b]) last.push_back((int)r - 1);
+    } catch (const std::exception&) {
+        return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
+    }
+    auto up = [&](int* dst, const int* src, size_t k) {
+        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
+    };
+    HIP_TRY(up(M.tokens, tokens, n));
+    HIP_TRY(up(B.cached, B.len.data(), n_seq));
+    HIP_TRY(up(B.count, counts, n_seq));
+    HIP_TRY(up(B.free_pages, B.free_host.data(), B.free_host.size()));
+    HIP_TRY(up(B.last_rows, last.data(), last.size()));
+    const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.free_host.size(), rdl::KV_PAGE, B.table,
+                                          (size_t)M.n_pages, B.row_start, B.kv_len, n, B.row_seq, B.positions, B.slots,
+                                          B.summary, M.stream);
+    if (st != RDL_OK) return st;
+    HIP_TRY(M.forward_batch(n, last.size()));
+    for (size_t b = 0, i = 0; b < n_seq; b++)
+        if (counts[b])
+            HIP_TRY(hipMemcpyAsync(logits + b * c.vocab, B.logits + i++ * c.vocab, (size_t)c.vocab * 4,
+                                   hipMemcpyDeviceToHost, M.stream));
+    HIP_TRY(hipStreamSynchronize(M.stream));
+    B.free_host.erase(B.free_host.begin(), B.free_host.begin() + (ptrdiff_t)pages);
+    for (size_t b = 0; b < n_seq; b++) B.len[b] += counts[b];
+    return api_ok();
+}
+
 rdl_status rdl_llama_forward(rdl_llama* model, const int32_t* tokens, size_t n, float* logits, size_t logits_len) {
     if (!model || !tokens || !logits) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
     rdl::LlamaModel& M = model->m;
     const rdl_llama_config& c = M.cfg;
+    if (M.batch.on) return api_fail(RDL_ERR_INVALID_DATA, "the cache holds several sequences (rdl_llama_reset first)");
     if (n == 0 || n > (size_t)c.max_batch)
         return api_fail(RDL_ERR_SHAPE_MISMATCH, "%zu tokens: 1 .. max_batch (%d) per call", n, c.max_batch);
     if (logits_len < (size_t)c.vocab)
@@ -1623,6 +1807,7 @@ rdl_status rdl_llama_generate_greedy(rdl_llama* model, const int32_t* prompt, si
         return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
     rdl::LlamaModel& M = model->m;
     const rdl_llama_config& c = M.cfg;
+    if (M.batch.on) return api_fail(RDL_ERR_INVALID_DATA, "the cache holds several sequences (rdl_llama_reset first)");
     if (n_prompt == 0) return api_fail(RDL_ERR_INVALID_DATA, "empty prompt");
     if (n_gen == 0) return api_ok();
     // the last sampled token is not fed back: positions used = prompt + n_gen - 1

@@ -38,6 +38,11 @@ _decl("rdl_llama_reset", _i32, _p)
 _decl("rdl_llama_position", _i32, _p, C.POINTER(_sz))
 _decl("rdl_llama_forward", _i32, _p, C.POINTER(C.c_int32), _sz, C.POINTER(C.c_float), _sz)
 _decl("rdl_llama_generate_greedy", _i32, _p, C.POINTER(C.c_int32), _sz, _sz, C.POINTER(C.c_int32))
+_decl("rdl_llama_batch_begin", _i32, _p, _sz)
+_decl("rdl_llama_batch_forward", _i32, _p, C.POINTER(C.c_int32), _sz, C.POINTER(C.c_int32), _sz, C.POINTER(C.c_float),
+      _sz)
+_decl("rdl_llama_batch_positions", _i32, _p, C.POINTER(_sz), _sz)
+_decl("rdl_llama_batch_drop", _i32, _p, _sz)
 _decl("rdl_llama_last_timing", _i32, _p, C.POINTER(C.c_float), C.POINTER(C.c_float))
 _decl("rdl_llama_rope_tables", _i32, _p, C.POINTER(C.c_float), C.POINTER(C.c_float), _sz)
 _decl("rdl_llama_get_config", _i32, _p, C.POINTER(_Config))
@@ -129,6 +134,7 @@ class LlamaModel:
         else:
             check(lib.rdl_llama_create(C.byref(cfg), C.byref(h)))
         self._h = h
+        self._n_seq = 0
 
     @classmethod
     def from_gguf(cls, gguf, max_seq: int = 0, max_batch: int = 32, kv_f16: bool = True) -> "LlamaModel":
@@ -150,6 +156,7 @@ class LlamaModel:
             check(status)
         self = cls.__new__(cls)
         self._h = h
+        self._n_seq = 0
         self.config = LlamaConfig(c.dim, c.n_layers, c.n_heads, c.n_kv_heads, c.head_dim, c.ffn_dim, c.vocab,
                                   c.max_seq, float(c.norm_eps), float(c.rope_theta), bool(c.kv_f16),
                                   c.max_batch, c.output_dtype)
@@ -222,6 +229,34 @@ class LlamaModel:
         check(lib.rdl_llama_forward(self._h, t.ctypes.data_as(C.POINTER(C.c_int32)), t.size,
                                     logits.ctypes.data_as(C.POINTER(C.c_float)), logits.size))
         return logits
+
+    def batch_begin(self, n_seq: int) -> None:
+        """n_seq empty sequences over the model's pages (empty cache only);
+        the cache is theirs until reset()."""
+        check(lib.rdl_llama_batch_begin(self._h, n_seq))
+        self._n_seq = n_seq
+
+    def batch_forward(self, tokens) -> np.ndarray:
+        """One step: tokens[b] (a list, maybe empty) behind sequence b.
+        Returns [n_seq, vocab] logits of the last rows; NaN for sequences
+        without tokens."""
+        counts = _i32_array([len(t) for t in tokens])
+        flat = _i32_array([t for seq in tokens for t in seq])
+        logits = np.full((counts.size, self.config.vocab), np.nan, dtype=np.float32)
+        ip = C.POINTER(C.c_int32)
+        check(lib.rdl_llama_batch_forward(self._h, counts.ctypes.data_as(ip), counts.size, flat.ctypes.data_as(ip),
+                                          flat.size, logits.ctypes.data_as(C.POINTER(C.c_float)), logits.size))
+        return logits
+
+    def batch_positions(self) -> list:
+        """Positions that each sequence has."""
+        out = (_sz * max(self._n_seq, 1))()
+        check(lib.rdl_llama_batch_positions(self._h, out, self._n_seq))
+        return [int(v) for v in out][:self._n_seq]
+
+    def batch_drop(self, seq: int) -> None:
+        """Empties one sequence; its pages are free for the others."""
+        check(lib.rdl_llama_batch_drop(self._h, seq))
 
     def prefill(self, tokens) -> np.ndarray:
         return self.forward_with_cache(tokens)
