@@ -46,7 +46,7 @@ enum {
 /* A layer's paged K and V memory.  Element d of position o of page pg and KV
  * head h is at pg * page_stride + h * head_stride + o * position_stride + d of
  * k_dev and of v_dev (strides in elements; multiples of 16 bytes, as both
- * bases; the heads and positions of a page and the pages must not overlap).
+ * bases; position_stride below 2^24; the heads and positions of a page and the pages must not overlap).
  * The decoder's own pools are [n_pages][n_kv_heads][page_positions][head_dim]. */
 typedef struct rdl_kv_pool {
     void* k_dev;
@@ -118,13 +118,18 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * not seen.  Rows row_start[n_seq] .. m - 1 of out are left as they were.
  * q and out: f32 rows stride floats apart (n_heads * head_dim or more, a
  * multiple of 4; bases 16-byte aligned); out must not overlap q.
- * What a row does not see has no effect on it, NaN and infinities included; a
- * NaN or an infinity in a key or query that is used makes its rows NaN.
+ * row_start ascends; where it does not, what the call's rows get is unspecified.
+ * What a row does not see has no effect on it, NaN and infinities included.  Of
+ * what it sees, a NaN in a key or in its query makes its outputs NaN, a value that is
+ * not finite makes that element NaN or infinite whatever its weight, and infinite
+ * keys or queries leave its outputs unspecified.
  * max_rows and max_kv tell the launch what to expect (the most rows of a
  * sequence, the longest kv_len; 0: unknown): results do not depend on them
  * beyond rounding, time does.  Products are formed on the matrix cores with
  * f32 sums from f16 pairs that carry 22 bits of q, of the weights and of f32
  * keys and values (f16 ones are exact); sums, maxima and exponents are f32.
+ * Of f32 values, elements far below the largest of their row or of the rows a
+ * query weighs with it end at 2^-28 of that.
  * n_heads must be a multiple of the pool's n_kv_heads. */
 rdl_status rdl_attention_paged_dev(const rdl_kv_pool* pool, const float* q_dev, size_t q_stride, size_t n_heads,
                                    size_t m, const int32_t* row_start_dev, const int32_t* kv_len_dev, size_t n_seq,

@@ -46,7 +46,7 @@ struct BatchArgs {
     float* part;              // [m][n_heads][part_splits][hd]
     float* part_ml;           // [m][n_heads][part_splits][2]
     int part_splits;
-    int* counters;            // [m][n_heads], zero between launches
+    int* counters;            // [tile, then sequence of few rows][n_kv], zero between launches
     // Split sources: tiles of TK keys as LDS holds them, numbered as row tiles
     // are (tile of TK rows * n_kv + KV head), and their exponents and flags
     const _Float16* images;
@@ -587,7 +587,9 @@ __device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int p)
 // maximum and sum (part_ml).  Publication as attention.hpp describes it:
 // agent-coherent stores, each wave waits for its own, a barrier, then the
 // counter; the last split to arrive joins all of them in order (so results
-// do not depend on which it is) and leaves the counter at zero.
+// do not depend on which it is) and leaves the counter at zero.  A counter belongs
+// to the workgroups of one slot of the launch, not to rows: whatever
+// row_start holds, they agree on how many they are.
 __device__ __forceinline__ int64_t place(const BatchArgs& a, const Seq& s, int kvh, int p) {
     const Pair x = pair_of(a, p);
     return (s.row0 + x.row) * a.n_heads + kvh * a.group + x.head;
@@ -621,12 +623,11 @@ template <int NT, int PAIRS>
 constexpr int JOIN_SPLITS = NT / PAIRS * JOIN_DEEP;
 template <int NT, int PAIRS>
 __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
-                                     float* wt, int* flag) {
+                                     int* c, float* wt, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const int tid = threadIdx.x;
     if (tid == 0) {
-        int* c = a.counters + place(a, s, kvh, p0);
         const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = old == splits - 1;
         if (old == splits - 1) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1113,7 +1114,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     const int g = lane >> 4, c = lane & 15;
     const int pairs = min(FEW_PAIRS, s.pairs - p0);
     const int keys = last_key(a, s, p0 + pairs - 1) + 1;
-    const int splits = min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
+    const int splits = p0 ? 1 : min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
     if (z >= splits) return 0;
     const int j_lo = z * a.few_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.few_span);
     const int p = p0 + c;
@@ -1345,14 +1346,16 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
             const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta, exps);
             // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
             if (splits > 1)
-                join<NT, TILE_PAIRS>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                join<NT, TILE_PAIRS>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, a.counters + slot * a.n_kv + kvh,
+                                     reinterpret_cast<float*>(smem), &flag);
         }
     } else {
         if constexpr ((KIND & FEW) != 0)
-            for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once only where max_rows was too small
+            for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once (and then not split) only where max_rows was too small
                 const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml, exps);
                 if (splits > 1)
-                    join<NT, FEW_PAIRS>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem), &flag);
+                    join<NT, FEW_PAIRS>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits,
+                                        a.counters + (a.tiles + slot) * a.n_kv + kvh, reinterpret_cast<float*>(smem), &flag);
                 __syncthreads();  // before the next rows take the LDS
             }
     }
@@ -1505,7 +1508,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     CallScratch work;
     if (part_bytes || pre) {
         const rdl_status st = call_scratch(s, part_room + (pre ? image_bytes + note_bytes : 0),
-                                           part_bytes ? (size_t)m * a.n_heads : 0, &work);
+                                           part_bytes ? ((size_t)a.tiles + (a.few_rows ? a.n_seq : 0)) * a.n_kv : 0, &work);
         if (st != RDL_OK) return st;
         a.part = reinterpret_cast<float*>(work.p);
         a.part_ml = a.part + (size_t)m * a.n_heads * a.part_splits * a.hd;

@@ -623,6 +623,20 @@ def test_packed_rows_before_the_first_and_bad_starts(rq, gpu):
     close(out[3:], *ref.attention(q[3:], k[3:], v[3:], 0, 0.1))
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_sequences_that_share_rows_leave_later_calls_alone(rq, gpu, kv):
+    """Split key ranges are joined by counters that the launches of a stream share."""
+    b = Batch([(2990, 20), (2990, 0), (2990, 20), (1500, 0)], 4, 2, 64, kv=kv)
+    want = b.run(max_rows=0, max_kv=0)
+    proper = b.row_start, b.kv_len
+    for _ in range(3):
+        b.row_start, b.kv_len = ints([0, 20, 0, 20, 40]), ints([3010, 2990, 1400, 1500])
+        b.run(max_rows=0, max_kv=0)
+        b.row_start, b.kv_len = proper
+        assert torch.equal(b.run(max_rows=0, max_kv=0), want)
+    close(want, *b.want())
+
+
 def test_packed_nan_behind_a_row(rq, gpu):
     torch.manual_seed(2)
     for dt in (torch.float16, torch.float32):
