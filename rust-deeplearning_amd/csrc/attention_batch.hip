@@ -42,11 +42,12 @@ struct BatchArgs {
     // (of 8 KV heads each has an XCD and its L2 to itself).
     int tiles, tile_splits, few_splits;
     int tile_span, few_span;  // keys a split
+    int tile_slots;           // not 0: the splits of all tiles that the launch has room for (tile_plan)
     int few_rows;             // sequences of at most this many (row, head of a group) pairs are few-row ones
     float* part;              // [m][n_heads][part_splits][hd]
     float* part_ml;           // [m][n_heads][part_splits][2]
     int part_splits;
-    int* counters;            // [tile, then sequence of few rows][n_kv], zero between launches
+    int* counters;            // [n_seq][n_kv] of few rows, zero between launches
     // Split sources: tiles of TK keys as LDS holds them, numbered as row tiles
     // are (tile of TK rows * n_kv + KV head), and their exponents and flags
     const _Float16* images;
@@ -118,6 +119,25 @@ __device__ __forceinline__ int lanes_max(int v) {
     v = max(v, dpp_i32<DPP_QUAD_XOR2>(v));
     if constexpr (N == 8) v = max(v, dpp_i32<DPP_ROW_HALF_MIRROR>(v));
     return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int lanes_sum(int v) {  // over the wave, uniform
+    v += dpp_i32<DPP_QUAD_XOR1>(v);
+    v += dpp_i32<DPP_QUAD_XOR2>(v);
+    v += dpp_i32<DPP_ROW_HALF_MIRROR>(v);
+    v += dpp_i32<DPP_ROW_MIRROR>(v);
+    v += __builtin_bit_cast(int, other16(__builtin_bit_cast(float, v)));
+    v += __builtin_bit_cast(int, other32(__builtin_bit_cast(float, v)));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int lanes_before(int v) {  // the sum over the lanes before this one
+    int t = v;
+    t += __builtin_amdgcn_update_dpp(0, t, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+    t += __builtin_amdgcn_update_dpp(0, t, 0x112, 0xF, 0xF, false);
+    t += __builtin_amdgcn_update_dpp(0, t, 0x114, 0xF, 0xF, false);
+    t += __builtin_amdgcn_update_dpp(0, t, 0x118, 0xF, 0xF, false);
+    t += __builtin_amdgcn_update_dpp(0, t, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+    t += __builtin_amdgcn_update_dpp(0, t, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
+    return t - v;
 }
 // floor(log2(v)) of a positive finite f32 given by its bits (-127 below 2^-126)
 __device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }
@@ -538,6 +558,17 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
     s.t = (int)max((int64_t)0, min(t, (int64_t)INT32_MAX - 4096));
     return s;
 }
+// Key ranges are split until the launch has about this many workgroups, as far
+// as a span has keys enough.  Measured (us): 48 single rows over up to 8192
+// keys with FEW_TARGET 512, 1024, 2048, 4096: 157.8, 163, 154.6, 163; 2048 rows over
+// 16048 keys with TILE_TARGET 512 (two workgroups a CU) and 768: 910 and 951, as each
+// split of a tile writes 65 KB that join_kernel reads; chunks and single rows in
+// one step (841 rows of 16 sequences) with MIXED_TARGET 512, 384, 320: 104, 95,
+// 126: the single rows run on what the tiles leave; 63 rows of 9 sequences over up
+// to 1900 f32 keys with TILE_MIN_SPAN 128, 256, 512: 22.8, 25.0, 36.7.
+constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512, MIXED_TARGET = 384;
+constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 128;
+
 // Tiles are numbered so that a sequence is found from row_start alone:
 // sequence b's are TILE_PAIRS pairs each and numbered from row_start[b] group
 // / TILE_PAIRS + b on, which leaves at least as many numbers as it has tiles before
@@ -615,25 +646,21 @@ __device__ __forceinline__ f2 get2(const float* p) {
 __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, float M, float L) {
     put2(a.part_ml + (at * a.part_splits + z) * 2, M, L);
 }
-// A join of up to PAIRS pairs: NT / PAIRS lanes a pair form the splits' weights,
-// while the first outputs are on their way; then a thread takes four dims of a
-// pair at a time.  Its latency is what it costs.
+// Joins up to FEW_PAIRS pairs: JOIN_LANES lanes a pair form the splits' weights
+// while the first outputs are on their way, then a thread takes four dims of a
+// pair at a time.  Its latency is what it costs.  COHERENT: the partials come from
+// the same launch.
 constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4;  // splits a lane, at most; splits whose outputs are read ahead
-template <int NT, int PAIRS>
-constexpr int JOIN_SPLITS = NT / PAIRS * JOIN_DEEP;
-template <int NT, int PAIRS>
-__device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits,
-                                     int* c, float* wt, int* flag) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
+constexpr int JOIN_FLOATS = FEW_PAIRS * (JOIN_SPLITS + 1);  // of LDS
+template <bool COHERENT>
+__device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int splits, float* wt) {
+    constexpr int NT = JOIN_THREADS, PAIRS = FEW_PAIRS;
     const int tid = threadIdx.x;
-    if (tid == 0) {
-        const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = old == splits - 1;
-        if (old == splits - 1) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!*flag) return;
+    auto get2 = [](const float* p) {
+        if constexpr (COHERENT) return rdl::get2(p);
+        else return *reinterpret_cast<const f2*>(p);
+    };
     constexpr int LP = NT / PAIRS;
     const int quads = a.hd >> 2;
     auto outputs = [&](int i) {  // item i's first split
@@ -668,7 +695,7 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     }
 #pragma unroll
     for (int d = 1; d < LP; d <<= 1) L += __shfl_xor(L, d);
-    float* inv = wt + PAIRS * JOIN_SPLITS<NT, PAIRS>;
+    float* inv = wt + PAIRS * JOIN_SPLITS;
     if (l == 0 && pi < pairs) inv[pi] = L != 0.0f ? 1.0f / L : 0.0f;
     __syncthreads();
     for (int i = tid; i < pairs * quads; i += NT) {
@@ -803,6 +830,41 @@ __device__ __forceinline__ void weigh_two(Get&& get, Put&& put, Value&& value, R
     }
 }
 
+// Of a few-row workgroup whose split's partial is stored: whether it is the last
+// of its splits, which the counter c knows.
+__device__ __forceinline__ bool last_to_arrive(int splits, int* c, int* flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int old = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = old == splits - 1;
+        if (old == splits - 1) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return *flag;
+}
+
+// How a tile's keys are split: into at most `parts` (its sequence's number), `share`
+// keys each, the last one's fewer.
+struct TileSplit {
+    int keys, share, splits;
+};
+__device__ __forceinline__ TileSplit tile_split(const BatchArgs& a, const Seq& s, int p0, int parts) {
+    TileSplit t;
+    t.keys = last_key(a, s, min(p0 + TILE_PAIRS - 1, s.pairs - 1)) + 1;
+    t.share = max(64, ((t.keys + parts - 1) / parts + 63) & ~63);
+    t.splits = max(1, (t.keys + t.share - 1) / t.share);
+    return t;
+}
+// (Nearly a division rounded up; what matters is that all who ask get the same.)
+__device__ __forceinline__ int parts_of(const BatchArgs& a, int keys, int span) {
+    return min(a.tile_splits, max(1, (int)fmaf((float)keys, __builtin_amdgcn_rcpf((float)span), 0.999f)));
+}
+// The tile of slot number `slot`: its sequence's last rows, which see the most keys, first.
+__device__ __forceinline__ int tile_start(const BatchArgs& a, const Seq& s, int b, int slot) {
+    return (tiles_of<TILE_PAIRS>(s.pairs) - 1 - (slot - first_tile<TILE_PAIRS>(s.row0, a.group, b))) * TILE_PAIRS;
+}
+
 // ---- many rows: waves of 32 pairs, tiles of TK keys shared through LDS -------------------
 // Each wave holds 32 pairs as the columns of both products, S^T = K Q^T and
 // O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a lane has 16 scores of one pair, so
@@ -812,8 +874,8 @@ __device__ __forceinline__ void weigh_two(Get&& get, Put&& put, Value&& value, R
 // fetch them.
 // Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
-__device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
-                                         int p0, int z, _Float16* lds, Meta* meta, int2* exps) {
+__device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
+                                         int p0, int z, int parts, _Float16* lds, Meta* meta, int2* exps) {
     using G = Geo<KV, HD>;
     typedef typename std::conditional<std::is_same<KV, Split>::value, float, KV>::type Elem;
     constexpr int TK = G::TK, W = G::W, SK = TK / W, KS = HD / 16, DT = HD / 32, HDP = G::HDP;
@@ -824,10 +886,11 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
     // this tile's keys and the split's share of them
-    const int keys = last_key(a, s, min(p0 + 32 * G::W - 1, s.pairs - 1)) + 1;
-    const int splits = min(a.tile_splits, max(1, (keys + a.tile_span - 1) / a.tile_span));
-    if (z >= splits) return 0;
-    const int j_lo = z * a.tile_span, j_hi = z == splits - 1 ? keys : min(keys, j_lo + a.tile_span);
+    static_assert(32 * W == TILE_PAIRS, "a wave 32 pairs");
+    const TileSplit ts = tile_split(a, s, p0, parts);
+    const int splits = ts.splits;
+    if (z >= splits) return;
+    const int j_lo = z * ts.share, j_hi = min(ts.keys, j_lo + ts.share);
     const int p = p0 + 32 * w + c;
     const bool live = p < s.pairs, work = p0 + 32 * w < s.pairs;
     const int last = live ? last_key(a, s, p) : -1;
@@ -1083,15 +1146,13 @@ __device__ __forceinline__ int tile_rows(const BatchArgs& a, const Seq& s, const
             if (splits == 1) {
                 *reinterpret_cast<f4*>(out_at(a, s, kvh, pr) + d) = y;
             } else {
-                float* dst = a.part + (place(a, s, kvh, pr) * a.part_splits + z) * a.hd + d;
-                put2(dst, y[0], y[1]);
-                put2(dst + 2, y[2], y[3]);
+                *reinterpret_cast<f4*>(a.part + (place(a, s, kvh, pr) * a.part_splits + z) * a.hd + d) = y;
             }
         }
         wave_sync();
     }
-    if (splits > 1 && live && h == 0) put_ml(a, place(a, s, kvh, p), z, M, L);
-    return splits;
+    if (splits > 1 && live && h == 0)
+        *reinterpret_cast<f2*>(a.part_ml + (place(a, s, kvh, p) * a.part_splits + z) * 2) = f2{M, L};
 }
 
 // ---- few rows: up to 16 pairs, each wave its own keys ------------------------------------------
@@ -1315,6 +1376,54 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     return splits;
 }
 
+// The splits of a step of up to 64 sequences, a lane each: the shortest span of
+// keys, in steps of 64, by which all tiles' splits find room in a.tile_slots
+// workgroups a KV head (one a tile does: there are as many), so that all start at once, numbered
+// without gaps.  Numbered over the most splits that any tile might have, every
+// fourth workgroup or so had nothing to do, and with them a quarter of the CUs:
+// workgroups are dealt to the parts of an XCD in turn.
+__device__ __forceinline__ int shortest_span(const BatchArgs& a, int tiles, int keys) {
+    int lo = TILE_MIN_SPAN / 64, hi = max(lo, ((int)wave_max_u32((uint32_t)keys) + 63) / 64);
+    for (int mid = lo; lo < hi; mid = (lo + hi) / 2) {
+        if (lanes_sum(tiles * parts_of(a, keys, 64 * mid)) <= a.tile_slots) hi = mid;
+        else lo = mid + 1;
+    }
+    return 64 * hi;
+}
+struct TilePlan {
+    int b, tile, z, parts;  // of number `slot`; b -1: none
+};
+__device__ __forceinline__ TilePlan tile_plan(const BatchArgs& a, int slot) {
+    const int lane = threadIdx.x & 63;
+    int tiles = 0, keys = 0;
+    if (lane < a.n_seq) {
+        const Seq s = sequence(a, lane);
+        if (s.pairs > a.few_rows) tiles = tiles_of<TILE_PAIRS>(s.pairs), keys = s.t;
+    }
+    const int parts = parts_of(a, keys, shortest_span(a, tiles, keys)), n = tiles * parts;
+    const int before = lanes_before(n);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(slot >= before && slot < before + n);
+    if (mask == 0) return {-1, 0, 0, 1};
+    TilePlan t;
+    t.b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(mask));
+    t.parts = __builtin_amdgcn_readlane(parts, t.b);
+    const int at = slot - __builtin_amdgcn_readlane(before, t.b);
+    t.tile = at / t.parts;
+    t.z = at - t.tile * t.parts;
+    return t;
+}
+// A sequence's parts, for those who come by its tiles' own numbers.
+__device__ __forceinline__ int planned_parts(const BatchArgs& a, const Seq& s, int b) {
+    if (!a.tile_slots) return parts_of(a, s.t, a.tile_span);
+    const int lane = threadIdx.x & 63;
+    int tiles = 0, keys = 0;
+    if (lane < a.n_seq) {
+        const Seq x = sequence(a, lane);
+        if (x.pairs > a.few_rows) tiles = tiles_of<TILE_PAIRS>(x.pairs), keys = x.t;
+    }
+    return parts_of(a, s.t, shortest_span(a, tiles, keys));
+}
+
 // KIND: which workgroups a launch has.  The two bodies in one kernel keep more
 // registers than either needs, so launches that need one of them have it alone.
 constexpr int TILE = 1, FEW = 2;
@@ -1327,38 +1436,58 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
     __shared__ float wml[W * 32];
     __shared__ int flag;
     _Float16* lds = reinterpret_cast<_Float16*>(smem);
-    const int tile_blocks = a.n_kv * a.tiles * a.tile_splits;
+    const int tile_blocks = a.n_kv * (a.tile_slots ? a.tile_slots : a.tiles * a.tile_splits);
     const bool tile = KIND == TILE || (KIND != FEW && (int)blockIdx.x < tile_blocks);
     int id = tile ? (int)blockIdx.x : (int)blockIdx.x - tile_blocks;
     const int kvh = id % a.n_kv;
     id /= a.n_kv;
-    const int most = tile ? a.tile_splits : a.few_splits;
-    const int z = id % most, slot = id / most;
-    const int b = tile ? sequence_of<TILE_PAIRS>(a, slot, a.group) : slot;
+    int z, slot, b, parts = 1;
+    if (KIND != FEW && tile && a.tile_slots) {
+        const TilePlan t = tile_plan(a, id);
+        b = t.b, z = t.z, slot = t.tile, parts = t.parts;
+    } else {
+        const int most = tile ? a.tile_splits : a.few_splits;
+        z = id % most, slot = id / most;
+        b = tile ? sequence_of<TILE_PAIRS>(a, slot, a.group) : slot;
+    }
     if (b < 0) return;
     const Seq s = sequence(a, b);
     if (s.pairs == 0 || (s.pairs > a.few_rows) != tile) return;
     const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
     if (tile) {
-        if constexpr (KIND & TILE) {
-            // the last rows, which see the most keys, first
-            const int p0 = (tiles_of<TILE_PAIRS>(s.pairs) - 1 - (slot - first_tile<TILE_PAIRS>(s.row0, a.group, b))) * TILE_PAIRS;
-            const int splits = tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, lds, meta, exps);
-            // (the keys' LDS is free: join's first barrier comes after every wave's last read of it)
-            if (splits > 1)
-                join<NT, TILE_PAIRS>(a, s, kvh, p0, min(TILE_PAIRS, s.pairs - p0), splits, a.counters + slot * a.n_kv + kvh,
-                                     reinterpret_cast<float*>(smem), &flag);
+        if constexpr ((KIND & TILE) != 0) {
+            int p0;
+            if (a.tile_slots) p0 = (tiles_of<TILE_PAIRS>(s.pairs) - 1 - slot) * TILE_PAIRS;
+            else p0 = tile_start(a, s, b, slot), parts = parts_of(a, s.t, a.tile_span);
+            tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, parts, lds, meta, exps);
         }
     } else {
         if constexpr ((KIND & FEW) != 0)
             for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once (and then not split) only where max_rows was too small
                 const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml, exps);
-                if (splits > 1)
-                    join<NT, FEW_PAIRS>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits,
-                                        a.counters + (a.tiles + slot) * a.n_kv + kvh, reinterpret_cast<float*>(smem), &flag);
+                if (splits > 1 && last_to_arrive(splits, a.counters + slot * a.n_kv + kvh, &flag))
+                    join<true>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem));
                 __syncthreads();  // before the next rows take the LDS
             }
     }
+}
+
+// The tiles' splits, FEW_PAIRS pairs a workgroup, in a launch behind theirs: the
+// last split to arrive would read a tile's partials (65 KB each) alone.
+__global__ __launch_bounds__(JOIN_THREADS) void join_kernel(BatchArgs a) {
+    constexpr int PER = TILE_PAIRS / FEW_PAIRS;
+    __shared__ float wt[JOIN_FLOATS];
+    int id = (int)blockIdx.x;
+    const int kvh = id % a.n_kv;
+    id /= a.n_kv;
+    const int slot = id / PER, b = sequence_of<TILE_PAIRS>(a, slot, a.group);
+    if (b < 0) return;
+    const Seq s = sequence(a, b);
+    if (s.pairs <= a.few_rows) return;
+    const int p0 = tile_start(a, s, b, slot), first = p0 + id % PER * FEW_PAIRS;
+    if (first >= s.pairs) return;
+    const TileSplit ts = tile_split(a, s, p0, planned_parts(a, s, b));
+    if (ts.splits > 1) join<false>(a, s, kvh, first, min(FEW_PAIRS, s.pairs - first), ts.splits, wt);
 }
 
 // ---- f32 rows as f16 parts, once a launch ---------------------------------------------
@@ -1434,8 +1563,12 @@ hipError_t launch(const BatchArgs& a, hipStream_t s) {
     const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD, KIND>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
-    const unsigned blocks = (unsigned)(a.n_kv * (a.tiles * a.tile_splits + (KIND & FEW ? a.n_seq * a.few_splits : 0)));
+    const int tile_blocks = a.tile_slots ? a.tile_slots : a.tiles * a.tile_splits;
+    const unsigned blocks = (unsigned)(a.n_kv * (tile_blocks + (KIND & FEW ? a.n_seq * a.few_splits : 0)));
+    static_assert(G::W * 64 == JOIN_THREADS && JOIN_FLOATS * 4 <= G::FEW_LDS, "few rows join with what they have");
     hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(G::W * 64), lds, s, a);
+    if (KIND != FEW && a.tile_splits > 1)
+        hipLaunchKernelGGL(join_kernel, dim3((unsigned)(a.n_kv * a.tiles * (TILE_PAIRS / FEW_PAIRS))), dim3(JOIN_THREADS), 0, s, a);
     return hipGetLastError();
 }
 template <typename KV, int HD>
@@ -1455,9 +1588,6 @@ hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
          : a.hd <= 128 ? launch_kind<KV, 128>(a, s) : launch_kind<KV, 256>(a, s);
 }
 
-// Key ranges are split until the launch has about this many workgroups.
-constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512;
-constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 256;
 constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
 // f32 prompts are split beforehand from this many tiles a sequence on, as far
 // as this much memory holds them.
@@ -1479,23 +1609,29 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && (a.n_seq == 1 || !a.kv.tables);
     a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
     a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
+    const int64_t most_parts =
+        std::max<int64_t>(1, (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float))));
     auto split = [&](int64_t base, int64_t target, int most, int unit, int64_t min_span, int* span, int* splits) {
         int64_t sp = std::max(min_span, keys * base / target);
         sp = (sp + unit - 1) / unit * unit;
         int64_t n = (keys + sp - 1) / sp;
-        const int64_t cap = (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float)));
-        if (n > cap) n = std::max<int64_t>(1, cap);
-        n = std::min<int64_t>(n, most);
+        n = std::min<int64_t>({n, most_parts, most});
         sp = ((keys + n - 1) / n + unit - 1) / unit * unit;
         *splits = (int)n;
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
     };
     if (only_tile) a.few_span = INT32_MAX / 2, a.few_splits = 1;
-    else split(pairs, FEW_TARGET, JOIN_SPLITS<256, FEW_PAIRS>, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
+    else split(pairs, FEW_TARGET, JOIN_SPLITS, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
     if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
-    else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, JOIN_SPLITS<256, TILE_PAIRS>, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
+    else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, JOIN_SPLITS, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
+    if (a.tile_splits > 1 && a.n_seq > 1 && a.n_seq <= 64) {
+        a.tile_slots = std::max(a.tiles, (int)((a.few_rows ? MIXED_TARGET : TILE_TARGET) / a.n_kv));
+        a.tile_splits = (int)std::min<int64_t>({(keys + TILE_MIN_SPAN - 1) / TILE_MIN_SPAN, most_parts, JOIN_SPLITS,
+                                                std::max(2 * a.tile_splits, a.few_splits)});
+    }
     a.part_splits = std::max(a.few_splits, a.tile_splits);
-    if (((int64_t)a.tiles * a.tile_splits + (int64_t)a.n_seq * a.few_splits) * a.n_kv > (int64_t)1 << 30)
+    if (((int64_t)a.tiles * std::max(a.tile_splits, TILE_PAIRS / FEW_PAIRS) + (int64_t)a.n_seq * a.few_splits) * a.n_kv >
+        (int64_t)1 << 30)
         return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows", a.n_seq, (long long)m);
     // f32 prompts whose keys several tiles read: split once
     const int hdp = a.hd <= 64 ? 64 : a.hd <= 128 ? 128 : 256, tk = a.hd <= 64 ? 64 : 32;  // Geo<Split, HD>
@@ -1508,7 +1644,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     CallScratch work;
     if (part_bytes || pre) {
         const rdl_status st = call_scratch(s, part_room + (pre ? image_bytes + note_bytes : 0),
-                                           part_bytes ? ((size_t)a.tiles + (a.few_rows ? a.n_seq : 0)) * a.n_kv : 0, &work);
+                                           part_bytes && a.few_rows ? (size_t)a.n_seq * a.n_kv : 0, &work);
         if (st != RDL_OK) return st;
         a.part = reinterpret_cast<float*>(work.p);
         a.part_ml = a.part + (size_t)m * a.n_heads * a.part_splits * a.hd;
