@@ -615,9 +615,9 @@ __device__ __forceinline__ int last_key(const BatchArgs& a, const Seq& s, int p)
 
 // ---- joining split key ranges ---------------------------------------------------------
 // A split's partial result: each pair's normalised outputs (part) with their
-// maximum and sum (part_ml).  Publication as attention.hpp describes it:
-// agent-coherent stores, each wave waits for its own, a barrier, then the
-// counter; the last split to arrive joins all of them in order (so results
+// maximum and sum (part_ml).  Tiles' are joined by join_kernel.  Few rows' are published
+// as attention.hpp describes it: agent-coherent stores, each wave waits for its own, a
+// barrier, then the counter; the last split to arrive joins all of them in order (so results
 // do not depend on which it is) and leaves the counter at zero.  A counter belongs
 // to the workgroups of one slot of the launch, not to rows: whatever
 // row_start holds, they agree on how many they are.
@@ -871,8 +871,13 @@ __device__ __forceinline__ int tile_start(const BatchArgs& a, const Seq& s, int 
 // the softmax needs one exchange with lane ^ 32, and its weights are already
 // the second product's B operand once the keys of a 16-key step are taken in
 // the order 4h .. 4h + 3, 8 + 4h .. (h = lane / 32), in which the transposed LDS reads of V
-// fetch them.
-// Returns the splits to join (1: the output is written, 0: no such split).
+// fetch them.  q and the weights are f16 pairs, so each product takes two
+// instructions (three with f32 keys and values); the matrix cores bound it: 2048 rows
+// over 16048 f16 keys (32 / 8 heads of 128) take 872 us, 1157 TFLOP/s of
+// those instructions where a large f16 library product reaches 1191.  32 pairs a wave
+// and 4 waves a workgroup: 64 pairs a wave left one wave a SIMD and took
+// twice the time, 8 waves a workgroup and wave priorities gave nothing.  f16
+// keys go straight to LDS (DirectSlab), two tiles deep, one barrier a tile.
 template <typename KV, int HD>
 __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
                                          int p0, int z, int parts, _Float16* lds, Meta* meta, int2* exps) {
@@ -1161,7 +1166,11 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
 // of its own without a barrier, with the next keys' loads in flight; at
 // the end they join through LDS.  The products as above, 16 columns wide
 // (v_mfma_f32_16x16x32_f16): a lane has the scores of keys 4g .. 4g + 3 and 16 +
-// 4g .. (g = lane / 16) of one pair.
+// 4g .. (g = lane / 16) of one pair.  HBM bounds it: 48 rows over 187420 keys of
+// 8 KV heads of 128 in f16, 769 MB, take 158 us, 4.9 TB/s (a large copy reaches
+// 4.7); a single row over 778 keys takes 11.3 us, which is latency: lengths,
+// page numbers, keys, then the splits' partials one behind the other.
+// Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
 __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
                                         _Float16* lds, float* wml, int2* exps) {
@@ -1376,12 +1385,11 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     return splits;
 }
 
-// The splits of a step of up to 64 sequences, a lane each: the shortest span of
-// keys, in steps of 64, by which all tiles' splits find room in a.tile_slots
-// workgroups a KV head (one a tile does: there are as many), so that all start at once, numbered
-// without gaps.  Numbered over the most splits that any tile might have, every
-// fourth workgroup or so had nothing to do, and with them a quarter of the CUs:
-// workgroups are dealt to the parts of an XCD in turn.
+// The splits of a step of up to 64 sequences, a lane each.  The span of keys is the
+// shortest, in steps of 64, by which all tiles' splits find room in a.tile_slots
+// workgroups a KV head (one a tile does: there are as many), so that all start at
+// once; by the longest kv_len alone, sequences of unlike lengths got
+// fewer and longer ones.
 __device__ __forceinline__ int shortest_span(const BatchArgs& a, int tiles, int keys) {
     int lo = TILE_MIN_SPAN / 64, hi = max(lo, ((int)wave_max_u32((uint32_t)keys) + 63) / 64);
     for (int mid = lo; lo < hi; mid = (lo + hi) / 2) {
@@ -1390,6 +1398,10 @@ __device__ __forceinline__ int shortest_span(const BatchArgs& a, int tiles, int 
     }
     return 64 * hi;
 }
+// The workgroups are numbered without gaps.  Numbered over the most splits that any
+// tile might have, every fourth or so had nothing to do, and with them a quarter of the
+// CUs: workgroups are dealt to the parts of an XCD in turn (132 us instead of
+// 100 for chunks and single rows of 16 sequences).
 struct TilePlan {
     int b, tile, z, parts;  // of number `slot`; b -1: none
 };
@@ -1473,7 +1485,8 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
 }
 
 // The tiles' splits, FEW_PAIRS pairs a workgroup, in a launch behind theirs: the
-// last split to arrive would read a tile's partials (65 KB each) alone.
+// last split to arrive would read a tile's partials (65 KB each) alone: 100 rows
+// over 3300 keys took 64.9 us so, and take 31.7.
 __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(BatchArgs a) {
     constexpr int PER = TILE_PAIRS / FEW_PAIRS;
     __shared__ float wt[JOIN_FLOATS];
@@ -1494,7 +1507,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(BatchArgs a) {
 // Where many tiles of rows read the same f32 keys, splitting them in every
 // tile (5 operations a value) cost more than the products' own work on them:
 // here a workgroup splits one tile of TK keys of a KV head and writes it as LDS will
-// hold it.
+// hold it.  It moves 8 + 8 bytes an element: 9910 rows of 8 KV heads of 128 take 32 us of
+// the call's 607, the products 1070 TFLOP/s.
 template <int HD>
 __global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* images, int4* notes, int2* exps) {
     using G = Geo<Split, HD>;
@@ -1590,7 +1604,9 @@ hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
 
 constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
 // f32 prompts are split beforehand from this many tiles a sequence on, as far
-// as this much memory holds them.
+// as this much memory holds them.  Prompts of 1, 2, 4, 8, 16, 32 tiles (us), split
+// beforehand: 13.4, 15.0, 19.6, 24.9, 33.6, 58.3; in every tile: 11.3, 14.3,
+// 20.2, 26.2, 36.3, 69.8 (32 / 8 heads of 128).
 constexpr int64_t SPLIT_MIN_TILES = 4;
 constexpr size_t SPLIT_BYTES = (size_t)1 << 30;
 
