@@ -46,7 +46,8 @@ enum {
 /* A layer's paged K and V memory.  Element d of position o of page pg and KV
  * head h is at pg * page_stride + h * head_stride + o * position_stride + d of
  * k_dev and of v_dev (strides in elements; multiples of 16 bytes, as both
- * bases; position_stride below 2^24; the heads and positions of a page and the pages must not overlap).
+ * bases; position_stride below 2^24; the heads and positions of a page and the
+ * pages must not overlap).
  * The decoder's own pools are [n_pages][n_kv_heads][page_positions][head_dim]. */
 typedef struct rdl_kv_pool {
     void* k_dev;

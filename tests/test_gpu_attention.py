@@ -623,6 +623,46 @@ def test_packed_rows_before_the_first_and_bad_starts(rq, gpu):
     close(out[3:], *ref.attention(q[3:], k[3:], v[3:], 0, 0.1))
 
 
+def chunks_and_tokens(n_seq):
+    """Chunks of 2 to 140 rows and single tokens behind caches of very different lengths."""
+    r = random.Random(n_seq)
+    return [(r.choice([0, 3, 700, 1900]) + r.randrange(60), r.choice([1, 1, 2, 20, 33, 140])) for _ in range(n_seq)]
+
+
+@pytest.mark.parametrize("n_seq,heads,kvh,hd", [(2, 32, 8, 128), (5, 8, 1, 64), (16, 14, 2, 96), (3, 4, 2, 256),
+                                                (64, 2, 1, 64), (70, 2, 1, 64)])
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_chunks_whose_keys_are_split(rq, gpu, n_seq, heads, kvh, hd, kv):
+    """Up to 64 sequences share the splits out on the device; more take the launch's own span."""
+    b = Batch(chunks_and_tokens(n_seq), heads, kvh, hd, kv=kv, pad=3)
+    b.check()
+    for hints in ((0, 0), (2, 300), (100000, 1 << 20)):
+        out = b.run(*hints)
+        close(out[:b.rows], *b.want())
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+def test_split_chunks_captured(rq, gpu, kv):
+    b = Batch([(2500, 90), (30, 1), (900, 200), (1400, 1)], 8, 2, 64, kv=kv)
+    out = torch.full((b.rows, 8, 64), -7.0, device="cuda")
+    b.run(out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.run(out=out)
+    starts, lens = b.row_start.clone(), b.kv_len.clone()
+    for drop in (0, 500, 0, 1300):  # fewer keys of each cache, other splits
+        b.kv_len.copy_((lens - drop).clamp(min=0))
+        b.q.normal_()
+        out.fill_(-7.0)
+        g.replay()
+        got = out.clone()
+        torch.randn(1000, device="cuda").sum().item()
+        assert torch.equal(b.run(), got)
+        if drop == 0:
+            close(got, *b.want())
+    assert torch.equal(b.row_start, starts)
+
+
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 def test_sequences_that_share_rows_leave_later_calls_alone(rq, gpu, kv):
     """Split key ranges are joined by counters that the launches of a stream share."""
