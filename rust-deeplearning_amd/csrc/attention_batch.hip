@@ -415,9 +415,11 @@ struct Slab {
 // l; an offset past the buffer writes zeros).  In asm, because the compiler
 // makes every LDS read wait for all such loads that it knows of, the next
 // tile's among them; they have no output register, and loads_done() stands
-// before the barrier that precedes the reads.
+// before the barrier that precedes the reads.  The compiler does not look into asm for the
+// 5 wait states between a v_readfirstlane, which forms the buffer's words, and a
+// load that reads them either: the block brings them (check_lds_loads.py looks).
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
                  : "memory");
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
