@@ -6,13 +6,15 @@ descriptor the compiler forms with v_readfirstlane.  gfx950 needs 5 wait states
 between a vector instruction that writes a scalar register and a
 vector-memory instruction that reads it, and one between the write of M0 and
 the load; the compiler keeps those distances for its own instructions only, so
-the asm block has to bring them.
+the asm block has to bring them.  And M0 is the block's: what the compiler
+holds there is lost.
 
 This script reads the device assembly (`hipcc -S --offload-device-only`, inline
 asm between `;;#ASMSTART` / `;;#ASMEND` markers) and checks of every inline-asm
-load to LDS that its own block writes M0 before it and gives 5 wait states in
-front of it (an instruction is one, `s_nop N` N + 1).  It exits non-zero,
-naming the function, where one does not hold.
+load to LDS that its own block writes M0 before it and gives 5 wait states in front
+of it (an instruction is one, `s_nop N` N + 1), and of every function that
+nothing outside the blocks reads M0 behind one without writing it first.  It
+exits non-zero, naming the function, where one does not hold.
 
 Usage: python check_lds_loads.py build/attention_batch.s
 """
@@ -25,12 +27,14 @@ WAIT_STATES = 5
 LDS_LOAD = re.compile(r"^buffer_load\w*\s.*\blds\b")
 NOP = re.compile(r"^s_nop\s+(0x[0-9a-fA-F]+|\d+)$")
 M0_WRITE = re.compile(r"^\w+\s+m0\b")
+M0 = re.compile(r"\bm0\b")
 
 
 def check_function(name, body):
     """Problems found in one function, and the number of loads checked."""
     problems, checked = [], 0
     in_asm = False
+    foreign = False  # M0 holds what an asm block wrote
     states = 0       # wait states since the block's start
     wrote = False    # the block has written M0
     for s in body:
@@ -44,6 +48,10 @@ def check_function(name, body):
         if not s or s.startswith(".") or s.endswith(":"):
             continue
         if not in_asm:
+            if M0_WRITE.match(s):
+                foreign = bool(foreign and M0.search(s.split(",", 1)[-1]))
+            if foreign and M0.search(s):
+                problems.append(f"{name}: M0 read behind an asm block that wrote it: {s}")
             continue
         if LDS_LOAD.match(s):
             checked += 1
@@ -52,7 +60,7 @@ def check_function(name, body):
             if states < WAIT_STATES:
                 problems.append(f"{name}: {states} wait states before a load to LDS, {WAIT_STATES} needed")
         if M0_WRITE.match(s):
-            wrote = True
+            wrote = foreign = True
         m = NOP.match(s)
         states += int(m.group(1), 0) + 1 if m else 1
     return problems, checked

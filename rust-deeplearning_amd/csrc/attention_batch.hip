@@ -418,10 +418,15 @@ struct Slab {
 // before the barrier that precedes the reads.  The compiler does not look into asm for the
 // 5 wait states between a v_readfirstlane, which forms the buffer's words, and a
 // load that reads them either: the block brings them (check_lds_loads.py looks).
+// M0 is named as written, so that the compiler sets it anew where it needs it (it warns that it
+// would not keep a value there over the block; it has none).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ i32x4 uniform_rsrc(const void* base, int bytes) {
     const uint64_t b = (uint64_t)base;

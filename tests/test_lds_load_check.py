@@ -1,7 +1,9 @@
 """The build check of the inline-asm loads to LDS
 (rust-deeplearning_amd/check_lds_loads.py): it passes on the compiled kernels
 and fails on planted mistakes in small assembly fragments."""
+import glob
 import os
+import re
 import sys
 
 import pytest
@@ -47,3 +49,22 @@ def test_a_load_without_its_address_fails():
 
 def test_other_loads_are_not_checked():
     assert cl.check(fn("global_load_dwordx4 v[4:7], v[2:3], off")) == ([], 0)
+
+
+def test_m0_read_behind_a_block_fails():
+    asm = ["s_mov_b32 m0, s4", "s_nop 3", LOAD]
+    problems, _ = cl.check(fn(*asm, before=["s_mov_b32 m0, s9"], after=["v_movrels_b32 v1, v2, m0"]))
+    assert problems and "M0 read" in problems[0]
+    assert cl.check(fn(*asm, after=["s_mov_b32 m0, s9", "s_add_u32 s1, m0, s2"])) == ([], 1)
+    assert cl.check(fn(*asm, after=["s_add_u32 m0, m0, s2"]))[0]
+
+
+def test_blocks_that_write_m0_say_so():
+    # the compiler may keep a value there over a block that does not name it
+    blocks = []
+    for path in glob.glob(os.path.join(PKG, "csrc", "*.h*")):
+        blocks += re.findall(r"\basm\b[^;]*?\)\s*;", open(path).read())
+    writers = [b for b in blocks if re.search(r"\bm0\s*,", b)]
+    assert len(blocks) > 5 and writers
+    for b in writers:
+        assert '"m0"' in b.rsplit(":", 1)[1], b
