@@ -85,9 +85,9 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
     *hi = __builtin_bit_cast(uint32_t, h);
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
 }
-// x 2^e, the factor from a product of scaled parts to a power of 2.  Not
-// below 2^-126, where it stands for scores of nothing in any case: masked
-// scores are -infinity before it.
+// x 2^e, the factor from a product of scaled parts (below 2^39) to a power of 2, e
+// the exponents of both factors together.  Not below 2^-126, where it stands for scores
+// of nothing in any case: masked scores are -infinity before it.
 __device__ __forceinline__ float score_factor(float x, int e) {
     return fmaxf(__builtin_amdgcn_ldexpf(x, e), 0x1p-126f);
 }
@@ -962,7 +962,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
-    const float cs = score_factor(a.scale * LOG2E, qe);
+    const float cs = a.scale * LOG2E, f16_factor = score_factor(cs, qe);  // (f32 keys have exponents too)
     int buf = 0;
     for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
         const int at = buf * TK * G::KEY;  // elements
@@ -996,12 +996,12 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
         [[maybe_unused]] const Meta* notes = meta + buf * W;
         const bool masked = j0 + TK - 1 > w_first || __builtin_amdgcn_ballot_w64(!note.valid);
         wide |= __builtin_amdgcn_ballot_w64(note.flags & SLAB_WIDE) != 0;
-        float f = cs;
+        float f = f16_factor;
         bool other_k = false, other_v = false;  // f32: keys held with other exponents than the rest
         if constexpr (TWO) {
             kref = lanes_max<W>(note.ke);
             vref = lanes_max<W>(note.ve);
-            f = score_factor(cs, kref);
+            f = score_factor(cs, qe + kref);
             other_k = __builtin_amdgcn_ballot_w64((note.ke != kref && note.ke != NO_EXPONENT) || (note.flags & SLAB_OTHER_K));
             other_v = __builtin_amdgcn_ballot_w64((note.ve != vref && note.ve != NO_EXPONENT) || (note.flags & SLAB_OTHER_V));
         }
@@ -1227,7 +1227,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
-        const float cs = score_factor(a.scale * LOG2E, qe);
+        const float cs = a.scale * LOG2E, f16_factor = score_factor(cs, qe);  // (f32 keys have exponents too)
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
             const Meta mt = slab.store(ks, vs, exps + FK * w, 0, PART, valid, j0 + FK - 1 > first, NO_EXPONENT, NO_EXPONENT);
             if (j0 + step < j_hi) {
@@ -1272,7 +1272,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) mx = fmaxf(mx, sc[b][t]);
-            const float f = F32 ? score_factor(cs, mt.ke) : cs;
+            const float f = F32 ? score_factor(cs, qe + mt.ke) : f16_factor;
             mx *= f;
             mx = fmaxf(mx, other16(mx));
             mx = max32(mx);

@@ -818,3 +818,26 @@ def test_two_streams_at_once(rq, gpu):
         assert all(torch.equal(o, w) for o in outs[i])
     for s in streams:
         rq.release_stream_work(s.cuda_stream)
+
+
+# ---- sizes at the ends of f32 --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("power", [-118, -112, -60, 60, 112, 118])
+def test_f32_queries_and_keys_of_opposite_extremes(rq, gpu, power):
+    """Queries by 2^-power and keys by 2^power: ordinary scores, in every kernel that takes f32 keys."""
+    def sized(x):  # every element keeps its 24 bits at 2^-118
+        return x.sign() * x.abs().clamp(0.01, 4.0)
+
+    for lens in ([(300, 1), (40, 1), (0, 1), (2500, 1)], [(130, 90), (0, 40), (1500, 33)]):
+        b = Batch(lens, 4, 2, 64, "f32")
+        b.q = sized(b.q) * 2.0**-power
+        b.kv = [(sized(k) * 2.0**power, v) for k, v in b.kv]
+        for t, (k, v) in zip(b.table, b.kv):
+            b.pool.put(t, k, v)
+        b.check()
+    for n in (3, 40, 1500):
+        torch.manual_seed(n)
+        q, k, v = torch.randn(3, n, 4, 64, device="cuda")
+        q, k = sized(q) * 2.0**-power, sized(k) * 2.0**power
+        close(run_packed(q, k, v, ints([0, n]), 0.125), *ref.attention(q, k, v, 0, 0.125))
