@@ -85,11 +85,23 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
     *hi = __builtin_bit_cast(uint32_t, h);
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
 }
-// x 2^e, the factor from a product of scaled parts (below 2^39) to a power of 2, e
+// scale 2^e, the factor from a product of scaled parts (below 2^39) to a power of 2, e
 // the exponents of both factors together.  Not below 2^-126, where it stands for scores
 // of nothing in any case: masked scores are -infinity before it.
-__device__ __forceinline__ float score_factor(float x, int e) {
-    return fmaxf(__builtin_amdgcn_ldexpf(x, e), 0x1p-126f);
+__device__ __forceinline__ float score_factor(float scale, int e) {
+    return fmaxf(__builtin_amdgcn_ldexpf(scale, e) * LOG2E, 0x1p-126f);
+}
+// And not above 2^FACTOR_MAX or so: past f32's range it would make NaN of a score
+// of 0, which queries and keys have however large they are.  f16 keys: a
+// row's products are whole steps of 2^-48, so from there on any two that differ are 2^40
+// apart, before a cap as behind it.  f32 keys: what is cut off the exponent, `lift`, comes on the
+// products first, as their rows' own exponents do.
+constexpr int FACTOR_MAX = 88;
+__device__ __forceinline__ float f16_factor(float scale, int e) {
+    return fminf(score_factor(scale, e), __builtin_bit_cast(float, (uint32_t)(FACTOR_MAX + 127) << 23));
+}
+__device__ __forceinline__ int lift_of(float scale, int e) {
+    return max(0, e + (int)(__builtin_bit_cast(uint32_t, scale) >> 23) - 127 - FACTOR_MAX);
 }
 __device__ __forceinline__ float weight(float s, float f, float off) { return __builtin_amdgcn_exp2f(fmaf(s, f, off)); }
 __device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
@@ -962,7 +974,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
-    const float cs = a.scale * LOG2E, f16_factor = score_factor(cs, qe);  // (f32 keys have exponents too)
+    [[maybe_unused]] const float f16_f = f16_factor(a.scale, qe);  // (f32 keys have exponents too)
     int buf = 0;
     for (int j0 = j_lo; j0 < j_hi; j0 += TK, buf ^= 1) {
         const int at = buf * TK * G::KEY;  // elements
@@ -996,13 +1008,15 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
         [[maybe_unused]] const Meta* notes = meta + buf * W;
         const bool masked = j0 + TK - 1 > w_first || __builtin_amdgcn_ballot_w64(!note.valid);
         wide |= __builtin_amdgcn_ballot_w64(note.flags & SLAB_WIDE) != 0;
-        float f = f16_factor;
+        float f = f16_f;
+        [[maybe_unused]] int lift = 0;
         bool other_k = false, other_v = false;  // f32: keys held with other exponents than the rest
         if constexpr (TWO) {
             kref = lanes_max<W>(note.ke);
             vref = lanes_max<W>(note.ve);
-            f = score_factor(cs, qe + kref);
-            other_k = __builtin_amdgcn_ballot_w64((note.ke != kref && note.ke != NO_EXPONENT) || (note.flags & SLAB_OTHER_K));
+            lift = lift_of(a.scale, qe + kref);
+            f = score_factor(a.scale, qe + kref - lift);
+            other_k = __builtin_amdgcn_ballot_w64((note.ke != kref && note.ke != NO_EXPONENT) || (note.flags & SLAB_OTHER_K) || lift);
             other_v = __builtin_amdgcn_ballot_w64((note.ve != vref && note.ve != NO_EXPONENT) || (note.flags & SLAB_OTHER_V));
         }
 #pragma unroll
@@ -1031,7 +1045,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
 #pragma unroll
                     for (int e = 0; e < 16; e++)
                         sc[b][e] = __builtin_amdgcn_ldexpf(
-                            sc[b][e], key_exps[32 * (b0 + b) + 8 * (e >> 2) + 4 * h + (e & 3)].x - kref);
+                            sc[b][e], key_exps[32 * (b0 + b) + 8 * (e >> 2) + 4 * h + (e & 3)].x - kref + lift);
             if (masked)
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
@@ -1227,7 +1241,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
-        const float cs = a.scale * LOG2E, f16_factor = score_factor(cs, qe);  // (f32 keys have exponents too)
+        [[maybe_unused]] const float f16_f = f16_factor(a.scale, qe);  // (f32 keys have exponents too)
         for (int j0 = j_w; j0 < j_hi; j0 += step) {
             const Meta mt = slab.store(ks, vs, exps + FK * w, 0, PART, valid, j0 + FK - 1 > first, NO_EXPONENT, NO_EXPONENT);
             if (j0 + step < j_hi) {
@@ -1254,12 +1268,13 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                     }
                 }
             }
-            if (F32 && (mt.flags & SLAB_OTHER_K))
+            [[maybe_unused]] const int lift = F32 ? lift_of(a.scale, qe + mt.ke) : 0;
+            if (F32 && ((mt.flags & SLAB_OTHER_K) || __builtin_amdgcn_ballot_w64(lift != 0)))
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int t = 0; t < 4; t++)
-                        sc[b][t] = __builtin_amdgcn_ldexpf(sc[b][t], exps[FK * w + 16 * b + 4 * g + t].x - mt.ke);
+                        sc[b][t] = __builtin_amdgcn_ldexpf(sc[b][t], exps[FK * w + 16 * b + 4 * g + t].x - mt.ke + lift);
             if (masked) {
                 const int rel = last - j0 - 4 * g;
 #pragma unroll
@@ -1272,7 +1287,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) mx = fmaxf(mx, sc[b][t]);
-            const float f = F32 ? score_factor(cs, qe + mt.ke) : f16_factor;
+            const float f = F32 ? score_factor(a.scale, qe + mt.ke - lift) : f16_f;
             mx *= f;
             mx = fmaxf(mx, other16(mx));
             mx = max32(mx);

@@ -841,3 +841,52 @@ def test_f32_queries_and_keys_of_opposite_extremes(rq, gpu, power):
         q, k, v = torch.randn(3, n, 4, 64, device="cuda")
         q, k = sized(q) * 2.0**-power, sized(k) * 2.0**power
         close(run_packed(q, k, v, ints([0, n]), 0.125), *ref.attention(q, k, v, 0, 0.125))
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("n", [1, 3, 40, 1500])
+def test_large_queries_and_keys_without_a_product(rq, gpu, kv, n):
+    """Queries and keys that share no dimension: scores of 0 whatever their sizes, the average of the values seen."""
+    torch.manual_seed(n)
+    q, k, v = torch.randn(3, n, 4, 64, device="cuda")
+    q[..., 32:], k[..., :32] = 0.0, 0.0
+    q, scale = q * 2.0**100, 2.0**60
+    k = k.half() if kv == "f16" else k * 2.0**110
+    v = v.to(k.dtype)
+    want = v.double().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]
+    # the weights are equal and exact; values of 22 bits, n f32 sums, a division, a product
+    bound = (v.double().abs().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]) * (n + 16) * 2.0**-23
+    out = run_packed(q, k, v, ints([0, n]), scale)
+    assert ((out.double() - want).abs() <= bound).all()
+    b = Batch([(n - 1, 1), (5, 0), (0, n)], 4, 4, 64, kv)  # the same over pages
+    for i in (0, 2):
+        b.pool.put(b.table[i], k, v)
+    b.q, b.scale = torch.cat([q[-1:], q]), scale
+    out = b.run().double()
+    assert ((out[0] - want[-1]).abs() <= bound[-1]).all() and ((out[1:] - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [3, 40, 1500])
+def test_scores_near_the_end_of_f32(rq, gpu, n):
+    """Scores about 2^119 beside parts whose product would pass f32: the keys of the largest score share the weight."""
+    torch.manual_seed(n)
+    q, k = torch.zeros(2, n, 2, 64, device="cuda")
+    v = torch.randn(n, 2, 64, device="cuda")
+    q[..., 0], k[..., 2] = 2.0**100, 2.0**80
+    q[..., 1] = 2.0**70
+    size = torch.tensor([1.0, 2.0, 4.0], device="cuda")[torch.randint(0, 3, (n,), device="cuda")]
+    k[..., 1] = 2.0**50 * size[:, None]
+    out = run_packed(q, k, v, ints([0, n]), 0.125).double()
+    b = Batch([(0, n), (n - 1, 1)], 2, 2, 64, "f32")
+    for t in b.table:
+        b.pool.put(t, k, v)
+    b.q = torch.cat([q, q[-1:]])
+    b.scale = 0.125
+    paged = b.run().double()
+    top = size[None] == size.cummax(0).values[:, None]
+    w = torch.where(torch.ones(n, n, device="cuda").tril() > 0, top, False).double()
+    w /= w.sum(1, keepdim=True)
+    want = (w @ v.double().view(n, 128)).view(n, 2, 64)
+    bound = (w @ v.double().abs().view(n, 128)).view(n, 2, 64) * (n + 16) * 2.0**-23
+    assert ((out - want).abs() <= bound).all()
+    assert ((paged[:n] - want).abs() <= bound).all() and ((paged[n] - want[-1]).abs() <= bound[-1]).all()
