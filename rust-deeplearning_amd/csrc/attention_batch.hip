@@ -801,7 +801,8 @@ struct Power {
 // would push its own below f16's smallest step.)  A weight's step of 2^-24 times a
 // value's 2^15 is so 2^-28 of the largest weighted row's size at most, 2^HOLD
 // of it for rows held with a larger one's exponent.  L sums 2^(x - M + SHIFT).
-// Where all keys have one exponent E the two differ by a factor only.
+// Where all keys have one exponent E the two differ by a factor only, which goes into the
+// exponent's offset, but not beside a maximum past 2^8: it would be rounded away there.
 // N scores of a lane: get(i), put(i, weight); value(i): key i's exponent;
 // rescale(c): o *= c; reduce: the maximum over a pair's lanes; mx: the pair's largest x.
 template <int N, typename Get, typename Put, typename Value, typename Rescale, typename Reduce>
@@ -829,8 +830,9 @@ __device__ __forceinline__ void weigh_two(Get&& get, Put&& put, Value&& value, R
         ref = rn;
     }
     const float r = ref == -__builtin_inff() ? (float)E : ref;
-    if (!other && !__builtin_amdgcn_ballot_w64(r - (float)E > 60.0f)) {
-        const float off = SHIFT - Mu + ((float)E - r);
+    const float base = SHIFT - Mu, up = (float)E - r;
+    if (!other && !__builtin_amdgcn_ballot_w64(up < -60.0f || fabsf(Mu) > 256.0f)) {
+        const float off = base + up;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -838,13 +840,13 @@ __device__ __forceinline__ void weigh_two(Get&& get, Put&& put, Value&& value, R
             sum += w;
             put(i, w);
         }
-        L += sum * __builtin_amdgcn_exp2f(r - (float)E);
+        L += sum * __builtin_amdgcn_exp2f(-up);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float x = fmaf(get(i), f, SHIFT - Mu);
+            const float x = fmaf(get(i), f, base);
             L += __builtin_amdgcn_exp2f(x);
-            put(i, __builtin_amdgcn_exp2f(x + ((other ? (float)value(i) : (float)E) - r)));
+            put(i, __builtin_amdgcn_exp2f(x + (other ? (float)value(i) - r : up)));
         }
     }
 }

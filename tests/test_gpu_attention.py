@@ -890,3 +890,32 @@ def test_scores_near_the_end_of_f32(rq, gpu, n):
     bound = (w @ v.double().abs().view(n, 128)).view(n, 2, 64) * (n + 16) * 2.0**-23
     assert ((out - want).abs() <= bound).all()
     assert ((paged[:n] - want).abs() <= bound).all() and ((paged[n] - want[-1]).abs() <= bound[-1]).all()
+
+
+@pytest.mark.parametrize("power", [4, 11, 21, 26])
+@pytest.mark.parametrize("n", [40, 700, 1500])
+def test_equal_large_scores_weigh_alike(rq, gpu, n, power):
+    """Equal scores of about 2^power beside f32 values whose sizes fall from key to key: equal weights."""
+    torch.manual_seed(n)
+    q = torch.zeros(n, 2, 64, device="cuda")
+    k = torch.zeros(n, 2, 64, device="cuda")
+    q[..., 0] = 2.0 ** (power // 2)
+    k[..., 0] = 2.0 ** (power - power // 2) * 1.375
+    # a first key whose score lies below the others': the running maximum moves, and the outputs' unit with it
+    k[0, :, 0] -= (6 if power < 26 else 32) / 2.0 ** (power // 2)
+    v = torch.randn(n, 2, 64, device="cuda")
+    v = v.sign() * v.abs().clamp(0.5, 2.0)
+    v *= 2.0 ** -(torch.arange(n, device="cuda") * (24 / n)).floor()[:, None, None]
+    want, _ = ref.attention(q, k, v, 0, 1.0)
+    mean, _ = ref.attention(q, k, v.abs(), 0, 1.0)
+    # keys and scores are exact in 22 and in 24 bits and the largest is exact, so the weights are off by a rounding of
+    # the first key's exponent and of its exponential; values of 22 bits, n f32 sums, a division, a product
+    bound = mean * (n + 32) * 2.0**-23
+    out = run_packed(q, k, v, ints([0, n]), 1.0).double()
+    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+    b = Batch([(0, n), (n - 1, 1)], 2, 2, 64, "f32")
+    for t in b.table:
+        b.pool.put(t, k, v)
+    b.q, b.scale = torch.cat([q, q[-1:]]), 1.0
+    out = b.run().double()
+    assert ((out[:n] - want).abs() <= bound).all() and ((out[n] - want[-1]).abs() <= bound[-1]).all()
