@@ -127,8 +127,9 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * max_rows and max_kv tell the launch what to expect (the most rows of a
  * sequence, the longest kv_len; 0: unknown): results do not depend on them
  * beyond rounding, time does.  Products are formed on the matrix cores with
- * f32 sums from f16 pairs that carry 22 bits of q, of the weights and of f32
- * keys and values (f16 ones are exact); sums, maxima and exponents are f32.
+ * f32 sums from f16 pairs: with f16 keys and values, which are exact, they
+ * carry 22 bits of q and of the weights; with f32 ones 23 bits of those and of
+ * keys and values.  Sums, maxima and exponents are f32.
  * Of f32 values, elements far below the largest of their row or of the rows a
  * query weighs with it end at 2^-28 of that.
  * n_heads must be a multiple of the pool's n_kv_heads. */

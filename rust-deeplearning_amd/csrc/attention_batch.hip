@@ -65,7 +65,7 @@ __device__ __forceinline__ Pair pair_of(const BatchArgs& a, int p) {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef __fp16 hp2 __attribute__((ext_vector_type(2)));  // v_cvt_pkrtz's type
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -77,13 +77,20 @@ constexpr float LOG2E = 1.44269504088896340736f;
 // instead take the same time: M seldom moves after a sequence's first tiles.)
 constexpr float SHIFT = 11.0f, SLACK = 4.0f;
 
-// a * 2^e as two f16 parts of 11 bits each (rounded toward zero, so both have
-// a's sign and hi + lo is off by less than 2^-21 of it).
+// a as two f16 parts of 11 bits each.  NEAREST (with f32 keys and values): both are rounded
+// to nearest, hi is off by at most 2^-11 of a, and lo, by its own half step, leaves
+// 2^-23.  Else both are cut toward zero and leave less than 2^-21, which with f16
+// keys and values, exact as they are, is below what the f32 sums are off by; the instruction
+// that rounds takes longer (1 % of a long chunk, 1 to 2 % of f32 prompts and chunks).
+template <bool NEAREST>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-    const hp2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const float ra = fmaf((float)h[0], -1.0f, a), rb = fmaf((float)h[1], -1.0f, b);
+    auto two = [](float x, float y) {
+        if constexpr (NEAREST) return h2{(_Float16)x, (_Float16)y};  // v_cvt_pk_f16_f32
+        else return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    };
+    const h2 h = two(a, b);
     *hi = __builtin_bit_cast(uint32_t, h);
-    *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+    *lo = __builtin_bit_cast(uint32_t, two(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b)));
 }
 // scale 2^e, the factor from a product of scaled parts (below 2^39) to a power of 2, e
 // the exponents of both factors together.  Not below 2^-126, where it stands for scores
@@ -163,7 +170,7 @@ __device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u3
             const float a = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].z : x[p].x)), -e);
             const float b = __builtin_amdgcn_ldexpf(as_f32((int32_t)(c ? x[p].w : x[p].y)), -e);
             uint32_t h, l;
-            split2(a, b, &h, &l);
+            split2<true>(a, b, &h, &l);
             (*hi)[2 * p + c] = h;
             (*lo)[2 * p + c] = l;
         }
@@ -753,7 +760,7 @@ struct QRow {
         }
     }
 };
-template <int NS, typename R>
+template <bool NEAREST, int NS, typename R>
 __device__ __forceinline__ int split_q(const QRow<NS>& row, h8 (&hi)[NS], h8 (&lo)[NS], R&& reduce) {
     const f4 (&x)[NS][2] = row.x;
     uint32_t m = 0;
@@ -771,8 +778,8 @@ __device__ __forceinline__ int split_q(const QRow<NS>& row, h8 (&hi)[NS], h8 (&l
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             uint32_t a, b;
-            split2(__builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2], -e),
-                   __builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2 + 1], -e), &a, &b);
+            split2<NEAREST>(__builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2], -e),
+                            __builtin_amdgcn_ldexpf(x[i][c >> 1][(c & 1) * 2 + 1], -e), &a, &b);
             h[c] = a;
             l[c] = b;
         }
@@ -973,7 +980,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     q.load(q_at(a, s, kvh, p), live, 8 * h, 16, a.hd);
     if (j_lo < j_hi) fetch(j_lo, 0);
     h8 qh[KS], ql[KS];
-    const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
+    const int qe = split_q<TWO, KS>(q, qh, ql, [](uint32_t m) {
         return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
     });
     [[maybe_unused]] const float f16_f = f16_factor(a.scale, qe);  // (f32 keys have exponents too)
@@ -1099,7 +1106,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         uint32_t hi, lo;
-                        split2(sc[b][8 * k + 2 * u], sc[b][8 * k + 2 * u + 1], &hi, &lo);
+                        split2<TWO>(sc[b][8 * k + 2 * u], sc[b][8 * k + 2 * u + 1], &hi, &lo);
                         ph[u] = hi;
                         pl[u] = lo;
                     }
@@ -1239,7 +1246,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             slab.pages(a.kv, table, j_w + step, s.t);
         }
         h8 qh[KS], ql[KS];
-        const int qe = split_q<KS>(q, qh, ql, [](uint32_t m) {
+        const int qe = split_q<F32, KS>(q, qh, ql, [](uint32_t m) {
             m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
             return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
         });
@@ -1322,7 +1329,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             uint32_t ph[2 * NB], pl[2 * NB];
 #pragma unroll
             for (int u = 0; u < 2 * NB; u++)
-                split2(sc[u >> 1][(u & 1) * 2], sc[u >> 1][(u & 1) * 2 + 1], &ph[u], &pl[u]);
+                split2<F32>(sc[u >> 1][(u & 1) * 2], sc[u >> 1][(u & 1) * 2 + 1], &ph[u], &pl[u]);
             const char* vr = reinterpret_cast<const char*>(vs);
             if constexpr (NB == 2) {
                 const h8 p8 = __builtin_bit_cast(h8, ph), q8 = __builtin_bit_cast(h8, pl);

@@ -919,3 +919,27 @@ def test_equal_large_scores_weigh_alike(rq, gpu, n, power):
     b.q, b.scale = torch.cat([q, q[-1:]]), 1.0
     out = b.run().double()
     assert ((out[:n] - want).abs() <= bound).all() and ((out[n] - want[-1]).abs() <= bound[-1]).all()
+
+
+@pytest.mark.parametrize("n", [3, 40, 1500])
+def test_f32_parts_round_to_nearest(rq, gpu, n):
+    """A row that sees one key returns that key's values to 23 bits, and its errors have both signs."""
+    torch.manual_seed(n)
+    v = torch.randn(n, 4, 64, device="cuda")
+    v = v.sign() * v.abs().clamp(0.01, 4.0)  # nothing far below a row's largest
+    q, k = torch.zeros_like(v), torch.zeros_like(v)
+    i = torch.arange(n, device="cuda")[:, None] * 128.0
+    q[..., 0], q[..., 1], k[..., 0], k[..., 1] = 1.0, -i, i, 1.0  # a score of 0 for the row's own key, -128 and less before
+    outs = [run_packed(q, k, v, ints([0, n]), 1.0)]
+    b = Batch([(0, n), (n - 1, 1)], 4, 4, 64, "f32")
+    for t in b.table:
+        b.pool.put(t, k, v)
+    b.q, b.scale = torch.cat([q, q[-1:]]), 1.0
+    out = b.run()
+    outs += [out[:n], out[n:]]
+    for o, w in zip(outs, (v, v, v[-1:])):
+        # the weight is a power of two and the others' are below 2^-180: the value's parts (2^-23) and a sum of two products
+        err = (o.double() - w.double()) / w.double()
+        assert err.abs().max() <= 2.0**-23 + 2 * 2.0**-24, float(err.abs().max())
+        if o.numel() >= 512:  # truncation would keep all of them below zero
+            assert (err > 0).double().mean() >= 0.1 and (err < 0).double().mean() >= 0.1
