@@ -121,9 +121,10 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * multiple of 4; bases 16-byte aligned); out must not overlap q.
  * row_start ascends; where it does not, what the call's rows get is unspecified.
  * What a row does not see has no effect on it, NaN and infinities included.  Of
- * what it sees, a NaN in a key or in its query makes its outputs NaN, a value that is
- * not finite makes that element NaN or infinite whatever its weight, and infinite
- * keys or queries leave its outputs unspecified.
+ * what it sees, a NaN in a key or in its query makes its outputs NaN, values that are
+ * not finite make that element their sum whatever their weights (infinite, or NaN for
+ * a NaN or both infinities), and infinite keys or queries, or scores past f32's range,
+ * leave its outputs unspecified.
  * max_rows and max_kv tell the launch what to expect (the most rows of a
  * sequence, the longest kv_len; 0: unknown): results do not depend on them
  * beyond rounding, time does.  Products are formed on the matrix cores with

@@ -565,6 +565,35 @@ __device__ __forceinline__ f4 wide4(const KV* v, bool on) {
     return y;
 }
 
+// What is not finite is summed apart from the products, where an infinity times a weight
+// of 0 (its small part, or underflown) would be NaN in one tile and not in the next:
+// values of masked tiles are zeroed before the products; of the others' outputs, of which
+// `all` is 0 times their sum, those that are not finite begin again from 0, but not where the
+// sum of weights L is NaN itself; wide4 then brings the values.
+__device__ __forceinline__ bool not_finite_of_values(float all, float L) {
+    return __builtin_amdgcn_ballot_w64(all != 0.0f && L == L) != 0;
+}
+__device__ __forceinline__ float finite_or(float x, bool zero) {
+    return zero && abs_bits(x) >= 0x7F800000u ? 0.0f : x;
+}
+// Partial outputs likewise, joined by y = sum(w x): an infinite x keeps its place whatever its weight.  y tells
+// whether there was any; if so its element is the sum of those, which `partial` gives one by one.
+__device__ __forceinline__ bool some_not_finite(f4 y) { return !(fmaf(y[0], 0.0f, fmaf(y[1], 0.0f, fmaf(y[2], 0.0f, y[3] * 0.0f))) == 0.0f); }
+template <typename Partial>
+__device__ __forceinline__ f4 sum_not_finite(f4 y, int n, Partial&& partial) {
+    f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int z = 0; z < n; z++) {
+        const f4 u = partial(z);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (abs_bits(u[i]) >= 0x7F800000u) x[i] += u[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (abs_bits(y[i]) >= 0x7F800000u) y[i] = x[i];
+    return y;
+}
+
 // The rows of a sequence that a launch works on.
 struct Seq {
     int64_t row0;   // its first row
@@ -735,11 +764,13 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
                 if (z < splits) y += w[z] * f4{ahead[z][0][0], ahead[z][0][1], ahead[z][1][0], ahead[z][1][1]};
             z0 = min(JOIN_AHEAD, splits);
         }
-#pragma unroll 4
-        for (int z = z0; z < splits; z++) {
+        auto partial = [&](int z) {
             const f2 u = get2(o + z * a.hd), v = get2(o + z * a.hd + 2);
-            y += w[z] * f4{u[0], u[1], v[0], v[1]};
-        }
+            return f4{u[0], u[1], v[0], v[1]};
+        };
+#pragma unroll 4
+        for (int z = z0; z < splits; z++) y += w[z] * partial(z);
+        if (some_not_finite(y)) y = sum_not_finite(y, splits, partial);
         *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y * inv[pr];
     }
 }
@@ -1139,6 +1170,20 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
             const float x = o[d][e] * inv;
             o[d][e] = TWO ? unit.times(x) : x;
         }
+    if constexpr (!TWO) {
+        float all = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) all = fmaf(o[d][e], 0.0f, all);
+        if (not_finite_of_values(all, L)) {
+            wide = 1;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] = finite_or(o[d][e], L == L);
+        }
+    }
     if (wide)  // rows that see a value that is not finite
         for (int j = j_lo; j < min(j_hi, w_last + 1); j++) {
             const Elem* v = value_row<Elem>(a.kv, s.row0, table, kvh, j);
@@ -1367,6 +1412,20 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
                 const float x = o[d][e] * inv;
                 o[d][e] = F32 ? unit.times(x) : x;
             }
+        if constexpr (!F32) {
+            float all = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) all = fmaf(o[d][e], 0.0f, all);
+            if (not_finite_of_values(all, L)) {
+                wide = 1;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[d][e] = finite_or(o[d][e], L == L);
+            }
+        }
         if (wide)  // rows that see a value that is not finite
             for (int j0 = j_w; j0 < j_hi; j0 += step)
                 for (int j = j0; j < min(j0 + FK, j_hi); j++) {
@@ -1393,6 +1452,9 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
 #pragma unroll
         for (int x = 0; x < W; x++)
             if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
+        auto partial = [&](int x) {
+            return *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * FK * G::KEY) + pi * OROW + dim);
+        };
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int x = 0; x < W; x++) {
@@ -1400,8 +1462,9 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             if (l == 0.0f) continue;
             const float wt = l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx);
             Ls += wt;
-            y += wt * *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * FK * G::KEY) + pi * OROW + dim);
+            y += wt * partial(x);
         }
+        if (some_not_finite(y)) y = sum_not_finite(y, W, partial);
         const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
         if (splits == 1) {
             *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y * inv;

@@ -943,3 +943,56 @@ def test_f32_parts_round_to_nearest(rq, gpu, n):
         assert err.abs().max() <= 2.0**-23 + 2 * 2.0**-24, float(err.abs().max())
         if o.numel() >= 512:  # truncation would keep all of them below zero
             assert (err > 0).double().mean() >= 0.1 and (err < 0).double().mean() >= 0.1
+
+
+def put_wide_values(v, at=(5, 0.5, -1)):
+    """Infinities and NaN in single places of v [n, 2, hd]."""
+    n = v.shape[0]
+    a, b, z = (int(x * n) if 0 < x < 1 else min(x, n - 1) if x > 0 else n + x for x in at)
+    v[a, 0, 1] = float("inf")
+    v[b, 1, 7] = -float("inf")
+    v[z, 0, 9] = float("nan")
+    v[a, 1, 20], v[b, 1, 20] = float("inf"), -float("inf")
+    v[b, 0, 30] = v[z, 0, 30] = -float("inf")
+
+
+def same_places(got, want, bound):
+    """close() without its figure for the whole, which takes scores of up to 2^4; here they reach 2^7."""
+    got = got.double()
+    assert torch.equal(got.isnan(), want.isnan())
+    fine = torch.isfinite(want)
+    assert torch.equal(got[~fine & ~want.isnan()], want[~fine & ~want.isnan()])
+    assert ((got - want)[fine].abs() <= bound[fine]).all(), float(((got - want)[fine].abs() / bound[fine]).max())
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("lens", [[(70, 60), (300, 1), (0, 200)], [(3000, 1), (1700, 1), (8, 1)],
+                                  [(2000, 90), (300, 40), (700, 1)], [(4000, 130)]])
+def test_what_is_not_finite_stays_in_its_place(rq, gpu, kv, lens):
+    """Every element of rows that see infinities or NaN: those elements by their sum, the others as without them, in
+    masked and unmasked tiles, with split and whole key ranges."""
+    b = Batch(lens, 4, 2, 64, kv, seed=7)
+    for i, (k, v) in enumerate(b.kv):
+        put_wide_values(v)
+        k[min(5, k.shape[0] - 1)] *= 30  # a weight of nearly 1 or of nothing
+        b.pool.put(b.table[i], k, v)
+    want, bound = b.want()
+    for hints in ((None, None), (0, 0), (1, 1), (1, 100000), (1000, 64)):
+        same_places(b.run(*hints)[:b.rows], want, bound)
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("lens", [[3, 40], [130, 64, 1, 700], [1500]])
+def test_packed_what_is_not_finite_stays_in_its_place(rq, gpu, kv, lens):
+    torch.manual_seed(8)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    q, k, v = torch.randn(3, starts[-1], 2, 64, device="cuda")
+    k, v = k.to(KV[kv][0]), v.to(KV[kv][0])
+    for a, z in zip(starts, starts[1:]):
+        put_wide_values(v[a:z])
+        k[min(a + 5, z - 1)] *= 30
+    out = run_packed(q, k, v, ints(starts), 0.1, max(lens))
+    for a, z in zip(starts, starts[1:]):
+        same_places(out[a:z], *ref.attention(q[a:z], k[a:z], v[a:z], 0, 0.1))
