@@ -703,7 +703,7 @@ __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, fl
 }
 // Joins up to FEW_PAIRS pairs: JOIN_LANES lanes a pair form the splits' weights
 // while the first outputs are on their way, then a thread takes four dims of a
-// pair at a time.  Its latency is what it costs.  COHERENT: the partials come from
+// pair at a time, by weights of at most 1 (large values stay in f32's range).  Its latency is what it costs.  COHERENT: the partials come from
 // the same launch.
 constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4;  // splits a lane, at most; splits whose outputs are read ahead
 constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
@@ -755,13 +755,13 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
     __syncthreads();
     for (int i = tid; i < pairs * quads; i += NT) {
         const int pr = i / quads;
-        const float *o = outputs(i), *w = wt + pr * splits;
+        const float *o = outputs(i), *w = wt + pr * splits, unit = inv[pr];
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
         int z0 = 0;
         if (i == tid) {
 #pragma unroll
             for (int z = 0; z < JOIN_AHEAD; z++)
-                if (z < splits) y += w[z] * f4{ahead[z][0][0], ahead[z][0][1], ahead[z][1][0], ahead[z][1][1]};
+                if (z < splits) y += w[z] * unit * f4{ahead[z][0][0], ahead[z][0][1], ahead[z][1][0], ahead[z][1][1]};
             z0 = min(JOIN_AHEAD, splits);
         }
         auto partial = [&](int z) {
@@ -769,9 +769,9 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
             return f4{u[0], u[1], v[0], v[1]};
         };
 #pragma unroll 4
-        for (int z = z0; z < splits; z++) y += w[z] * partial(z);
+        for (int z = z0; z < splits; z++) y += w[z] * unit * partial(z);
         if (some_not_finite(y)) y = sum_not_finite(y, splits, partial);
-        *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y * inv[pr];
+        *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y;
     }
 }
 
@@ -1455,24 +1455,25 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         auto partial = [&](int x) {
             return *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * FK * G::KEY) + pi * OROW + dim);
         };
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        float wt[W];
 #pragma unroll
         for (int x = 0; x < W; x++) {
             const float l = wml[x * 32 + 16 + pi];
-            if (l == 0.0f) continue;
-            const float wt = l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx);
-            Ls += wt;
-            y += wt * partial(x);
+            wt[x] = l != 0.0f ? l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx) : 0.0f;
+            Ls += wt[x];
         }
-        if (some_not_finite(y)) y = sum_not_finite(y, W, partial);
         const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < W; x++) y += wt[x] * inv * partial(x);  // weights of at most 1: large values stay in range
+        if (some_not_finite(y)) y = sum_not_finite(y, W, partial);
         if (splits == 1) {
-            *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y * inv;
+            *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y;
         } else {
             const int64_t at = place(a, s, kvh, p0 + pi);
             float* pt = a.part + (at * a.part_splits + z) * a.hd + dim;
-            put2(pt, y[0] * inv, y[1] * inv);
-            put2(pt + 2, y[2] * inv, y[3] * inv);
+            put2(pt, y[0], y[1]);
+            put2(pt + 2, y[2], y[3]);
             if (dim == 0) put_ml(a, at, z, Mx, Ls);
         }
     }

@@ -996,3 +996,18 @@ def test_packed_what_is_not_finite_stays_in_its_place(rq, gpu, kv, lens):
     out = run_packed(q, k, v, ints(starts), 0.1, max(lens))
     for a, z in zip(starts, starts[1:]):
         same_places(out[a:z], *ref.attention(q[a:z], k[a:z], v[a:z], 0, 0.1))
+
+
+@pytest.mark.parametrize("power", [112, 122])
+@pytest.mark.parametrize("lens", [[(20000, 1), (70, 1)], [(9000, 40)], [(3000, 5), (1200, 200)]])
+def test_f32_values_near_the_end_of_f32_over_split_keys(rq, gpu, lens, power):
+    """Values up to 2^(power + 2): their weighted means are in range, and so is every step to them."""
+    b = Batch(lens, 4, 2, 64, "f32")
+    for i, (k, v) in enumerate(b.kv):
+        v.copy_(v.abs().clamp(0.5, 4.0))
+        b.pool.put(b.table[i], k, v)
+    want, bound = b.want()
+    close(b.run()[:b.rows], want, bound)
+    for i, (k, v) in enumerate(b.kv):
+        b.pool.put(b.table[i], k, v * 2.0**power)
+    close(b.run()[:b.rows].double() * 2.0**-power, want, bound)
