@@ -1697,6 +1697,8 @@ hipError_t launch_hd(const BatchArgs& a, hipStream_t s) {
          : a.hd <= 128 ? launch_kind<KV, 128>(a, s) : launch_kind<KV, 256>(a, s);
 }
 
+// A launch has fewer than 2^32 threads.
+constexpr int64_t MAX_BLOCKS = (((int64_t)1 << 32) - 1) / JOIN_THREADS;
 constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial results
 // f32 prompts are split beforehand from this many tiles a sequence on, as far
 // as this much memory holds them.  Prompts of 1, 2, 4, 8, 16, 32 tiles (us), split
@@ -1741,9 +1743,12 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
                                                 std::max(2 * a.tile_splits, a.few_splits)});
     }
     a.part_splits = std::max(a.few_splits, a.tile_splits);
-    if (((int64_t)a.tiles * std::max(a.tile_splits, TILE_PAIRS / FEW_PAIRS) + (int64_t)a.n_seq * a.few_splits) * a.n_kv >
-        (int64_t)1 << 30)
-        return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows", a.n_seq, (long long)m);
+    // (join_kernel, behind split tiles, has TILE_PAIRS / FEW_PAIRS workgroups a tile)
+    const int64_t tile_blocks = a.tile_slots ? a.tile_slots : (int64_t)a.tiles * a.tile_splits;
+    const int64_t blocks = a.n_kv * std::max(tile_blocks + (only_tile ? 0 : (int64_t)a.n_seq * a.few_splits),
+                                             a.tile_splits > 1 ? (int64_t)a.tiles * (TILE_PAIRS / FEW_PAIRS) : 0);
+    if (blocks > MAX_BLOCKS)
+        return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows: %lld workgroups", a.n_seq, (long long)m, (long long)blocks);
     // f32 prompts whose keys several tiles read: split once
     const int hdp = a.hd <= 64 ? 64 : a.hd <= 128 ? 128 : 256, tk = a.hd <= 64 ? 64 : 32;  // Geo<Split, HD>
     const int64_t tiles = m / tk + a.n_seq;

@@ -130,3 +130,17 @@ def test_columns_of_the_same_rows_do_not_overlap(rq):
     with pytest.raises(rq.InvalidData):
         paged(pool(), q=Q, qs=512, out=Q + 1008, os=512, rs=0)
     assert C.sizeof(A.KvPool) == 64
+
+
+@pytest.mark.parametrize("n_seq,kvh,m", [(1 << 24, 1, 1 << 24), (1 << 23, 2, 1 << 23), (1 << 24, 2, 8), (1 << 22, 16, 1 << 22)])
+def test_more_workgroups_than_a_launch_has(rq, n_seq, kvh, m):
+    far = dict(q=1 << 40, out=1 << 50)
+    w = kvh * 8
+    one = pool(n_kv_heads=kvh, head_dim=8, position_stride=8, head_stride=512, page_stride=512 * kvh)
+    for call in (lambda: paged(one, qs=w, os=w, heads=kvh, m=m, n_seq=n_seq, **far),
+                 lambda: A.attention_paged_dev(one, far["q"], w, kvh, m, INTS, INTS, n_seq, INTS, 4, 0.1, far["out"], w, 1,
+                                               4, 0),
+                 lambda: packed(qs=w, os=w, heads=kvh, ks=w, vs=w, kvh=kvh, hd=8, m=m, n_seq=n_seq, **far)):
+        with pytest.raises(rq.DeviceError) as e:
+            call()
+        assert e.value.status == rq.ERR_UNSUPPORTED, e.value
