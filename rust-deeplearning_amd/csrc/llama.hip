@@ -699,6 +699,7 @@ struct LlamaModel {
         float *x = nullptr, *logits = nullptr;  // [cap][dim], [cap][vocab]
         size_t max_rows = 0, max_kv = 0;        // of the step
         std::vector<int> len, free_host;
+        rdl_status status = RDL_OK;  // of the step's cache operators, whose message stands
     } batch;
 
     ~LlamaModel() {
@@ -818,6 +819,7 @@ struct LlamaModel {
             st = rdl_attention_paged_dev(&pool, qkv, qkv_dim, cfg.n_heads, m, batch.row_start, batch.kv_len, batch.n_seq,
                                          batch.table, n_pages, 1.0f / sqrtf((float)hd), att, q_dim, batch.max_rows,
                                          batch.max_kv, stream);
+        batch.status = st;
         return st == RDL_OK ? hipSuccess : hipErrorUnknown;
     }
 
@@ -1760,11 +1762,17 @@ rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size
     HIP_TRY(up(B.count, counts, n_seq));
     HIP_TRY(up(B.free_pages, B.free_host.data(), B.free_host.size()));
     HIP_TRY(up(B.last_rows, last.data(), last.size()));
+    B.status = RDL_OK;
     const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.free_host.size(), rdl::KV_PAGE, B.table,
                                           (size_t)M.n_pages, B.row_start, B.kv_len, n, B.row_seq, B.positions, B.slots,
                                           B.summary, M.stream);
     if (st != RDL_OK) return st;
-    HIP_TRY(M.forward_batch(n, last.size()));
+    const hipError_t run = M.forward_batch(n, last.size());
+    if (B.status != RDL_OK) {
+        (void)hipStreamSynchronize(M.stream);  // nothing of the step is in use any more
+        return B.status;
+    }
+    HIP_TRY(run);
     for (size_t b = 0, i = 0; b < n_seq; b++)
         if (counts[b])
             HIP_TRY(hipMemcpyAsync(logits + b * c.vocab, B.logits + i++ * c.vocab, (size_t)c.vocab * 4,
