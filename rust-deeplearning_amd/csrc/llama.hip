@@ -696,7 +696,8 @@ struct LlamaModel {
         int *table = nullptr, *cached = nullptr, *count = nullptr, *free_pages = nullptr, *row_start = nullptr,
             *kv_len = nullptr, *row_seq = nullptr, *positions = nullptr, *slots = nullptr, *summary = nullptr,
             *last_rows = nullptr;
-        float *x = nullptr, *logits = nullptr;  // [cap][dim], [cap][vocab]
+        float *x = nullptr, *logits = nullptr;  // [last][dim], [last][vocab]: a step's last rows, at most min(cap, max_batch)
+        void* mem = nullptr;                    // all of it, one allocation
         size_t max_rows = 0, max_kv = 0;        // of the step
         std::vector<int> len, free_host;
         rdl_status status = RDL_OK;  // of the step's cache operators, whose message stands
@@ -704,6 +705,7 @@ struct LlamaModel {
 
     ~LlamaModel() {
         if (batch.cap) (void)rdl_release_stream_work(stream);  // the attention's
+        (void)hipFree(batch.mem);
         if (decode_exec) (void)hipGraphExecDestroy(decode_exec);
         if (decode_graph) (void)hipGraphDestroy(decode_graph);
         for (hipEvent_t e : ev)
@@ -1664,7 +1666,6 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
                         c.dim);
     if (M.host_pos != 0 || B.on)
         return api_fail(RDL_ERR_INVALID_DATA, "sequences can begin only on an empty cache (rdl_llama_reset first)");
-    auto fail_free = [&](hipError_t e) { return api_fail(RDL_ERR_HIP, "allocation failed: %s", hipGetErrorString(e)); };
     try {
         B.len.assign(n_seq, 0);
         B.free_host.resize((size_t)M.n_pages);
@@ -1672,15 +1673,27 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
     }
     for (int p = 0; p < M.n_pages; p++) B.free_host[p] = p;
-    hipError_t e;
-    if (n_seq > B.cap) {  // (memory of an earlier, smaller batch stays until the model is freed)
-        const size_t mb = c.max_batch, pg = M.n_pages;
-        for (auto& a : {std::make_pair(&B.table, n_seq * pg), {&B.cached, n_seq}, {&B.count, n_seq}, {&B.free_pages, pg},
-                        {&B.row_start, n_seq + 1}, {&B.kv_len, n_seq}, {&B.row_seq, mb}, {&B.positions, mb},
-                        {&B.slots, mb}, {&B.summary, (size_t)4}, {&B.last_rows, n_seq}})
-            if ((e = M.alloc_t(a.first, a.second)) != hipSuccess) return fail_free(e);
-        if ((e = M.alloc_t(&B.x, n_seq * c.dim)) != hipSuccess) return fail_free(e);
-        if ((e = M.alloc_t(&B.logits, n_seq * c.vocab)) != hipSuccess) return fail_free(e);
+    if (n_seq > B.cap) {
+        const size_t mb = c.max_batch, pg = M.n_pages, last = std::min(n_seq, mb);
+        const std::pair<int**, size_t> ints[] = {
+            {&B.table, n_seq * pg}, {&B.cached, n_seq}, {&B.count, n_seq}, {&B.free_pages, pg}, {&B.row_start, n_seq + 1},
+            {&B.kv_len, n_seq}, {&B.row_seq, mb}, {&B.positions, mb}, {&B.slots, mb}, {&B.summary, 4}, {&B.last_rows, last}};
+        const std::pair<float**, size_t> floats[] = {{&B.x, last * c.dim}, {&B.logits, last * c.vocab}};
+        auto room = [](size_t n) { return (n * 4 + 255) & ~(size_t)255; };
+        size_t bytes = 0;
+        for (const auto& a : ints) bytes += room(a.second);
+        for (const auto& a : floats) bytes += room(a.second);
+        void* mem = nullptr;
+        const hipError_t e = hipMalloc(&mem, bytes);
+        if (e != hipSuccess) {  // what an earlier batch had stays as it is
+            (void)hipGetLastError();
+            return api_fail(RDL_ERR_HIP, "allocation failed: %s", hipGetErrorString(e));
+        }
+        HIP_TRY(hipFree(B.mem));
+        B.mem = mem;
+        uint8_t* at = static_cast<uint8_t*>(mem);
+        for (const auto& a : ints) *a.first = reinterpret_cast<int*>(at), at += room(a.second);
+        for (const auto& a : floats) *a.first = reinterpret_cast<float*>(at), at += room(a.second);
         B.cap = n_seq;
     }
     B.n_seq = n_seq;

@@ -146,3 +146,28 @@ def test_refusals(rq, gpu):
     with pytest.raises(rq.DeviceError) as e:
         LlamaModel(bad).batch_begin(2)
     assert e.value.status == rq.ERR_UNSUPPORTED
+
+
+def test_memory_of_a_batch(rq, gpu):
+    """Logits are kept of the rows that a step can have, not of every sequence, and a larger batch takes the smaller
+    one's place."""
+    import torch
+    cfg = tiny_config(vocab=32000, max_seq=64 * 8, max_batch=16)
+    m, new = build(cfg)
+    used = lambda: -torch.cuda.mem_get_info()[0]  # noqa: E731
+    m.batch_begin(2)
+    check_step(m, [new(), new()], [[1, 2], [3]])
+    m.reset()
+    before = used()
+    for n in (600, 1200, 2400, 4096):
+        m.batch_begin(n)
+        m.reset()
+        # 16 rows of logits (2 MB), 4096 page tables of 8 and a few ints a sequence
+        assert used() - before <= 16 << 20, n
+    m.batch_begin(4096)
+    refs = [new() for _ in range(3)]
+    toks = [[]] * 4096
+    toks[5], toks[2000], toks[4095] = [1, 2, 3], [7], [9, 9]
+    got = m.batch_forward(toks)
+    for r, b in zip(refs, (5, 2000, 4095)):
+        assert_close(got[b], r.forward_with_cache(toks[b]))
