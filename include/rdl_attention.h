@@ -97,12 +97,13 @@ rdl_status rdl_kv_plan_dev(const int32_t* cached_dev, const int32_t* new_rows_de
  * update), in one launch.  Row r of q (n_heads heads), k and v (the pool's KV
  * heads) starts r * stride floats behind its base, heads head_dim apart;
  * strides and bases are multiples of 16 bytes.  q_out rows may be the q rows
- * themselves (the same base and stride) and may not overlap them otherwise;
- * n_heads = 0: no q.  positions (NULL without RoPE) select the rows of cos
- * and sin [n_positions][head_dim / 2] f32; cos and sin NULL: no RoPE, q is
- * copied.  slots: page * page_positions + offset.  A row whose slot is
- * negative or past the pool, or whose position is outside the tables, is left
- * out: nothing of it is written.  The slots of two rows must differ. */
+ * themselves (the same base and stride) and may not overlap them otherwise,
+ * nor the k and v rows (RDL_ERR_INVALID_DATA) or the pool; n_heads = 0: no q.
+ * positions (NULL without RoPE) select the rows of cos and sin
+ * [n_positions][head_dim / 2] f32; cos and sin NULL: no RoPE, q is copied.
+ * slots: page * page_positions + offset.  A row whose slot is negative or past
+ * the pool, or whose position is outside the tables, is left out: nothing of it
+ * is written.  The slots of two rows must differ. */
 rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_dev, size_t q_stride, float* q_out_dev,
                             size_t q_out_stride, size_t n_heads, const float* k_dev, size_t k_stride,
                             const float* v_dev, size_t v_stride, const int32_t* positions_dev,
@@ -118,7 +119,8 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * no key gives zeros, and a key on a page that is not in the pool counts as
  * not seen.  Rows row_start[n_seq] .. m - 1 of out are left as they were.
  * q and out: f32 rows stride floats apart (n_heads * head_dim or more, a
- * multiple of 4; bases 16-byte aligned); out must not overlap q.
+ * multiple of 4; bases 16-byte aligned); out must not overlap q (RDL_ERR_INVALID_DATA),
+ * the pool or the int arrays.
  * row_start ascends; where it does not, what the call's rows get is unspecified.
  * What a row does not see has no effect on it, NaN and infinities included.  Of
  * what it sees, a NaN in a key or in its query makes its outputs NaN, values that are
@@ -143,8 +145,9 @@ rdl_status rdl_attention_paged_dev(const rdl_kv_pool* pool, const float* q_dev, 
  * cache (MultiHeadAttention::forward, attention.rs): sequence b's rows
  * row_start[b] .. row_start[b + 1] - 1 see one another up to their own place.
  * k and v rows are kv_dtype (f32 as a Linear leaves them, or f16), stride
- * elements apart (multiples of 16 bytes, as the bases), heads head_dim apart.
- * Otherwise as rdl_attention_paged_dev. */
+ * elements apart (multiples of 16 bytes, as the bases), heads head_dim apart;
+ * out must not overlap them either (RDL_ERR_INVALID_DATA).  Otherwise as
+ * rdl_attention_paged_dev. */
 rdl_status rdl_attention_packed_dev(const float* q_dev, size_t q_stride, size_t n_heads, const void* k_dev,
                                     size_t k_stride, const void* v_dev, size_t v_stride, int32_t kv_dtype,
                                     size_t n_kv_heads, size_t head_dim, size_t m, const int32_t* row_start_dev,

@@ -1796,7 +1796,7 @@ rdl_status check_attention(BatchArgs* a, const float* q, size_t q_stride, size_t
     rdl_status st = check_rows("q", q, q_stride, n_heads * hd, m, 4);
     if (st != RDL_OK) return st;
     if ((st = check_rows("out", out, out_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
-    if (rows_overlap(q, q_stride, n_heads * hd, out, out_stride, n_heads * hd, m))
+    if (rows_overlap(q, q_stride * 4, n_heads * hd * 4, out, out_stride * 4, n_heads * hd * 4, m))
         return api_fail(RDL_ERR_INVALID_DATA, "out overlaps q");
     if (!row_start) return api_fail(RDL_ERR_NULL_POINTER, "row_start is NULL");
     if ((st = check_stream((hipStream_t)stream)) != RDL_OK) return st;
@@ -1861,6 +1861,9 @@ rdl_status rdl_attention_packed_dev(const float* q_dev, size_t q_stride, size_t 
     const size_t elem = kv_dtype == RDL_DTYPE_F16 ? 2 : 4, width = n_kv_heads * head_dim;
     if ((st = rdl::check_rows("k", k_dev, k_stride, width, m, elem)) != RDL_OK) return st;
     if ((st = rdl::check_rows("v", v_dev, v_stride, width, m, elem)) != RDL_OK) return st;
+    if (rdl::rows_overlap(k_dev, k_stride * elem, width * elem, out_dev, out_stride * 4, n_heads * head_dim * 4, m) ||
+        rdl::rows_overlap(v_dev, v_stride * elem, width * elem, out_dev, out_stride * 4, n_heads * head_dim * 4, m))
+        return api_fail(RDL_ERR_INVALID_DATA, "out overlaps k or v");
     if ((st = rdl::check_position_stride(k_stride > v_stride ? k_stride : v_stride)) != RDL_OK) return st;
     a.kv = {k_dev, v_dev, (int64_t)k_stride, (int64_t)v_stride, (int64_t)head_dim, 0, nullptr, 0, 0, 0};
     return rdl::run(a, kv_dtype == RDL_DTYPE_F16, max_rows, max_rows, (hipStream_t)stream);

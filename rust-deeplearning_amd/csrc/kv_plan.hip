@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
+#include <utility>
+
 #include "../../include/rdl_attention.h"
 #include "kv_pool.hpp"
 #include "rdl_device.hpp"
@@ -315,16 +317,14 @@ rdl_status check_rows(const char* what, const void* p, size_t stride, size_t wid
     return RDL_OK;
 }
 
-bool rows_overlap(const float* a, size_t a_stride, size_t a_width, const float* b, size_t b_stride, size_t b_width,
-                  size_t m) {
-    const uintptr_t a0 = (uintptr_t)a, a1 = a0 + ((m - 1) * a_stride + a_width) * sizeof(float);
-    const uintptr_t b0 = (uintptr_t)b, b1 = b0 + ((m - 1) * b_stride + b_width) * sizeof(float);
+bool rows_overlap(const void* a, size_t a_pitch, size_t a_width, const void* b, size_t b_pitch, size_t b_width, size_t m) {
+    const uintptr_t a0 = (uintptr_t)a, a1 = a0 + (m - 1) * a_pitch + a_width;
+    const uintptr_t b0 = (uintptr_t)b, b1 = b0 + (m - 1) * b_pitch + b_width;
     if (a1 <= b0 || b1 <= a0) return false;
-    if (a_stride != b_stride || m == 1) return true;
-    // rows of one stride: columns apart (q and out as two parts of the same rows)
-    const size_t pitch = a_stride * sizeof(float);
-    const size_t off = (b0 + pitch - a0 % pitch) % pitch;  // b's column in a's rows
-    return off < a_width * sizeof(float) || off + b_width * sizeof(float) > pitch;
+    if (a_pitch != b_pitch || m == 1) return true;
+    // rows of one pitch: columns apart (q and out as two parts of the same rows)
+    const size_t off = (b0 + a_pitch - a0 % a_pitch) % a_pitch;  // b's column in a's rows
+    return off < a_width || off + b_width > a_pitch;
 }
 
 rdl_status check_stream(hipStream_t s) {
@@ -395,11 +395,15 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
         if ((st = rdl::check_rows("q", q_dev, q_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
         if ((st = rdl::check_rows("q_out", q_out_dev, q_out_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
         if (!(q_dev == q_out_dev && q_stride == q_out_stride) &&
-            rdl::rows_overlap(q_dev, q_stride, n_heads * hd, q_out_dev, q_out_stride, n_heads * hd, m))
+            rdl::rows_overlap(q_dev, q_stride * 4, n_heads * hd * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
             return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps q (the same rows, or none of them)");
     }
     if ((st = rdl::check_rows("k", k_dev, k_stride, kvw, m, 4)) != RDL_OK) return st;
     if ((st = rdl::check_rows("v", v_dev, v_stride, kvw, m, 4)) != RDL_OK) return st;
+    if (n_heads)
+        for (const auto& x : {std::make_pair(k_dev, k_stride), std::make_pair(v_dev, v_stride)})
+            if (rdl::rows_overlap(x.first, x.second * 4, kvw * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
+                return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps k or v");
     if (!slots_dev || !cos_dev != !sin_dev || (cos_dev && !positions_dev))
         return api_fail(RDL_ERR_NULL_POINTER, "NULL device pointer");
     if (((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15)

@@ -29,9 +29,8 @@ rdl_status check_head_dim(size_t hd);
 rdl_status check_position_stride(size_t n);
 // m rows of `width` elements, `stride` apart, 16-byte aligned and not NULL
 rdl_status check_rows(const char* what, const void* p, size_t stride, size_t width, size_t m, size_t elem);
-// whether two sets of m >= 1 f32 rows share an element
-bool rows_overlap(const float* a, size_t a_stride, size_t a_width, const float* b, size_t b_stride, size_t b_width,
-                  size_t m);
+// whether two sets of m >= 1 rows, pitch bytes apart and width bytes long, share a byte
+bool rows_overlap(const void* a, size_t a_pitch, size_t a_width, const void* b, size_t b_pitch, size_t b_width, size_t m);
 // RDL_ERR_INVALID_DATA for a stream of another device than the current one
 rdl_status check_stream(hipStream_t s);
 

@@ -144,3 +144,30 @@ def test_more_workgroups_than_a_launch_has(rq, n_seq, kvh, m):
         with pytest.raises(rq.DeviceError) as e:
             call()
         assert e.value.status == rq.ERR_UNSUPPORTED, e.value
+
+
+@pytest.mark.parametrize("kw", [dict(qo=K), dict(qo=V + 16), dict(qo=K - 256 * 4 * 4 + 16), dict(k=OUT + 512),
+                                dict(q=Q, qs=512, qo=Q, qos=512, k=Q + 1008, ks=512),
+                                dict(q=Q, qs=512, qo=Q, qos=512, k=Q + 1024, ks=512, v=Q + 1008, vs=512)])
+def test_store_refuses_q_out_over_k_or_v(rq, kw):
+    with pytest.raises(rq.InvalidData) as e:
+        store(pool(), **kw)
+    assert "q_out overlaps k or v" in str(e.value)
+
+
+def test_store_takes_parts_of_the_same_rows(rq):
+    # q in place, k and v behind it in rows of one stride: past the overlap checks, up to the null check
+    with pytest.raises(rq.DeviceError) as e:
+        store(pool(), q=Q, qs=512, qo=Q, qos=512, k=Q + 1024, ks=512, v=Q + 1536, vs=512, slots=0)
+    assert e.value.status == rq.ERR_NULL_POINTER
+    with pytest.raises(rq.DeviceError) as e:
+        store(pool(), heads=0, q=0, qo=K, slots=0)  # no q: no q_out
+    assert e.value.status == rq.ERR_NULL_POINTER
+
+
+@pytest.mark.parametrize("kw", [dict(out=K), dict(out=V + 16), dict(out=K, dtype=1, ks=512), dict(k=OUT + 512),
+                                dict(q=Q, qs=1024, out=Q + 1024, os=1024, k=Q + 2032, ks=1024)])
+def test_packed_refuses_out_over_k_or_v(rq, kw):
+    with pytest.raises(rq.InvalidData) as e:
+        packed(**kw)
+    assert "out overlaps k or v" in str(e.value)
