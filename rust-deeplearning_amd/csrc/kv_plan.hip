@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "../../include/rdl_attention.h"
@@ -23,12 +24,13 @@ namespace {
 // entries, a thread a row or an entry, each finding its sequence by bisection
 // in LDS.  Nothing passes between workgroups: the slot of a row on a new page
 // comes from the free list, not from the table entry that another workgroup
-// writes.  Sums stop at 2^31 - 1, which no row or free page number reaches.
+// writes.  Past PLAN_WG workgroups each takes more rows, since every one of them walks
+// all the sequences.  Sums stop at 2^31 - 1, which no row or free page number reaches.
 // Latency bounds it (one load of the lengths, the scan, a bisection and a
 // dependent load): 4.1 us for 16 sequences, 7.4 us for 1500 with 20600 rows, where
 // an empty launch takes about as much as the former.
 constexpr int PLAN_NT = 512, PLAN_PER = 4, PLAN_CHUNK = PLAN_NT * PLAN_PER;
-constexpr int PLAN_ROWS = 1024;  // rows a workgroup
+constexpr int PLAN_ROWS = 1024, PLAN_WG = 2048;  // rows a workgroup, at least; workgroups, at most
 
 struct PlanArgs {
     const int32_t *cached, *new_rows;
@@ -39,7 +41,7 @@ struct PlanArgs {
     int32_t* tables;
     int table_stride;
     int32_t *row_start, *kv_len;
-    int m;
+    int m, wg_rows;  // rows; of a workgroup
     int32_t *row_seq, *positions, *slots, *summary;
 };
 
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(PLAN_NT) void plan_kernel(PlanArgs a) {
     __shared__ int start[PLAN_CHUNK], first[PLAN_CHUNK], have[PLAN_CHUNK], before[PLAN_CHUNK];
     __shared__ int wrows[PLAN_NT / 64], wpages[PLAN_NT / 64], wflag[PLAN_NT / 64], wlong[PLAN_NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int r_lo = min((int)blockIdx.x * PLAN_ROWS, a.m), r_hi = min(r_lo + PLAN_ROWS, a.m);
+    const int r_lo = min((int)blockIdx.x * a.wg_rows, a.m), r_hi = min(r_lo + a.wg_rows, a.m);  // m <= 2^30
     const int mask = (1 << a.shift) - 1;
     int rows = 0, pages = 0;  // of the chunks before this one
     int flags = 0, longest = 0;
@@ -374,7 +376,9 @@ rdl_status rdl_kv_plan_dev(const int32_t* cached_dev, const int32_t* new_rows_de
     a.positions = positions_dev;
     a.slots = slots_dev;
     a.summary = summary_dev;
-    const size_t wg = (m + rdl::PLAN_ROWS - 1) / rdl::PLAN_ROWS;
+    const size_t rows = std::max((size_t)rdl::PLAN_ROWS, (m + rdl::PLAN_WG - 1) / rdl::PLAN_WG);
+    const size_t wg = (m + rows - 1) / rows;
+    a.wg_rows = (int)rows;
     hipLaunchKernelGGL(rdl::plan_kernel, dim3((unsigned)(wg ? wg : 1)), dim3(rdl::PLAN_NT), 0, (hipStream_t)stream, a);
     HIP_TRY(hipGetLastError());
     return api_ok();

@@ -1011,3 +1011,34 @@ def test_f32_values_near_the_end_of_f32_over_split_keys(rq, gpu, lens, power):
     for i, (k, v) in enumerate(b.kv):
         b.pool.put(b.table[i], k, v * 2.0**power)
     close(b.run()[:b.rows].double() * 2.0**-power, want, bound)
+
+
+@pytest.mark.parametrize("n_seq,m", [(3, 2**21 + 1), (5000, 2**22 + 77)])
+def test_plan_of_more_rows_than_its_workgroups_take_at_once(rq, gpu, n_seq, m):
+    r = random.Random(m)
+    new = [2 * m // n_seq // 2 - r.randrange(50) for _ in range(n_seq)]
+    cached = [r.randrange(300) for _ in range(n_seq)]
+    page, pad = 1024, m - sum(new)
+    need = [-(-(c + n) // page) - -(-c // page) for c, n in zip(cached, new)]
+    width = max(-(-(c + n) // page) for c, n in zip(cached, new))
+    tables = torch.full((n_seq, width), -1, dtype=torch.int32, device="cuda")
+    tables[:, 0] = torch.arange(n_seq, device="cuda") + sum(need)  # the pages of what is cached
+    free = torch.randperm(sum(need), device="cuda").int()
+    cd, nd = ints(cached), ints(new)
+    rs, kl, sm = (torch.zeros(k, dtype=torch.int32, device="cuda") for k in (n_seq + 1, n_seq, 4))
+    seq, pos, slot = (torch.full((m,), -7, dtype=torch.int32, device="cuda") for _ in range(3))
+    A.plan_dev(cd.data_ptr(), nd.data_ptr(), n_seq, free.data_ptr(), free.numel(), page, tables.data_ptr(), width,
+               rs.data_ptr(), kl.data_ptr(), m, seq.data_ptr(), pos.data_ptr(), slot.data_ptr(), sm.data_ptr(), stream())
+    assert pad >= 0 and sm.tolist() == [sum(new), sum(need), 0, max(c + n for c, n in zip(cached, new))]
+    ids = torch.repeat_interleave(torch.arange(n_seq, device="cuda"), nd)
+    start = torch.cumsum(nd, 0) - nd
+    want = cd[ids] + (torch.arange(sum(new), device="cuda") - start[ids])
+    assert torch.equal(seq[:m - pad].long(), ids) and (seq[m - pad:] == -1).all()
+    assert torch.equal(pos[:m - pad].long(), want) and (pos[m - pad:] == 0).all()
+    # the new pages come off the free list in order; the table names them
+    have = torch.tensor([-(-c // page) for c in cached], device="cuda")
+    first = torch.cumsum(torch.tensor(need, device="cuda"), 0) - torch.tensor(need, device="cuda")
+    p = want // page
+    pages = torch.where(p < have[ids], tables[ids, 0].long(), free.long()[(first[ids] + p - have[ids]).clamp(0)])
+    assert torch.equal(slot[:m - pad].long(), pages * page + want % page) and (slot[m - pad:] == -1).all()
+    assert torch.equal(tables[ids, p].long(), pages)
