@@ -19,8 +19,12 @@
  * RDL_ERR_INVALID_DATA), stream-ordered, no synchronisation; lengths, tables
  * and slots are read on the device, so a captured graph follows their contents
  * at each replay.  Activations are f32, the cache f16 or f32.  Work memory
- * (the attention's partial results of split key ranges) is the stream's, as
- * rdl_linear_forward_dev describes; under graph capture the graph owns it.
+ * (the attention's partial results of split key ranges, at most 256 MB, and, for
+ * long packed f32 prompts, 16-bit parts of their k and v, at most about 1 GB) is the
+ * stream's, as rdl_linear_forward_dev describes (rdl_release_stream_work frees
+ * it); under graph capture the graph owns it.  Steps of more than 2^24 - 1
+ * workgroups (a sequence has one a KV head at least, or one a KV head for 128
+ * pairs of row and query head of a group) are RDL_ERR_UNSUPPORTED.
  * What device-side arrays hold is never trusted with an address: page numbers,
  * slots and positions outside their array are skipped, row numbers and lengths
  * are cut to m and to the table's width.  Inference only: there is no backward
@@ -79,7 +83,8 @@ enum {
  *   tables        the entries of the new pages (no others are written);
  *   row_start     [n_seq + 1];    kv_len  [n_seq];
  *   row_seq, positions, slots     [m]: the row's sequence, its position in it
- *                 and page * page_positions + offset of that position;
+ *                 and page * page_positions + offset of that position
+ *                 (-1 past 2^31 - 1);
  *   summary       [4]: rows of the step, pages taken from the free list,
  *                 RDL_PLAN_* flags, the longest kv_len.
  * Rows row_start[n_seq] .. m - 1 of a padded batch get sequence -1, position 0
@@ -133,8 +138,10 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * f32 sums from f16 pairs: with f16 keys and values, which are exact, they
  * carry 22 bits of q and of the weights; with f32 ones 23 bits of those and of
  * keys and values.  Sums, maxima and exponents are f32.
- * Of f32 values, elements far below the largest of their row or of the rows a
- * query weighs with it end at 2^-28 of that.
+ * Errors are then about those of plain f32 sums and products.  What pairs cannot
+ * hold: f32 elements far below the largest of their row end at 2^-38 of that in
+ * queries and at 2^-33 in keys, and in values at 2^-28 of the largest of their
+ * row or of the rows a query weighs with it.
  * n_heads must be a multiple of the pool's n_kv_heads. */
 rdl_status rdl_attention_paged_dev(const rdl_kv_pool* pool, const float* q_dev, size_t q_stride, size_t n_heads,
                                    size_t m, const int32_t* row_start_dev, const int32_t* kv_len_dev, size_t n_seq,

@@ -190,8 +190,9 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq);
  * chunks may share a step.  A step that needs more pages than are free or passes
  * max_seq is RDL_ERR_INVALID_DATA and changes nothing.  Synchronous; after
  * RDL_ERR_HIP the cache contents are undefined.  The rows run as a prompt chunk's do, the
- * cache through rdl_kv_plan_dev, rdl_kv_store_dev and rdl_attention_paged_dev
- * (rdl_attention.h). */
+ * cache through rdl_kv_plan_dev, rdl_kv_store_dev and rdl_attention_paged_dev, with
+ * the arithmetic that rdl_attention.h describes: over an f32 cache too (where
+ * rdl_llama_forward multiplies in f32) products are formed from 23-bit pairs. */
 rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
                                    size_t n, float* logits, size_t logits_len);
 /* Positions that each of the n (= n_seq) sequences has. */

@@ -932,10 +932,10 @@ __device__ __forceinline__ int tile_start(const BatchArgs& a, const Seq& s, int 
 // the order 4h .. 4h + 3, 8 + 4h .. (h = lane / 32), in which the transposed LDS reads of V
 // fetch them.  q and the weights are f16 pairs, so each product takes two
 // instructions (three with f32 keys and values); the matrix cores bound it: 2048 rows
-// over 16048 f16 keys (32 / 8 heads of 128) take 872 us, 1157 TFLOP/s of
-// those instructions where a large f16 library product reaches 1191.  32 pairs a wave
-// and 4 waves a workgroup: 64 pairs a wave left one wave a SIMD and took
-// twice the time, 8 waves a workgroup and wave priorities gave nothing.  f16
+// over 16048 f16 keys (32 / 8 heads of 128) take 870 to 935 us from card to card,
+// 1160 to 1080 TFLOP/s of those instructions (a large f16 library product on
+// the first card: 1191).  32 pairs a wave and 4 waves a workgroup: 64 pairs a wave left one
+// wave a SIMD and took twice the time, 8 waves a workgroup and wave priorities gave nothing.  f16
 // keys go straight to LDS (DirectSlab), two tiles deep, one barrier a tile.
 template <typename KV, int HD>
 __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, const int32_t* table, int b, int kvh,
@@ -1243,7 +1243,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
 // (v_mfma_f32_16x16x32_f16): a lane has the scores of keys 4g .. 4g + 3 and 16 +
 // 4g .. (g = lane / 16) of one pair.  HBM bounds it: 48 rows over 187420 keys of
 // 8 KV heads of 128 in f16, 769 MB, take 158 us, 4.9 TB/s (a large copy reaches
-// 4.7); a single row over 778 keys takes 11.3 us, which is latency: lengths,
+// 4.7); a single row over 778 keys takes 11.4 us, which is latency: lengths,
 // page numbers, keys, then the splits' partials one behind the other.
 // Returns the splits to join (1: the output is written, 0: no such split).
 template <typename KV, int HD>
@@ -1603,7 +1603,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_kernel(BatchArgs a) {
 // tile (5 operations a value) cost more than the products' own work on them:
 // here a workgroup splits one tile of TK keys of a KV head and writes it as LDS will
 // hold it.  It moves 8 + 8 bytes an element: 9910 rows of 8 KV heads of 128 take 32 us of
-// the call's 607, the products 1070 TFLOP/s.
+// the call's 602, the products 1020 TFLOP/s.
 template <int HD>
 __global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* images, int4* notes, int2* exps) {
     using G = Geo<Split, HD>;
