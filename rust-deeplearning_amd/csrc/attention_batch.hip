@@ -576,9 +576,12 @@ __device__ __forceinline__ bool not_finite_of_values(float all, float L) {
 __device__ __forceinline__ float finite_or(float x, bool zero) {
     return zero && abs_bits(x) >= 0x7F800000u ? 0.0f : x;
 }
-// Partial outputs likewise, joined by y = sum(w x): an infinite x keeps its place whatever its weight.  y tells
-// whether there was any; if so its element is the sum of those, which `partial` gives one by one.
-__device__ __forceinline__ bool some_not_finite(f4 y) { return !(fmaf(y[0], 0.0f, fmaf(y[1], 0.0f, fmaf(y[2], 0.0f, y[3] * 0.0f))) == 0.0f); }
+// Partial outputs likewise, joined by y = sum(w x): an infinite x keeps its place
+// whatever its weight.  y tells whether there was any; if so its element is the
+// sum of those, which `partial` gives one by one.
+__device__ __forceinline__ bool some_not_finite(f4 y) {
+    return !(fmaf(y[0], 0.0f, fmaf(y[1], 0.0f, fmaf(y[2], 0.0f, y[3] * 0.0f))) == 0.0f);
+}
 template <typename Partial>
 __device__ __forceinline__ f4 sum_not_finite(f4 y, int n, Partial&& partial) {
     f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -703,8 +706,8 @@ __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, fl
 }
 // Joins up to FEW_PAIRS pairs: JOIN_LANES lanes a pair form the splits' weights
 // while the first outputs are on their way, then a thread takes four dims of a
-// pair at a time, by weights of at most 1 (large values stay in f32's range).  Its latency is what it costs.  COHERENT: the partials come from
-// the same launch.
+// pair at a time, by weights of at most 1 (large values stay in f32's range).  Its
+// latency is what it costs.  COHERENT: the partials come from the same launch.
 constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4;  // splits a lane, at most; splits whose outputs are read ahead
 constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
 constexpr int JOIN_FLOATS = FEW_PAIRS * (JOIN_SPLITS + 1);  // of LDS
