@@ -41,10 +41,23 @@
 extern "C" {
 #endif
 
-/* Cache element types: GGML type ids (rustml/gguf/main/src/api/types.rs:5-20). */
+/* Cache element types: GGML type ids (rustml/gguf/main/src/api/types.rs:5-20), and
+ * one of this library's own, RDL_KV_Q4: 4 bits and a share of a scale, 4.5 bits a
+ * value.  32 consecutive values of a position and KV head are a block of a scale
+ * d and codes 0 .. 15, value = d (code - 8).  d has the size of the block's largest
+ * magnitude over 8, rounded to 8 significant bits, as f16, at most 8160, and the sign
+ * that takes that value to code 0 (of a positive and a negative one as large, the
+ * positive); a code is value / d rounded to nearest, halves to even, between -8
+ * and 7, plus 8.  A block that holds a value that is not finite reads as NaN.  With such a
+ * scale every value is an f16 number; with one of more bits it is rounded to f16.
+ * A page of a head is one run of bytes: page_positions * head_dim / 2 of codes,
+ * then page_positions * head_dim / 32 f16 scales, positions in order.  In each
+ * 4 bytes of codes, as a little-endian word, codes 0, 2, 4, 6 of 8 are the nibbles of the
+ * low half and 1, 3, 5, 7 those of the high half, from the lowest bits up. */
 enum {
     RDL_DTYPE_F32 = 0,
-    RDL_DTYPE_F16 = 1
+    RDL_DTYPE_F16 = 1,
+    RDL_KV_Q4 = 0x104
 };
 
 /* A layer's paged K and V memory.  Element d of position o of page pg and KV
@@ -52,11 +65,13 @@ enum {
  * k_dev and of v_dev (strides in elements; multiples of 16 bytes, as both
  * bases; position_stride below 2^24; the heads and positions of a page and the
  * pages must not overlap).
- * The decoder's own pools are [n_pages][n_kv_heads][page_positions][head_dim]. */
+ * The decoder's own pools are [n_pages][n_kv_heads][page_positions][head_dim].
+ * RDL_KV_Q4: strides in bytes (multiples of 16), position_stride = head_dim / 2,
+ * head_dim a multiple of 32. */
 typedef struct rdl_kv_pool {
     void* k_dev;
     void* v_dev;
-    int32_t dtype;          /* RDL_DTYPE_F16 or RDL_DTYPE_F32 */
+    int32_t dtype;          /* RDL_DTYPE_F16, RDL_DTYPE_F32 or RDL_KV_Q4 */
     int32_t n_pages;
     int32_t page_positions; /* a power of two, 16 .. 1024 */
     int32_t n_kv_heads;
@@ -115,6 +130,59 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
                             const int32_t* slots_dev, const float* cos_dev, const float* sin_dev, size_t n_positions,
                             void* stream);
 
+/* The same with an RMS norm of every query and key head before its rotation
+ * (MultiHeadAttention's q_norm and k_norm, rustml/nn/main/src/core/attention.rs):
+ *   y = (x * r) * gamma,  r = 1 / sqrt(mean(x^2) + eps) over the head's values,
+ * the mean square in 64 bits, r rounded to f32.  q_gamma and k_gamma: [head_dim] f32,
+ * 16-byte aligned, the same for all heads; NULL: no norm of those rows.  eps is
+ * finite and not negative.  Products and sums of the norm and of the rotation are
+ * rounded one by one (rdl_kv_store_dev fuses a product with its sum, except over a 4-bit pool).  Otherwise as
+ * rdl_kv_store_dev. */
+rdl_status rdl_kv_store_norm_dev(const rdl_kv_pool* pool, size_t m, const float* q_dev, size_t q_stride,
+                                 float* q_out_dev, size_t q_out_stride, size_t n_heads, const float* k_dev,
+                                 size_t k_stride, const float* v_dev, size_t v_stride, const float* q_gamma_dev,
+                                 const float* k_gamma_dev, float eps, const int32_t* positions_dev,
+                                 const int32_t* slots_dev, const float* cos_dev, const float* sin_dev,
+                                 size_t n_positions, void* stream);
+
+/* What rdl_kv_fork_dev found wrong (summary[1], 0: nothing). */
+enum {
+    RDL_FORK_BAD_SEQUENCE = 1, /* a parent or child that is no sequence, or one that is both: the pair is left out */
+    RDL_FORK_BAD_LENGTH = 2,   /* a parent's length that is negative (taken as 0) or past its table row (cut) */
+    RDL_FORK_NO_PAGES = 4      /* the free list is shorter than the pages needed */
+};
+
+/* Forks sequences over shared pages, in one launch: for each of n pairs (int32,
+ * device) the sequence children[i] becomes a copy of parents[i].  Its table
+ * row names the parent's pages, except that a last page that is not full is the
+ * child's own: the next page of the free list, and -1 where that is used up.  src_pages
+ * and dst_pages [n] receive the pages to copy, the parent's last and the child's
+ * own (-1, -1: none), for rdl_kv_copy_pages_dev on every layer.
+ *   tables [n_seq][table_stride], kv_len [n_seq]: the children's rows (as far as
+ *                 the parent's length) and lengths are written;
+ *   summary [2]:  pages taken from the free list, RDL_FORK_* flags.
+ * Several children of one parent are its copies with a page of their own
+ * each.  A child may not be another pair's parent or child (its row is then unspecified).
+ * Full pages are shared: the caller frees a page when no sequence names it.
+ * page_positions: a power of two, 16 .. 1024.  Outputs must not overlap. */
+rdl_status rdl_kv_fork_dev(int32_t* tables_dev, size_t table_stride, int32_t* kv_len_dev, size_t n_seq,
+                           size_t page_positions, const int32_t* parents_dev, const int32_t* children_dev, size_t n,
+                           const int32_t* free_pages_dev, size_t n_free, int32_t* src_pages_dev,
+                           int32_t* dst_pages_dev, int32_t* summary_dev, void* stream);
+
+/* Copies whole pages, K and V of every KV head, for n_pools (src, dst) pairs of pools
+ * at once (a model's layers): page src_pages[i] of src[l] to page dst_pages[i] of
+ * dst[l], i < n (int32, device).  A pair with a page outside its pool is left out.  src
+ * and dst may be the same pools (a fork, compaction) or others of the same pages,
+ * heads and head_dim in any types and strides: values of another type are rounded
+ * to nearest (f16: past its range infinite; 4 bits as RDL_KV_Q4 says), those of the same type are
+ * copied bit by bit.  All src pools agree in everything but their addresses, and so do
+ * all dst pools (RDL_ERR_INVALID_DATA).  dst pages differ from one another, and
+ * in the same pool none is also a pair's src, unless it is its own (its contents are
+ * then unspecified); pools that are not the same must not overlap. */
+rdl_status rdl_kv_copy_pages_dev(const rdl_kv_pool* src, const rdl_kv_pool* dst, size_t n_pools,
+                                 const int32_t* src_pages_dev, const int32_t* dst_pages_dev, size_t n, void* stream);
+
 /* Causal attention of a step's rows over the paged cache, which holds the
  * rows' own keys already: row i of sequence b's new_b = row_start[b + 1] -
  * row_start[b] rows sees the keys 0 .. kv_len[b] - new_b + i, and
@@ -135,7 +203,7 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
  * max_rows and max_kv tell the launch what to expect (the most rows of a
  * sequence, the longest kv_len; 0: unknown): results do not depend on them
  * beyond rounding, time does.  Products are formed on the matrix cores with
- * f32 sums from f16 pairs: with f16 keys and values, which are exact, they
+ * f32 sums from f16 pairs: with f16 keys and values, and 4-bit ones, which are exact in f16, they
  * carry 22 bits of q and of the weights; with f32 ones 23 bits of those and of
  * keys and values.  Sums, maxima and exponents are f32.
  * Errors are then about those of plain f32 sums and products.  What pairs cannot

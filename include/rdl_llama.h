@@ -200,6 +200,24 @@ rdl_status rdl_llama_batch_positions(const rdl_llama* model, size_t* out, size_t
 /* Empties one sequence; its pages are free for the others. */
 rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq);
 
+/* Log probabilities of logit rows on the device, in one launch: row r's vocab
+ * (1 .. 2^28) f32 logits start r * stride floats behind logits_dev.  With
+ * lse = log(sum_j exp(l_j)):
+ *   logprobs [m]:  l[tokens[r]] - lse (a token outside the vocabulary: NaN);
+ *   entropies [m]: -sum_j p_j log p_j, p_j = exp(l_j - lse);
+ *   top_ids, top_logprobs [m][n_top]: the n_top (0 .. 64, at most vocab) largest
+ *                  logits, largest first, of equal ones the lower index first,
+ *                  and their log probabilities.
+ * tokens and logprobs NULL: none of those; entropies NULL: none; n_top 0: no
+ * alternatives.  Logits of minus infinity have no probability.  A row that holds a NaN
+ * or an infinity, or nothing but minus infinity, has none at all: NaN, and
+ * top_ids of -1.  Sums are f32.  Conventions of rdl_quant.h's device entry points;
+ * rows of few are split over workgroups, whose partial results are the stream's
+ * work memory.  The reference samples on the host (rustml/nlp/main/src/core/sampling.rs). */
+rdl_status rdl_logprobs_dev(const float* logits_dev, size_t stride, size_t m, size_t vocab, const int32_t* tokens_dev,
+                            float* logprobs_dev, float* entropies_dev, size_t n_top, int32_t* top_ids_dev,
+                            float* top_logprobs_dev, void* stream);
+
 /* Greedy generation (Generator::generate with argmax sampling): prefill of
  * the prompt (in chunks of max_batch), then n_gen - 1 decode steps, each one
  * replay of a captured graph; out_tokens receives the n_gen sampled ids.

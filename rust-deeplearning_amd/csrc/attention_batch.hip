@@ -10,6 +10,7 @@
 #include "../../include/rdl_attention.h"
 #include "attention.hpp"
 #include "kv_pool.hpp"
+#include "kv_q4.hpp"
 #include "rdl_device.hpp"
 #include "rdl_internal.hpp"
 
@@ -176,8 +177,10 @@ __device__ __forceinline__ void split8(const u32x4 (&x)[2], int e, u32x4* hi, u3
         }
 }
 // Where a launch's keys and values come from: _Float16 and float as they
-// are, Split as f32 rows that split_kernel has made f16 parts of before.
+// are, Split as f32 rows that split_kernel has made f16 parts of before, Q4
+// as 4-bit blocks, whose values are f16 numbers (kv_q4.hpp).
 struct Split {};
+struct Q4 {};
 
 // LDS rows of one key, HDP f16 values without a pad (direct loads fill them
 // 16 bytes a lane in order).  The 16-byte pieces of a row stand in the order
@@ -185,7 +188,7 @@ struct Split {};
 // piece (K) and the transposed reads of 4 rows' 64 bytes (V) fall on all 64 banks.
 template <typename KV, int HD>
 struct Geo {
-    static constexpr bool TWO = !std::is_same<KV, _Float16>::value;  // hi, lo parts
+    static constexpr bool TWO = !std::is_same<KV, _Float16>::value && !std::is_same<KV, Q4>::value;  // hi, lo parts
     static constexpr int PARTS = TWO ? 2 : 1;
     static constexpr int HDP = HD == 96 ? 128 : HD;
     static constexpr int KEY = 2 * HDP * PARTS;              // f16 elements a key
@@ -534,6 +537,103 @@ __device__ __forceinline__ h4 read_t(const void* p) {
     return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
 
+// One wave's slab of SK 4-bit keys: code pieces of 32 values (16 where a slab
+// has fewer than 64 pieces) and their scales into registers, issued a step ahead, then the
+// values as f16 into LDS, laid out as an f16 cache's.
+template <int HD, int SK>
+struct Slab<Q4, HD, SK> {
+    using G = Geo<Q4, HD>;
+    static constexpr int GK = SK < 16 ? SK : 16, NG = SK / GK;       // keys of a page's group
+    static constexpr int LANE = GK * G::HDP / 128;                   // code bytes of a group a lane
+    static constexpr int PB = LANE < 16 ? LANE : 16, LPG = LANE / PB;  // of a piece; pieces a lane
+    static constexpr int NW = PB / 4, PPK = G::HDP / 2 / PB;          // words of a piece, pieces a key
+    static_assert(PB * LPG == LANE && (PB == 8 || PB == 16), "whole pieces");
+    uint32_t k[NG * LPG][NW], v[NG * LPG][NW], kd[NG * LPG], vd[NG * LPG];
+    uint32_t off[LPG], soff[LPG];
+    int pg[NG], row_scales, scales;
+
+    __device__ __forceinline__ void init(const KvSource& s, int hd) {
+        row_scales = hd / Q4_BLOCK * 2;
+        scales = (hd / 2) << s.shift;
+#pragma unroll
+        for (int i = 0; i < LPG; i++) {
+            const int pc = (threadIdx.x & 63) + 64 * i, key = pc / PPK, byte = pc % PPK * PB;
+            const bool in = byte * 2 < hd;
+            off[i] = in ? (uint32_t)(key * (hd / 2) + byte) : RSRC_OOB;
+            soff[i] = in ? (uint32_t)(key * row_scales + byte / 16 * 2) : RSRC_OOB;
+        }
+    }
+    __device__ __forceinline__ void pages(const KvSource& s, const int32_t* table, int j, int t) {
+#pragma unroll
+        for (int g = 0; g < NG; g++) pg[g] = j + g * GK < t ? table[(j + g * GK) >> s.shift] : 0;
+    }
+    __device__ __forceinline__ int load(const KvSource& s, int64_t, int kvh, int j, int t) {
+        int valid = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const int jg = j + g * GK, nv = max(0, min(GK, t - jg));
+            const int p = __builtin_amdgcn_readfirstlane(pg[g]);
+            const bool ok = (uint32_t)p < (uint32_t)s.n_pages;
+            valid |= (int)ok << g;
+            const int rows = ok ? nv : 0;
+            const int64_t run = rows ? p * s.page + kvh * s.head : 0;
+            const int o = rows ? jg & ((1 << s.shift) - 1) : 0;
+            const uint8_t *kb = reinterpret_cast<const uint8_t*>(s.k) + run, *vb = reinterpret_cast<const uint8_t*>(s.v) + run;
+            const int at = o * (int)s.k_position, bytes = rows * (int)s.k_position;
+            const int sat = scales + o * row_scales, sbytes = rows * row_scales;
+            const auto kr = make_rsrc(kb + at, (uint32_t)bytes), vr = make_rsrc(vb + at, (uint32_t)bytes);
+            const auto ks = make_rsrc(kb + sat, (uint32_t)sbytes), vs = make_rsrc(vb + sat, (uint32_t)sbytes);
+#pragma unroll
+            for (int i = 0; i < LPG; i++) {
+                const int n = g * LPG + i;
+                piece(kr, off[i], k[n]);
+                piece(vr, off[i], v[n]);
+                kd[n] = buf_load_b16(ks, soff[i]);
+                vd[n] = buf_load_b16(vs, soff[i]);
+            }
+        }
+        return valid;
+    }
+    static __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, uint32_t at, uint32_t (&w)[NW]) {
+        if constexpr (NW == 4) {
+            const u32x4 x = buf_load_b128(r, at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = x[i];
+        } else {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, 0, 0);
+            w[0] = x[0];
+            w[1] = x[1];
+        }
+    }
+    // Registers to LDS rows row0 .. of ks and vs.  check: whether blocks without
+    // finite values have to be found; their values are then zeroed.
+    __device__ __forceinline__ Meta store(_Float16* ks, _Float16* vs, int2*, int row0, int, int valid, bool check, int, int) {
+        const int lane = threadIdx.x & 63;
+        Meta mt{valid, 0, 0, 0};
+        if (check) {
+            bool found = false;
+#pragma unroll
+            for (int n = 0; n < NG * LPG; n++) {
+                const bool bad = (vd[n] & 0x7C00u) == 0x7C00u;
+                found |= bad;
+                if (bad) vd[n] = 0;
+            }
+            if (__builtin_amdgcn_ballot_w64(found)) mt.flags = SLAB_WIDE;
+        }
+#pragma unroll
+        for (int n = 0; n < NG * LPG; n++) {
+            const int pc = lane + 64 * (n % LPG), row = row0 + n / LPG * GK + pc / PPK, col = pc % PPK * NW;
+            const uint32_t d = kd[n] * 0x10001u, e = vd[n] * 0x10001u;
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+                *reinterpret_cast<u32x4*>(ks + row * G::HDP + ((col + i) ^ G::k_swap(row)) * 8) = q4_values(k[n][i], d);
+                *reinterpret_cast<u32x4*>(vs + row * G::HDP + ((col + i) ^ G::v_swap(row)) * 8) = q4_values(v[n][i], e);
+            }
+        }
+        return mt;
+    }
+};
+
 // Orders a wave's LDS accesses between its lanes.
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -554,7 +654,41 @@ __device__ __forceinline__ const KV* value_row(const KvSource& s, int64_t row0, 
     return reinterpret_cast<const KV*>(s.v) + at;
 }
 
+// The same of a 4-bit cache: a place in the codes of its position's row.
+struct Q4Row {
+    const uint8_t *codes, *scales;
+    int dim;
+    __device__ __forceinline__ explicit operator bool() const { return codes != nullptr; }
+    __device__ __forceinline__ Q4Row operator+(int d) const { return {codes, scales, dim + d}; }
+};
+template <typename KV>
+struct ValueRow {
+    static __device__ __forceinline__ const KV* at(const BatchArgs& a, int64_t row0, const int32_t* table, int kvh, int j) {
+        return value_row<KV>(a.kv, row0, table, kvh, j);
+    }
+};
+template <>
+struct ValueRow<Q4> {
+    static __device__ __forceinline__ Q4Row at(const BatchArgs& a, int64_t, const int32_t* table, int kvh, int j) {
+        const KvSource& s = a.kv;
+        const int32_t p = table[j >> s.shift];
+        if ((uint32_t)p >= (uint32_t)s.n_pages) return {nullptr, nullptr, 0};
+        const int o = j & ((1 << s.shift) - 1);
+        const uint8_t* run = reinterpret_cast<const uint8_t*>(s.v) + p * s.page + kvh * s.head;
+        return {run + o * (a.hd / 2), run + q4_scale_at(1 << s.shift, a.hd, o, 0), 0};
+    }
+};
+
 // Of 4 values those that are not finite, the others (and all without `on`) as 0.
+__device__ __forceinline__ f4 wide4(Q4Row v, bool on) {
+    const uint32_t d = reinterpret_cast<const uint16_t*>(v.scales)[v.dim / Q4_BLOCK];
+    const u32x4 w = q4_values(reinterpret_cast<const uint32_t*>(v.codes)[v.dim / 8], d * 0x10001u);
+    const h4 x = __builtin_bit_cast(h4, (uint64_t)(v.dim & 4 ? w[3] : w[1]) << 32 | (v.dim & 4 ? w[2] : w[0]));
+    f4 y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = on && abs_bits((float)x[i]) >= 0x7F800000u ? (float)x[i] : 0.0f;
+    return y;
+}
 template <typename KV>
 __device__ __forceinline__ f4 wide4(const KV* v, bool on) {
     typedef KV kv4 __attribute__((ext_vector_type(4)));
@@ -946,7 +1080,8 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     using G = Geo<KV, HD>;
     typedef typename std::conditional<std::is_same<KV, Split>::value, float, KV>::type Elem;
     constexpr int TK = G::TK, W = G::W, SK = TK / W, KS = HD / 16, DT = HD / 32, HDP = G::HDP;
-    constexpr bool TWO = G::TWO, RAW32 = std::is_same<KV, float>::value, PRE = std::is_same<KV, Split>::value;
+    constexpr bool TWO = G::TWO, PRE = std::is_same<KV, Split>::value;
+    constexpr bool REGS = std::is_same<KV, float>::value || std::is_same<KV, Q4>::value;  // keys pass through registers
     // blocks of 32 keys that take one softmax step together: two where registers hold their scores
     constexpr int NB = TWO || HD == 256 ? 1 : 2;
     constexpr int PART = TK * HDP;  // a part's elements
@@ -980,7 +1115,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     const int v_row = 4 * h + ((lane & 15) >> 2);
     const uint32_t v_off = (PART * G::PARTS + v_row * HDP +
                             ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ G::v_swap(v_row)) * 8 + 4 * (lane & 1)) * 2;
-    typedef typename std::conditional<RAW32, Slab<float, HD, SK>, DirectSlab<HD, (SK < 16 ? SK : 16)>>::type Stage;
+    typedef typename std::conditional<REGS, Slab<KV, HD, SK>, DirectSlab<HD, (SK < 16 ? SK : 16)>>::type Stage;
     Stage slab;
     int valid = 1;
     [[maybe_unused]] int4 note_next = {0, 0, 0, 0};
@@ -995,7 +1130,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
 #pragma unroll
             for (int i = 0; i < SHARE / 1024; i++)
                 load_to_lds(r, 1024 * i + 16 * lane, lds0 + to * TK * G::KEY * 2 + w * SHARE + 1024 * i);
-        } else if constexpr (RAW32) {
+        } else if constexpr (REGS) {
             valid = slab.load(a.kv, s.row0, kvh, j + SK * w, j_hi);
             slab.pages(a.kv, table, j + TK + SK * w, s.t);
         } else {
@@ -1005,7 +1140,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
         }
     };
     if (j_lo < j_hi) {
-        if constexpr (RAW32) slab.init(a.kv, a.hd);
+        if constexpr (REGS) slab.init(a.kv, a.hd);
         else if constexpr (!PRE) slab.init(a.kv, a.hd, SK * w);
         if constexpr (!PRE) slab.pages(a.kv, table, j_lo + SK * w, s.t);
     }
@@ -1023,8 +1158,9 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
         const int at = buf * TK * G::KEY;  // elements
         Meta note;
         [[maybe_unused]] const int2* key_exps = exps + buf * TK;
-        if constexpr (RAW32) {
-            const Meta mine = slab.store(lds + at, lds + at + PART * 2, exps + buf * TK, SK * w, PART, valid, true, kref, vref);
+        if constexpr (REGS) {
+            const Meta mine = slab.store(lds + at, lds + at + PART * G::PARTS, exps + buf * TK, SK * w, PART, valid,
+                                         TWO || j0 + TK - 1 > wg_first, kref, vref);
             if (lane == 0) meta[buf * W + w] = mine;
             if (j0 + TK < j_hi) fetch(j0 + TK, 0);
             __syncthreads();
@@ -1189,7 +1325,7 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
     }
     if (wide)  // rows that see a value that is not finite
         for (int j = j_lo; j < min(j_hi, w_last + 1); j++) {
-            const Elem* v = value_row<Elem>(a.kv, s.row0, table, kvh, j);
+            const auto v = ValueRow<Elem>::at(a, s.row0, table, kvh, j);
             if (!v) continue;
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -1432,7 +1568,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
         if (wide)  // rows that see a value that is not finite
             for (int j0 = j_w; j0 < j_hi; j0 += step)
                 for (int j = j0; j < min(j0 + FK, j_hi); j++) {
-                    const KV* v = value_row<KV>(a.kv, s.row0, table, kvh, j);
+                    const auto v = ValueRow<KV>::at(a, s.row0, table, kvh, j);
                     if (!v) continue;
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
@@ -1710,7 +1846,7 @@ constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial resu
 constexpr int64_t SPLIT_MIN_TILES = 4;
 constexpr size_t SPLIT_BYTES = (size_t)1 << 30;
 
-rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_t s) {
+rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipStream_t s) {
     const int64_t m = a.m, rows = max_rows == 0 || (int64_t)max_rows > m ? m : (int64_t)max_rows;
     int64_t keys = a.kv.tables ? a.kv.table_stride << a.kv.shift : m;
     if (max_kv != 0 && (int64_t)max_kv < keys) keys = (int64_t)max_kv;
@@ -1756,7 +1892,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
     const int hdp = a.hd <= 64 ? 64 : a.hd <= 128 ? 128 : 256, tk = a.hd <= 64 ? 64 : 32;  // Geo<Split, HD>
     const int64_t tiles = m / tk + a.n_seq;
     const size_t image_bytes = (size_t)tiles * a.n_kv * tk * hdp * 8, note_bytes = (size_t)tiles * a.n_kv * (sizeof(int4) + tk * sizeof(int2));
-    const bool pre = !f16 && !a.kv.tables && only_tile && m * G >= SPLIT_MIN_TILES * TILE_PAIRS * a.n_seq &&
+    const bool pre = dtype == RDL_DTYPE_F32 && !a.kv.tables && only_tile && m * G >= SPLIT_MIN_TILES * TILE_PAIRS * a.n_seq &&
                      image_bytes <= SPLIT_BYTES;
     const size_t part_bytes = a.part_splits > 1 ? (size_t)m * a.n_heads * a.part_splits * (a.hd + 2) * sizeof(float) : 0;
     const size_t part_room = (part_bytes + 255) & ~(size_t)255;
@@ -1780,7 +1916,7 @@ rdl_status run(BatchArgs a, bool f16, size_t max_rows, size_t max_kv, hipStream_
         auto go = a.hd <= 64 ? launch_split<64> : a.hd <= 96 ? launch_split<96> : a.hd <= 128 ? launch_split<128> : launch_split<256>;
         e = go(a, images, notes, exps, (int)tiles, s);
     } else {
-        e = f16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
+        e = dtype == RDL_KV_Q4 ? launch_hd<Q4>(a, s) : dtype == RDL_DTYPE_F16 ? launch_hd<_Float16>(a, s) : launch_hd<float>(a, s);
     }
     const rdl_status done = call_scratch_done(s, &work);
     HIP_TRY(e);
@@ -1843,7 +1979,7 @@ rdl_status rdl_attention_paged_dev(const rdl_kv_pool* pool, const float* q_dev, 
     a.kv = {p.k, p.v, p.position_stride, p.position_stride, p.head_stride, p.page_stride, tables_dev,
             (int64_t)table_stride, p.n_pages, p.shift};
     a.kv_len = kv_len_dev;
-    return rdl::run(a, p.f16, max_rows, max_kv, (hipStream_t)stream);
+    return rdl::run(a, p.dtype, max_rows, max_kv, (hipStream_t)stream);
 }
 
 rdl_status rdl_attention_packed_dev(const float* q_dev, size_t q_stride, size_t n_heads, const void* k_dev,
@@ -1869,7 +2005,7 @@ rdl_status rdl_attention_packed_dev(const float* q_dev, size_t q_stride, size_t 
         return api_fail(RDL_ERR_INVALID_DATA, "out overlaps k or v");
     if ((st = rdl::check_position_stride(k_stride > v_stride ? k_stride : v_stride)) != RDL_OK) return st;
     a.kv = {k_dev, v_dev, (int64_t)k_stride, (int64_t)v_stride, (int64_t)head_dim, 0, nullptr, 0, 0, 0};
-    return rdl::run(a, kv_dtype == RDL_DTYPE_F16, max_rows, max_rows, (hipStream_t)stream);
+    return rdl::run(a, kv_dtype, max_rows, max_rows, (hipStream_t)stream);
 }
 
 }  // extern "C"

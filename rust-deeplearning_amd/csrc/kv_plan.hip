@@ -3,12 +3,15 @@
 // lengths, and RoPE with the write of k and v rows through the slots.
 #include <hip/hip_runtime.h>
 #include <limits.h>
+#include <math.h>
 
 #include <algorithm>
 #include <utility>
 
 #include "../../include/rdl_attention.h"
 #include "kv_pool.hpp"
+#include "kv_q4.hpp"
+#include "kv_store_norm.hpp"
 #include "rdl_device.hpp"
 #include "rdl_internal.hpp"
 
@@ -250,23 +253,29 @@ __global__ __launch_bounds__(STORE_NT) void store_kernel(StoreArgs a) {
 
 rdl_status check_pool(const rdl_kv_pool* p, PoolView* v) {
     if (!p) return api_fail(RDL_ERR_NULL_POINTER, "pool is NULL");
-    if (p->dtype != RDL_DTYPE_F16 && p->dtype != RDL_DTYPE_F32)
-        return api_fail(RDL_ERR_DTYPE_MISMATCH, "cache dtype %d: F32 (0) or F16 (1)", p->dtype);
+    const bool q4 = p->dtype == RDL_KV_Q4;
+    if (p->dtype != RDL_DTYPE_F16 && p->dtype != RDL_DTYPE_F32 && !q4)
+        return api_fail(RDL_ERR_DTYPE_MISMATCH, "cache dtype %d: F32 (0), F16 (1) or Q4 (%d)", p->dtype, RDL_KV_Q4);
     int shift = 0;
     rdl_status st = check_page_positions(p->page_positions > 0 ? (size_t)p->page_positions : 0, &shift);
     if (st != RDL_OK) return st;
     if ((st = check_head_dim(p->head_dim > 0 ? (size_t)p->head_dim : 0)) != RDL_OK) return st;
+    if (q4 && p->head_dim % Q4_BLOCK)
+        return api_fail(RDL_ERR_UNSUPPORTED, "head_dim %d in 4 bits: a multiple of 32", p->head_dim);
     if (p->n_kv_heads <= 0 || p->n_kv_heads > 65535 || p->n_pages < 0)
         return api_fail(RDL_ERR_INVALID_DATA, "pool of %d pages, %d KV heads", p->n_pages, p->n_kv_heads);
-    const int64_t unit = p->dtype == RDL_DTYPE_F16 ? 8 : 4;
-    if (p->page_stride % unit || p->head_stride % unit || p->position_stride % unit || ((uintptr_t)p->k_dev & 15) ||
+    if (q4 && p->position_stride != p->head_dim / 2)
+        return api_fail(RDL_ERR_SHAPE_MISMATCH, "position stride %lld: %d bytes of codes", (long long)p->position_stride,
+                        p->head_dim / 2);
+    const int64_t unit = q4 ? 16 : p->dtype == RDL_DTYPE_F16 ? 8 : 4;
+    if (p->page_stride % unit || p->head_stride % unit || (!q4 && p->position_stride % unit) || ((uintptr_t)p->k_dev & 15) ||
         ((uintptr_t)p->v_dev & 15))
         return api_fail(RDL_ERR_INVALID_DATA, "pool strides and bases must be multiples of 16 bytes");
     if (p->position_stride > 0 && (st = check_position_stride((size_t)p->position_stride)) != RDL_OK) return st;
     // the axes from the innermost out: each must step over all that the ones inside it span
     struct Axis {
         int64_t stride, count;
-    } ax[3] = {{p->page_stride, p->n_pages}, {p->head_stride, p->n_kv_heads}, {p->position_stride, p->page_positions}};
+    } ax[3] = {{p->page_stride, p->n_pages}, {p->head_stride, p->n_kv_heads}, {p->position_stride, q4 ? 1 : p->page_positions}};
     for (int i = 0; i < 3; i++)
         for (int j = i + 1; j < 3; j++)
             if (ax[j].stride < ax[i].stride) {
@@ -274,7 +283,8 @@ rdl_status check_pool(const rdl_kv_pool* p, PoolView* v) {
                 ax[i] = ax[j];
                 ax[j] = t;
             }
-    int64_t span = p->head_dim;  // elements the axes inside take
+    // elements the axes inside take (4 bits: bytes of a head's page, which is one run)
+    int64_t span = q4 ? q4_run_bytes(p->page_positions, p->head_dim) : p->head_dim;
     for (const Axis& x : ax) {
         if (x.count <= 1) continue;
         int64_t reach = 0;
@@ -284,7 +294,7 @@ rdl_status check_pool(const rdl_kv_pool* p, PoolView* v) {
                             (long long)p->page_stride, (long long)p->head_stride, (long long)p->position_stride);
     }
     if (p->n_pages > 0 && (!p->k_dev || !p->v_dev)) return api_fail(RDL_ERR_NULL_POINTER, "NULL pool memory");
-    *v = PoolView{p->k_dev, p->v_dev, p->dtype == RDL_DTYPE_F16, p->n_pages, shift, p->n_kv_heads, p->head_dim,
+    *v = PoolView{p->k_dev, p->v_dev, p->dtype, p->n_pages, shift, p->n_kv_heads, p->head_dim,
                   p->page_stride, p->head_stride, p->position_stride};
     return RDL_OK;
 }
@@ -339,6 +349,53 @@ rdl_status check_stream(hipStream_t s) {
     return RDL_OK;
 }
 
+// The checks of the two cache writes; fills all of `a` but the norms. (m 0: the pool alone is checked.)
+static rdl_status check_store(const rdl_kv_pool* pool, size_t m, const float* q_dev, size_t q_stride, float* q_out_dev,
+                              size_t q_out_stride, size_t n_heads, const float* k_dev, size_t k_stride,
+                              const float* v_dev, size_t v_stride, const int32_t* positions_dev,
+                              const int32_t* slots_dev, const float* cos_dev, const float* sin_dev, size_t n_positions,
+                              void* stream, StoreNormArgs* out) {
+    StoreNormArgs& a = *out;
+    rdl_status st = check_pool(pool, &a.pool);
+    if (st != RDL_OK || m == 0) return st;
+    const size_t hd = (size_t)pool->head_dim, kvw = (size_t)pool->n_kv_heads * hd;
+    if (n_heads > 65535) return api_fail(RDL_ERR_UNSUPPORTED, "%zu heads", n_heads);
+    if (n_heads) {
+        if ((st = check_rows("q", q_dev, q_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
+        if ((st = check_rows("q_out", q_out_dev, q_out_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
+        if (!(q_dev == q_out_dev && q_stride == q_out_stride) &&
+            rows_overlap(q_dev, q_stride * 4, n_heads * hd * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
+            return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps q (the same rows, or none of them)");
+    }
+    if ((st = check_rows("k", k_dev, k_stride, kvw, m, 4)) != RDL_OK) return st;
+    if ((st = check_rows("v", v_dev, v_stride, kvw, m, 4)) != RDL_OK) return st;
+    if (n_heads)
+        for (const auto& x : {std::make_pair(k_dev, k_stride), std::make_pair(v_dev, v_stride)})
+            if (rows_overlap(x.first, x.second * 4, kvw * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
+                return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps k or v");
+    if (!slots_dev || !cos_dev != !sin_dev || (cos_dev && !positions_dev))
+        return api_fail(RDL_ERR_NULL_POINTER, "NULL device pointer");
+    if (((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15)
+        return api_fail(RDL_ERR_INVALID_DATA, "cos and sin must be 16-byte aligned");
+    if ((st = check_stream((hipStream_t)stream)) != RDL_OK) return st;
+    a.m = (int64_t)m;
+    a.q = q_dev;
+    a.q_stride = (int64_t)q_stride;
+    a.q_out = q_out_dev;
+    a.q_out_stride = (int64_t)q_out_stride;
+    a.n_heads = (int)n_heads;
+    a.k = k_dev;
+    a.v = v_dev;
+    a.k_stride = (int64_t)k_stride;
+    a.v_stride = (int64_t)v_stride;
+    a.positions = positions_dev;
+    a.slots = slots_dev;
+    a.cos_t = cos_dev;
+    a.sin_t = sin_dev;
+    a.n_positions = (int64_t)n_positions;
+    return RDL_OK;
+}
+
 }  // namespace rdl
 
 using rdl::api_fail;
@@ -389,52 +446,47 @@ rdl_status rdl_kv_store_dev(const rdl_kv_pool* pool, size_t m, const float* q_de
                             const float* v_dev, size_t v_stride, const int32_t* positions_dev,
                             const int32_t* slots_dev, const float* cos_dev, const float* sin_dev, size_t n_positions,
                             void* stream) {
-    rdl::StoreArgs a{};
-    rdl_status st = rdl::check_pool(pool, &a.pool);
+    rdl::StoreNormArgs n{};
+    const rdl_status st = rdl::check_store(pool, m, q_dev, q_stride, q_out_dev, q_out_stride, n_heads, k_dev, k_stride,
+                                           v_dev, v_stride, positions_dev, slots_dev, cos_dev, sin_dev, n_positions,
+                                           stream, &n);
     if (st != RDL_OK) return st;
     if (m == 0) return api_ok();
-    const size_t hd = (size_t)pool->head_dim, kvw = (size_t)pool->n_kv_heads * hd;
-    if (n_heads > 65535) return api_fail(RDL_ERR_UNSUPPORTED, "%zu heads", n_heads);
-    if (n_heads) {
-        if ((st = rdl::check_rows("q", q_dev, q_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
-        if ((st = rdl::check_rows("q_out", q_out_dev, q_out_stride, n_heads * hd, m, 4)) != RDL_OK) return st;
-        if (!(q_dev == q_out_dev && q_stride == q_out_stride) &&
-            rdl::rows_overlap(q_dev, q_stride * 4, n_heads * hd * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
-            return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps q (the same rows, or none of them)");
+    if (n.pool.dtype == RDL_KV_Q4) {
+        HIP_TRY(rdl::launch_store_norm(n, (hipStream_t)stream));
+        return api_ok();
     }
-    if ((st = rdl::check_rows("k", k_dev, k_stride, kvw, m, 4)) != RDL_OK) return st;
-    if ((st = rdl::check_rows("v", v_dev, v_stride, kvw, m, 4)) != RDL_OK) return st;
-    if (n_heads)
-        for (const auto& x : {std::make_pair(k_dev, k_stride), std::make_pair(v_dev, v_stride)})
-            if (rdl::rows_overlap(x.first, x.second * 4, kvw * 4, q_out_dev, q_out_stride * 4, n_heads * hd * 4, m))
-                return api_fail(RDL_ERR_INVALID_DATA, "q_out overlaps k or v");
-    if (!slots_dev || !cos_dev != !sin_dev || (cos_dev && !positions_dev))
-        return api_fail(RDL_ERR_NULL_POINTER, "NULL device pointer");
-    if (((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15)
-        return api_fail(RDL_ERR_INVALID_DATA, "cos and sin must be 16-byte aligned");
-    if ((st = rdl::check_stream((hipStream_t)stream)) != RDL_OK) return st;
-    a.m = (int64_t)m;
-    a.q = q_dev;
-    a.q_stride = (int64_t)q_stride;
-    a.q_out = q_out_dev;
-    a.q_out_stride = (int64_t)q_out_stride;
-    a.n_heads = (int)n_heads;
-    a.k = k_dev;
-    a.v = v_dev;
-    a.k_stride = (int64_t)k_stride;
-    a.v_stride = (int64_t)v_stride;
-    a.positions = positions_dev;
-    a.slots = slots_dev;
-    a.cos_t = cos_dev;
-    a.sin_t = sin_dev;
-    a.n_positions = (int64_t)n_positions;
-    const size_t units = (n_heads + 2 * (size_t)pool->n_kv_heads) * (hd / 8);
+    const rdl::StoreArgs a{n.pool, n.m, n.q, n.q_stride, n.q_out, n.q_out_stride, n.n_heads, n.k, n.v, n.k_stride, n.v_stride,
+                           n.positions, n.slots, n.cos_t, n.sin_t, n.n_positions};
+    const size_t units = (n_heads + 2 * (size_t)pool->n_kv_heads) * ((size_t)pool->head_dim / 8);
     const dim3 grid((unsigned)((units + rdl::STORE_NT - 1) / rdl::STORE_NT), (unsigned)(m < 65535 ? m : 65535));
-    if (a.pool.f16)
+    if (a.pool.dtype == RDL_DTYPE_F16)
         hipLaunchKernelGGL(rdl::store_kernel<_Float16>, grid, dim3(rdl::STORE_NT), 0, (hipStream_t)stream, a);
     else
         hipLaunchKernelGGL(rdl::store_kernel<float>, grid, dim3(rdl::STORE_NT), 0, (hipStream_t)stream, a);
     HIP_TRY(hipGetLastError());
+    return api_ok();
+}
+
+rdl_status rdl_kv_store_norm_dev(const rdl_kv_pool* pool, size_t m, const float* q_dev, size_t q_stride,
+                                 float* q_out_dev, size_t q_out_stride, size_t n_heads, const float* k_dev,
+                                 size_t k_stride, const float* v_dev, size_t v_stride, const float* q_gamma_dev,
+                                 const float* k_gamma_dev, float eps, const int32_t* positions_dev,
+                                 const int32_t* slots_dev, const float* cos_dev, const float* sin_dev,
+                                 size_t n_positions, void* stream) {
+    rdl::StoreNormArgs n{};
+    if (!(eps >= 0.0f) || !isfinite(eps)) return api_fail(RDL_ERR_INVALID_DATA, "eps %g: finite, not negative", eps);
+    if (((uintptr_t)q_gamma_dev | (uintptr_t)k_gamma_dev) & 15)
+        return api_fail(RDL_ERR_INVALID_DATA, "q_gamma and k_gamma must be 16-byte aligned");
+    const rdl_status st = rdl::check_store(pool, m, q_dev, q_stride, q_out_dev, q_out_stride, n_heads, k_dev, k_stride,
+                                           v_dev, v_stride, positions_dev, slots_dev, cos_dev, sin_dev, n_positions,
+                                           stream, &n);
+    if (st != RDL_OK) return st;
+    if (m == 0) return api_ok();
+    n.q_gamma = q_gamma_dev;
+    n.k_gamma = k_gamma_dev;
+    n.eps = eps;
+    HIP_TRY(rdl::launch_store_norm(n, (hipStream_t)stream));
     return api_ok();
 }
 

@@ -12,11 +12,11 @@ namespace rdl {
 
 struct PoolView {
     void *k, *v;
-    bool f16;
+    int32_t dtype;  // RDL_DTYPE_F16, RDL_DTYPE_F32 or RDL_KV_Q4 (strides in bytes)
     int n_pages, shift;  // shift: log2(page_positions)
     int n_kv_heads, head_dim;
     int64_t page_stride, head_stride, position_stride;
-    // element offset of position pos (any multiple of the page size may be added) on page pg
+    // element offset (4 bits: that of the codes) of position pos (any multiple of the page size may be added) on page pg
     __device__ __forceinline__ int64_t at(int pg, int kvh, int pos) const {
         return pg * page_stride + kvh * head_stride + (pos & ((1 << shift) - 1)) * position_stride;
     }

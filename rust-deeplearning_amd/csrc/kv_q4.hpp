@@ -1,0 +1,68 @@
+// kv_q4.hpp -- the 4-bit cache's blocks on the device (RDL_KV_Q4,
+// include/rdl_attention.h): 32 values of one position and head as a scale d
+// and codes n, value = d (n - 8).  d has 8 significant bits and n - 8 at most
+// 3, so a value is an f16 number without a rounding: the attention's products
+// are those of an f16 cache.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "rdl_device.hpp"
+
+namespace rdl {
+
+constexpr int Q4_BLOCK = 32;
+constexpr float Q4_MOST = 8160.0f;         // largest scale: 8 times it lies within f16
+constexpr uint32_t Q4_NAN = 0x7E00u;       // the scale of a block with a value that is not finite
+// A head's page: the codes of its positions, then their scales.
+__host__ __device__ __forceinline__ int64_t q4_run_bytes(int64_t positions, int hd) {
+    return positions * (hd / 2 + hd / Q4_BLOCK * 2);
+}
+__device__ __forceinline__ int q4_scale_at(int positions, int hd, int pos, int dim) {
+    return positions * (hd / 2) + (pos * (hd / Q4_BLOCK) + dim / Q4_BLOCK) * 2;
+}
+
+typedef _Float16 q4h2 __attribute__((ext_vector_type(2)));
+
+// The 8 values of a code word, in order, times the scale in both halves of d.
+// A nibble under an exponent is a whole number of steps above a power of two:
+// 1024 + n in bits 0 .. 3 of f16, 64 + n in bits 4 .. 7.
+__device__ __forceinline__ u32x4 q4_values(uint32_t w, uint32_t d) {
+    const q4h2 dd = __builtin_bit_cast(q4h2, d);
+    u32x4 out;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t x = w >> (8 * i);
+        const q4h2 a = __builtin_bit_cast(q4h2, (x & 0x000F000Fu) | 0x64006400u);
+        const q4h2 b = __builtin_bit_cast(q4h2, (x & 0x00F000F0u) | 0x54005400u);
+        const q4h2 va = (a - q4h2{(_Float16)1032.0f, (_Float16)1032.0f}) * dd;
+        const q4h2 vb = (b - q4h2{(_Float16)72.0f, (_Float16)72.0f}) * dd;
+        out[2 * i] = __builtin_bit_cast(uint32_t, va);
+        out[2 * i + 1] = __builtin_bit_cast(uint32_t, vb);
+    }
+    return out;
+}
+
+// The scale of a block: mag, the bits of its largest magnitude, and whether a
+// positive value has it.  f16 bits.
+__device__ __forceinline__ uint32_t q4_scale(uint32_t mag, bool positive) {
+    if (mag >= 0x7F800000u) return Q4_NAN;
+    const uint32_t u = __builtin_bit_cast(uint32_t, as_f32((int32_t)mag) * 0.125f);
+    const uint32_t b = (u + 0x7FFFu + (u >> 16 & 1)) & 0xFFFF0000u;  // 8 significant bits, to nearest
+    const _Float16 h = (_Float16)fminf(as_f32((int32_t)b), Q4_MOST);
+    return (uint32_t)__builtin_bit_cast(uint16_t, h) | (positive ? 0x8000u : 0u);
+}
+// The code of x under scale d (as f32; inv: 1 / d or so): x / d to the nearest
+// whole number, halves to even, which the rounded quotient alone would miss
+// beside a half: the remainder of the nearest code, exact in f32, decides.
+__device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
+    float c = rintf(x * inv);
+    const float rest = fmaf(-c, d, x), twice = 2.0f * fabsf(rest), size = fabsf(d);
+    const float step = (__builtin_bit_cast(uint32_t, rest) ^ __builtin_bit_cast(uint32_t, d)) >> 31 ? -1.0f : 1.0f;
+    const bool odd = ((int)c & 1) != 0;  // (far out, where the code is cut, either will do)
+    if (twice > size || (twice == size && odd)) c += step;
+    return (uint32_t)(int)(fminf(fmaxf(c, -8.0f), 7.0f) + 8.0f);
+}
+
+}  // namespace rdl

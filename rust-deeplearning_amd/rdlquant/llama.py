@@ -64,6 +64,16 @@ class _GgufOptions(C.Structure):
 
 
 _decl("rdl_llama_load_gguf", _i32, _p, C.POINTER(_GgufOptions), C.POINTER(_p))
+_decl("rdl_logprobs_dev", _i32, _p, _sz, _sz, _sz, _p, _p, _p, _sz, _p, _p, _p)
+
+
+def logprobs_dev(logits_ptr, stride, m, vocab, tokens_ptr, logprobs_ptr, entropies_ptr, n_top, top_ids_ptr,
+                 top_logprobs_ptr, stream=0):
+    """rdl_logprobs_dev: log probabilities of given tokens, entropies and the
+    n_top most likely tokens of m rows of f32 logits on the device (pointers as
+    ints; tokens and logprobs 0, entropies 0, n_top 0: none of those)."""
+    check(lib.rdl_logprobs_dev(logits_ptr, stride, m, vocab, tokens_ptr or None, logprobs_ptr or None,
+                               entropies_ptr or None, n_top, top_ids_ptr or None, top_logprobs_ptr or None, stream))
 
 
 @dataclass
