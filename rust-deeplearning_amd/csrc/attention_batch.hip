@@ -44,6 +44,8 @@ struct BatchArgs {
     int tiles, tile_splits, few_splits;
     int tile_span, few_span;  // keys a split
     int tile_slots;           // not 0: the splits of all tiles that the launch has room for (tile_plan)
+    int few_slots;            // not 0: the splits of all sequences that the launch has room for (few_plan)
+    bool packed;              // few rows of at most 8 pairs over a 4-bit cache (few_rows_q4)
     int few_rows;             // sequences of at most this many (row, head of a group) pairs are few-row ones
     float* part;              // [m][n_heads][part_splits][hd]
     float* part_ml;           // [m][n_heads][part_splits][2]
@@ -195,7 +197,11 @@ struct Geo {
     static constexpr int W = 4;                              // waves of a workgroup, 32 pairs each of a tile
     static constexpr int TK = HD == 64 ? 64 : TWO || HD == 256 ? 32 : 64;  // keys of a tile
     static constexpr int FK = TWO ? 16 : 32;                 // keys a wave takes at a time for few rows
-    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = (size_t)W * FK * KEY * 2;
+    // of few rows: a wave's keys, then its 16 pairs' outputs; 4-bit keys stay in registers
+    static constexpr int FHD = HD == 96 && std::is_same<KV, Q4>::value ? 128 : HD, FROW = FHD + 4;
+    static constexpr size_t FEW_WAVE = std::is_same<KV, Q4>::value ? 16 * FROW * 4 : (size_t)FK * KEY * 2;
+    static_assert(16 * FROW * 4 <= FEW_WAVE, "the output fits the wave's key rows");
+    static constexpr size_t TILE_LDS = (size_t)2 * TK * KEY * 2, FEW_LDS = W * FEW_WAVE;
     static constexpr size_t LDS = TILE_LDS > FEW_LDS ? TILE_LDS : FEW_LDS;
     static_assert(LDS <= 160 * 1024 - 6144, "LDS of a CU");
     static __device__ __forceinline__ int k_swap(int row) { return HDP == 64 ? (row >> 1) & 7 : row & 15; }
@@ -620,14 +626,15 @@ struct Slab<Q4, HD, SK> {
             }
             if (__builtin_amdgcn_ballot_w64(found)) mt.flags = SLAB_WIDE;
         }
+        const Q4Decoder decode;
 #pragma unroll
         for (int n = 0; n < NG * LPG; n++) {
             const int pc = lane + 64 * (n % LPG), row = row0 + n / LPG * GK + pc / PPK, col = pc % PPK * NW;
-            const uint32_t d = kd[n] * 0x10001u, e = vd[n] * 0x10001u;
+            const q4h2 d = __builtin_bit_cast(q4h2, perm(kd[n], kd[n], 0x05040100u)), e = __builtin_bit_cast(q4h2, perm(vd[n], vd[n], 0x05040100u));
 #pragma unroll
             for (int i = 0; i < NW; i++) {
-                *reinterpret_cast<u32x4*>(ks + row * G::HDP + ((col + i) ^ G::k_swap(row)) * 8) = q4_values(k[n][i], d);
-                *reinterpret_cast<u32x4*>(vs + row * G::HDP + ((col + i) ^ G::v_swap(row)) * 8) = q4_values(v[n][i], e);
+                *reinterpret_cast<u32x4*>(ks + row * G::HDP + ((col + i) ^ G::k_swap(row)) * 8) = decode.word(k[n][i], d);
+                *reinterpret_cast<u32x4*>(vs + row * G::HDP + ((col + i) ^ G::v_swap(row)) * 8) = decode.word(v[n][i], e);
             }
         }
         return mt;
@@ -682,7 +689,7 @@ struct ValueRow<Q4> {
 // Of 4 values those that are not finite, the others (and all without `on`) as 0.
 __device__ __forceinline__ f4 wide4(Q4Row v, bool on) {
     const uint32_t d = reinterpret_cast<const uint16_t*>(v.scales)[v.dim / Q4_BLOCK];
-    const u32x4 w = q4_values(reinterpret_cast<const uint32_t*>(v.codes)[v.dim / 8], d * 0x10001u);
+    const u32x4 w = Q4Decoder().word(reinterpret_cast<const uint32_t*>(v.codes)[v.dim / 8], __builtin_bit_cast(q4h2, d * 0x10001u));
     const h4 x = __builtin_bit_cast(h4, (uint64_t)(v.dim & 4 ? w[3] : w[1]) << 32 | (v.dim & 4 ? w[2] : w[0]));
     f4 y;
 #pragma unroll
@@ -760,6 +767,8 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
 // to 1900 f32 keys with TILE_MIN_SPAN 128, 256, 512: 22.8, 25.0, 36.7.
 constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512, MIXED_TARGET = 384;
 constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 128;
+// few_plan: workgroups that run at once (wide heads: a third of them), and the keys that one's waves take in a turn.
+constexpr int FEW_SLOTS = 768, FEW_UNIT = 128, FEW_BEGIN = 4;
 
 // Tiles are numbered so that a sequence is found from row_start alone:
 // sequence b's are TILE_PAIRS pairs each and numbered from row_start[b] group
@@ -919,9 +928,13 @@ template <int NS>
 struct QRow {
     f4 x[NS][2];
     __device__ __forceinline__ void load(const float* q, bool live, int d0, int step, int hd) {
+        load_at(q, live, [=](int i) { return d0 + i * step; }, hd);
+    }
+    template <typename Dim>
+    __device__ __forceinline__ void load_at(const float* q, bool live, Dim&& dim, int hd) {
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-            const int d = d0 + i * step;
+            const int d = dim(i);
 #pragma unroll
             for (int c = 0; c < 2; c++)
                 x[i][c] = live && d < hd ? *reinterpret_cast<const f4*>(q + d + 4 * c) : f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1374,6 +1387,47 @@ __device__ __forceinline__ void tile_rows(const BatchArgs& a, const Seq& s, cons
         *reinterpret_cast<f2*>(a.part_ml + (place(a, s, kvh, p) * a.part_splits + z) * 2) = f2{M, L};
 }
 
+// The waves' outputs of few rows (in each wave's LDS), maxima and sums: joined
+// and written, or stored as a split's partial.  Returns the splits to join.
+template <typename G>
+__device__ __forceinline__ int join_waves(const BatchArgs& a, const Seq& s, int kvh, int p0, int pairs, int z, int splits,
+                                          const _Float16* lds, const float* wml) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs * (G::FHD / 4); i += G::W * 64) {
+        const int pi = i / (G::FHD / 4), dim = (i % (G::FHD / 4)) * 4;
+        if (dim >= a.hd) continue;
+        float Mx = -__builtin_inff(), Ls = 0.0f;
+#pragma unroll
+        for (int x = 0; x < G::W; x++)
+            if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
+        auto partial = [&](int x) {
+            return *reinterpret_cast<const f4*>(reinterpret_cast<const uint8_t*>(lds) + x * G::FEW_WAVE + (pi * G::FROW + dim) * 4);
+        };
+        float wt[G::W];
+#pragma unroll
+        for (int x = 0; x < G::W; x++) {
+            const float l = wml[x * 32 + 16 + pi];
+            wt[x] = l != 0.0f ? l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx) : 0.0f;
+            Ls += wt[x];
+        }
+        const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < G::W; x++) y += wt[x] * inv * partial(x);  // weights of at most 1: large values stay in range
+        if (some_not_finite(y)) y = sum_not_finite(y, G::W, partial);
+        if (splits == 1) {
+            *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y;
+        } else {
+            const int64_t at = place(a, s, kvh, p0 + pi);
+            float* pt = a.part + (at * a.part_splits + z) * a.hd + dim;
+            put2(pt, y[0], y[1]);
+            put2(pt + 2, y[2], y[3]);
+            if (dim == 0) put_ml(a, at, z, Mx, Ls);
+        }
+    }
+    return splits;
+}
+
 // ---- few rows: up to 16 pairs, each wave its own keys ------------------------------------------
 // A decode step reads the cache once and computes little: the waves of a
 // workgroup take the split's keys 32 at a time in turn, each through LDS rows
@@ -1392,8 +1446,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
     constexpr int KS = HD / 32, DT = HD / 16, FK = G::FK, NB = FK / 16, W = G::W, HDP = G::HDP;
     constexpr bool F32 = G::TWO;
     constexpr int PART = FK * HDP;
-    constexpr int OROW = HD + 4;  // f32 elements of a pair's joined output
-    static_assert(16 * OROW * 4 <= FK * G::KEY * 2, "the output fits the wave's key rows");
+    constexpr int OROW = G::FROW;  // f32 elements of a pair's joined output
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int pairs = min(FEW_PAIRS, s.pairs - p0);
@@ -1583,40 +1636,297 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
             wml[w * 32 + 16 + c] = L;
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs * (HD / 4); i += W * 64) {
-        const int pi = i / (HD / 4), dim = (i % (HD / 4)) * 4;
-        if (dim >= a.hd) continue;
-        float Mx = -__builtin_inff(), Ls = 0.0f;
+    return join_waves<G>(a, s, kvh, p0, pairs, z, splits, lds, wml);
+}
+
+// Few rows over 4-bit keys: the same products with both operands formed in
+// registers, so that nothing passes through LDS before the waves join.  A slab of
+// 32 keys a wave, its two groups of 16 each on a page:
+//   K: lane (g, c) = (lane / 16, lane % 16) loads the codes of 32 dims of key c (32 g .., 64-wide heads 16 of
+//      them), one load and one scale, which are the A operands of four steps of
+//      S^T = K Q^T, a code word a step; q is laid out to match;
+//   V: O^T = V^T P^T needs a dim's values of eight keys a lane.  Lane (g, c) loads
+//      the word of dims 8 c .. 8 c + 7 of each of the eight keys whose weights it holds,
+//      an 8 x 8 block of nibbles: dim 8 c + t of all of them, two keys an instruction, is its A
+//      operand of tile t, whose 16 rows are the dims t of the 16 words (64-wide
+//      heads: half words of 4 dims each).
+template <int HD>
+struct FourBits {
+    static constexpr int NH = HD > 128 ? 2 : 1;         // 128-dim parts
+    static constexpr bool HALF = HD == 64;
+    static constexpr int KW = HALF ? 2 : 4;              // words of a K piece
+    static constexpr int TILES = HALF ? 4 : 8;           // of 16 dims a part
+    typedef typename std::conditional<HALF, uint16_t, uint32_t>::type Word;
+    uint32_t k[2][NH][KW];
+    Word v[8][NH];
+    struct alignas(4) Scale {  // a register each
+        _Float16 x;
+    };
+    Scale kd[2][NH], vd[8][NH];
+};
+template <int HD>
+struct FourSlab {
+    typedef FourBits<HD> Bits;
+    uint32_t k_off[Bits::NH], kd_off[Bits::NH], v_off[Bits::NH], vd_off[Bits::NH];  // of V: the first of four keys
+    int pg[2], row, row_scales, scales;
+    __device__ __forceinline__ void init(const KvSource& s, int hd) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        row = hd / 2;
+        row_scales = hd / Q4_BLOCK * 2;
+        scales = row << s.shift;
 #pragma unroll
-        for (int x = 0; x < W; x++)
-            if (wml[x * 32 + 16 + pi] != 0.0f) Mx = fmaxf(Mx, wml[x * 32 + pi]);
-        auto partial = [&](int x) {
-            return *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + x * FK * G::KEY) + pi * OROW + dim);
-        };
-        float wt[W];
-#pragma unroll
-        for (int x = 0; x < W; x++) {
-            const float l = wml[x * 32 + 16 + pi];
-            wt[x] = l != 0.0f ? l * __builtin_amdgcn_exp2f(wml[x * 32 + pi] - Mx) : 0.0f;
-            Ls += wt[x];
-        }
-        const float inv = Ls != 0.0f ? 1.0f / Ls : 0.0f;
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int x = 0; x < W; x++) y += wt[x] * inv * partial(x);  // weights of at most 1: large values stay in range
-        if (some_not_finite(y)) y = sum_not_finite(y, W, partial);
-        if (splits == 1) {
-            *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pi) + dim) = y;
-        } else {
-            const int64_t at = place(a, s, kvh, p0 + pi);
-            float* pt = a.part + (at * a.part_splits + z) * a.hd + dim;
-            put2(pt, y[0], y[1]);
-            put2(pt + 2, y[2], y[3]);
-            if (dim == 0) put_ml(a, at, z, Mx, Ls);
+        for (int i = 0; i < Bits::NH; i++) {
+            const int kb = 64 * i + g * Bits::KW * 4, vb = 64 * i + c * (Bits::HALF ? 2 : 4);  // bytes in a row
+            k_off[i] = kb < row ? (uint32_t)(c * row + kb) : RSRC_OOB;
+            kd_off[i] = kb < row ? (uint32_t)(c * row_scales + kb / 16 * 2) : RSRC_OOB;
+            v_off[i] = vb < row ? (uint32_t)(4 * g * row + vb) : RSRC_OOB;
+            vd_off[i] = vb < row ? (uint32_t)(4 * g * row_scales + vb / 16 * 2) : RSRC_OOB;
         }
     }
-    return splits;
+    __device__ __forceinline__ void pages(const KvSource& s, const int32_t* table, int j, int t) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) pg[b] = j + 16 * b < t ? table[(j + 16 * b) >> s.shift] : 0;
+    }
+    static __device__ __forceinline__ _Float16 half_of(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+        return __builtin_bit_cast(_Float16, __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0));
+    }
+    // issues the loads of the slab at key j; bit b: group b's page is in the pool
+    __device__ __forceinline__ int load(const KvSource& s, int kvh, int j, int t, Bits* x) const {
+        int valid = 0;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int jb = j + 16 * b, p = __builtin_amdgcn_readfirstlane(pg[b]);
+            const bool ok = (uint32_t)p < (uint32_t)s.n_pages;
+            valid |= (int)ok << b;
+            const int rows = ok ? max(0, min(16, t - jb)) : 0;
+            const int64_t run = rows ? p * s.page + kvh * s.head : 0;
+            const int o = rows ? jb & ((1 << s.shift) - 1) : 0;
+            const uint8_t *kb = reinterpret_cast<const uint8_t*>(s.k) + run, *vb = reinterpret_cast<const uint8_t*>(s.v) + run;
+            const int at = o * row, sat = scales + o * row_scales;
+            const auto kr = make_rsrc(kb + at, (uint32_t)(rows * row)), vr = make_rsrc(vb + at, (uint32_t)(rows * row));
+            const auto ks = make_rsrc(kb + sat, (uint32_t)(rows * row_scales)), vs = make_rsrc(vb + sat, (uint32_t)(rows * row_scales));
+#pragma unroll
+            for (int i = 0; i < Bits::NH; i++) {
+                if constexpr (Bits::HALF) {
+                    const auto w = __builtin_amdgcn_raw_buffer_load_b64(kr, (int)k_off[i], 0, 0);
+                    x->k[b][i][0] = w[0], x->k[b][i][1] = w[1];
+                } else {
+                    const u32x4 w = buf_load_b128(kr, k_off[i]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) x->k[b][i][u] = w[u];
+                }
+                // (16 bits stay as they are until their use: a widening here would wait for the load)
+                x->kd[b][i].x = half_of(ks, kd_off[i]);
+                uint32_t va = v_off[i], da = vd_off[i];
+                asm("" : "+v"(va), "+v"(da));  // sums of a step, not registers of the loop
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t at = va + e * row;
+                    if constexpr (Bits::HALF) x->v[4 * b + e][i] = __builtin_amdgcn_raw_buffer_load_b16(vr, (int)at, 0, 0);
+                    else x->v[4 * b + e][i] = buf_load_b32(vr, at);
+                    x->vd[4 * b + e][i].x = half_of(vs, da + e * row_scales);
+                }
+            }
+        }
+        return valid;
+    }
+};
+// PACKED: at most 8 pairs, whose small parts of q and of the weights take columns 8 .. 15
+// of the products: half the matrix instructions.  Columns c and c + 8 then
+// hold the two parts of a pair's scores, which are added (both get the sum), and of
+// its outputs, which are added at the end.
+__device__ __forceinline__ float other8(float v) { return dpp_f32<0x128>(v); }  // row_ror:8
+template <int FHD, typename G, bool PACKED>
+__device__ __forceinline__ int few_rows_q4(const BatchArgs& a, const Seq& s, const int32_t* table, int kvh, int p0, int z,
+                                           int parts, int j_lo, int j_hi, _Float16* lds, float* wml) {
+    typedef FourBits<FHD> Bits;
+    constexpr int W = G::W, NS = Bits::NH * Bits::KW, DT = Bits::NH * Bits::TILES, FK = 32, PAIRS = PACKED ? 8 : FEW_PAIRS;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & (PAIRS - 1);
+    [[maybe_unused]] const bool small = PACKED && (lane & 8);
+    const int pairs = min(PAIRS, s.pairs - p0);
+    const int keys = last_key(a, s, p0 + pairs - 1) + 1;
+    const int splits = p0 ? 1 : parts;
+    if (z >= splits) return 0;
+    if (p0) j_lo = 0;
+    j_hi = z == splits - 1 ? keys : min(keys, j_hi);
+    const int p = p0 + c;
+    const bool live = c < pairs;
+    const int last = live ? last_key(a, s, p) : -1;
+    const int first = last_key(a, s, p0);
+    float M = -__builtin_inff(), L = 0.0f;
+    f4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    int wide = 0;
+    const int step = W * FK, j_w = j_lo + FK * w;
+    FourSlab<FHD> slab;
+    Bits bits[2];
+    slab.init(a.kv, a.hd);
+    // the row of q on its way while the page numbers are
+    int valid = 0;
+    if (j_w < j_hi) slab.pages(a.kv, table, j_w, s.t);
+    QRow<NS> q;
+    q.load_at(q_at(a, s, kvh, p), live, [g](int i) { return i / Bits::KW * 128 + g * Bits::KW * 8 + i % Bits::KW * 8; }, a.hd);
+    if (j_w < j_hi) {
+        valid = slab.load(a.kv, kvh, j_w, j_hi, &bits[0]);
+        slab.pages(a.kv, table, j_w + step, s.t);
+    }
+    h8 qh[NS], ql[NS];
+    const int qe = split_q<false, NS>(q, qh, ql, [](uint32_t m) {
+        m = max(m, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, m))));
+        return max(m, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, m))));
+    });
+    if constexpr (PACKED)
+#pragma unroll
+        for (int n = 0; n < NS; n++) qh[n] = small ? ql[n] : qh[n];
+    const float f = f16_factor(a.scale, qe);
+    const Q4Decoder decode;
+    // the slab at j0 from x, the next one's loads into `next`
+    auto turn = [&](int j0, Bits& x, Bits& next) {
+        const bool masked = j0 + FK - 1 > first || valid != 3;
+        const int now = valid;
+        if (j0 + step < j_hi) {
+            valid = slab.load(a.kv, kvh, j0 + step, j_hi, &next);
+            slab.pages(a.kv, table, j0 + 2 * step, s.t);
+        }
+        f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int n = 0; n < NS; n++) {
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const _Float16 d = x.kd[b][n / Bits::KW].x;
+                const h8 kf = __builtin_bit_cast(h8, decode.word(x.k[b][n / Bits::KW][n % Bits::KW], q4h2{d, d}));
+                sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[n], sc[b], 0, 0, 0);
+                if constexpr (!PACKED) sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[n], sc[b], 0, 0, 0);
+            }
+        }
+        if constexpr (PACKED)
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) sc[b][t] += other8(sc[b][t]);
+        if (masked) {
+            const int rel = last - j0 - 4 * g;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) sc[b][t] = (now >> b & 1) && 16 * b + t <= rel ? sc[b][t] : -__builtin_inff();
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) mx = fmaxf(mx, sc[b][t]);
+        mx *= f;
+        if (__builtin_amdgcn_ballot_w64(mx > M + SLACK)) {  // M is the pair's, mx the lane's so far
+            mx = fmaxf(mx, other16(mx));
+            mx = max32(mx);
+            const float Mn = fmaxf(M, mx);
+            const float corr = Mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - Mn);
+            L *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= corr;
+            M = Mn;
+        }
+        const float off = SHIFT - (M == -__builtin_inff() ? 0.0f : M);
+        u32x4 ph, pl;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float w0 = weight(sc[u >> 1][(u & 1) * 2], f, off), w1 = weight(sc[u >> 1][(u & 1) * 2 + 1], f, off);
+            L += w0;
+            L += w1;
+            uint32_t hi, lo;
+            split2<false>(w0, w1, &hi, &lo);
+            ph[u] = small ? lo : hi;
+            pl[u] = lo;
+        }
+        const h8 p8 = __builtin_bit_cast(h8, ph);
+        [[maybe_unused]] const h8 q8 = __builtin_bit_cast(h8, pl);
+#pragma unroll
+        for (int n = 0; n < Bits::NH; n++) {
+            uint32_t dd[4], half[2][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // keys 2 i and 2 i + 1
+                dd[i] = __builtin_bit_cast(uint32_t, q4h2{x.vd[2 * i][n].x, x.vd[2 * i + 1][n].x});
+                half[0][i] = perm(x.v[2 * i + 1][n], x.v[2 * i][n], 0x05040100u);
+                if constexpr (!Bits::HALF) half[1][i] = perm(x.v[2 * i + 1][n], x.v[2 * i][n], 0x07060302u);
+            }
+            if (masked) {  // blocks without finite values are zeroed: not all rows see them
+                bool found = false;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t lo = (dd[i] & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0, hi = (dd[i] & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0;
+                    found |= (lo | hi) != 0;
+                    dd[i] &= ~(lo | hi);
+                }
+                if (__builtin_amdgcn_ballot_w64(found)) wide = 1;
+            }
+#pragma unroll
+            for (int t = 0; t < Bits::TILES; t++) {
+                u32x4 vf;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    vf[i] = decode.pair(half[Bits::HALF ? 0 : t & 1][i], Bits::HALF ? t : t >> 1, __builtin_bit_cast(q4h2, dd[i]));
+                f4& ot = o[n * Bits::TILES + t];
+                ot = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vf), p8, ot, 0, 0, 0);
+                if constexpr (!PACKED) ot = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vf), q8, ot, 0, 0, 0);
+            }
+        }
+    };
+    for (int j0 = j_w; j0 < j_hi; j0 += 2 * step) {  // two register sets in turn: nothing is moved
+        turn(j0, bits[0], bits[1]);
+        if (j0 + step < j_hi) turn(j0 + step, bits[1], bits[0]);
+    }
+    L += other16(L);
+    L += other32(L);
+    // the wave's normalised output to its LDS, its maximum and sum beside; row r of a tile is word r's dim
+    auto dim_of = [](int d, int r) {
+        const int n = d / Bits::TILES, t = d % Bits::TILES;
+        return Bits::HALF ? 8 * (r >> 1) + 2 * t + (r & 1) : 128 * n + 8 * r + t;
+    };
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    float all = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (PACKED) o[d][e] += other8(o[d][e]);
+            o[d][e] *= inv;
+            all = fmaf(o[d][e], 0.0f, all);
+        }
+    if (not_finite_of_values(all, L)) {
+        wide = 1;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[d][e] = finite_or(o[d][e], L == L);
+    }
+    float* os = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(lds) + w * G::FEW_WAVE);
+    if (!small)
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) os[c * G::FROW + dim_of(d, 4 * g + e)] = o[d][e];
+    if (wide) {  // rows that see a value that is not finite, from LDS: a loop of few registers
+        wave_sync();
+        for (int j0 = j_w; j0 < j_hi; j0 += step)
+            for (int j = j0; j < min(j0 + FK, j_hi); j++) {
+                const auto v = ValueRow<Q4>::at(a, s.row0, table, kvh, j);
+                if (!v) continue;
+#pragma unroll 1
+                for (int i = lane; i < pairs * (a.hd / 4); i += 64) {
+                    const int pi = i / (a.hd / 4), dim = i % (a.hd / 4) * 4;
+                    f4* y = reinterpret_cast<f4*>(os + pi * G::FROW + dim);
+                    *y = *y + wide4(v + dim, j <= last_key(a, s, p0 + pi));
+                }
+            }
+    }
+    if (g == 0 && !small) {
+        wml[w * 32 + c] = M;
+        wml[w * 32 + 16 + c] = L;
+    }
+    return join_waves<G>(a, s, kvh, p0, pairs, z, splits, lds, wml);
 }
 
 // The splits of a step of up to 64 sequences, a lane each.  The span of keys is the
@@ -1670,12 +1980,67 @@ __device__ __forceinline__ int planned_parts(const BatchArgs& a, const Seq& s, i
     return parts_of(a, s.t, shortest_span(a, tiles, keys));
 }
 
+// Sequences of few rows alone (over a 4-bit cache): all their keys, one sequence
+// behind the other in units of FEW_UNIT, are dealt out evenly to as many workgroups as run at
+// once, a.few_slots a KV head; one may so work on the end of one sequence and on the
+// next.  To begin a sequence costs a workgroup about as much as FEW_BEGIN units (its first keys
+// are some 7 us away), so each sequence has that many more in front of its own, of
+// which nothing comes.  A lane a sequence.
+// (48 rows over up to 8192 keys: 91 us with a span for the longest kv_len, whose 1250
+// workgroups took more than two turns; 84 with the shortest span by which all start
+// at once, some with a third more keys than the others; 81 without FEW_BEGIN.)
+struct FewPlan {
+    Seq s;                   // of the lane
+    int units, before, per;  // of the lane's sequence, with FEW_BEGIN; of those before it; of a workgroup
+};
+__device__ __forceinline__ FewPlan few_plan(const BatchArgs& a) {
+    const int lane = threadIdx.x & 63;
+    FewPlan p{{0, 0, 0, 0}, 0, 0, 1};
+    if (lane < a.n_seq) {
+        p.s = sequence(a, lane);
+        if (p.s.pairs) p.units = FEW_BEGIN + max(1, (p.s.t + FEW_UNIT - 1) / FEW_UNIT);
+    }
+    p.before = lanes_before(p.units);
+    const int all = lanes_sum(p.units), longest = (int)wave_max_u32((uint32_t)p.units);  // below 2^31: 64 of 2^31 / FEW_UNIT
+    // a sequence lies in at most units / per + 2 parts, of which there may be few_splits
+    p.per = max(1, max((all + a.few_slots - 1) / a.few_slots, (longest + a.few_splits - 3) / max(1, a.few_splits - 2)));
+    return p;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), lane) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uint64_t)v, lane));
+}
+
+// Split z of `parts` of a few-row sequence b, its keys j_lo .. j_hi - 1 (of the last all that are left).
+template <typename KV, int HD, bool PACKED>
+__device__ __forceinline__ void few_pairs(const BatchArgs& a, const Seq& s, int b, int kvh, int z, int parts, int j_lo, int j_hi,
+                                          _Float16* lds, float* wml, int2* exps, int* flag) {
+    const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
+    constexpr int PAIRS = PACKED ? 8 : FEW_PAIRS;
+    for (int p0 = 0; p0 < s.pairs; p0 += PAIRS) {  // more than once (and then not split) only where max_rows was too small
+        int splits;
+        if constexpr (std::is_same<KV, Q4>::value) splits = few_rows_q4<Geo<KV, HD>::FHD, Geo<KV, HD>, PACKED>(a, s, table, kvh, p0, z, parts, j_lo, j_hi, lds, wml);
+        else splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml, exps);
+        if (splits > 1 && last_to_arrive(splits, a.counters + b * a.n_kv + kvh, flag))
+            join<true>(a, s, kvh, p0, min(PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(lds));
+        __syncthreads();  // before the next rows take the LDS
+    }
+}
+
 // KIND: which workgroups a launch has.  The two bodies in one kernel keep more
 // registers than either needs, so launches that need one of them have it alone.
 constexpr int TILE = 1, FEW = 2;
+// Waves of a SIMD at least, which bounds the registers.  Few rows over 4-bit keys
+// need little LDS: three waves (168 registers, none of the loop's in memory) took 75 us
+// where two took 76 and four, with registers in memory, 145.
 template <typename KV, int HD, int KIND>
-__global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void attend_kernel(BatchArgs a) {
-    constexpr int W = Geo<KV, HD>::W, NT = W * 64;
+constexpr int waves_per_simd() {
+    if (std::is_same<KV, Q4>::value && KIND == FEW && HD != 256) return 3;
+    return HD == 256 ? 1 : 2;
+}
+template <typename KV, int HD, int KIND, bool PACKED = false>
+__global__ __launch_bounds__((Geo<KV, HD>::W * 64), (waves_per_simd<KV, HD, KIND>())) void attend_kernel(BatchArgs a) {
+    constexpr int W = Geo<KV, HD>::W;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ Meta meta[2 * W];
     __shared__ int2 exps[2 * 64];  // of a tile's keys, twice, or of each wave's
@@ -1697,24 +2062,47 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), HD == 256 ? 1 : 2) void atte
         b = tile ? sequence_of<TILE_PAIRS>(a, slot, a.group) : slot;
     }
     if (b < 0) return;
-    const Seq s = sequence(a, b);
-    if (s.pairs == 0 || (s.pairs > a.few_rows) != tile) return;
-    const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
-    if (tile) {
+    if (KIND != FEW && tile) {
+        const Seq s = sequence(a, b);
+        if (s.pairs == 0 || s.pairs <= a.few_rows) return;
+        const int32_t* table = a.kv.tables ? a.kv.tables + b * a.kv.table_stride : nullptr;
         if constexpr ((KIND & TILE) != 0) {
             int p0;
             if (a.tile_slots) p0 = (tiles_of<TILE_PAIRS>(s.pairs) - 1 - slot) * TILE_PAIRS;
             else p0 = tile_start(a, s, b, slot), parts = parts_of(a, s.t, a.tile_span);
             tile_rows<KV, HD>(a, s, table, b, kvh, p0, z, parts, lds, meta, exps);
         }
-    } else {
-        if constexpr ((KIND & FEW) != 0)
-            for (int p0 = 0; p0 < s.pairs; p0 += FEW_PAIRS) {  // more than once (and then not split) only where max_rows was too small
-                const int splits = few_rows<KV, HD>(a, s, table, kvh, p0, z, lds, wml, exps);
-                if (splits > 1 && last_to_arrive(splits, a.counters + slot * a.n_kv + kvh, &flag))
-                    join<true>(a, s, kvh, p0, min(FEW_PAIRS, s.pairs - p0), splits, reinterpret_cast<float*>(smem));
-                __syncthreads();  // before the next rows take the LDS
+        return;
+    }
+    if constexpr ((KIND & FEW) != 0) {
+        uint64_t left = 1;  // sequences of this workgroup
+        FewPlan p{{0, 0, 0, 0}, 0, 0, 1};
+        const bool planned = KIND == FEW && std::is_same<KV, Q4>::value && a.few_slots;
+        const int lo = planned ? id * (p = few_plan(a)).per : 0, hi = lo + p.per;
+        // (of a sequence's units the first FEW_BEGIN have no keys)
+        if (planned) left = __builtin_amdgcn_ballot_w64(p.units && p.before + FEW_BEGIN < hi && p.before + p.units > lo);
+        for (; left; left &= left - 1) {
+            int j_lo = 0, j_hi = 0;
+            Seq s;
+            if (planned) {
+                b = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(left));
+                const int u0 = __builtin_amdgcn_readlane(p.before, b) + FEW_BEGIN;
+                const int u1 = u0 - FEW_BEGIN + __builtin_amdgcn_readlane(p.units, b), first = u0 / p.per;
+                z = id - first, parts = (u1 - 1) / p.per - first + 1;
+                j_lo = (max(lo, u0) - u0) * FEW_UNIT, j_hi = (min(hi, u1) - u0) * FEW_UNIT;
+                s = {lane_value(p.s.row0, b), __builtin_amdgcn_readlane(p.s.pairs, b), lane_value(p.s.first, b),
+                     __builtin_amdgcn_readlane(p.s.t, b)};
+            } else {
+                s = sequence(a, b);
+                if (s.pairs == 0 || s.pairs > a.few_rows) return;
             }
+            if (!planned) {
+                const int keys = last_key(a, s, min(PACKED ? 8 : FEW_PAIRS, s.pairs) - 1) + 1;
+                parts = min(a.few_splits, max(1, (keys + a.few_span - 1) / a.few_span));
+                j_lo = z * a.few_span, j_hi = j_lo + a.few_span;
+            }
+            few_pairs<KV, HD, PACKED>(a, s, b, kvh, z, parts, j_lo, j_hi, lds, wml, exps, &flag);
+        }
     }
 }
 
@@ -1804,23 +2192,25 @@ __global__ __launch_bounds__(256) void split_kernel(BatchArgs a, _Float16* image
     }
 }
 
-template <typename KV, int HD, int KIND>
+template <typename KV, int HD, int KIND, bool PACKED = false>
 hipError_t launch(const BatchArgs& a, hipStream_t s) {
     using G = Geo<KV, HD>;
     constexpr size_t lds = KIND == TILE ? G::TILE_LDS : KIND == FEW ? G::FEW_LDS : G::LDS;
-    const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD, KIND>,
+    const hipError_t e = hipFuncSetAttribute((const void*)attend_kernel<KV, HD, KIND, PACKED>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     const int tile_blocks = a.tile_slots ? a.tile_slots : a.tiles * a.tile_splits;
-    const unsigned blocks = (unsigned)(a.n_kv * (tile_blocks + (KIND & FEW ? a.n_seq * a.few_splits : 0)));
+    const unsigned blocks = (unsigned)(a.n_kv * (tile_blocks + (!(KIND & FEW) ? 0 : a.few_slots ? a.few_slots : a.n_seq * a.few_splits)));
     static_assert(G::W * 64 == JOIN_THREADS && JOIN_FLOATS * 4 <= G::FEW_LDS, "few rows join with what they have");
-    hipLaunchKernelGGL((attend_kernel<KV, HD, KIND>), dim3(blocks), dim3(G::W * 64), lds, s, a);
+    hipLaunchKernelGGL((attend_kernel<KV, HD, KIND, PACKED>), dim3(blocks), dim3(G::W * 64), lds, s, a);
     if (KIND != FEW && a.tile_splits > 1)
         hipLaunchKernelGGL(join_kernel, dim3((unsigned)(a.n_kv * a.tiles * (TILE_PAIRS / FEW_PAIRS))), dim3(JOIN_THREADS), 0, s, a);
     return hipGetLastError();
 }
 template <typename KV, int HD>
 hipError_t launch_kind(const BatchArgs& a, hipStream_t s) {
+    if constexpr (std::is_same<KV, Q4>::value)
+        if (a.packed) return launch<KV, HD, FEW, true>(a, s);
     return a.few_rows == 0 ? launch<KV, HD, TILE>(a, s) : a.tiles == 0 ? launch<KV, HD, FEW>(a, s)
                                                                        : launch<KV, HD, TILE | FEW>(a, s);
 }
@@ -1860,6 +2250,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
     // (packed prompts of few rows have few keys: tiles serve them too)
     const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && (a.n_seq == 1 || !a.kv.tables);
     a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
+    a.packed = dtype == RDL_KV_Q4 && rows * G <= 8;
     a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
     const int64_t most_parts =
         std::max<int64_t>(1, (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float))));
@@ -1881,10 +2272,16 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
         a.tile_splits = (int)std::min<int64_t>({(keys + TILE_MIN_SPAN - 1) / TILE_MIN_SPAN, most_parts, JOIN_SPLITS,
                                                 std::max(2 * a.tile_splits, a.few_splits)});
     }
+    if (dtype == RDL_KV_Q4 && only_few && a.n_seq <= 64 && a.few_splits > 1) {
+        const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS / 3 : FEW_SLOTS) / a.n_kv);
+        const int64_t most = std::min<int64_t>({(keys + FEW_UNIT - 1) / FEW_UNIT, most_parts, JOIN_SPLITS, slots});
+        if (most > 1) a.few_slots = (int)slots, a.few_splits = (int)most;
+    }
     a.part_splits = std::max(a.few_splits, a.tile_splits);
     // (join_kernel, behind split tiles, has TILE_PAIRS / FEW_PAIRS workgroups a tile)
     const int64_t tile_blocks = a.tile_slots ? a.tile_slots : (int64_t)a.tiles * a.tile_splits;
-    const int64_t blocks = a.n_kv * std::max(tile_blocks + (only_tile ? 0 : (int64_t)a.n_seq * a.few_splits),
+    const int64_t few_blocks = only_tile ? 0 : a.few_slots ? a.few_slots : (int64_t)a.n_seq * a.few_splits;
+    const int64_t blocks = a.n_kv * std::max(tile_blocks + few_blocks,
                                              a.tile_splits > 1 ? (int64_t)a.tiles * (TILE_PAIRS / FEW_PAIRS) : 0);
     if (blocks > MAX_BLOCKS)
         return api_fail(RDL_ERR_UNSUPPORTED, "%d sequences, %lld rows: %lld workgroups", a.n_seq, (long long)m, (long long)blocks);

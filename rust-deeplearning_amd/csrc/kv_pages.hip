@@ -172,7 +172,7 @@ struct Unit<Q4, false> {
         w = reinterpret_cast<const uint32_t*>(run)[u];
         d = *reinterpret_cast<const uint16_t*>(run + q4_scale_at(a.page_positions, a.head_dim, pos, col * 8)) * 0x10001u;
     }
-    __device__ __forceinline__ u32x4 halves() const { return q4_values(w, d); }
+    __device__ __forceinline__ u32x4 halves() const { return Q4Decoder().word(w, __builtin_bit_cast(q4h2, d)); }
     __device__ __forceinline__ void get(float (&v)[8]) const {
         const h8 x = __builtin_bit_cast(h8, halves());
 #pragma unroll

@@ -25,24 +25,24 @@ __device__ __forceinline__ int q4_scale_at(int positions, int hd, int pos, int d
 
 typedef _Float16 q4h2 __attribute__((ext_vector_type(2)));
 
-// The 8 values of a code word, in order, times the scale in both halves of d.
-// A nibble under an exponent is a whole number of steps above a power of two:
-// 1024 + n in bits 0 .. 3 of f16, 64 + n in bits 4 .. 7.
-__device__ __forceinline__ u32x4 q4_values(uint32_t w, uint32_t d) {
-    const q4h2 dd = __builtin_bit_cast(q4h2, d);
-    u32x4 out;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t x = w >> (8 * i);
-        const q4h2 a = __builtin_bit_cast(q4h2, (x & 0x000F000Fu) | 0x64006400u);
-        const q4h2 b = __builtin_bit_cast(q4h2, (x & 0x00F000F0u) | 0x54005400u);
-        const q4h2 va = (a - q4h2{(_Float16)1032.0f, (_Float16)1032.0f}) * dd;
-        const q4h2 vb = (b - q4h2{(_Float16)72.0f, (_Float16)72.0f}) * dd;
-        out[2 * i] = __builtin_bit_cast(uint32_t, va);
-        out[2 * i + 1] = __builtin_bit_cast(uint32_t, vb);
+// From codes to values.  A nibble under an exponent is a whole number of steps above a power of two:
+// 1024 + n in bits 0 .. 3 of f16, 64 + n in bits 4 .. 7.  The constants are kept from
+// the compiler, so that they are registers and v_and_or_b32 takes both at once.
+struct Q4Decoder {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, from1024 = 0x64006400u, from64 = 0x54005400u;
+    __device__ __forceinline__ Q4Decoder() {
+        asm("" : "+s"(low), "+s"(high), "+v"(from1024), "+v"(from64));
     }
-    return out;
-}
+    // nibble t of both halves of x, times d
+    __device__ __forceinline__ uint32_t pair(uint32_t x, int t, q4h2 d) const {
+        const uint32_t y = t & 2 ? x >> 8 : x;
+        const q4h2 n = __builtin_bit_cast(q4h2, t & 1 ? (y & high) | from64 : (y & low) | from1024);
+        const _Float16 bias = t & 1 ? (_Float16)72.0f : (_Float16)1032.0f;
+        return __builtin_bit_cast(uint32_t, (n - q4h2{bias, bias}) * d);
+    }
+    // the 8 values of a code word, in order
+    __device__ __forceinline__ u32x4 word(uint32_t w, q4h2 d) const { return {pair(w, 0, d), pair(w, 1, d), pair(w, 2, d), pair(w, 3, d)}; }
+};
 
 // The scale of a block: mag, the bits of its largest magnitude, and whether a
 // positive value has it.  f16 bits.
