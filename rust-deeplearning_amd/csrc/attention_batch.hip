@@ -114,26 +114,7 @@ __device__ __forceinline__ int lift_of(float scale, int e) {
     return max(0, e + (int)(__builtin_bit_cast(uint32_t, scale) >> 23) - 127 - FACTOR_MAX);
 }
 __device__ __forceinline__ float weight(float s, float f, float off) { return __builtin_amdgcn_exp2f(fmaf(s, f, off)); }
-__device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
-                                                    false, false);
-    const uint32_t a = r[0], b = r[1];
-    return __builtin_bit_cast(float, threadIdx.x & 32 ? a : b);
-}
 __device__ __forceinline__ float max32(float v) { return fmaxf(v, other32(v)); }
-__device__ __forceinline__ float other16(float v) {  // the value of lane ^ 16
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
-                                                    false, false);
-    const uint32_t a = r[0], b = r[1];
-    return __builtin_bit_cast(float, threadIdx.x & 16 ? a : b);
-}
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-    v = max8_u32(v);
-    v = max(v, (uint32_t)dpp_i32<DPP_ROW_MIRROR>((int)v));
-    v = max(v, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, v))));
-    v = max(v, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, v))));
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
-}
 // Maximum over the first N lanes of each N (4 or 8), uniform.
 template <int N>
 __device__ __forceinline__ int lanes_max(int v) {
@@ -2272,7 +2253,8 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
         a.tile_splits = (int)std::min<int64_t>({(keys + TILE_MIN_SPAN - 1) / TILE_MIN_SPAN, most_parts, JOIN_SPLITS,
                                                 std::max(2 * a.tile_splits, a.few_splits)});
     }
-    if (dtype == RDL_KV_Q4 && only_few && a.n_seq <= 64 && a.few_splits > 1) {
+    // (fewer workgroups than run at once need no plan: one row over 778 keys took 14.0 us with it, 11.1 without)
+    if (dtype == RDL_KV_Q4 && only_few && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS) {
         const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS / 3 : FEW_SLOTS) / a.n_kv);
         const int64_t most = std::min<int64_t>({(keys + FEW_UNIT - 1) / FEW_UNIT, most_parts, JOIN_SPLITS, slots});
         if (most > 1) a.few_slots = (int)slots, a.few_splits = (int)most;

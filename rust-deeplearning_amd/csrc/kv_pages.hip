@@ -212,7 +212,7 @@ __device__ __forceinline__ void store_unit(const Unit<S, __is_same(S, D)>& u, vo
             const float d = h2f(scale), by = d == 0.0f ? __builtin_inff() : d, inv = __builtin_amdgcn_rcpf(by);
             uint32_t w = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) w |= q4_code(v[i], by, inv) << ((i >> 1) * 4 + (i & 1) * 16);
+            for (int i = 0; i < 8; i++) w |= q4_code<__is_same(S, _Float16)>(v[i], by, inv) << ((i >> 1) * 4 + (i & 1) * 16);
             if (!on) return;
             uint8_t* run = reinterpret_cast<uint8_t*>(head);
             reinterpret_cast<uint32_t*>(run)[at] = w;

@@ -56,7 +56,14 @@ __device__ __forceinline__ uint32_t q4_scale(uint32_t mag, bool positive) {
 // The code of x under scale d (as f32; inv: 1 / d or so): x / d to the nearest
 // whole number, halves to even, which the rounded quotient alone would miss
 // beside a half: the remainder of the nearest code, exact in f32, decides.
+// HALF: x is an f16 number, 2^-14 of itself or more away from the halves that it is not: the quotient rounded
+// to f32 has the same nearest whole number.
+template <bool HALF = false>
 __device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
+    if constexpr (HALF) {
+        const float q = x * inv;
+        return (uint32_t)(int)(fminf(fmaxf(rintf(fmaf(fmaf(-q, d, x), inv, q)), -8.0f), 7.0f) + 8.0f);
+    }
     float c = rintf(x * inv);
     const float rest = fmaf(-c, d, x), twice = 2.0f * fabsf(rest), size = fabsf(d);
     const float step = (__builtin_bit_cast(uint32_t, rest) ^ __builtin_bit_cast(uint32_t, d)) >> 31 ? -1.0f : 1.0f;

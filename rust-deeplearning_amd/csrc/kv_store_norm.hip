@@ -21,11 +21,16 @@ constexpr int STORE_NT = 256;
 
 struct Q4 {};
 
+template <typename F>
+__device__ __forceinline__ double two_words(double v, F&& f) {  // another lane's value, a word at a time
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_bit_cast(uint32_t, f(as_f32((int32_t)(uint32_t)u)));
+    const uint32_t hi = __builtin_bit_cast(uint32_t, f(as_f32((int32_t)(uint32_t)(u >> 32))));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 template <int CTRL>
 __device__ __forceinline__ double dpp_f64(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)dpp_i32<CTRL>((int)(uint32_t)u), hi = (uint32_t)dpp_i32<CTRL>((int)(uint32_t)(u >> 32));
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    return two_words(v, [](float w) { return dpp_f32<CTRL>(w); });
 }
 template <int G>
 __device__ __forceinline__ double group_sum(double v) {
@@ -33,8 +38,8 @@ __device__ __forceinline__ double group_sum(double v) {
     if constexpr (G >= 4) v += dpp_f64<DPP_QUAD_XOR2>(v);
     if constexpr (G >= 8) v += dpp_f64<DPP_ROW_HALF_MIRROR>(v);
     if constexpr (G >= 16) v += dpp_f64<DPP_ROW_MIRROR>(v);
-    if constexpr (G >= 32) v += __shfl_xor(v, 16);
-    if constexpr (G >= 64) v += __shfl_xor(v, 32);
+    if constexpr (G >= 32) v += two_words(v, [](float w) { return other16(w); });
+    if constexpr (G >= 64) v += two_words(v, [](float w) { return other32(w); });
     return v;
 }
 // f32(1 / sqrt(a)): two steps of Newton's method from the 24 bits of the instruction.
@@ -44,6 +49,18 @@ __device__ __forceinline__ float inverse_root(double a) {
     y = y * (1.5 - 0.5 * a * (y * y));
     y = y * (1.5 - 0.5 * a * (y * y));
     return (float)y;
+}
+
+// The value of the lane that holds the other half of the rotation's pairs.  Where the head fills its G
+// lanes that is lane ^ G / 2, without a way through LDS.
+template <int G>
+__device__ __forceinline__ float half_away(float v, int l, int quarter) {
+    if (2 * quarter == G) {
+        if constexpr (G == 16) return dpp_f32<0x128>(v);  // row_ror:8
+        if constexpr (G == 32) return other16(v);
+        if constexpr (G == 64) return other32(v);
+    }
+    return __shfl(v, l < quarter ? l + quarter : l - quarter, G);
 }
 
 // A thread's four dims of a cached row.
@@ -79,7 +96,13 @@ __device__ __forceinline__ void put(const PoolView& p, void* base, int64_t page,
     }
 }
 
-template <typename KV, int G>
+// ROWS rows at a time, whose loads are on their way together: slot and position,
+// then cos and sin, are two trips to memory one behind the other, and what is in
+// flight meanwhile bounds the rate, with the norm's 64-bit sums behind it.  4096 rows of 32 + 2 * 8
+// heads of 128 take 45 us one at a time, 40 by two (4.6 TB/s, a large copy reaches
+// 5.1), 42 by four and 48 by eight, whose registers leave fewer waves.
+// Few rows take one each, so that they spread over the CUs.
+template <typename KV, int G, int ROWS>
 __global__ __launch_bounds__(STORE_NT) void store_norm_kernel(StoreNormArgs a) {
 #pragma clang fp contract(off)
     const int hd = a.pool.head_dim, quarter = hd >> 3, n_kv = a.pool.n_kv_heads;  // quarter: lanes of half a head
@@ -89,50 +112,66 @@ __global__ __launch_bounds__(STORE_NT) void store_norm_kernel(StoreNormArgs a) {
     const bool live = dim < hd, is_q = head < a.n_heads, is_v = head >= a.n_heads + n_kv;
     const int kvh = is_v ? head - a.n_heads - n_kv : head - a.n_heads;
     const float* gamma = is_q ? a.q_gamma : is_v ? nullptr : a.k_gamma;
+    const float* src = is_q ? a.q + (int64_t)head * hd : is_v ? a.v + (int64_t)kvh * hd : a.k + (int64_t)kvh * hd;
+    const int64_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
     const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const f4 g = gamma && live ? *reinterpret_cast<const f4*>(gamma + dim) : zero;
     const int64_t capacity = (int64_t)a.pool.n_pages << a.pool.shift;
-    for (int64_t r = blockIdx.y; r < a.m; r += gridDim.y) {
-        const float* src = is_q ? a.q + r * a.q_stride + (int64_t)head * hd
-                         : is_v ? a.v + r * a.v_stride + (int64_t)kvh * hd
-                                : a.k + r * a.k_stride + (int64_t)kvh * hd;
-        f4 x = live ? *reinterpret_cast<const f4*>(src + dim) : zero;
-        const int32_t slot = a.slots[r];
-        if (slot < 0 || slot >= capacity) continue;
-        if (a.cos_t) {
-            const int32_t pos = a.positions[r];
-            if (pos < 0 || pos >= a.n_positions) continue;
-        }
-        if (gamma) {
-            double ss = 0.0;
+    const bool turns = a.cos_t && !is_v;
+    for (int64_t r0 = (int64_t)blockIdx.y * ROWS; r0 < a.m; r0 += (int64_t)gridDim.y * ROWS) {
+        f4 x[ROWS], c[ROWS], s[ROWS];
+        int32_t slot[ROWS], pos[ROWS];
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss = __builtin_fma((double)x[i], (double)x[i], ss);
-            const float inv = inverse_root(group_sum<G>(ss) / (double)hd + (double)a.eps);
-            x = x * inv;
-            x = x * g;
+        for (int i = 0; i < ROWS; i++) {
+            const int64_t r = min(r0 + i, a.m - 1);
+            slot[i] = a.slots[r];
+            pos[i] = a.cos_t ? a.positions[r] : 0;
+            x[i] = live ? *reinterpret_cast<const f4*>(src + r * stride + dim) : zero;
         }
-        if (a.cos_t && !is_v) {
-            const int64_t at = (int64_t)a.positions[r] * (hd >> 1) + (l < quarter ? dim : dim - (hd >> 1));
-            const f4 c = live ? *reinterpret_cast<const f4*>(a.cos_t + at) : zero;
-            const f4 s = live ? *reinterpret_cast<const f4*>(a.sin_t + at) : zero;
-            f4 other;
 #pragma unroll
-            for (int i = 0; i < 4; i++) other[i] = __shfl(x[i], l < quarter ? l + quarter : l - quarter, G);
-            x = l < quarter ? x * c - other * s : other * s + x * c;
+        for (int i = 0; i < ROWS; i++) {
+            if (r0 + i >= a.m || slot[i] < 0 || slot[i] >= capacity || (a.cos_t && (pos[i] < 0 || pos[i] >= a.n_positions))) slot[i] = -1;
+            const int64_t at = (int64_t)(slot[i] < 0 ? 0 : pos[i]) * (hd >> 1) + (l < quarter ? dim : dim - (hd >> 1));
+            const bool load = turns && live && slot[i] >= 0;
+            c[i] = load ? *reinterpret_cast<const f4*>(a.cos_t + at) : zero;
+            s[i] = load ? *reinterpret_cast<const f4*>(a.sin_t + at) : zero;
         }
-        if (is_q) {
-            if (live) *reinterpret_cast<f4*>(a.q_out + r * a.q_out_stride + (int64_t)head * hd + dim) = x;
-        } else {
-            put<KV>(a.pool, is_v ? a.pool.v : a.pool.k, slot >> a.pool.shift, kvh, slot & ((1 << a.pool.shift) - 1), dim, live, x);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            if (slot[i] < 0) continue;  // (the same in all lanes)
+            if (gamma) {
+                double ss = 0.0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) ss = __builtin_fma((double)x[i][e], (double)x[i][e], ss);
+                const float inv = inverse_root(__builtin_fma(group_sum<G>(ss), a.share, (double)a.eps));
+                x[i] = x[i] * inv;
+                x[i] = x[i] * g;
+            }
+            if (turns) {
+                f4 other;
+#pragma unroll
+                for (int e = 0; e < 4; e++) other[e] = half_away<G>(x[i][e], l, quarter);
+                x[i] = l < quarter ? x[i] * c[i] - other * s[i] : other * s[i] + x[i] * c[i];
+            }
+            if (is_q) {
+                if (live) *reinterpret_cast<f4*>(a.q_out + (r0 + i) * a.q_out_stride + (int64_t)head * hd + dim) = x[i];
+            } else {
+                put<KV>(a.pool, is_v ? a.pool.v : a.pool.k, slot[i] >> a.pool.shift, kvh, slot[i] & ((1 << a.pool.shift) - 1), dim, live, x[i]);
+            }
         }
     }
 }
 
+constexpr int STORE_ROWS = 2;
+constexpr int64_t STORE_MANY = 512;  // rows from which on a workgroup takes STORE_ROWS at a time
 template <typename KV, int G>
 void go(const StoreNormArgs& a, hipStream_t s) {
     const unsigned heads = (unsigned)(a.n_heads + 2 * a.pool.n_kv_heads), per = STORE_NT / G;
-    const dim3 grid((heads + per - 1) / per, (unsigned)(a.m < 65535 ? a.m : 65535));
-    hipLaunchKernelGGL((store_norm_kernel<KV, G>), grid, dim3(STORE_NT), 0, s, a);
+    const bool many = a.m >= STORE_MANY;
+    const int64_t rows = many ? (a.m + STORE_ROWS - 1) / STORE_ROWS : a.m;
+    const dim3 grid((heads + per - 1) / per, (unsigned)(rows < 65535 ? rows : 65535));
+    if (many) hipLaunchKernelGGL((store_norm_kernel<KV, G, STORE_ROWS>), grid, dim3(STORE_NT), 0, s, a);
+    else hipLaunchKernelGGL((store_norm_kernel<KV, G, 1>), grid, dim3(STORE_NT), 0, s, a);
 }
 template <typename KV>
 void go_hd(const StoreNormArgs& a, hipStream_t s) {
@@ -145,7 +184,8 @@ void go_hd(const StoreNormArgs& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_store_norm(const StoreNormArgs& a, hipStream_t s) {
+hipError_t launch_store_norm(StoreNormArgs a, hipStream_t s) {
+    a.share = 1.0 / a.pool.head_dim;
     if (a.pool.dtype == RDL_KV_Q4) go_hd<Q4>(a, s);
     else if (a.pool.dtype == RDL_DTYPE_F16) go_hd<_Float16>(a, s);
     else go_hd<float>(a, s);

@@ -21,7 +21,8 @@ struct StoreNormArgs {
     const int32_t *positions, *slots;
     const float *cos_t, *sin_t;
     int64_t n_positions;
+    double share;  // 1 / head_dim (launch_store_norm sets it)
 };
-hipError_t launch_store_norm(const StoreNormArgs& a, hipStream_t s);
+hipError_t launch_store_norm(StoreNormArgs a, hipStream_t s);
 
 }  // namespace rdl

@@ -139,6 +139,26 @@ __device__ __forceinline__ float fold16(float x, float y) {
     return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
 }
 
+__device__ __forceinline__ float other32(float v) {  // the value of lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    const uint32_t a = r[0], b = r[1];
+    return __builtin_bit_cast(float, threadIdx.x & 32 ? a : b);
+}
+__device__ __forceinline__ float other16(float v) {  // the value of lane ^ 16
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    const uint32_t a = r[0], b = r[1];
+    return __builtin_bit_cast(float, threadIdx.x & 16 ? a : b);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max8_u32(v);
+    v = max(v, (uint32_t)dpp_i32<DPP_ROW_MIRROR>((int)v));
+    v = max(v, __builtin_bit_cast(uint32_t, other16(__builtin_bit_cast(float, v))));
+    v = max(v, __builtin_bit_cast(uint32_t, other32(__builtin_bit_cast(float, v))));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
 // Row sums of a wave: v[r] holds lane partials of row r (R <= 4).  Returns,
 // in every lane, the 64-lane total of row (lane >> 4) for R = 3, 4, of row
 // (lane >> 5) for R = 2 and of row 0 for R = 1 (rows >= R read as zero).
