@@ -31,6 +31,11 @@
 extern "C" {
 #endif
 
+/* kv_f16 of a cache of 4 bits a value (RDL_KV_Q4, rdl_attention.h). */
+enum {
+    RDL_LLAMA_KV_Q4 = 2
+};
+
 /* ModelConfig fields used by the Llama path (rustml/nlp/main/src/api/types.rs:186). */
 typedef struct rdl_llama_config {
     int32_t dim;         /* hidden size */
@@ -43,7 +48,8 @@ typedef struct rdl_llama_config {
     int32_t max_seq;     /* KV cache capacity (max_seq_len) */
     float norm_eps;
     float rope_theta;
-    int32_t kv_f16;      /* 1: f16 KV cache, 0: f32 (the reference's) */
+    int32_t kv_f16;      /* 1: f16 KV cache, 0: f32 (the reference's), RDL_LLAMA_KV_Q4:
+                            4 bits (head_dim % 32 == 0; rdl_llama_batch_* alone) */
     int32_t max_batch;   /* most rows one forward call takes (prefill chunk) */
     int32_t output_dtype; /* GGML type of the output matrix: RDL_DTYPE_Q4_0 (also
                              when 0), _Q8_0, _Q4_1, _Q4_K or _Q6_K (K-quants:
@@ -195,6 +201,20 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq);
  * rdl_llama_forward multiplies in f32) products are formed from 23-bit pairs. */
 rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
                                    size_t n, float* logits, size_t logits_len);
+/* The same step with log probabilities (rdl_logprobs_dev) of the last rows' logits
+ * instead of the logits, which stay on the device: logprobs[b] of token targets[b]
+ * (both NULL: none), entropies[b] (NULL: none), and the n_top (0 .. 64) most likely
+ * tokens and their log probabilities at [b * n_top ..]; those of a sequence without
+ * tokens are left as they were. */
+rdl_status rdl_llama_batch_logprobs(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
+                                    size_t n, const int32_t* targets, float* logprobs, float* entropies, size_t n_top,
+                                    int32_t* top_ids, float* top_logprobs);
+/* Forks sequences: for each of n pairs the empty sequence children[i] becomes a copy
+ * of parents[i], whose full pages it shares; a last page that is not full is copied in
+ * every layer (rdl_kv_fork_dev, rdl_kv_copy_pages_dev).  Children differ, and none is a
+ * parent.  RDL_ERR_INVALID_DATA, and nothing changes, where the pages do
+ * not suffice.  rdl_llama_batch_drop frees a page with the last sequence that holds it.  Synchronous. */
+rdl_status rdl_llama_batch_fork(rdl_llama* model, const int32_t* parents, const int32_t* children, size_t n);
 /* Positions that each of the n (= n_seq) sequences has. */
 rdl_status rdl_llama_batch_positions(const rdl_llama* model, size_t* out, size_t n);
 /* Empties one sequence; its pages are free for the others. */
@@ -241,7 +261,7 @@ rdl_status rdl_llama_get_config(const rdl_llama* model, rdl_llama_config* out);
 typedef struct rdl_llama_gguf_options {
     int32_t max_seq;   /* KV cache capacity; 0: the file's context_length (2048 if absent) */
     int32_t max_batch; /* rows per forward call; 0: 32 */
-    int32_t kv_f16;    /* 1: f16 KV cache, 0: f32 */
+    int32_t kv_f16;    /* 1: f16 KV cache, 0: f32, RDL_LLAMA_KV_Q4: 4 bits */
 } rdl_llama_gguf_options;
 
 /* LlmModel::from_pretrained over GGUFFile::load_and_remap, the Llama branch

@@ -35,6 +35,7 @@
 #include "../../include/rdl_gguf.h"
 #include "../../include/rdl_llama.h"
 #include "attention.hpp"
+#include "kv_q4.hpp"
 #include "rdl_device.hpp"
 #include "rdl_internal.hpp"
 
@@ -42,6 +43,7 @@ namespace rdl {
 namespace {
 
 constexpr int NT = 256;  // threads of the element-wise / reduction kernels
+constexpr size_t LLAMA_TOP = 64;  // most alternatives of rdl_llama_batch_logprobs
 
 // Sum over a 256-thread block, returned to every thread.
 __device__ __forceinline__ float block_sum(float v, float* red) {
@@ -696,10 +698,15 @@ struct LlamaModel {
         int *table = nullptr, *cached = nullptr, *count = nullptr, *free_pages = nullptr, *row_start = nullptr,
             *kv_len = nullptr, *row_seq = nullptr, *positions = nullptr, *slots = nullptr, *summary = nullptr,
             *last_rows = nullptr;
+        int *parents = nullptr, *children = nullptr, *src = nullptr, *dst = nullptr, *forked = nullptr;  // of a fork
+        int *targets = nullptr, *top_ids = nullptr;  // of a step's log probabilities
+        float *logprobs = nullptr, *entropies = nullptr, *top_logprobs = nullptr;
         float *x = nullptr, *logits = nullptr;  // [last][dim], [last][vocab]: a step's last rows, at most min(cap, max_batch)
         void* mem = nullptr;                    // all of it, one allocation
         size_t max_rows = 0, max_kv = 0;        // of the step
         std::vector<int> len, free_host;
+        std::vector<int> holders;    // of each page: the sequences whose tables name it
+        std::vector<int> row_host;  // room for a table row
         rdl_status status = RDL_OK;  // of the step's cache operators, whose message stands
     } batch;
 
@@ -723,8 +730,11 @@ struct LlamaModel {
     hipError_t alloc_t(T** p, size_t count) {
         return alloc(reinterpret_cast<void**>(p), count * sizeof(T));
     }
-    size_t kv_elem() const { return cfg.kv_f16 ? 2 : 4; }
-    size_t kv_layer_elems() const { return (size_t)n_pages * cfg.n_kv_heads * KV_PAGE * cfg.head_dim; }
+    bool kv_q4() const { return cfg.kv_f16 == RDL_LLAMA_KV_Q4; }
+    size_t kv_layer_bytes() const {
+        const size_t heads = (size_t)n_pages * cfg.n_kv_heads;
+        return heads * (kv_q4() ? (size_t)q4_run_bytes(KV_PAGE, cfg.head_dim) : (size_t)KV_PAGE * cfg.head_dim * (cfg.kv_f16 ? 2 : 4));
+    }
 
     // Every matrix that prompt chunks multiply with.
     template <typename F>
@@ -805,15 +815,21 @@ struct LlamaModel {
     }
 
     void* kv_layer(void* base, int l) const {
-        return reinterpret_cast<uint8_t*>(base) + (size_t)l * kv_layer_elems() * kv_elem();
+        return reinterpret_cast<uint8_t*>(base) + (size_t)l * kv_layer_bytes();
+    }
+
+    rdl_kv_pool batch_pool(int l) const {
+        const int hd = cfg.head_dim;
+        // a head's page, in elements or, in 4 bits, bytes
+        const int64_t head = kv_q4() ? q4_run_bytes(KV_PAGE, hd) : (int64_t)KV_PAGE * hd;
+        return {kv_layer(kc, l), kv_layer(vc, l), kv_q4() ? RDL_KV_Q4 : cfg.kv_f16 ? RDL_DTYPE_F16 : RDL_DTYPE_F32, n_pages,
+                KV_PAGE, cfg.n_kv_heads, hd, cfg.n_kv_heads * head, head, kv_q4() ? hd / 2 : hd};
     }
 
     // The same for a step of several sequences.
     hipError_t batch_attention(int l, size_t m) {
         const int hd = cfg.head_dim;
-        const rdl_kv_pool pool = {kv_layer(kc, l), kv_layer(vc, l), cfg.kv_f16 ? RDL_DTYPE_F16 : RDL_DTYPE_F32, n_pages,
-                                  KV_PAGE, cfg.n_kv_heads, hd, (int64_t)cfg.n_kv_heads * KV_PAGE * hd,
-                                  (int64_t)KV_PAGE * hd, hd};
+        const rdl_kv_pool pool = batch_pool(l);
         rdl_status st = rdl_kv_store_dev(&pool, m, qkv, qkv_dim, qkv, qkv_dim, cfg.n_heads, qkv + q_dim, qkv_dim,
                                          qkv + q_dim + kv_dim, qkv_dim, batch.positions, batch.slots, cos_t, sin_t,
                                          cfg.max_seq, stream);
@@ -1255,7 +1271,7 @@ bool valid_config(const rdl_llama_config& c) {
            c.head_dim % 2 == 0 && c.head_dim <= 256 && c.n_heads % c.n_kv_heads == 0 && c.ffn_dim > 0 &&
            c.vocab > 0 && c.max_seq > 0 && c.max_seq <= 65536 && c.max_batch > 0 && c.dim % 32 == 0 && c.ffn_dim % 32 == 0 &&
            (c.n_heads * c.head_dim) % 32 == 0 && c.dim <= 16384 && c.ffn_dim <= 16384 &&
-           c.n_heads * c.head_dim <= 16384;
+           c.n_heads * c.head_dim <= 16384 && (c.kv_f16 != RDL_LLAMA_KV_Q4 || c.head_dim % 32 == 0);
 }
 
 // Where a weight slot's bytes go: `rows` rows of row_bytes, at dst with row
@@ -1486,7 +1502,7 @@ rdl_status rdl_llama_create_typed(const rdl_llama_config* cfg, const int32_t* ty
     if ((e = alloc_mat(M.out)) != hipSuccess) return fail_free(e);
     if ((e = M.alloc_t(&M.final_norm, c.dim)) != hipSuccess) return fail_free(e);
     M.n_pages = (c.max_seq + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
-    const size_t kv_bytes = (size_t)c.n_layers * M.kv_layer_elems() * M.kv_elem();
+    const size_t kv_bytes = (size_t)c.n_layers * M.kv_layer_bytes();
     if ((e = M.alloc(&M.kc, kv_bytes)) != hipSuccess) return fail_free(e);
     if ((e = M.alloc(&M.vc, kv_bytes)) != hipSuccess) return fail_free(e);
     {  // identity page table: the layout of a contiguous cache
@@ -1669,6 +1685,8 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
     try {
         B.len.assign(n_seq, 0);
         B.free_host.resize((size_t)M.n_pages);
+        B.holders.assign((size_t)M.n_pages, 0);
+        B.row_host.resize((size_t)M.n_pages);
     } catch (const std::exception&) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
     }
@@ -1677,8 +1695,11 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
         const size_t mb = c.max_batch, pg = M.n_pages, last = std::min(n_seq, mb);
         const std::pair<int**, size_t> ints[] = {
             {&B.table, n_seq * pg}, {&B.cached, n_seq}, {&B.count, n_seq}, {&B.free_pages, pg}, {&B.row_start, n_seq + 1},
-            {&B.kv_len, n_seq}, {&B.row_seq, mb}, {&B.positions, mb}, {&B.slots, mb}, {&B.summary, 4}, {&B.last_rows, last}};
-        const std::pair<float**, size_t> floats[] = {{&B.x, last * c.dim}, {&B.logits, last * c.vocab}};
+            {&B.kv_len, n_seq}, {&B.row_seq, mb}, {&B.positions, mb}, {&B.slots, mb}, {&B.summary, 4}, {&B.last_rows, last},
+            {&B.parents, n_seq}, {&B.children, n_seq}, {&B.src, n_seq}, {&B.dst, n_seq}, {&B.forked, 2}, {&B.targets, last},
+            {&B.top_ids, last * rdl::LLAMA_TOP}};
+        const std::pair<float**, size_t> floats[] = {{&B.x, last * c.dim}, {&B.logits, last * c.vocab}, {&B.logprobs, last},
+                                                     {&B.entropies, last}, {&B.top_logprobs, last * rdl::LLAMA_TOP}};
         auto room = [](size_t n) { return (n * 4 + 255) & ~(size_t)255; };
         size_t bytes = 0;
         for (const auto& a : ints) bytes += room(a.second);
@@ -1717,31 +1738,24 @@ rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq) {
     if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
     if (seq >= B.n_seq) return api_fail(RDL_ERR_INVALID_DATA, "sequence %zu of %zu", seq, B.n_seq);
     const size_t held = ((size_t)B.len[seq] + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
-    const size_t had = B.free_host.size();
-    B.free_host.resize(had + held);  // within the capacity it began with
-    if (held) {
-        const hipError_t e = hipMemcpy(B.free_host.data() + had, B.table + seq * M.n_pages, held * sizeof(int),
-                                       hipMemcpyDeviceToHost);
-        if (e != hipSuccess) {
-            B.free_host.resize(had);
-            return api_fail(RDL_ERR_HIP, "page table read failed: %s", hipGetErrorString(e));
-        }
-    }
+    if (held)
+        HIP_TRY(hipMemcpy(B.row_host.data(), B.table + seq * M.n_pages, held * sizeof(int), hipMemcpyDeviceToHost));
+    for (size_t i = 0; i < held; i++)
+        if (--B.holders[B.row_host[i]] == 0) B.free_host.push_back(B.row_host[i]);  // within the capacity it began with
     B.len[seq] = 0;
     return api_ok();
 }
 
-rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
-                                   size_t n, float* logits, size_t logits_len) {
-    if (!model || !counts || !tokens || !logits) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
-    rdl::LlamaModel& M = model->m;
+// A step of several sequences up to the logits of the *n_last sequences with tokens, in B.logits;
+// *pages: taken from the free list.  Nothing of the host's state moves before batch_done.
+static rdl_status batch_step(rdl::LlamaModel& M, const int32_t* counts, size_t n_seq, const int32_t* tokens, size_t n,
+                             size_t* n_last, size_t* pages_taken) {
     const rdl_llama_config& c = M.cfg;
     rdl::LlamaModel::Batch& B = M.batch;
     if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
     if (n_seq != B.n_seq) return rdl::api_shape_fail("sequences", {B.n_seq}, {n_seq});
     if (n == 0 || n > (size_t)c.max_batch)
         return api_fail(RDL_ERR_SHAPE_MISMATCH, "%zu tokens: 1 .. max_batch (%d) per call", n, c.max_batch);
-    if (logits_len < n_seq * (size_t)c.vocab) return rdl::api_shape_fail("logits length", {n_seq * (size_t)c.vocab}, {logits_len});
     size_t rows = 0, pages = 0;
     B.max_rows = B.max_kv = 0;
     for (size_t b = 0; b < n_seq; b++) {
@@ -1786,13 +1800,147 @@ rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size
         return B.status;
     }
     HIP_TRY(run);
+    *n_last = last.size();
+    *pages_taken = pages;
+    return RDL_OK;
+}
+// Behind it, once the stream has been waited for.
+static void batch_done(rdl::LlamaModel& M, const int32_t* counts, size_t pages) {
+    rdl::LlamaModel::Batch& B = M.batch;
+    for (size_t i = 0; i < pages; i++) B.holders[B.free_host[i]] = 1;
+    B.free_host.erase(B.free_host.begin(), B.free_host.begin() + (ptrdiff_t)pages);
+    for (size_t b = 0; b < B.n_seq; b++) B.len[b] += counts[b];
+}
+
+rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
+                                   size_t n, float* logits, size_t logits_len) {
+    if (!model || !counts || !tokens || !logits) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
+    rdl::LlamaModel& M = model->m;
+    const rdl_llama_config& c = M.cfg;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (B.on && n_seq == B.n_seq && n > 0 && n <= (size_t)c.max_batch && logits_len < n_seq * (size_t)c.vocab)
+        return rdl::api_shape_fail("logits length", {n_seq * (size_t)c.vocab}, {logits_len});
+    size_t n_last = 0, pages = 0;
+    const rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last, &pages);
+    if (st != RDL_OK) return st;
     for (size_t b = 0, i = 0; b < n_seq; b++)
         if (counts[b])
             HIP_TRY(hipMemcpyAsync(logits + b * c.vocab, B.logits + i++ * c.vocab, (size_t)c.vocab * 4,
                                    hipMemcpyDeviceToHost, M.stream));
     HIP_TRY(hipStreamSynchronize(M.stream));
+    batch_done(M, counts, pages);
+    return api_ok();
+}
+
+rdl_status rdl_llama_batch_logprobs(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
+                                    size_t n, const int32_t* targets, float* logprobs, float* entropies, size_t n_top,
+                                    int32_t* top_ids, float* top_logprobs) {
+    if (!model || !counts || !tokens || !targets != !logprobs || (n_top && (!top_ids || !top_logprobs)))
+        return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
+    rdl::LlamaModel& M = model->m;
+    const rdl_llama_config& c = M.cfg;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (n_top > rdl::LLAMA_TOP || n_top > (size_t)c.vocab)
+        return api_fail(RDL_ERR_UNSUPPORTED, "%zu alternatives of %d tokens: at most %zu", n_top, c.vocab, rdl::LLAMA_TOP);
+    std::vector<int> given, ids;
+    std::vector<float> lp, en, tl;
+    try {
+        given.resize(std::min(n, n_seq)), lp.resize(given.size()), en.resize(given.size());
+        ids.resize(given.size() * n_top), tl.resize(given.size() * n_top);
+    } catch (const std::exception&) {
+        return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
+    }
+    size_t n_last = 0, pages = 0;
+    rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last, &pages);  // (checks n and n_seq)
+    if (st != RDL_OK) return st;
+    for (size_t b = 0, i = 0; targets && b < n_seq; b++)
+        if (counts[b]) given[i++] = targets[b];
+    auto failed = [&](hipError_t e) {
+        (void)hipStreamSynchronize(M.stream);  // the copies' host memory goes
+        return api_fail(RDL_ERR_HIP, "log probabilities: %s", hipGetErrorString(e));
+    };
+    hipError_t e = targets ? hipMemcpyAsync(B.targets, given.data(), n_last * 4, hipMemcpyHostToDevice, M.stream) : hipSuccess;
+    if (e != hipSuccess) return failed(e);
+    st = rdl_logprobs_dev(B.logits, (size_t)c.vocab, n_last, (size_t)c.vocab, targets ? B.targets : nullptr,
+                          targets ? B.logprobs : nullptr, B.entropies, n_top, B.top_ids, B.top_logprobs, M.stream);
+    if (st != RDL_OK) {
+        (void)hipStreamSynchronize(M.stream);
+        return st;
+    }
+    auto down = [&](void* to, const void* from, size_t k) {
+        if (k && e == hipSuccess) e = hipMemcpyAsync(to, from, k * 4, hipMemcpyDeviceToHost, M.stream);
+    };
+    if (targets) down(lp.data(), B.logprobs, n_last);
+    down(en.data(), B.entropies, n_last);
+    down(ids.data(), B.top_ids, n_last * n_top);
+    down(tl.data(), B.top_logprobs, n_last * n_top);
+    if (e != hipSuccess) return failed(e);
+    HIP_TRY(hipStreamSynchronize(M.stream));
+    for (size_t b = 0, i = 0; b < n_seq; b++) {
+        if (!counts[b]) continue;
+        if (logprobs) logprobs[b] = lp[i];
+        if (entropies) entropies[b] = en[i];
+        for (size_t t = 0; t < n_top; t++) top_ids[b * n_top + t] = ids[i * n_top + t], top_logprobs[b * n_top + t] = tl[i * n_top + t];
+        i++;
+    }
+    batch_done(M, counts, pages);
+    return api_ok();
+}
+
+rdl_status rdl_llama_batch_fork(rdl_llama* model, const int32_t* parents, const int32_t* children, size_t n) {
+    if (!model || (n && (!parents || !children))) return api_fail(RDL_ERR_NULL_POINTER, "NULL argument");
+    rdl::LlamaModel& M = model->m;
+    rdl::LlamaModel::Batch& B = M.batch;
+    if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
+    if (n > B.n_seq) return api_fail(RDL_ERR_INVALID_DATA, "%zu forks of %zu sequences", n, B.n_seq);
+    if (n == 0) return api_ok();
+    std::vector<char> used;
+    std::vector<rdl_kv_pool> pools;
+    std::vector<int> table;
+    try {
+        used.assign(B.n_seq, 0);
+        pools.resize((size_t)M.cfg.n_layers);
+        table.resize(B.n_seq * (size_t)M.n_pages);
+    } catch (const std::exception&) {
+        return api_fail(RDL_ERR_INVALID_DATA, "%zu forks", n);
+    }
+    size_t pages = 0;
+    for (size_t i = 0; i < n; i++) {
+        const int p = parents[i], ch = children[i];
+        if (p < 0 || (size_t)p >= B.n_seq || ch < 0 || (size_t)ch >= B.n_seq)
+            return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d from %d of %zu", i, ch, p, B.n_seq);
+        if (B.len[ch] != 0) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d is not empty", i, ch);
+        if (used[ch]) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d again", i, ch);
+        used[ch] = 1;
+        pages += B.len[p] % rdl::KV_PAGE != 0;
+    }
+    for (size_t i = 0; i < n; i++)
+        if (used[parents[i]]) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d is forked itself", i, parents[i]);
+    if (pages > B.free_host.size())
+        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.free_host.size());
+    for (size_t l = 0; l < pools.size(); l++) pools[l] = M.batch_pool((int)l);
+    auto up = [&](int* dst, const int* src, size_t k) {
+        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
+    };
+    HIP_TRY(up(B.cached, B.len.data(), B.n_seq));
+    HIP_TRY(up(B.parents, parents, n));
+    HIP_TRY(up(B.children, children, n));
+    HIP_TRY(up(B.free_pages, B.free_host.data(), pages));
+    rdl_status st = rdl_kv_fork_dev(B.table, (size_t)M.n_pages, B.cached, B.n_seq, rdl::KV_PAGE, B.parents, B.children, n,
+                                    B.free_pages, pages, B.src, B.dst, B.forked, M.stream);
+    if (st == RDL_OK) st = rdl_kv_copy_pages_dev(pools.data(), pools.data(), pools.size(), B.src, B.dst, n, M.stream);
+    if (st != RDL_OK) {
+        (void)hipStreamSynchronize(M.stream);
+        return st;
+    }
+    HIP_TRY(hipMemcpyAsync(table.data(), B.table, table.size() * sizeof(int), hipMemcpyDeviceToHost, M.stream));
+    HIP_TRY(hipStreamSynchronize(M.stream));
+    for (size_t i = 0; i < n; i++) {
+        B.len[children[i]] = B.len[parents[i]];
+        const int* row = table.data() + (size_t)children[i] * M.n_pages;
+        for (int p = 0; p < (B.len[children[i]] + rdl::KV_PAGE - 1) / rdl::KV_PAGE; p++) B.holders[row[p]]++;
+    }
     B.free_host.erase(B.free_host.begin(), B.free_host.begin() + (ptrdiff_t)pages);
-    for (size_t b = 0; b < n_seq; b++) B.len[b] += counts[b];
     return api_ok();
 }
 
@@ -1801,6 +1949,7 @@ rdl_status rdl_llama_forward(rdl_llama* model, const int32_t* tokens, size_t n, 
     rdl::LlamaModel& M = model->m;
     const rdl_llama_config& c = M.cfg;
     if (M.batch.on) return api_fail(RDL_ERR_INVALID_DATA, "the cache holds several sequences (rdl_llama_reset first)");
+    if (M.kv_q4()) return api_fail(RDL_ERR_UNSUPPORTED, "a 4-bit cache serves rdl_llama_batch_* alone");
     if (n == 0 || n > (size_t)c.max_batch)
         return api_fail(RDL_ERR_SHAPE_MISMATCH, "%zu tokens: 1 .. max_batch (%d) per call", n, c.max_batch);
     if (logits_len < (size_t)c.vocab)
@@ -1829,6 +1978,7 @@ rdl_status rdl_llama_generate_greedy(rdl_llama* model, const int32_t* prompt, si
     rdl::LlamaModel& M = model->m;
     const rdl_llama_config& c = M.cfg;
     if (M.batch.on) return api_fail(RDL_ERR_INVALID_DATA, "the cache holds several sequences (rdl_llama_reset first)");
+    if (M.kv_q4()) return api_fail(RDL_ERR_UNSUPPORTED, "a 4-bit cache serves rdl_llama_batch_* alone");
     if (n_prompt == 0) return api_fail(RDL_ERR_INVALID_DATA, "empty prompt");
     if (n_gen == 0) return api_ok();
     // the last sampled token is not fed back: positions used = prompt + n_gen - 1

@@ -18,6 +18,7 @@ from . import _decl, _i32, _p, _sz, check, lib
 
 TOKEN_EMBEDDING, ATTN_NORM, WQ, WK, WV, WO, FFN_NORM, W_GATE, W_UP, W_DOWN, FINAL_NORM, OUTPUT = range(12)
 SLOTS = 12
+KV_Q4 = 2  # RDL_LLAMA_KV_Q4: kv_f16 of a 4-bit cache (batch_* alone)
 
 
 class _Config(C.Structure):
@@ -43,6 +44,8 @@ _decl("rdl_llama_batch_forward", _i32, _p, C.POINTER(C.c_int32), _sz, C.POINTER(
       _sz)
 _decl("rdl_llama_batch_positions", _i32, _p, C.POINTER(_sz), _sz)
 _decl("rdl_llama_batch_drop", _i32, _p, _sz)
+_decl("rdl_llama_batch_logprobs", _i32, _p, C.POINTER(C.c_int32), _sz, C.POINTER(C.c_int32), _sz, _p, _p, _p, _sz, _p, _p)
+_decl("rdl_llama_batch_fork", _i32, _p, C.POINTER(C.c_int32), C.POINTER(C.c_int32), _sz)
 _decl("rdl_llama_last_timing", _i32, _p, C.POINTER(C.c_float), C.POINTER(C.c_float))
 _decl("rdl_llama_rope_tables", _i32, _p, C.POINTER(C.c_float), C.POINTER(C.c_float), _sz)
 _decl("rdl_llama_get_config", _i32, _p, C.POINTER(_Config))
@@ -89,7 +92,7 @@ class LlamaConfig:
     max_seq: int = 2048
     norm_eps: float = 1e-5
     rope_theta: float = 10000.0
-    kv_f16: bool = True
+    kv_f16: bool | int = True  # False: f32, KV_Q4: 4 bits
     max_batch: int = 128
     output_dtype: int = 2  # GGML type of the output matrix (Q4_0; also Q8_0, Q4_1, Q4_K, Q6_K)
 
@@ -147,7 +150,7 @@ class LlamaModel:
         self._n_seq = 0
 
     @classmethod
-    def from_gguf(cls, gguf, max_seq: int = 0, max_batch: int = 32, kv_f16: bool = True) -> "LlamaModel":
+    def from_gguf(cls, gguf, max_seq: int = 0, max_batch: int = 32, kv_f16: bool | int = True) -> "LlamaModel":
         """LlmModel::from_pretrained over a GGUF file (a path or an open
         rdlquant.gguf.GGUFFile): config from the metadata, tensors through the
         Llama weight map, bytes from the file mapping straight to HBM
@@ -168,7 +171,8 @@ class LlamaModel:
         self._h = h
         self._n_seq = 0
         self.config = LlamaConfig(c.dim, c.n_layers, c.n_heads, c.n_kv_heads, c.head_dim, c.ffn_dim, c.vocab,
-                                  c.max_seq, float(c.norm_eps), float(c.rope_theta), bool(c.kv_f16),
+                                  c.max_seq, float(c.norm_eps), float(c.rope_theta),
+                                  KV_Q4 if c.kv_f16 == KV_Q4 else bool(c.kv_f16),
                                   c.max_batch, c.output_dtype)
         return self
 
@@ -257,6 +261,32 @@ class LlamaModel:
         check(lib.rdl_llama_batch_forward(self._h, counts.ctypes.data_as(ip), counts.size, flat.ctypes.data_as(ip),
                                           flat.size, logits.ctypes.data_as(C.POINTER(C.c_float)), logits.size))
         return logits
+
+    def batch_logprobs(self, tokens, targets=None, n_top: int = 0):
+        """batch_forward with log probabilities instead of logits: (logprobs of
+        `targets`, one a sequence, or None; entropies; ids and log probabilities of
+        the n_top most likely tokens), NaN and -1 for sequences without tokens."""
+        n = len(tokens)
+        counts, flat = _i32_array([len(t) for t in tokens]), _i32_array([t for seq in tokens for t in seq])
+        given = None if targets is None else _i32_array(targets)
+        if given is not None and given.size != n:
+            raise ValueError(f"{given.size} targets of {n} sequences")
+        lp, en = (np.full(n, np.nan, dtype=np.float32) for _ in range(2))
+        ids, tl = np.full((n, n_top), -1, dtype=np.int32), np.full((n, n_top), np.nan, dtype=np.float32)
+        ip = C.POINTER(C.c_int32)
+        check(lib.rdl_llama_batch_logprobs(self._h, counts.ctypes.data_as(ip), n, flat.ctypes.data_as(ip), flat.size,
+                                           None if given is None else given.ctypes.data,
+                                           None if given is None else lp.ctypes.data, en.ctypes.data, n_top,
+                                           ids.ctypes.data if n_top else None, tl.ctypes.data if n_top else None))
+        return (None if given is None else lp), en, ids, tl
+
+    def batch_fork(self, parents, children) -> None:
+        """The empty sequences `children` become copies of `parents` over shared pages."""
+        p, c = _i32_array(parents), _i32_array(children)
+        if p.size != c.size:
+            raise ValueError(f"{p.size} parents, {c.size} children")
+        ip = C.POINTER(C.c_int32)
+        check(lib.rdl_llama_batch_fork(self._h, p.ctypes.data_as(ip), c.ctypes.data_as(ip), p.size))
 
     def batch_positions(self) -> list:
         """Positions that each sequence has."""
