@@ -612,10 +612,25 @@ struct Slab<Q4, HD, SK> {
         for (int n = 0; n < NG * LPG; n++) {
             const int pc = lane + 64 * (n % LPG), row = row0 + n / LPG * GK + pc / PPK, col = pc % PPK * NW;
             const q4h2 d = __builtin_bit_cast(q4h2, perm(kd[n], kd[n], 0x05040100u)), e = __builtin_bit_cast(q4h2, perm(vd[n], vd[n], 0x05040100u));
+            // V's rows begin turned by their key, or the pieces that 16 lanes write together would fall on a quarter of
+            // the banks (K's order spreads them as it is)
+            const int turn = NW == 4 ? row & 3 : row >> 1 & 1;
+            uint32_t u[NW];
+#pragma unroll
+            for (int i = 0; i < NW; i++) u[i] = v[n][i];
+#pragma unroll
+            for (int bit = 1; bit < NW; bit <<= 1)
+#pragma unroll
+                for (int i = 0; i < NW; i++)
+                    if (!(i & bit)) {
+                        const uint32_t x = u[i], y = u[i | bit];
+                        u[i] = turn & bit ? y : x;
+                        u[i | bit] = turn & bit ? x : y;
+                    }
 #pragma unroll
             for (int i = 0; i < NW; i++) {
                 *reinterpret_cast<u32x4*>(ks + row * G::HDP + ((col + i) ^ G::k_swap(row)) * 8) = decode.word(k[n][i], d);
-                *reinterpret_cast<u32x4*>(vs + row * G::HDP + ((col + i) ^ G::v_swap(row)) * 8) = decode.word(v[n][i], e);
+                *reinterpret_cast<u32x4*>(vs + row * G::HDP + ((col + (i ^ turn)) ^ G::v_swap(row)) * 8) = decode.word(u[i], e);
             }
         }
         return mt;

@@ -301,6 +301,7 @@ extern "C" rdl_status rdl_logprobs_dev(const float* logits_dev, size_t stride, s
         return api_fail(RDL_ERR_NULL_POINTER, "NULL device pointer");
     if (m == 0) return api_ok();
     if (!logits_dev) return api_fail(RDL_ERR_NULL_POINTER, "logits is NULL");
+    if ((uintptr_t)logits_dev & 3) return api_fail(RDL_ERR_INVALID_DATA, "logits must be 4-byte aligned");
     rdl_status st = rdl::check_stream((hipStream_t)stream);
     if (st != RDL_OK) return st;
     rdl::Args a{logits_dev, (int64_t)stride, (int64_t)m, (int)vocab, (int)n_top, tokens_dev, logprobs_dev, entropies_dev,

@@ -76,12 +76,12 @@ def rope32(x, c, s):
     return torch.cat([a * c - b * s, b * c + a * s], -1)
 
 
-@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 256, 8, 40, 80])
-@pytest.mark.parametrize("kv,layout", [("q4", "heads"), ("f16", "padded"), ("f32", "positions"), ("q4", "padded"), ("q4", "positions")])
+@pytest.mark.parametrize("kv,layout,hd", [
+    (kv, layout, hd) for hd in (32, 64, 96, 128, 160, 256, 8, 40, 80)
+    for kv, layout in (("q4", "heads"), ("f16", "padded"), ("f32", "positions"), ("q4", "padded"), ("q4", "positions"))
+    if kv != "q4" or hd % 32 == 0])
 @pytest.mark.parametrize("rope,in_place,norms", [(True, False, "qk"), (True, True, "k"), (False, False, "q"), (True, True, "")])
 def test_store_norm(rq, gpu, hd, kv, layout, rope, in_place, norms):
-    if kv == "q4" and hd % 32:
-        pytest.skip("4-bit blocks are 32 values")
     torch.manual_seed(hd)
     rows, heads, kvh, page, npos, eps = 37, 6, 2, 32, 90, 2.0 ** -17  # (f32 as 64 bits)
     pool = Pool(5, page, kvh, hd, kv, layout)
@@ -408,6 +408,94 @@ def test_attention(rq, gpu, case, hd, heads, kvh, page):
         attend(pool, q, heads, lens, kv, tables, hd ** -0.5, out, max(lens) * hint, max(kv) * hint)
         check(pool, q[:m - 2], heads, lens, kv, tables, out, hd ** -0.5)
         assert out[m - 2:].isnan().all()  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("lens,kv,hd,heads,kvh,page", [
+    ([1] * 48, [int(3000 * ((i * 37) % 48) / 47) + 1 for i in range(48)], 128, 8, 2, 64),  # dealt out over the launch
+    ([1, 0, 1, 1, 0, 2], [5000, 300, 0, 1, 64, 2500], 64, 8, 2, 16),                       # sequences without rows or keys
+    ([1] * 64, [700 + 13 * i for i in range(64)], 64, 4, 4, 32),                           # a lane each
+    ([1] * 100, [300 + 7 * i for i in range(100)], 128, 4, 1, 128),                        # too many for a plan
+    ([1], [40000], 128, 4, 1, 64),                                                          # more parts than are joined
+    ([1, 2], [9000, 7000], 128, 8, 2, 64),                                                  # 4 and 8 pairs: packed
+    ([1, 3], [9000, 7000], 128, 8, 2, 64),                                                  # 12 pairs: not
+    ([1, 1], [9000, 7000], 256, 16, 1, 16),                                                 # 16 pairs, wide heads
+    ([2, 1], [4000, 3000], 32, 3, 1, 16),
+    ([1] * 5 + [40], [3000, 10, 700, 1500, 64, 900], 128, 8, 2, 32)])                       # single rows beside a chunk
+def test_attention_of_split_keys(rq, gpu, lens, kv, hd, heads, kvh, page):
+    torch.manual_seed(len(kv) + hd)
+    pool = Pool(sum(-(-n // page) for n in kv) + 3, page, kvh, hd, "q4")
+    tables = sequences(pool, kv, random.Random(hd))
+    q = torch.randn(sum(lens), heads * hd, device="cuda")
+    last = None
+    for rows, keys in ((max(lens), max(kv)), (0, 0), (1, max(kv)), (1, 129)):  # the last two: less than there is
+        out = torch.full_like(q, float("nan"))
+        attend(pool, q, heads, lens, kv, tables, hd ** -0.5, out, rows, keys)
+        check(pool, q, heads, lens, kv, tables, out, hd ** -0.5)
+        again = torch.full_like(q, float("nan"))
+        attend(pool, q, heads, lens, kv, tables, hd ** -0.5, again, rows, keys)
+        assert torch.equal(out, again)  # whichever part arrives last
+        last = out if last is None else last
+        assert (out - last).abs().max() < 1e-4
+
+
+def test_two_streams(rq, gpu):
+    torch.manual_seed(5)
+    hd, heads, kvh, page = 128, 8, 2, 64
+    lens, kv = [1] * 20, [200 + 190 * i for i in range(20)]
+    pool = Pool(sum(-(-n // page) for n in kv), page, kvh, hd, "q4")
+    tables = sequences(pool, kv, random.Random(7))
+    qs = [torch.randn(20, heads * hd, device="cuda") for _ in range(2)]
+    want = [torch.empty_like(q) for q in qs]
+    rs, kl = ints(list(range(21))), ints(kv)
+
+    def call(q, out, s):
+        A.attention_paged_dev(pool.c, q.data_ptr(), heads * hd, heads, 20, rs.data_ptr(), kl.data_ptr(), 20, tables.data_ptr(),
+                              tables.shape[1], 0.1, out.data_ptr(), heads * hd, 1, max(kv), s)
+
+    for q, w in zip(qs, want):
+        call(q, w, stream())
+    torch.cuda.synchronize()
+    got, streams = [torch.empty_like(q) for q in qs], [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(30):
+        for q, o, s in zip(qs, got, streams):
+            call(q, o, s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(got, want))
+
+
+def test_offsets_past_32_bits(rq, gpu):
+    """Pages 3 GB apart: stored, attended to, copied."""
+    torch.manual_seed(6)
+    hd, heads, kvh, page, far = 64, 4, 1, 16, 3 << 30
+    n = q4.run_bytes(page, hd)
+    mem = [torch.empty(2 * far + n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    runs = [torch.as_strided(t, (3, kvh, n), (far, n, 1)) for t in mem]
+    pool = Pool(1, page, kvh, hd, "q4")
+    pool.k, pool.v = (q4.Runs(t, page, hd) for t in runs)
+    pool.pages = 3
+    pool.c = A.KvPool(mem[0].data_ptr(), mem[1].data_ptr(), A.KV_Q4, 3, page, kvh, hd, far, n, hd // 2)
+    rows = 40
+    x = torch.randn(rows, (heads + 2) * hd, device="cuda")
+    q, k, v = x[:, :heads * hd], x[:, heads * hd:(heads + 1) * hd], x[:, (heads + 1) * hd:]
+    tables = ints([[2, 0, 1]])
+    slots = ints([[2, 0, 1][i // page] * page + i % page for i in range(rows)])
+    w = x.shape[1]
+    out = torch.empty(rows, heads * hd, device="cuda")
+    A.store_dev(pool.c, rows, q.data_ptr(), w, out.data_ptr(), heads * hd, heads, k.data_ptr(), w, v.data_ptr(), w, 0, slots.data_ptr(), 0,
+                0, 0, stream())
+    d, c = q4.quantize(k.cpu().view(rows, 1, hd))
+    sl = slots.long()
+    assert torch.equal(pool.k.codes[sl // page, :, sl % page].cpu(), q4.pack(c))
+    got = torch.full((rows, heads * hd), float("nan"), device="cuda")
+    for lens in ([rows], [1]):
+        m = lens[0]
+        attend(pool, q[rows - m:], heads, lens, [rows], tables, 0.125, got[rows - m:])
+        check(pool, q[rows - m:].contiguous(), heads, lens, [rows], tables, got[rows - m:], 0.125)
+    dst = Pool(2, page, kvh, hd, "f16")
+    f, t = ints([2, 1]), ints([0, 1])
+    A.copy_pages_dev([pool.c], [dst.c], f.data_ptr(), t.data_ptr(), 2, stream())
+    both = pool.both()
+    assert torch.equal(dst.k[0].double(), both[0, 2]) and torch.equal(dst.v[0].double(), both[1, 2])
 
 
 @pytest.mark.parametrize("lens,kv", [([1, 1], [200, 130]), ([40, 70], [200, 130])])

@@ -139,7 +139,7 @@ def test_fork_sizes(rq, at):
     (dict(vocab=0), "DeviceError"), (dict(vocab=1 << 29, stride=1 << 29), "DeviceError"), (dict(stride=99), "ShapeMismatch"),
     (dict(top=65), "DeviceError"), (dict(top=3, vocab=2), "DeviceError"), (dict(m=1 << 24), "DeviceError"),
     (dict(stride=1 << 33), "DeviceError"), (dict(tokens=0), "DeviceError"), (dict(lp=0), "DeviceError"),
-    (dict(ids=0), "DeviceError"), (dict(tl=0), "DeviceError"), (dict(x=0), "DeviceError"),
+    (dict(ids=0), "DeviceError"), (dict(tl=0), "DeviceError"), (dict(x=0), "DeviceError"), (dict(x=Q + 2), "InvalidData"),
 ])
 def test_logprobs_refusals(rq, kw, kind):
     a = {**dict(x=Q, stride=100, m=2, vocab=100, tokens=INTS, lp=OUT, en=OUT, top=5, ids=INTS, tl=OUT), **kw}
