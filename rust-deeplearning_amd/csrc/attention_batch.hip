@@ -763,7 +763,8 @@ __device__ __forceinline__ Seq sequence(const BatchArgs& a, int b) {
 // to 1900 f32 keys with TILE_MIN_SPAN 128, 256, 512: 22.8, 25.0, 36.7.
 constexpr int64_t FEW_TARGET = 2048, TILE_TARGET = 512, MIXED_TARGET = 384;
 constexpr int FEW_MIN_SPAN = 128, TILE_MIN_SPAN = 128;
-// few_plan: workgroups that run at once (wide heads: a third of them), and the keys that one's waves take in a turn.
+// few_plan: workgroups that run at once (wide heads: two thirds of them), the keys that one's waves take in
+// a turn, and those that the begin of a sequence stands for.
 constexpr int FEW_SLOTS = 768, FEW_UNIT = 128, FEW_BEGIN = 4;
 
 // Tiles are numbered so that a sequence is found from row_start alone:
@@ -1641,7 +1642,7 @@ __device__ __forceinline__ int few_rows(const BatchArgs& a, const Seq& s, const 
 //   K: lane (g, c) = (lane / 16, lane % 16) loads the codes of 32 dims of key c (32 g .., 64-wide heads 16 of
 //      them), one load and one scale, which are the A operands of four steps of
 //      S^T = K Q^T, a code word a step; q is laid out to match;
-//   V: O^T = V^T P^T needs a dim's values of eight keys a lane.  Lane (g, c) loads
+//   V: O^T = V^T P^T needs a dim's values of eight keys a lane (a quad's lanes load a scale each of the four).  Lane (g, c) loads
 //      the word of dims 8 c .. 8 c + 7 of each of the eight keys whose weights it holds,
 //      an 8 x 8 block of nibbles: dim 8 c + t of all of them, two keys an instruction, is its A
 //      operand of tile t, whose 16 rows are the dims t of the 16 words (64-wide
@@ -1658,7 +1659,7 @@ struct FourBits {
     struct alignas(4) Scale {  // a register each
         _Float16 x;
     };
-    Scale kd[2][NH], vd[8][NH];
+    Scale kd[2][NH], vd[2][NH];  // of V: key 4 g + c % 4's of each group, which its quad shares
 };
 template <int HD>
 struct FourSlab {
@@ -1676,7 +1677,7 @@ struct FourSlab {
             k_off[i] = kb < row ? (uint32_t)(c * row + kb) : RSRC_OOB;
             kd_off[i] = kb < row ? (uint32_t)(c * row_scales + kb / 16 * 2) : RSRC_OOB;
             v_off[i] = vb < row ? (uint32_t)(4 * g * row + vb) : RSRC_OOB;
-            vd_off[i] = vb < row ? (uint32_t)(4 * g * row_scales + vb / 16 * 2) : RSRC_OOB;
+            vd_off[i] = vb < row ? (uint32_t)((4 * g + c % 4) * row_scales + vb / 16 * 2) : RSRC_OOB;
         }
     }
     __device__ __forceinline__ void pages(const KvSource& s, const int32_t* table, int j, int t) {
@@ -1713,14 +1714,14 @@ struct FourSlab {
                 }
                 // (16 bits stay as they are until their use: a widening here would wait for the load)
                 x->kd[b][i].x = half_of(ks, kd_off[i]);
-                uint32_t va = v_off[i], da = vd_off[i];
-                asm("" : "+v"(va), "+v"(da));  // sums of a step, not registers of the loop
+                x->vd[b][i].x = half_of(vs, vd_off[i]);
+                uint32_t va = v_off[i];
+                asm("" : "+v"(va));  // sums of a step, not registers of the loop
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t at = va + e * row;
                     if constexpr (Bits::HALF) x->v[4 * b + e][i] = __builtin_amdgcn_raw_buffer_load_b16(vr, (int)at, 0, 0);
                     else x->v[4 * b + e][i] = buf_load_b32(vr, at);
-                    x->vd[4 * b + e][i].x = half_of(vs, da + e * row_scales);
                 }
             }
         }
@@ -1844,7 +1845,9 @@ __device__ __forceinline__ int few_rows_q4(const BatchArgs& a, const Seq& s, con
             uint32_t dd[4], half[2][4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {  // keys 2 i and 2 i + 1
-                dd[i] = __builtin_bit_cast(uint32_t, q4h2{x.vd[2 * i][n].x, x.vd[2 * i + 1][n].x});
+                const uint32_t d = __builtin_bit_cast(uint16_t, x.vd[i >> 1][n].x);
+                dd[i] = i & 1 ? perm((uint32_t)dpp_i32<0xFF>((int)d), (uint32_t)dpp_i32<0xAA>((int)d), 0x05040100u)   // of lanes 2, 3
+                              : perm((uint32_t)dpp_i32<0x55>((int)d), (uint32_t)dpp_i32<0x00>((int)d), 0x05040100u);  // of lanes 0, 1
                 half[0][i] = perm(x.v[2 * i + 1][n], x.v[2 * i][n], 0x05040100u);
                 if constexpr (!Bits::HALF) half[1][i] = perm(x.v[2 * i + 1][n], x.v[2 * i][n], 0x07060302u);
             }
@@ -2027,11 +2030,12 @@ __device__ __forceinline__ void few_pairs(const BatchArgs& a, const Seq& s, int 
 // registers than either needs, so launches that need one of them have it alone.
 constexpr int TILE = 1, FEW = 2;
 // Waves of a SIMD at least, which bounds the registers.  Few rows over 4-bit keys
-// need little LDS: three waves (168 registers, none of the loop's in memory) took 75 us
-// where two took 76 and four, with registers in memory, 145.
+// need little LDS: 48 rows over up to 8192 keys took 71 us with three waves (168 registers, none of
+// the loop's in memory), 76 with two and 98 with four, with registers in memory; heads
+// of 256 (half as many of them) 71 with two and 83 with one.
 template <typename KV, int HD, int KIND>
 constexpr int waves_per_simd() {
-    if (std::is_same<KV, Q4>::value && KIND == FEW && HD != 256) return 3;
+    if (std::is_same<KV, Q4>::value && KIND == FEW) return HD == 256 ? 2 : 3;
     return HD == 256 ? 1 : 2;
 }
 template <typename KV, int HD, int KIND, bool PACKED = false>
@@ -2270,7 +2274,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
     }
     // (fewer workgroups than run at once need no plan: one row over 778 keys took 14.0 us with it, 11.1 without)
     if (dtype == RDL_KV_Q4 && only_few && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS) {
-        const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS / 3 : FEW_SLOTS) / a.n_kv);
+        const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS * 2 / 3 : FEW_SLOTS) / a.n_kv);
         const int64_t most = std::min<int64_t>({(keys + FEW_UNIT - 1) / FEW_UNIT, most_parts, JOIN_SPLITS, slots});
         if (most > 1) a.few_slots = (int)slots, a.few_splits = (int)most;
     }
