@@ -28,6 +28,9 @@ namespace {
 // 32003 take 44 us, 5.8 TB/s (a large copy reaches 5.1).
 constexpr int NT = 256, W = NT / 64, PER = 16, STEP = 64 * PER, TOP = 64;
 constexpr int WG_TARGET = 1024, MOST_PARTS = 64;
+// A list begins by counting (first_list), where that is faster than one by one: 16 rows of 32000 with 5,
+// 20 and 64 alternatives took 10.3, 12.4 and 71.7 us so, 10.4, 23.6 and 63.3 one by one.
+__host__ __device__ constexpr bool counted(int n) { return n > 4 && n <= 32; }
 constexpr float LOG2E = 1.44269504088896340736f;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -71,16 +74,32 @@ __device__ __forceinline__ float wave_sum(float v) {
     v += other16(v);
     return v + other32(v);
 }
-// The largest key: of those with the largest upper word the largest lower one.
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
-    const uint32_t hi = wave_max_u32((uint32_t)(v >> 32));
-    return (uint64_t)hi << 32 | wave_max_u32((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0);
+__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {  // lane's, uniform
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 // The value of the lane before (0 in lane 0).
 __device__ __forceinline__ uint64_t lane_before(uint64_t v) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, 0x138, 0xF, 0xF, false);  // wave_shr:1
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
     return (uint64_t)hi << 32 | lo;
+}
+
+// Orders a wave's LDS accesses between its lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// How many of n keys in LDS (8-byte, from a 16-byte boundary, a 0 behind an odd number) are larger than k.
+__device__ __forceinline__ int larger(const uint64_t* keys, int n, uint64_t k) {
+    int c = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; i += 2) {  // (reads of LDS in flight together)
+        const u32x4 two = *reinterpret_cast<const u32x4*>(keys + i);
+        c += ((uint64_t)two[1] << 32 | two[0]) > k;
+        c += ((uint64_t)two[3] << 32 | two[2]) > k;
+    }
+    return c;
 }
 
 struct Stats {
@@ -112,10 +131,81 @@ __device__ __forceinline__ f4 load4(const float* row, int i, int hi) {
     return x;
 }
 
+// The n largest keys of the wave's step x, the i-th in lane i, by counting: the n-th
+// largest of the lanes' own largest keys is a bound that n lanes' values at most reach, whose places in
+// the order are then counted.  room: room_of(n) keys of LDS.
+__device__ __forceinline__ uint64_t first_list(const f4 (&x)[PER / 4], float top, int i0, int n, uint64_t* room) {
+    const int lane = threadIdx.x & 63;
+    int at = INT_MAX;
+#pragma unroll
+    for (int j = PER / 4 - 1; j >= 0; j--)
+#pragma unroll
+        for (int t = 3; t >= 0; t--)
+            if (x[j][t] == top) at = i0 + (j * 64 + lane) * 4 + t;
+    const uint64_t own = at == INT_MAX ? 0 : key_of(top, at);
+    room[lane] = own;
+    wave_sync();
+    const int before = larger(room, 64, own);
+    const uint64_t nth = __builtin_amdgcn_ballot_w64(own != 0 && before == n - 1);
+    uint64_t bound = 1;
+    if (nth) {
+        bound = lane_key(own, (int)__builtin_ctzll(nth));
+    }
+    wave_sync();
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < PER / 4; j++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint64_t k = x[j][t] == x[j][t] ? key_of(x[j][t], i0 + (j * 64 + lane) * 4 + t) : 0;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(k >= bound);
+            if (k >= bound) room[count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = k;
+            count += (int)__builtin_popcountll(m);
+        }
+    if (lane == 0) room[count] = 0;
+    wave_sync();
+    // into order: the lanes' keys, 64 at a time, to their places (room for n behind the others)
+    uint64_t* sorted = room + n * PER + 2;
+    if (lane < n) sorted[lane] = 0;
+    wave_sync();
+    for (int i = lane; i < count; i += 64) {
+        const uint64_t k = room[i];
+        const int place = larger(room, count, k);
+        if (place < n) sorted[place] = k;
+    }
+    wave_sync();
+    return lane < n ? sorted[lane] : 0;
+}
+__host__ __device__ constexpr int room_of(int n) { return counted(n) ? n * PER + 2 + ((n + 1) & ~1) : 0; }
+// `count` lists of n keys each in LDS, largest first, to one, by counting, four at a
+// time, between src and dst; both have a key's room behind their lists.
+__device__ __forceinline__ const uint64_t* merge_lists(uint64_t* src, uint64_t* dst, int count, int n) {
+    const int tid = threadIdx.x;
+    while (count > 1) {
+        const int groups = (count + 3) / 4;
+        for (int i = tid; i <= groups * n; i += NT) dst[i] = 0;
+        if (tid == 0) src[count * n] = 0;
+        __syncthreads();
+        for (int i = tid; i < count * n; i += NT) {
+            const uint64_t k = src[i];
+            const int g = i / (4 * n), lists = min(4, count - 4 * g);
+            const int place = k ? larger(src + g * 4 * n, lists * n, k) : n;
+            if (place < n) dst[g * n + place] = k;
+        }
+        __syncthreads();
+        uint64_t* t = src;
+        src = dst, dst = t;
+        count = groups;
+    }
+    return src;
+}
+
 template <bool TOPS>
-__global__ __launch_bounds__(NT) void logprobs_kernel(Args a) {
+__global__ __launch_bounds__(NT, 4) void logprobs_kernel(Args a) {
     __shared__ float wave_stats[W][4];
-    __shared__ uint64_t lists[TOPS ? MOST_PARTS * TOP : 1];
+    // the waves' rooms for their first lists, the lists of the waves or parts, and those merged
+    extern __shared__ __attribute__((aligned(16))) uint64_t smem[];
+    uint64_t *lists = smem + W * room_of(a.n_top), *merged = lists + ((max(W, a.parts) * a.n_top + 2) & ~1);
     __shared__ int flag;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t r = blockIdx.x / a.parts;
@@ -171,6 +261,11 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Args a) {
                 s.T = fmaf(e, d, s.T);
             }
         if constexpr (TOPS) {
+            if (i0 == lo && counted(a.n_top)) {
+                list = first_list(x, top, i0, a.n_top, smem + w * room_of(a.n_top));
+                least = lane_key(list, a.n_top - 1);
+                continue;
+            }
             // the step's values that belong into the list, largest first; one that is as large as the list's last
             // lies behind it in the row
             while (__builtin_amdgcn_ballot_w64(least == 0 || top > value_of(least))) {
@@ -185,8 +280,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Args a) {
                 at = (int)~wave_max_u32(~(uint32_t)at);
                 if (at == INT_MAX) break;  // nothing left of the step
                 list = insert(list, key_of(V, at));
-                least = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(list >> 32), a.n_top - 1) << 32 |
-                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)list, a.n_top - 1);
+                least = lane_key(list, a.n_top - 1);
                 top = -__builtin_inff();
 #pragma unroll
                 for (int j = 0; j < PER / 4; j++)
@@ -209,26 +303,18 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Args a) {
     if constexpr (TOPS)
         if (lane < a.n_top) lists[w * a.n_top + lane] = list;
     __syncthreads();
-    // n lists of n_top keys, largest first, in LDS: their largest, the i-th in lane i (wave 0)
+    uint64_t best = 0;  // wave 0: the largest keys, the i-th in lane i
     auto merge = [&](int n) {
-        uint64_t best = 0;
         if constexpr (TOPS) {
-            int head = 0;
-            for (int i = 0; i < a.n_top; i++) {
-                const uint64_t mine = lane < n && head < a.n_top ? lists[lane * a.n_top + head] : 0;
-                const uint64_t k = wave_max_key(mine);
-                if (k == mine && k != 0) head++;  // keys differ
-                if (lane == i) best = k;
-            }
+            const uint64_t* r = merge_lists(lists, merged, n, a.n_top);
+            best = lane < a.n_top ? r[lane] : 0;
         }
-        return best;
     };
-    uint64_t best = 0;
+    merge(W);
     if (w == 0) {
         s = lane < W ? Stats{wave_stats[lane][0], wave_stats[lane][1], wave_stats[lane][2]} : Stats{-__builtin_inff(), 0.0f, 0.0f};
         bad = __builtin_amdgcn_ballot_w64(lane < W && wave_stats[lane & (W - 1)][3] != 0.0f) != 0;
         s = join(s);
-        best = merge(W);
     }
     if (a.parts > 1) {
         // the workgroup's result, agent-coherent, then its arrival
@@ -267,8 +353,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Args a) {
             }
             bad = __builtin_amdgcn_ballot_w64(b) != 0;
             s = join(s);
-            best = merge(a.parts);
         }
+        merge(a.parts);
     }
     if (w != 0) return;
     const bool none = bad || s.M == -__builtin_inff();
@@ -318,8 +404,14 @@ extern "C" rdl_status rdl_logprobs_dev(const float* logits_dev, size_t stride, s
         a.counters = work.counters;
     }
     const dim3 grid((unsigned)(m * (size_t)a.parts));
-    hipLaunchKernelGGL((n_top ? rdl::logprobs_kernel<true> : rdl::logprobs_kernel<false>), grid, dim3(rdl::NT), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
+    const int lists = std::max(rdl::W, a.parts);
+    const size_t lds = n_top ? 8 * (size_t)(rdl::W * rdl::room_of(a.n_top) + ((lists * a.n_top + 2) & ~1) + (lists + 3) / 4 * a.n_top + 2) : 0;
+    auto kernel = n_top ? rdl::logprobs_kernel<true> : rdl::logprobs_kernel<false>;
+    hipError_t e = lds > 64 * 1024 ? hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) : hipSuccess;
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(kernel, grid, dim3(rdl::NT), lds, (hipStream_t)stream, a);
+        e = hipGetLastError();
+    }
     const rdl_status done = a.parts > 1 ? rdl::call_scratch_done((hipStream_t)stream, &work) : RDL_OK;
     HIP_TRY(e);
     return done == RDL_OK ? api_ok() : done;
