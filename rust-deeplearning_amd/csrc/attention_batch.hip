@@ -2078,7 +2078,9 @@ __global__ __launch_bounds__((Geo<KV, HD>::W * 64), (waves_per_simd<KV, HD, KIND
         uint64_t left = 1;  // sequences of this workgroup
         FewPlan p{{0, 0, 0, 0}, 0, 0, 1};
         const bool planned = KIND == FEW && std::is_same<KV, Q4>::value && a.few_slots;
-        const int lo = planned ? id * (p = few_plan(a)).per : 0, hi = lo + p.per;
+        if (planned) p = few_plan(a);
+        // (a hint far below the longest sequence makes parts so long that the last workgroups would begin past 2^31)
+        const int lo = (int)min((int64_t)id * p.per, (int64_t)INT32_MAX - p.per), hi = lo + p.per;
         // (of a sequence's units the first FEW_BEGIN have no keys)
         if (planned) left = __builtin_amdgcn_ballot_w64(p.units && p.before + FEW_BEGIN < hi && p.before + p.units > lo);
         for (; left; left &= left - 1) {

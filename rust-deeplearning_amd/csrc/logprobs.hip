@@ -23,13 +23,13 @@ namespace {
 // steps, so that a comparison a step is what the alternatives cost.  The waves of a
 // workgroup join through LDS, the workgroups of a row (rows that are few are split, down to a
 // step a wave) through partial results that the last of them to arrive joins.
-// Few rows: latency.  16 rows of 32000, five alternatives: 10.5 us, of which the lists are nothing; one workgroup of 16 waves a
+// Few rows: latency.  16 rows of 32000, five alternatives: 10.5 us (8.7 with one alternative); one workgroup of 16 waves a
 // row took 16.3, the waves' lists then share one CU.  Many rows: HBM bounds it: 2000 rows of
 // 32003 take 44 us, 5.8 TB/s (a large copy reaches 5.1).
 constexpr int NT = 256, W = NT / 64, PER = 16, STEP = 64 * PER, TOP = 64;
 constexpr int WG_TARGET = 1024, MOST_PARTS = 64;
 // A list begins by counting (first_list), where that is faster than one by one: 16 rows of 32000 with 5,
-// 20 and 64 alternatives took 10.3, 12.4 and 71.7 us so, 10.4, 23.6 and 63.3 one by one.
+// 20 and 64 alternatives take 10.4, 12.8 and 71.7 us so, 10.5, 23.7 and 50.5 one by one.
 __host__ __device__ constexpr bool counted(int n) { return n > 4 && n <= 32; }
 constexpr float LOG2E = 1.44269504088896340736f;
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -406,12 +406,10 @@ extern "C" rdl_status rdl_logprobs_dev(const float* logits_dev, size_t stride, s
     const dim3 grid((unsigned)(m * (size_t)a.parts));
     const int lists = std::max(rdl::W, a.parts);
     const size_t lds = n_top ? 8 * (size_t)(rdl::W * rdl::room_of(a.n_top) + ((lists * a.n_top + 2) & ~1) + (lists + 3) / 4 * a.n_top + 2) : 0;
-    auto kernel = n_top ? rdl::logprobs_kernel<true> : rdl::logprobs_kernel<false>;
-    hipError_t e = lds > 64 * 1024 ? hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) : hipSuccess;
-    if (e == hipSuccess) {
-        hipLaunchKernelGGL(kernel, grid, dim3(rdl::NT), lds, (hipStream_t)stream, a);
-        e = hipGetLastError();
-    }
+    static_assert(8 * (rdl::W * rdl::room_of(32) + rdl::MOST_PARTS * 32 * 5 / 4 + 4) <= 64 * 1024 &&
+                  8 * (rdl::W * rdl::room_of(rdl::TOP) + rdl::MOST_PARTS * rdl::TOP * 5 / 4 + 4) <= 64 * 1024, "LDS of a launch");
+    hipLaunchKernelGGL(n_top ? rdl::logprobs_kernel<true> : rdl::logprobs_kernel<false>, grid, dim3(rdl::NT), lds, (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
     const rdl_status done = a.parts > 1 ? rdl::call_scratch_done((hipStream_t)stream, &work) : RDL_OK;
     HIP_TRY(e);
     return done == RDL_OK ? api_ok() : done;
