@@ -848,7 +848,10 @@ __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, fl
 // while the first outputs are on their way, then a thread takes four dims of a
 // pair at a time, by weights of at most 1 (large values stay in f32's range).  Its
 // latency is what it costs.  COHERENT: the partials come from the same launch.
-constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4;  // splits a lane, at most; splits whose outputs are read ahead
+// Behind those read ahead, JOIN_BATCH splits a trip to memory: one row over 4000 and 16000 4-bit keys (32 and 96 splits)
+// took 20.4 and 34.2 us with four, 15.2 and 22.8 with 8, 14.9 and 22.3 with 12, more with 16, whose
+// registers the launch did not have.
+constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4, JOIN_BATCH = 12;  // splits a lane, at most; splits whose outputs are read ahead
 constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
 constexpr int JOIN_FLOATS = FEW_PAIRS * (JOIN_SPLITS + 1);  // of LDS
 template <bool COHERENT>
@@ -911,8 +914,18 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
             const f2 u = get2(o + z * a.hd), v = get2(o + z * a.hd + 2);
             return f4{u[0], u[1], v[0], v[1]};
         };
-#pragma unroll 4
-        for (int z = z0; z < splits; z++) y += w[z] * unit * partial(z);
+        auto batch = [&](auto n) {  // splits whose loads are on their way together
+            constexpr int N = decltype(n)::value;
+            f4 x[N];
+#pragma unroll
+            for (int t = 0; t < N; t++) x[t] = partial(min(z0 + t, splits - 1));
+#pragma unroll
+            for (int t = 0; t < N; t++)
+                if (z0 + t < splits) y += w[z0 + t] * unit * x[t];
+            z0 += N;
+        };
+        while (splits - z0 > JOIN_AHEAD) batch(std::integral_constant<int, JOIN_BATCH>());
+        if (z0 < splits) batch(std::integral_constant<int, JOIN_AHEAD>());
         if (some_not_finite(y)) y = sum_not_finite(y, splits, partial);
         *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y;
     }
@@ -2238,6 +2251,18 @@ constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial resu
 constexpr int64_t SPLIT_MIN_TILES = 4;
 constexpr size_t SPLIT_BYTES = (size_t)1 << 30;
 
+// The shortest span of a split of few rows over 4-bit keys.  A turn of 128 keys takes 1.2 us of a workgroup that waits
+// for each, a split 0.2 us of the join: their sum is least near 4 sqrt(keys).  One row over 4000, 16000 and 60000
+// keys took 15.0, 22.4 and 37.3 us with spans of 128 keys (or dealt out in units of as many), 13.0, 18.4
+// and 32.6 with 256, 512 and 1024.  Short keys of many sequences are not split, which spares the join: 24
+// rows over up to 600 keys (192 workgroups) 13.0 us instead of 15.0, 48 over up to 250 12.0 instead
+// of 14.3; one row over 777 alone 14.9 instead of 10.8.
+constexpr int64_t FOUR_WHOLE_KEYS = 640, FOUR_WHOLE_PAIRS = 128;
+int64_t few_min_span(int64_t pairs, int64_t keys) {
+    if (pairs >= FOUR_WHOLE_PAIRS && keys <= FOUR_WHOLE_KEYS) return FOUR_WHOLE_KEYS;
+    return std::max<int64_t>(FEW_MIN_SPAN, (int64_t)(4.0 * sqrt((double)keys)));
+}
+
 rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipStream_t s) {
     const int64_t m = a.m, rows = max_rows == 0 || (int64_t)max_rows > m ? m : (int64_t)max_rows;
     int64_t keys = a.kv.tables ? a.kv.table_stride << a.kv.shift : m;
@@ -2253,6 +2278,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
     const bool only_few = rows * G <= FEW_PAIRS, only_tile = !only_few && (a.n_seq == 1 || !a.kv.tables);
     a.few_rows = only_few ? INT32_MAX : only_tile ? 0 : FEW_PAIRS;
     a.packed = dtype == RDL_KV_Q4 && rows * G <= 8;
+    const bool only_four = dtype == RDL_KV_Q4 && only_few;
     a.tiles = only_few ? 0 : (int)(m * G / TILE_PAIRS + a.n_seq);
     const int64_t most_parts =
         std::max<int64_t>(1, (int64_t)(PART_BYTES / ((size_t)m * a.n_heads * (a.hd + 2) * sizeof(float))));
@@ -2266,7 +2292,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
         *span = (int)std::min<int64_t>(sp, INT32_MAX / 2);
     };
     if (only_tile) a.few_span = INT32_MAX / 2, a.few_splits = 1;
-    else split(pairs, FEW_TARGET, JOIN_SPLITS, 128, FEW_MIN_SPAN, &a.few_span, &a.few_splits);
+    else split(pairs, FEW_TARGET, JOIN_SPLITS, 128, only_four ? few_min_span(pairs, keys) : FEW_MIN_SPAN, &a.few_span, &a.few_splits);
     if (only_few) a.tile_span = INT32_MAX / 2, a.tile_splits = 1;
     else split((int64_t)a.tiles * a.n_kv, TILE_TARGET, JOIN_SPLITS, 64, TILE_MIN_SPAN, &a.tile_span, &a.tile_splits);
     if (a.tile_splits > 1 && a.n_seq > 1 && a.n_seq <= 64) {
@@ -2275,7 +2301,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
                                                 std::max(2 * a.tile_splits, a.few_splits)});
     }
     // (fewer workgroups than run at once need no plan: one row over 778 keys took 14.0 us with it, 11.1 without)
-    if (dtype == RDL_KV_Q4 && only_few && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS) {
+    if (only_four && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS) {
         const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS * 2 / 3 : FEW_SLOTS) / a.n_kv);
         const int64_t most = std::min<int64_t>({(keys + FEW_UNIT - 1) / FEW_UNIT, most_parts, JOIN_SPLITS, slots});
         if (most > 1) a.few_slots = (int)slots, a.few_splits = (int)most;
