@@ -850,7 +850,7 @@ __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, fl
 // latency is what it costs.  COHERENT: the partials come from the same launch.
 // Behind those read ahead, JOIN_BATCH splits a trip to memory: one row over 4000 and 16000 4-bit keys (32 and 96 splits)
 // took 20.4 and 34.2 us with four, 15.2 and 22.8 with 8, 14.9 and 22.3 with 12, more with 16, whose
-// registers the launch did not have.
+// registers the launch did not have.  join_kernel takes four: its waves are many (841 rows over up to 3000 f16 keys 10.9 us, 12.8 by 12).
 constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4, JOIN_BATCH = 12;  // splits a lane, at most; splits whose outputs are read ahead
 constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
 constexpr int JOIN_FLOATS = FEW_PAIRS * (JOIN_SPLITS + 1);  // of LDS
@@ -924,7 +924,7 @@ __device__ __forceinline__ void join(const BatchArgs& a, const Seq& s, int kvh, 
                 if (z0 + t < splits) y += w[z0 + t] * unit * x[t];
             z0 += N;
         };
-        while (splits - z0 > JOIN_AHEAD) batch(std::integral_constant<int, JOIN_BATCH>());
+        while (splits - z0 > JOIN_AHEAD) batch(std::integral_constant<int, COHERENT ? JOIN_BATCH : JOIN_AHEAD>());
         if (z0 < splits) batch(std::integral_constant<int, JOIN_AHEAD>());
         if (some_not_finite(y)) y = sum_not_finite(y, splits, partial);
         *reinterpret_cast<f4*>(out_at(a, s, kvh, p0 + pr) + (i - pr * quads) * 4) = y;
