@@ -101,7 +101,9 @@ __device__ __forceinline__ void put(const PoolView& p, void* base, int64_t page,
 // flight meanwhile bounds the rate, with the norm's 64-bit sums behind it.  4096 rows of 32 + 2 * 8
 // heads of 128 take 45 us one at a time, 40 by two (4.6 TB/s, a large copy reaches
 // 5.1), 42 by four and 48 by eight, whose registers leave fewer waves.
-// Few rows take one each, so that they spread over the CUs.
+// Few rows take one each, so that they spread over the CUs.  The first rows' loads stand before the loop and the next
+// ones' behind those of cos and sin: with all of a turn's in the turn the same took 49 us from cold caches, so 44, and
+// with 1536 .. 4096 workgroups that take several turns 46 to 56.
 template <typename KV, int G, int ROWS>
 __global__ __launch_bounds__(STORE_NT) void store_norm_kernel(StoreNormArgs a) {
 #pragma clang fp contract(off)
@@ -118,24 +120,34 @@ __global__ __launch_bounds__(STORE_NT) void store_norm_kernel(StoreNormArgs a) {
     const f4 g = gamma && live ? *reinterpret_cast<const f4*>(gamma + dim) : zero;
     const int64_t capacity = (int64_t)a.pool.n_pages << a.pool.shift;
     const bool turns = a.cos_t && !is_v;
-    for (int64_t r0 = (int64_t)blockIdx.y * ROWS; r0 < a.m; r0 += (int64_t)gridDim.y * ROWS) {
-        f4 x[ROWS], c[ROWS], s[ROWS];
-        int32_t slot[ROWS], pos[ROWS];
+    f4 x[ROWS], c[ROWS], s[ROWS], x_next[ROWS];
+    int32_t slot[ROWS], pos[ROWS], slot_next[ROWS], pos_next[ROWS];
+    auto fetch = [&](int64_t r0) {
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             const int64_t r = min(r0 + i, a.m - 1);
-            slot[i] = a.slots[r];
-            pos[i] = a.cos_t ? a.positions[r] : 0;
-            x[i] = live ? *reinterpret_cast<const f4*>(src + r * stride + dim) : zero;
+            slot_next[i] = a.slots[r];
+            pos_next[i] = a.cos_t ? a.positions[r] : 0;
+            x_next[i] = live ? *reinterpret_cast<const f4*>(src + r * stride + dim) : zero;
         }
+    };
+    const int64_t step = (int64_t)gridDim.y * ROWS;
+    fetch((int64_t)blockIdx.y * ROWS);
+    for (int64_t r0 = (int64_t)blockIdx.y * ROWS; r0 < a.m; r0 += step) {
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) x[i] = x_next[i], slot[i] = slot_next[i], pos[i] = pos_next[i];
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
-            if (r0 + i >= a.m || slot[i] < 0 || slot[i] >= capacity || (a.cos_t && (pos[i] < 0 || pos[i] >= a.n_positions))) slot[i] = -1;
+            // (no short circuits: from branches around the assignment the compiler lost that of an even row)
+            const bool in = (r0 + i < a.m) & (slot[i] >= 0) & (slot[i] < capacity) &
+                            (!a.cos_t | ((pos[i] >= 0) & (pos[i] < a.n_positions)));
+            slot[i] = in ? slot[i] : -1;
             const int64_t at = (int64_t)(slot[i] < 0 ? 0 : pos[i]) * (hd >> 1) + (l < quarter ? dim : dim - (hd >> 1));
             const bool load = turns && live && slot[i] >= 0;
             c[i] = load ? *reinterpret_cast<const f4*>(a.cos_t + at) : zero;
             s[i] = load ? *reinterpret_cast<const f4*>(a.sin_t + at) : zero;
         }
+        if (r0 + step < a.m) fetch(r0 + step);
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             if (slot[i] < 0) continue;  // (the same in all lanes)

@@ -132,6 +132,39 @@ def test_store_norm(rq, gpu, hd, kv, layout, rope, in_place, norms):
         assert torch.equal(mem.view(torch.uint8), was.view(torch.uint8))
 
 
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+def test_more_rows_than_a_launch_has_workgroups(rq, gpu, kv):
+    """Each workgroup then takes rows several times: one call, in place too, is bit for bit the calls of 499 and of 50000
+    rows (which take one turn each)."""
+    torch.manual_seed(4)
+    rows, heads, hd, page, npos = 140001, 1, 32, 1024, 300
+    q, k, v = torch.randn(3, rows, hd, device="cuda")
+    g = 1 + 0.5 * torch.randn(hd, device="cuda")
+    pos = torch.randint(-2, npos + 2, (rows,), device="cuda").int()
+    slots = torch.randperm(140 * page, device="cuda")[:rows].int()
+    slots[::1000] = -1
+    ang = torch.rand(npos, hd // 2, device="cuda") * 6
+    cos, sin = ang.cos(), ang.sin()
+
+    def call(x, out, pool, r0, r1):
+        A.store_norm_dev(pool.c, r1 - r0, x[r0:].data_ptr(), hd, out[r0:].data_ptr(), hd, heads, k[r0:].data_ptr(), hd,
+                         v[r0:].data_ptr(), hd, g.data_ptr(), g.data_ptr(), 1e-6, pos[r0:].data_ptr(), slots[r0:].data_ptr(),
+                         cos.data_ptr(), sin.data_ptr(), npos, stream())
+
+    got = []
+    for cuts in ([0, rows], [0, rows], [0, 499, 50499, 100499, rows]):
+        pool = Pool(140, page, 1, hd, kv, fill=7.0)
+        x = q.clone()
+        out = x if len(got) == 1 else torch.full_like(q, 5.0)
+        for r0, r1 in zip(cuts, cuts[1:]):
+            call(x, out, pool, r0, r1)
+        ok = (slots >= 0) & (pos >= 0) & (pos < npos)
+        assert torch.equal(out[~ok], q[~ok] if len(got) == 1 else torch.full_like(q[~ok], 5.0))
+        got.append([out[ok]] + [t.clone() for t in pool.mem])
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
 def test_norm_against_the_formula(rq, gpu):
     """Against 64 bits: r is off by half a step, two products and a rotation (two products and a sum) round once each."""
     torch.manual_seed(3)
