@@ -526,7 +526,8 @@ __device__ __forceinline__ h4 read_t(const void* p) {
 
 // One wave's slab of SK 4-bit keys: code pieces of 32 values (16 where a slab
 // has fewer than 64 pieces) and their scales into registers, issued a step ahead, then the
-// values as f16 into LDS, laid out as an f16 cache's.
+// values as f16 into LDS, laid out as an f16 cache's.  2048 rows over 16048 keys take 887 us and more, an f16
+// cache's 855: the matrix cores bound both, and every tile dequantises its keys again (213 M VALU instructions, 165 M).
 template <int HD, int SK>
 struct Slab<Q4, HD, SK> {
     using G = Geo<Q4, HD>;
@@ -2045,7 +2046,9 @@ constexpr int TILE = 1, FEW = 2;
 // Waves of a SIMD at least, which bounds the registers.  Few rows over 4-bit keys
 // need little LDS: 48 rows over up to 8192 keys took 71 us with three waves (168 registers, none of
 // the loop's in memory), 76 with two and 98 with four, with registers in memory; heads
-// of 256 (half as many of them) 71 with two and 83 with one.
+// of 256 (half as many of them) 71 with two and 83 with one.  (With the small parts in idle columns and scales a lane
+// of a quad the 48 rows have come to 57 .. 62 us, 3.5 TB/s or more: half of the cycles are VALU issue, the rest the
+// first keys' three trips to memory and the join.)
 template <typename KV, int HD, int KIND>
 constexpr int waves_per_simd() {
     if (std::is_same<KV, Q4>::value && KIND == FEW) return HD == 256 ? 2 : 3;
