@@ -211,7 +211,7 @@ __device__ __forceinline__ void store_unit(const Unit<S, __is_same(S, D)>& u, vo
             mag = max4_u32(mag);
             top = max4_f32(top);
             const uint32_t scale = q4_scale(mag, __builtin_bit_cast(uint32_t, top) == mag);
-            const float d = h2f(scale), by = d == 0.0f ? __builtin_inff() : d, inv = __builtin_amdgcn_rcpf(by);
+            const float by = q4_divisor(scale), inv = __builtin_amdgcn_rcpf(by);
             uint32_t w = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) w |= q4_code<__is_same(S, _Float16)>(v[i], by, inv) << ((i >> 1) * 4 + (i & 1) * 16);

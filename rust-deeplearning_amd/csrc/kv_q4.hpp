@@ -53,7 +53,13 @@ __device__ __forceinline__ uint32_t q4_scale(uint32_t mag, bool positive) {
     const _Float16 h = (_Float16)fminf(as_f32((int32_t)b), Q4_MOST);
     return (uint32_t)__builtin_bit_cast(uint16_t, h) | (positive ? 0x8000u : 0u);
 }
-// The code of x under scale d (as f32; inv: 1 / d or so): x / d to the nearest
+// What a block's values are divided by: its scale as f32, or 1 where that is 0 (its values, below 2^-21 all of
+// them, then have code 8; 1 / 0 would make NaN of their quotients).
+__device__ __forceinline__ float q4_divisor(uint32_t scale) {
+    const float d = h2f(scale);
+    return d == 0.0f ? 1.0f : d;
+}
+// The code of x under divisor d (inv: 1 / d or so): x / d to the nearest
 // whole number, halves to even, which the rounded quotient alone would miss
 // beside a half: the remainder of the nearest code, exact in f32, decides.
 // HALF: x is an f16 number, 2^-14 of itself or more away from the halves that it is not: the quotient rounded
