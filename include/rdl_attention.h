@@ -47,7 +47,7 @@ extern "C" {
  * d and codes 0 .. 15, value = d (code - 8).  d has the size of the block's largest
  * magnitude over 8, rounded to 8 significant bits, as f16, at most 8160, and the sign
  * that takes that value to code 0 (of a positive and a negative one as large, the
- * positive); a code is value / d rounded to nearest, halves to even,
+ * positive; zeros are positive); a code is value / d rounded to nearest, halves to even,
  * between -8 and 7, plus 8; where d rounds to 0 (magnitudes up to 2^-22) the codes are 8.  A
  * block that holds a value that is not finite reads as NaN (d is NaN, its codes unspecified).  With such a
  * scale every value is an f16 number; with one of more bits it is rounded to f16.

@@ -210,7 +210,7 @@ __device__ __forceinline__ void store_unit(const Unit<S, __is_same(S, D)>& u, vo
             for (int i = 0; i < 8; i++) mag = max(mag, abs_bits(v[i])), top = fmaxf(top, v[i]);
             mag = max4_u32(mag);
             top = max4_f32(top);
-            const uint32_t scale = q4_scale(mag, __builtin_bit_cast(uint32_t, top) == mag);
+            const uint32_t scale = q4_scale(mag, top == as_f32((int32_t)mag));
             const float by = q4_divisor(scale), inv = __builtin_amdgcn_rcpf(by);
             uint32_t w = 0;
 #pragma unroll

@@ -45,7 +45,7 @@ struct Q4Decoder {
 };
 
 // The scale of a block: mag, the bits of its largest magnitude, and whether a
-// positive value has it.  f16 bits.
+// positive value, or a zero of either sign, has it.  f16 bits.
 __device__ __forceinline__ uint32_t q4_scale(uint32_t mag, bool positive) {
     if (mag >= 0x7F800000u) return Q4_NAN;
     const uint32_t u = __builtin_bit_cast(uint32_t, as_f32((int32_t)mag) * 0.125f);

@@ -74,7 +74,7 @@ __device__ __forceinline__ void put(const PoolView& p, void* base, int64_t page,
         for (int i = 0; i < 4; i++) mag = max(mag, abs_bits(y[i])), top = fmaxf(top, y[i]);
         mag = max8_u32(mag);
         top = max8_f32(top);
-        const uint32_t scale = q4_scale(mag, __builtin_bit_cast(uint32_t, top) == mag);
+        const uint32_t scale = q4_scale(mag, top == as_f32((int32_t)mag));
         const float by = q4_divisor(scale), inv = __builtin_amdgcn_rcpf(by);
         uint32_t w = 0;
 #pragma unroll

@@ -53,3 +53,13 @@ def test_codes_of_blocks_whose_scale_is_zero(rq, gpu, via):
         assert torch.equal(runs.codes.cpu(), q4.pack(q4.quantize(y)[1]))
         assert (q4.unpack(runs.codes.cpu())[0, 0, :7] == 8).all()
     assert (dst.both()[:, 0, 0, :7] == 0).all()
+
+
+@WAYS
+def test_scales_of_zeros(rq, gpu, via):
+    """Zeros of either sign, in any order, are the same bytes: a zero counts as positive."""
+    x = small_rows(16, 64)
+    dst = put(via, x)
+    for runs, y in ((dst.k, x), (dst.v, -x)):
+        assert torch.equal(runs.scales.cpu().view(torch.int16), q4.quantize(y)[0].view(torch.int16))
+        assert (runs.scales.cpu().view(torch.int16)[0, 0, :3] == -0x8000).all()
