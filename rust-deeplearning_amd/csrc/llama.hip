@@ -707,6 +707,7 @@ struct LlamaModel {
         std::vector<int> len, free_host;
         std::vector<int> holders;    // of each page: the sequences whose tables name it
         std::vector<int> row_host;  // room for a table row
+        std::vector<int> last_host;  // of a step, until the stream has been waited for: what last_rows gets
         rdl_status status = RDL_OK;  // of the step's cache operators, whose message stands
     } batch;
 
@@ -1687,6 +1688,7 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
         B.free_host.resize((size_t)M.n_pages);
         B.holders.assign((size_t)M.n_pages, 0);
         B.row_host.resize((size_t)M.n_pages);
+        B.last_host.reserve(std::min(n_seq, (size_t)c.max_batch));
     } catch (const std::exception&) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
     }
@@ -1746,8 +1748,31 @@ rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq) {
     return api_ok();
 }
 
+// The uploads and launches of a checked step (batch_step).
+static rdl_status batch_launch(rdl::LlamaModel& M, const int32_t* counts, size_t n_seq, const int32_t* tokens, size_t n) {
+    rdl::LlamaModel::Batch& B = M.batch;
+    auto up = [&](int* dst, const int* src, size_t k) {
+        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
+    };
+    HIP_TRY(up(M.tokens, tokens, n));
+    HIP_TRY(up(B.cached, B.len.data(), n_seq));
+    HIP_TRY(up(B.count, counts, n_seq));
+    HIP_TRY(up(B.free_pages, B.free_host.data(), B.free_host.size()));
+    HIP_TRY(up(B.last_rows, B.last_host.data(), B.last_host.size()));
+    B.status = RDL_OK;
+    const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.free_host.size(), rdl::KV_PAGE, B.table,
+                                          (size_t)M.n_pages, B.row_start, B.kv_len, n, B.row_seq, B.positions, B.slots,
+                                          B.summary, M.stream);
+    if (st != RDL_OK) return st;
+    const hipError_t run = M.forward_batch(n, B.last_host.size());
+    if (B.status != RDL_OK) return B.status;
+    HIP_TRY(run);
+    return RDL_OK;
+}
+
 // A step of several sequences up to the logits of the *n_last sequences with tokens, in B.logits;
-// *pages: taken from the free list.  Nothing of the host's state moves before batch_done.
+// *pages: taken from the free list.  Nothing of the host's state moves before batch_done.  The uploads may still
+// be reading the caller's memory; where the step fails nothing of it is in use any more.
 static rdl_status batch_step(rdl::LlamaModel& M, const int32_t* counts, size_t n_seq, const int32_t* tokens, size_t n,
                              size_t* n_last, size_t* pages_taken) {
     const rdl_llama_config& c = M.cfg;
@@ -1774,33 +1799,15 @@ static rdl_status batch_step(rdl::LlamaModel& M, const int32_t* counts, size_t n
     for (size_t i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= c.vocab)
             return api_fail(RDL_ERR_INVALID_DATA, "token %d out of bounds for embedding with %d entries", tokens[i], c.vocab);
-    std::vector<int> last;
-    try {
-        for (size_t b = 0, r = 0; b < n_seq; b++)
-            if (r += (size_t)counts[b]; counts[b]) last.push_back((int)r - 1);
-    } catch (const std::exception&) {
-        return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
+    B.last_host.clear();  // (at most n_seq and n entries: room since the sequences began)
+    for (size_t b = 0, r = 0; b < n_seq; b++)
+        if (r += (size_t)counts[b]; counts[b]) B.last_host.push_back((int)r - 1);
+    const rdl_status st = batch_launch(M, counts, n_seq, tokens, n);
+    if (st != RDL_OK) {
+        (void)hipStreamSynchronize(M.stream);
+        return st;
     }
-    auto up = [&](int* dst, const int* src, size_t k) {
-        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
-    };
-    HIP_TRY(up(M.tokens, tokens, n));
-    HIP_TRY(up(B.cached, B.len.data(), n_seq));
-    HIP_TRY(up(B.count, counts, n_seq));
-    HIP_TRY(up(B.free_pages, B.free_host.data(), B.free_host.size()));
-    HIP_TRY(up(B.last_rows, last.data(), last.size()));
-    B.status = RDL_OK;
-    const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.free_host.size(), rdl::KV_PAGE, B.table,
-                                          (size_t)M.n_pages, B.row_start, B.kv_len, n, B.row_seq, B.positions, B.slots,
-                                          B.summary, M.stream);
-    if (st != RDL_OK) return st;
-    const hipError_t run = M.forward_batch(n, last.size());
-    if (B.status != RDL_OK) {
-        (void)hipStreamSynchronize(M.stream);  // nothing of the step is in use any more
-        return B.status;
-    }
-    HIP_TRY(run);
-    *n_last = last.size();
+    *n_last = B.last_host.size();
     *pages_taken = pages;
     return RDL_OK;
 }
@@ -1823,11 +1830,14 @@ rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size
     size_t n_last = 0, pages = 0;
     const rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last, &pages);
     if (st != RDL_OK) return st;
-    for (size_t b = 0, i = 0; b < n_seq; b++)
+    hipError_t e = hipSuccess;
+    for (size_t b = 0, i = 0; b < n_seq && e == hipSuccess; b++)
         if (counts[b])
-            HIP_TRY(hipMemcpyAsync(logits + b * c.vocab, B.logits + i++ * c.vocab, (size_t)c.vocab * 4,
-                                   hipMemcpyDeviceToHost, M.stream));
-    HIP_TRY(hipStreamSynchronize(M.stream));
+            e = hipMemcpyAsync(logits + b * c.vocab, B.logits + i++ * c.vocab, (size_t)c.vocab * 4, hipMemcpyDeviceToHost,
+                               M.stream);
+    const hipError_t done = hipStreamSynchronize(M.stream);  // before the caller's memory goes, also after an error
+    HIP_TRY(e);
+    HIP_TRY(done);
     batch_done(M, counts, pages);
     return api_ok();
 }
