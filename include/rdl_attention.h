@@ -148,7 +148,7 @@ rdl_status rdl_kv_store_norm_dev(const rdl_kv_pool* pool, size_t m, const float*
 
 /* What rdl_kv_fork_dev found wrong (summary[1], 0: nothing). */
 enum {
-    RDL_FORK_BAD_SEQUENCE = 1, /* a parent or child that is no sequence, or one that is both: the pair is left out */
+    RDL_FORK_BAD_SEQUENCE = 1, /* a parent or child that is no sequence, or a parent that is its own child: the pair is left out */
     RDL_FORK_BAD_LENGTH = 2,   /* a parent's length that is negative (taken as 0) or past its table row (cut) */
     RDL_FORK_NO_PAGES = 4      /* the free list is shorter than the pages needed */
 };
@@ -163,7 +163,10 @@ enum {
  *                 the parent's length) and lengths are written;
  *   summary [2]:  pages taken from the free list, RDL_FORK_* flags.
  * Several children of one parent are its copies with a page of their own
- * each.  A child may not be another pair's parent or child (its row is then unspecified).
+ * each.  All pairs go by the parents' lengths from before the call.  A child may not be another
+ * pair's parent or child: the row of a sequence that two pairs name so, and what is copied from it
+ * (the row, length and src_pages entry of its own children), are unspecified; other pairs, all of
+ * dst_pages and the summary are what those lengths make them.
  * Full pages are shared: the caller frees a page when no sequence names it.
  * page_positions: a power of two, 16 .. 1024.  Outputs must not overlap. */
 rdl_status rdl_kv_fork_dev(int32_t* tables_dev, size_t table_stride, int32_t* kv_len_dev, size_t n_seq,

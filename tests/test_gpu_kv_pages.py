@@ -1,10 +1,12 @@
 """GPU tests of page copies and forks at their edges (include/rdl_attention.h)."""
+import random
+
 import pytest
 import torch
 
 import kv_q4_ref as q4
 from rdlquant import attention as A
-from test_gpu_kv_q4 import Pool, ints, stream
+from test_gpu_kv_q4 import Pool, ints, plain_fork, run_fork, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +65,84 @@ def test_scales_of_zeros(rq, gpu, via):
     for runs, y in ((dst.k, x), (dst.v, -x)):
         assert torch.equal(runs.scales.cpu().view(torch.int16), q4.quantize(y)[0].view(torch.int16))
         assert (runs.scales.cpu().view(torch.int16)[0, 0, :3] == -0x8000).all()
+
+
+# ---- forks ----------------------------------------------------------------------------------------------
+
+
+def chained(n, page, seed):
+    """n pairs of which every fourth child is the parent of later and of earlier pairs."""
+    r = random.Random(seed)
+    width, roots = 9, 1 + n // 5
+    lens = [r.randrange(width * page + 1) for _ in range(roots + n)]
+    tables = [[r.randrange(10000) for _ in range(width)] for _ in lens]
+    children = list(range(roots, roots + n))
+    r.shuffle(children)
+    parents = [children[r.randrange(n)] if i % 4 == 3 else r.randrange(roots) for i in range(n)]
+    parents = [p if p != c else 0 for p, c in zip(parents, children)]
+    return tables, lens, page, parents, children, r.sample(range(20000, 60000), n + 7)
+
+
+@pytest.mark.parametrize("n,page", [(4, 16), (150, 16), (700, 64), (2600, 32)])
+def test_children_that_are_parents_spoil_their_own_copies_alone(rq, gpu, n, page):
+    args = chained(n, page, n)
+    parents, children = args[3:5]
+    want, got = plain_fork(*args), run_fork(*args)
+    assert got[3] == want[3] and got[4] == want[4]  # pages and summary
+    own = {c for p, c in zip(parents, children) if p in set(children)}
+    for s in range(len(args[1])):
+        if s not in own:
+            assert got[0][s] == want[0][s] and got[1][s] == want[1][s]
+    assert all(g == w for g, w, c in zip(got[2], want[2], children) if c not in own)
+
+
+def test_forks_on_streams_and_in_graphs(rq, gpu):
+    r = random.Random(3)
+    n, page, width = 60, 16, 7
+    lens = [r.randrange(width * page + 1) for _ in range(20)] + [0] * n
+    tables = [[r.randrange(10000) for _ in range(width)] for _ in lens]
+    parents, children, free = [r.randrange(20) for _ in range(n)], list(range(20, 20 + n)), r.sample(range(20000, 60000), n)
+    want = plain_fork(tables, lens, page, parents, children, free)
+    f, c, fr = ints(parents), ints(children), ints(free)
+
+    class Side:
+        def __init__(self):
+            self.stream = torch.cuda.Stream()
+            self.t, self.k = ints(tables), ints(lens)
+            self.out = [torch.zeros(s, dtype=torch.int32, device="cuda") for s in (n, n, 2)]
+
+        def call(self):
+            A.fork_dev(self.t.data_ptr(), width, self.k.data_ptr(), len(lens), page, f.data_ptr(), c.data_ptr(), n, fr.data_ptr(), n,
+                       *(o.data_ptr() for o in self.out), self.stream.cuda_stream)
+
+        def restore(self):
+            self.t.copy_(ints(tables)), self.k.copy_(ints(lens))
+            for o in self.out:
+                o.fill_(-5)
+
+        def check(self):
+            assert (self.t.tolist(), self.k.tolist(), *(o.tolist() for o in self.out)) == want
+
+    sides = [Side(), Side()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s in sides:
+            s.call()
+    torch.cuda.synchronize()
+    for s in sides:
+        s.check()
+    graphs = []
+    for s in sides:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s.stream), torch.cuda.graph(g, stream=s.stream):
+            s.call()
+        graphs.append(g)
+    for _ in range(4):
+        for s in sides:
+            s.restore()
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for s in sides:
+            s.check()
