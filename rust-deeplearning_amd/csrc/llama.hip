@@ -36,6 +36,7 @@
 #include "../../include/rdl_llama.h"
 #include "attention.hpp"
 #include "kv_q4.hpp"
+#include "page_book.hpp"
 #include "rdl_device.hpp"
 #include "rdl_internal.hpp"
 
@@ -704,9 +705,7 @@ struct LlamaModel {
         float *x = nullptr, *logits = nullptr;  // [last][dim], [last][vocab]: a step's last rows, at most min(cap, max_batch)
         void* mem = nullptr;                    // all of it, one allocation
         size_t max_rows = 0, max_kv = 0;        // of the step
-        std::vector<int> len, free_host;
-        std::vector<int> holders;    // of each page: the sequences whose tables name it
-        std::vector<int> row_host;  // room for a table row
+        PageBook book;
         std::vector<int> last_host;  // of a step, until the stream has been waited for: what last_rows gets
         rdl_status status = RDL_OK;  // of the step's cache operators, whose message stands
     } batch;
@@ -1684,15 +1683,11 @@ rdl_status rdl_llama_batch_begin(rdl_llama* model, size_t n_seq) {
     if (M.host_pos != 0 || B.on)
         return api_fail(RDL_ERR_INVALID_DATA, "sequences can begin only on an empty cache (rdl_llama_reset first)");
     try {
-        B.len.assign(n_seq, 0);
-        B.free_host.resize((size_t)M.n_pages);
-        B.holders.assign((size_t)M.n_pages, 0);
-        B.row_host.resize((size_t)M.n_pages);
+        B.book.begin(n_seq, (size_t)M.n_pages, rdl::KV_PAGE);
         B.last_host.reserve(std::min(n_seq, (size_t)c.max_batch));
     } catch (const std::exception&) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
     }
-    for (int p = 0; p < M.n_pages; p++) B.free_host[p] = p;
     if (n_seq > B.cap) {
         const size_t mb = c.max_batch, pg = M.n_pages, last = std::min(n_seq, mb);
         const std::pair<int**, size_t> ints[] = {
@@ -1729,7 +1724,7 @@ rdl_status rdl_llama_batch_positions(const rdl_llama* model, size_t* out, size_t
     const rdl::LlamaModel::Batch& B = model->m.batch;
     if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
     if (n != B.n_seq) return rdl::api_shape_fail("sequences", {B.n_seq}, {n});
-    for (size_t b = 0; b < n; b++) out[b] = (size_t)B.len[b];
+    for (size_t b = 0; b < n; b++) out[b] = (size_t)B.book.len[b];
     return api_ok();
 }
 
@@ -1739,12 +1734,7 @@ rdl_status rdl_llama_batch_drop(rdl_llama* model, size_t seq) {
     rdl::LlamaModel::Batch& B = M.batch;
     if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
     if (seq >= B.n_seq) return api_fail(RDL_ERR_INVALID_DATA, "sequence %zu of %zu", seq, B.n_seq);
-    const size_t held = ((size_t)B.len[seq] + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
-    if (held)
-        HIP_TRY(hipMemcpy(B.row_host.data(), B.table + seq * M.n_pages, held * sizeof(int), hipMemcpyDeviceToHost));
-    for (size_t i = 0; i < held; i++)
-        if (--B.holders[B.row_host[i]] == 0) B.free_host.push_back(B.row_host[i]);  // within the capacity it began with
-    B.len[seq] = 0;
+    B.book.drop(seq);
     return api_ok();
 }
 
@@ -1755,12 +1745,12 @@ static rdl_status batch_launch(rdl::LlamaModel& M, const int32_t* counts, size_t
         return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
     };
     HIP_TRY(up(M.tokens, tokens, n));
-    HIP_TRY(up(B.cached, B.len.data(), n_seq));
+    HIP_TRY(up(B.cached, B.book.len.data(), n_seq));
     HIP_TRY(up(B.count, counts, n_seq));
-    HIP_TRY(up(B.free_pages, B.free_host.data(), B.free_host.size()));
+    HIP_TRY(up(B.free_pages, B.book.free.data(), B.book.free.size()));
     HIP_TRY(up(B.last_rows, B.last_host.data(), B.last_host.size()));
     B.status = RDL_OK;
-    const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.free_host.size(), rdl::KV_PAGE, B.table,
+    const rdl_status st = rdl_kv_plan_dev(B.cached, B.count, n_seq, B.free_pages, B.book.free.size(), rdl::KV_PAGE, B.table,
                                           (size_t)M.n_pages, B.row_start, B.kv_len, n, B.row_seq, B.positions, B.slots,
                                           B.summary, M.stream);
     if (st != RDL_OK) return st;
@@ -1770,32 +1760,32 @@ static rdl_status batch_launch(rdl::LlamaModel& M, const int32_t* counts, size_t
     return RDL_OK;
 }
 
-// A step of several sequences up to the logits of the *n_last sequences with tokens, in B.logits;
-// *pages: taken from the free list.  Nothing of the host's state moves before batch_done.  The uploads may still
-// be reading the caller's memory; where the step fails nothing of it is in use any more.
+// A step of several sequences up to the logits of the *n_last sequences with tokens, in B.logits,
+// for the page book to follow once the stream has been waited for.  The uploads may still be reading the caller's
+// memory; where the step fails nothing of it is in use any more.
 static rdl_status batch_step(rdl::LlamaModel& M, const int32_t* counts, size_t n_seq, const int32_t* tokens, size_t n,
-                             size_t* n_last, size_t* pages_taken) {
+                             size_t* n_last) {
     const rdl_llama_config& c = M.cfg;
     rdl::LlamaModel::Batch& B = M.batch;
     if (!B.on) return api_fail(RDL_ERR_INVALID_DATA, "no sequences (rdl_llama_batch_begin first)");
     if (n_seq != B.n_seq) return rdl::api_shape_fail("sequences", {B.n_seq}, {n_seq});
     if (n == 0 || n > (size_t)c.max_batch)
         return api_fail(RDL_ERR_SHAPE_MISMATCH, "%zu tokens: 1 .. max_batch (%d) per call", n, c.max_batch);
-    size_t rows = 0, pages = 0;
+    size_t rows = 0;
     B.max_rows = B.max_kv = 0;
     for (size_t b = 0; b < n_seq; b++) {
         if (counts[b] < 0) return api_fail(RDL_ERR_INVALID_DATA, "sequence %zu: %d tokens", b, counts[b]);
-        const size_t len = (size_t)B.len[b], t = len + (size_t)counts[b];
+        const size_t len = (size_t)B.book.len[b], t = len + (size_t)counts[b];
         if (t > (size_t)c.max_seq)
             return api_fail(RDL_ERR_INVALID_DATA, "sequence length %zu exceeds maximum %d (start_pos=%zu)", t, c.max_seq, len);
         rows += (size_t)counts[b];
-        pages += (t + rdl::KV_PAGE - 1) / rdl::KV_PAGE - (len + rdl::KV_PAGE - 1) / rdl::KV_PAGE;
         B.max_rows = std::max(B.max_rows, (size_t)counts[b]);
         if (counts[b]) B.max_kv = std::max(B.max_kv, t);
     }
     if (rows != n) return rdl::api_shape_fail("tokens", {rows}, {n});
-    if (pages > B.free_host.size())
-        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.free_host.size());
+    const size_t pages = B.book.step_pages(counts);
+    if (pages > B.book.free.size())
+        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.book.free.size());
     for (size_t i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= c.vocab)
             return api_fail(RDL_ERR_INVALID_DATA, "token %d out of bounds for embedding with %d entries", tokens[i], c.vocab);
@@ -1808,15 +1798,7 @@ static rdl_status batch_step(rdl::LlamaModel& M, const int32_t* counts, size_t n
         return st;
     }
     *n_last = B.last_host.size();
-    *pages_taken = pages;
     return RDL_OK;
-}
-// Behind it, once the stream has been waited for.
-static void batch_done(rdl::LlamaModel& M, const int32_t* counts, size_t pages) {
-    rdl::LlamaModel::Batch& B = M.batch;
-    for (size_t i = 0; i < pages; i++) B.holders[B.free_host[i]] = 1;
-    B.free_host.erase(B.free_host.begin(), B.free_host.begin() + (ptrdiff_t)pages);
-    for (size_t b = 0; b < B.n_seq; b++) B.len[b] += counts[b];
 }
 
 rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size_t n_seq, const int32_t* tokens,
@@ -1827,8 +1809,8 @@ rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size
     rdl::LlamaModel::Batch& B = M.batch;
     if (B.on && n_seq == B.n_seq && n > 0 && n <= (size_t)c.max_batch && logits_len < n_seq * (size_t)c.vocab)
         return rdl::api_shape_fail("logits length", {n_seq * (size_t)c.vocab}, {logits_len});
-    size_t n_last = 0, pages = 0;
-    const rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last, &pages);
+    size_t n_last = 0;
+    const rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last);
     if (st != RDL_OK) return st;
     hipError_t e = hipSuccess;
     for (size_t b = 0, i = 0; b < n_seq && e == hipSuccess; b++)
@@ -1838,7 +1820,7 @@ rdl_status rdl_llama_batch_forward(rdl_llama* model, const int32_t* counts, size
     const hipError_t done = hipStreamSynchronize(M.stream);  // before the caller's memory goes, also after an error
     HIP_TRY(e);
     HIP_TRY(done);
-    batch_done(M, counts, pages);
+    B.book.step(counts);
     return api_ok();
 }
 
@@ -1860,8 +1842,8 @@ rdl_status rdl_llama_batch_logprobs(rdl_llama* model, const int32_t* counts, siz
     } catch (const std::exception&) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu sequences", n_seq);
     }
-    size_t n_last = 0, pages = 0;
-    rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last, &pages);  // (checks n and n_seq)
+    size_t n_last = 0;
+    rdl_status st = batch_step(M, counts, n_seq, tokens, n, &n_last);  // (checks n and n_seq)
     if (st != RDL_OK) return st;
     for (size_t b = 0, i = 0; targets && b < n_seq; b++)
         if (counts[b]) given[i++] = targets[b];
@@ -1893,8 +1875,27 @@ rdl_status rdl_llama_batch_logprobs(rdl_llama* model, const int32_t* counts, siz
         for (size_t t = 0; t < n_top; t++) top_ids[b * n_top + t] = ids[i * n_top + t], top_logprobs[b * n_top + t] = tl[i * n_top + t];
         i++;
     }
-    batch_done(M, counts, pages);
+    B.book.step(counts);
     return api_ok();
+}
+
+// The uploads and launches of checked forks, which take `pages` pages; what they found, to `forked`.
+static rdl_status fork_launch(rdl::LlamaModel& M, const int32_t* parents, const int32_t* children, size_t n, size_t pages,
+                              const std::vector<rdl_kv_pool>& pools, int (&forked)[2]) {
+    rdl::LlamaModel::Batch& B = M.batch;
+    auto up = [&](int* dst, const int* src, size_t k) {
+        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
+    };
+    HIP_TRY(up(B.cached, B.book.len.data(), B.n_seq));
+    HIP_TRY(up(B.parents, parents, n));
+    HIP_TRY(up(B.children, children, n));
+    HIP_TRY(up(B.free_pages, B.book.free.data(), pages));
+    rdl_status st = rdl_kv_fork_dev(B.table, (size_t)M.n_pages, B.cached, B.n_seq, rdl::KV_PAGE, B.parents, B.children, n,
+                                    B.free_pages, pages, B.src, B.dst, B.forked, M.stream);
+    if (st == RDL_OK) st = rdl_kv_copy_pages_dev(pools.data(), pools.data(), pools.size(), B.src, B.dst, n, M.stream);
+    if (st != RDL_OK) return st;
+    HIP_TRY(hipMemcpyAsync(forked, B.forked, sizeof(forked), hipMemcpyDeviceToHost, M.stream));
+    return RDL_OK;
 }
 
 rdl_status rdl_llama_batch_fork(rdl_llama* model, const int32_t* parents, const int32_t* children, size_t n) {
@@ -1906,51 +1907,34 @@ rdl_status rdl_llama_batch_fork(rdl_llama* model, const int32_t* parents, const 
     if (n == 0) return api_ok();
     std::vector<char> used;
     std::vector<rdl_kv_pool> pools;
-    std::vector<int> table;
     try {
         used.assign(B.n_seq, 0);
         pools.resize((size_t)M.cfg.n_layers);
-        table.resize(B.n_seq * (size_t)M.n_pages);
     } catch (const std::exception&) {
         return api_fail(RDL_ERR_INVALID_DATA, "%zu forks", n);
     }
-    size_t pages = 0;
     for (size_t i = 0; i < n; i++) {
         const int p = parents[i], ch = children[i];
         if (p < 0 || (size_t)p >= B.n_seq || ch < 0 || (size_t)ch >= B.n_seq)
             return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d from %d of %zu", i, ch, p, B.n_seq);
-        if (B.len[ch] != 0) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d is not empty", i, ch);
+        if (B.book.len[ch] != 0) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d is not empty", i, ch);
         if (used[ch]) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d again", i, ch);
         used[ch] = 1;
-        pages += B.len[p] % rdl::KV_PAGE != 0;
     }
     for (size_t i = 0; i < n; i++)
         if (used[parents[i]]) return api_fail(RDL_ERR_INVALID_DATA, "fork %zu: sequence %d is forked itself", i, parents[i]);
-    if (pages > B.free_host.size())
-        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.free_host.size());
+    const size_t pages = B.book.fork_pages(parents, n);
+    if (pages > B.book.free.size())
+        return api_fail(RDL_ERR_INVALID_DATA, "the cache is full: %zu pages needed, %zu free", pages, B.book.free.size());
     for (size_t l = 0; l < pools.size(); l++) pools[l] = M.batch_pool((int)l);
-    auto up = [&](int* dst, const int* src, size_t k) {
-        return k ? hipMemcpyAsync(dst, src, k * sizeof(int), hipMemcpyHostToDevice, M.stream) : hipSuccess;
-    };
-    HIP_TRY(up(B.cached, B.len.data(), B.n_seq));
-    HIP_TRY(up(B.parents, parents, n));
-    HIP_TRY(up(B.children, children, n));
-    HIP_TRY(up(B.free_pages, B.free_host.data(), pages));
-    rdl_status st = rdl_kv_fork_dev(B.table, (size_t)M.n_pages, B.cached, B.n_seq, rdl::KV_PAGE, B.parents, B.children, n,
-                                    B.free_pages, pages, B.src, B.dst, B.forked, M.stream);
-    if (st == RDL_OK) st = rdl_kv_copy_pages_dev(pools.data(), pools.data(), pools.size(), B.src, B.dst, n, M.stream);
-    if (st != RDL_OK) {
-        (void)hipStreamSynchronize(M.stream);
-        return st;
-    }
-    HIP_TRY(hipMemcpyAsync(table.data(), B.table, table.size() * sizeof(int), hipMemcpyDeviceToHost, M.stream));
-    HIP_TRY(hipStreamSynchronize(M.stream));
-    for (size_t i = 0; i < n; i++) {
-        B.len[children[i]] = B.len[parents[i]];
-        const int* row = table.data() + (size_t)children[i] * M.n_pages;
-        for (int p = 0; p < (B.len[children[i]] + rdl::KV_PAGE - 1) / rdl::KV_PAGE; p++) B.holders[row[p]]++;
-    }
-    B.free_host.erase(B.free_host.begin(), B.free_host.begin() + (ptrdiff_t)pages);
+    int forked[2] = {-1, -1};  // pages taken, flags
+    const rdl_status st = fork_launch(M, parents, children, n, pages, pools, forked);
+    const hipError_t done = hipStreamSynchronize(M.stream);  // before `forked` and the caller's memory go
+    if (st != RDL_OK) return st;
+    HIP_TRY(done);
+    if (forked[0] != (int)pages || forked[1] != 0)
+        return api_fail(RDL_ERR_HIP, "fork of %zu sequences: %d pages taken, flags %d, instead of %zu pages", n, forked[0], forked[1], pages);
+    B.book.fork(parents, children, n);
     return api_ok();
 }
 
