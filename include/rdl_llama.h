@@ -31,9 +31,9 @@
 extern "C" {
 #endif
 
-/* kv_f16 of a cache of 4 bits a value (RDL_KV_Q4, rdl_attention.h). */
+/* kv_f16 of a cache of 4 bits a value (RDL_KV_Q4, rdl_attention.h, the same number). */
 enum {
-    RDL_LLAMA_KV_Q4 = 2
+    RDL_LLAMA_KV_Q4 = 0x104
 };
 
 /* ModelConfig fields used by the Llama path (rustml/nlp/main/src/api/types.rs:186). */
@@ -49,7 +49,8 @@ typedef struct rdl_llama_config {
     float norm_eps;
     float rope_theta;
     int32_t kv_f16;      /* 1: f16 KV cache, 0: f32 (the reference's), RDL_LLAMA_KV_Q4:
-                            4 bits (head_dim % 32 == 0; rdl_llama_batch_* alone) */
+                            4 bits (head_dim % 32 == 0; rdl_llama_batch_* alone);
+                            any other value: f16 */
     int32_t max_batch;   /* most rows one forward call takes (prefill chunk) */
     int32_t output_dtype; /* GGML type of the output matrix: RDL_DTYPE_Q4_0 (also
                              when 0), _Q8_0, _Q4_1, _Q4_K or _Q6_K (K-quants:

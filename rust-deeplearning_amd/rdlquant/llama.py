@@ -18,7 +18,7 @@ from . import _decl, _i32, _p, _sz, check, lib
 
 TOKEN_EMBEDDING, ATTN_NORM, WQ, WK, WV, WO, FFN_NORM, W_GATE, W_UP, W_DOWN, FINAL_NORM, OUTPUT = range(12)
 SLOTS = 12
-KV_Q4 = 2  # RDL_LLAMA_KV_Q4: kv_f16 of a 4-bit cache (batch_* alone)
+KV_Q4 = 0x104  # RDL_LLAMA_KV_Q4: kv_f16 of a 4-bit cache (batch_* alone)
 
 
 class _Config(C.Structure):
