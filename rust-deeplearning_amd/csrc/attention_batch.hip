@@ -2254,15 +2254,21 @@ constexpr size_t PART_BYTES = (size_t)256 << 20;  // most memory of partial resu
 constexpr int64_t SPLIT_MIN_TILES = 4;
 constexpr size_t SPLIT_BYTES = (size_t)1 << 30;
 
-// The shortest span of a split of few rows over 4-bit keys.  A turn of 128 keys takes 1.2 us of a workgroup that waits
+// Few rows over 4-bit keys: short keys of many sequences are neither split nor dealt out (few_plan), which
+// spares the join.  pairs: sequences times KV heads.  Lengths from an eighth of the longest on, us, whole and split or
+// dealt out: 16, 24, 48, 64 sequences of 8 KV heads of 128 over up to 640 keys 12.2, 12.2, 16.7, 17.6 and 14.0, 15.9,
+// 21.1, 21.1, heads of 64 (32 and 64 sequences) 10.5, 13.3 and 15.4, 16.3, of 256 (16 and 48) 17.4, 25.7 and 19.4, 26.9; more
+// workgroups than run at once, 64 of 16 KV heads over up to 250 and 600 keys, 17.9, 29.3 and 23.5, 35.0, equal lengths 19.3,
+// 29.4 and 20.2, 30.5.  Up to 900 keys whole ones still took no longer in any of these, over 1300 from 2 us less (64
+// sequences) to 3 more, over 2000 up to 13 more.  Fewer than 128 pairs leave CUs idle: one row over 777 keys 14.9 whole, 10.8 split.
+constexpr int64_t FOUR_WHOLE_KEYS = 640, FOUR_WHOLE_PAIRS = 128;
+bool four_whole(int64_t pairs, int64_t keys) { return pairs >= FOUR_WHOLE_PAIRS && keys <= FOUR_WHOLE_KEYS; }
+// The shortest span of a split of them.  A turn of 128 keys takes 1.2 us of a workgroup that waits
 // for each, a split 0.2 us of the join: their sum is least near 4 sqrt(keys).  One row over 4000, 16000 and 60000
 // keys took 15.0, 22.4 and 37.3 us with spans of 128 keys (or dealt out in units of as many), 13.0, 18.4
-// and 32.6 with 256, 512 and 1024.  Short keys of many sequences are not split, which spares the join: 24
-// rows over up to 600 keys (192 workgroups) 13.0 us instead of 15.0, 48 over up to 250 12.0 instead
-// of 14.3; one row over 777 alone 14.9 instead of 10.8.
-constexpr int64_t FOUR_WHOLE_KEYS = 640, FOUR_WHOLE_PAIRS = 128;
+// and 32.6 with 256, 512 and 1024.
 int64_t few_min_span(int64_t pairs, int64_t keys) {
-    if (pairs >= FOUR_WHOLE_PAIRS && keys <= FOUR_WHOLE_KEYS) return FOUR_WHOLE_KEYS;
+    if (four_whole(pairs, keys)) return FOUR_WHOLE_KEYS;
     return std::max<int64_t>(FEW_MIN_SPAN, (int64_t)(4.0 * sqrt((double)keys)));
 }
 
@@ -2304,7 +2310,7 @@ rdl_status run(BatchArgs a, int32_t dtype, size_t max_rows, size_t max_kv, hipSt
                                                 std::max(2 * a.tile_splits, a.few_splits)});
     }
     // (fewer workgroups than run at once need no plan: one row over 778 keys took 14.0 us with it, 11.1 without)
-    if (only_four && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS) {
+    if (only_four && a.n_seq <= 64 && pairs * a.few_splits > FEW_SLOTS && !four_whole(pairs, keys)) {
         const int64_t slots = std::max<int64_t>(a.n_seq, (a.hd > 128 ? FEW_SLOTS * 2 / 3 : FEW_SLOTS) / a.n_kv);
         const int64_t most = std::min<int64_t>({(keys + FEW_UNIT - 1) / FEW_UNIT, most_parts, JOIN_SPLITS, slots});
         if (most > 1) a.few_slots = (int)slots, a.few_splits = (int)most;
