@@ -153,7 +153,7 @@ enum {
     RDL_FORK_NO_PAGES = 4      /* the free list is shorter than the pages needed */
 };
 
-/* Forks sequences over shared pages, in one launch: for each of n pairs (int32,
+/* Forks sequences over shared pages: for each of n pairs (int32,
  * device) the sequence children[i] becomes a copy of parents[i].  Its table
  * row names the parent's pages, except that a last page that is not full is the
  * child's own: the next page of the free list, and -1 where that is used up.  src_pages

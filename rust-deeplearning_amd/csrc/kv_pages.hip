@@ -18,9 +18,11 @@ namespace {
 // ---- fork -----------------------------------------------------------------------------
 // A workgroup a pair.  The pair's place in the free list is the number of
 // pairs before it that need a page, which each workgroup counts for itself (a
-// length and two numbers a pair, in every L2) instead of a second launch.  They all count by the lengths
-// from before the call: the last workgroup to arrive writes the children's, so that a child which is
-// another pair's parent spoils nothing but its own copies.  Latency: 3.4 us for one pair, 4.1 for 32.
+// length and two numbers a pair, in every L2).  They all count by the lengths from before the
+// call: a second launch writes the children's (one pair's workgroup its own), so that a child which is
+// another pair's parent spoils nothing but its own copies.  Written by the last workgroup to arrive they
+// cost as much, and 4 us more of a captured call, whose counter is the graph's to allocate and clear.
+// Latency: 3.4 us for one pair, 4.1 for 32.
 constexpr int FORK_NT = 256, FORK_WG = 2048;
 
 struct ForkArgs {
@@ -33,7 +35,6 @@ struct ForkArgs {
     const int32_t* free_pages;
     int n_free;
     int32_t *src, *dst, *summary;
-    int* arrived;  // zero between launches (NULL: one workgroup)
 };
 struct ForkPair {
     int parent, child, pages, flags;  // pages: full ones
@@ -68,7 +69,7 @@ __device__ __forceinline__ int block_sum(int v, int* red) {
 }
 
 __global__ __launch_bounds__(FORK_NT) void fork_kernel(ForkArgs a) {
-    __shared__ int red[FORK_NT / 64], last_one;
+    __shared__ int red[FORK_NT / 64];
     const int tid = threadIdx.x;
     int before = 0, counted = 0;
     for (int i = (int)blockIdx.x; i < a.n; i += (int)gridDim.x) {
@@ -91,35 +92,28 @@ __global__ __launch_bounds__(FORK_NT) void fork_kernel(ForkArgs a) {
             a.dst[i] = fresh;
         }
     }
-    if (blockIdx.x == 0) {
-        int needed = 0, flags = 0;
-        for (int j = tid; j < a.n; j += FORK_NT) {
-            const ForkPair p = fork_pair(a, j);
-            needed += p.part;
-            flags |= p.flags;
-        }
-        needed = block_sum(needed, red);
-        const int bad = block_sum((flags & RDL_FORK_BAD_SEQUENCE) != 0, red), cut = block_sum((flags & RDL_FORK_BAD_LENGTH) != 0, red);
-        if (tid == 0) {
-            a.summary[0] = min(needed, a.n_free);
-            a.summary[1] = (bad ? RDL_FORK_BAD_SEQUENCE : 0) | (cut ? RDL_FORK_BAD_LENGTH : 0) |
-                           (needed > a.n_free ? RDL_FORK_NO_PAGES : 0);
-        }
-    }
-    // every length that this workgroup needs has been read
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (a.arrived) {
-        if (tid == 0) {
-            const int old = __hip_atomic_fetch_add(a.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last_one = old == (int)gridDim.x - 1;
-            if (last_one) __hip_atomic_store(a.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!last_one) return;
-    }
+    if (blockIdx.x != 0) return;
+    int needed = 0, flags = 0;
     for (int j = tid; j < a.n; j += FORK_NT) {
         const ForkPair p = fork_pair(a, j);
+        needed += p.part;
+        flags |= p.flags;
+    }
+    needed = block_sum(needed, red);
+    const int bad = block_sum((flags & RDL_FORK_BAD_SEQUENCE) != 0, red), cut = block_sum((flags & RDL_FORK_BAD_LENGTH) != 0, red);
+    if (tid == 0) {
+        a.summary[0] = min(needed, a.n_free);
+        a.summary[1] = (bad ? RDL_FORK_BAD_SEQUENCE : 0) | (cut ? RDL_FORK_BAD_LENGTH : 0) |
+                       (needed > a.n_free ? RDL_FORK_NO_PAGES : 0);
+    }
+    if (a.n != 1) return;
+    __syncthreads();  // every thread has read the length
+    const ForkPair p = fork_pair(a, 0);
+    if (tid == 0 && p.ok) a.kv_len[p.child] = p.length;
+}
+__global__ __launch_bounds__(FORK_NT) void fork_lengths_kernel(ForkArgs a) {
+    for (int i = (int)(blockIdx.x * FORK_NT + threadIdx.x); i < a.n; i += (int)(gridDim.x * FORK_NT)) {
+        const ForkPair p = fork_pair(a, i);
         if (p.ok) a.kv_len[p.child] = p.length;
     }
 }
@@ -350,17 +344,12 @@ rdl_status rdl_kv_fork_dev(int32_t* tables_dev, size_t table_stride, int32_t* kv
     a.dst = dst_pages_dev;
     a.summary = summary_dev;
     const unsigned wg = (unsigned)std::max<size_t>(1, std::min<size_t>(n, rdl::FORK_WG));
-    rdl::CallScratch work;
-    if (wg > 1) {
-        st = rdl::call_scratch((hipStream_t)stream, 0, 1, &work);
-        if (st != RDL_OK) return st;
-        a.arrived = work.counters;
-    }
     hipLaunchKernelGGL(rdl::fork_kernel, dim3(wg), dim3(rdl::FORK_NT), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    const rdl_status done = rdl::call_scratch_done((hipStream_t)stream, &work);
-    HIP_TRY(e);
-    return done == RDL_OK ? api_ok() : done;
+    if (n > 1)
+        hipLaunchKernelGGL(rdl::fork_lengths_kernel, dim3((unsigned)std::min<size_t>((n + rdl::FORK_NT - 1) / rdl::FORK_NT, rdl::FORK_WG)),
+                           dim3(rdl::FORK_NT), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError());
+    return api_ok();
 }
 
 rdl_status rdl_kv_copy_pages_dev(const rdl_kv_pool* src, const rdl_kv_pool* dst, size_t n_pools,
