@@ -16,13 +16,15 @@ namespace rdl {
 namespace {
 
 // ---- fork -----------------------------------------------------------------------------
-// A workgroup a pair.  The pair's place in the free list is the number of
-// pairs before it that need a page, which each workgroup counts for itself (a
-// length and two numbers a pair, in every L2).  They all count by the lengths from before the
-// call: a second launch writes the children's (one pair's workgroup its own), so that a child which is
-// another pair's parent spoils nothing but its own copies.  Written by the last workgroup to arrive they
-// cost as much, and 4 us more of a captured call, whose counter is the graph's to allocate and clear.
-// Latency: 3.4 us for one pair, 4.1 for 32.
+// A pair's place in the free list is the number of pairs before it that need a
+// page, counted by the parents' lengths from before the call: the children's are
+// written when all counts are done, so that a child which is another pair's parent
+// spoils nothing but its own copies.  Latency is what it costs: a call of 1, 32, 64 pairs of rows of 16 entries takes
+// 2.4, 2.6, 3.0 us as one workgroup, one of 65 or 300 5.2, 5.4 as a workgroup a pair with a launch behind (with
+// rows of 128 entries 2.5, 2.9, 3.6 and 5.2, 5.4).  One workgroup copies long rows alone: of 1024 entries 16, 32 and 64 pairs
+// take 4.2, 6.3 and 10.6 so, 5.5 the other way, so it has at most 16 rows' worth of those.
+constexpr int FORK_SMALL = 64, FORK_SMALL_WAVES = 16;
+constexpr size_t FORK_SMALL_ENTRIES = 16384;
 constexpr int FORK_NT = 256, FORK_WG = 2048;
 
 struct ForkArgs {
@@ -55,6 +57,46 @@ __device__ __forceinline__ ForkPair fork_pair(const ForkArgs& a, int i) {
     p.part = (p.length & ((1 << a.shift) - 1)) != 0;
     return p;
 }
+// Up to 64 pairs: one workgroup, whose waves have a pair a lane and copy the rows of every
+// 16th.
+__global__ __launch_bounds__(FORK_SMALL_WAVES * 64) void fork_small_kernel(ForkArgs a) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    ForkPair p{-1, -1, 0, 0, 0, false, false};
+    if (lane < a.n) p = fork_pair(a, lane);
+    const uint64_t wanted = __builtin_amdgcn_ballot_w64(p.part), ok = __builtin_amdgcn_ballot_w64(p.ok);
+    for (int i = w; i < a.n; i += FORK_SMALL_WAVES) {
+        if (!(ok >> i & 1)) continue;
+        const int pages = __builtin_amdgcn_readlane(p.pages, i);
+        const int32_t* from = a.tables + __builtin_amdgcn_readlane(p.parent, i) * a.table_stride;
+        int32_t* to = a.tables + __builtin_amdgcn_readlane(p.child, i) * a.table_stride;
+        for (int k = lane; k < pages; k += 64) to[k] = from[k];
+    }
+    if (w == 0) {
+        const int before = (int)__builtin_popcountll(wanted & (((uint64_t)1 << lane) - 1)), needed = (int)__builtin_popcountll(wanted);
+        int fresh = -1, last = -1;
+        if (p.part) {
+            fresh = before < a.n_free ? a.free_pages[before] : -1;
+            last = a.tables[p.parent * a.table_stride + p.pages];
+            a.tables[p.child * a.table_stride + p.pages] = fresh;
+        }
+        if (lane < a.n) {
+            a.src[lane] = fresh < 0 ? -1 : last;
+            a.dst[lane] = fresh;
+        }
+        const bool bad = __builtin_amdgcn_ballot_w64((p.flags & RDL_FORK_BAD_SEQUENCE) != 0) != 0;
+        const bool cut = __builtin_amdgcn_ballot_w64((p.flags & RDL_FORK_BAD_LENGTH) != 0) != 0;
+        if (lane == 0) {
+            a.summary[0] = min(needed, a.n_free);
+            a.summary[1] = (bad ? RDL_FORK_BAD_SEQUENCE : 0) | (cut ? RDL_FORK_BAD_LENGTH : 0) |
+                           (needed > a.n_free ? RDL_FORK_NO_PAGES : 0);
+        }
+    }
+    __syncthreads();  // every wave has read the lengths
+    if (w == 0 && p.ok) a.kv_len[p.child] = p.length;
+}
+
+// More pairs: a workgroup each, which counts the pairs before its own for itself (a length and two
+// numbers a pair, in every L2); the lengths come from a launch behind.
 // Sum over the workgroup (twice in a row: a barrier between).
 __device__ __forceinline__ int block_sum(int v, int* red) {
 #pragma unroll
@@ -106,10 +148,6 @@ __global__ __launch_bounds__(FORK_NT) void fork_kernel(ForkArgs a) {
         a.summary[1] = (bad ? RDL_FORK_BAD_SEQUENCE : 0) | (cut ? RDL_FORK_BAD_LENGTH : 0) |
                        (needed > a.n_free ? RDL_FORK_NO_PAGES : 0);
     }
-    if (a.n != 1) return;
-    __syncthreads();  // every thread has read the length
-    const ForkPair p = fork_pair(a, 0);
-    if (tid == 0 && p.ok) a.kv_len[p.child] = p.length;
 }
 __global__ __launch_bounds__(FORK_NT) void fork_lengths_kernel(ForkArgs a) {
     for (int i = (int)(blockIdx.x * FORK_NT + threadIdx.x); i < a.n; i += (int)(gridDim.x * FORK_NT)) {
@@ -343,11 +381,15 @@ rdl_status rdl_kv_fork_dev(int32_t* tables_dev, size_t table_stride, int32_t* kv
     a.src = src_pages_dev;
     a.dst = dst_pages_dev;
     a.summary = summary_dev;
-    const unsigned wg = (unsigned)std::max<size_t>(1, std::min<size_t>(n, rdl::FORK_WG));
-    hipLaunchKernelGGL(rdl::fork_kernel, dim3(wg), dim3(rdl::FORK_NT), 0, (hipStream_t)stream, a);
-    if (n > 1)
-        hipLaunchKernelGGL(rdl::fork_lengths_kernel, dim3((unsigned)std::min<size_t>((n + rdl::FORK_NT - 1) / rdl::FORK_NT, rdl::FORK_WG)),
-                           dim3(rdl::FORK_NT), 0, (hipStream_t)stream, a);
+    if (n <= (size_t)rdl::FORK_SMALL && n * table_stride <= rdl::FORK_SMALL_ENTRIES) {
+        hipLaunchKernelGGL(rdl::fork_small_kernel, dim3(1), dim3(rdl::FORK_SMALL_WAVES * 64), 0, (hipStream_t)stream, a);
+    } else {
+        const size_t lengths = (n + rdl::FORK_NT - 1) / rdl::FORK_NT;
+        hipLaunchKernelGGL(rdl::fork_kernel, dim3((unsigned)std::min<size_t>(n, rdl::FORK_WG)), dim3(rdl::FORK_NT), 0,
+                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL(rdl::fork_lengths_kernel, dim3((unsigned)std::min<size_t>(lengths, rdl::FORK_WG)), dim3(rdl::FORK_NT), 0,
+                           (hipStream_t)stream, a);
+    }
     HIP_TRY(hipGetLastError());
     return api_ok();
 }

@@ -83,7 +83,7 @@ def chained(n, page, seed):
     return tables, lens, page, parents, children, r.sample(range(20000, 60000), n + 7)
 
 
-@pytest.mark.parametrize("n,page", [(4, 16), (150, 16), (700, 64), (2600, 32)])
+@pytest.mark.parametrize("n,page", [(4, 16), (63, 32), (64, 16), (65, 16), (150, 16), (700, 64), (2600, 32)])
 def test_children_that_are_parents_spoil_their_own_copies_alone(rq, gpu, n, page):
     args = chained(n, page, n)
     parents, children = args[3:5]
@@ -146,3 +146,21 @@ def test_forks_on_streams_and_in_graphs(rq, gpu):
         torch.cuda.synchronize()
         for s in sides:
             s.check()
+
+
+@pytest.mark.parametrize("n", [1, 3, 17, 40, 64, 65, 100])
+@pytest.mark.parametrize("short", [0, 5])
+def test_forks_of_long_rows(rq, gpu, n, short):
+    """Rows of many pages, free lists that end within the pairs, parents and children that are none."""
+    r = random.Random(n)
+    width, page, roots = 1100, 16, 5
+    lens = [width * page, width * page - 1, 64 * page + 3, 7, 20 * width * page] + [0] * n
+    tables = [[r.randrange(10000) for _ in range(width)] for _ in lens]
+    parents, children = [r.randrange(roots) for _ in range(n)], list(range(roots, roots + n))
+    if n > 10:
+        parents[4], children[7], parents[9] = -1, roots + n, children[9]
+    want = sum(0 <= p < roots + n and 0 <= c < roots + n and p != c and min(lens[p], width * page) % page != 0
+               for p, c in zip(parents, children))
+    free = r.sample(range(20000, 60000), max(0, want - short))
+    args = (tables, lens, page, parents, children, free)
+    assert run_fork(*args) == plain_fork(*args)
