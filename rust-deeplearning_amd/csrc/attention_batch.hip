@@ -849,9 +849,9 @@ __device__ __forceinline__ void put_ml(const BatchArgs& a, int64_t at, int z, fl
 // while the first outputs are on their way, then a thread takes four dims of a
 // pair at a time, by weights of at most 1 (large values stay in f32's range).  Its
 // latency is what it costs.  COHERENT: the partials come from the same launch.
-// Behind those read ahead, JOIN_BATCH splits a trip to memory: one row over 4000 and 16000 4-bit keys (32 and 96 splits)
+// Behind those read ahead, JOIN_BATCH splits a trip to memory: of one row over 4000 and 16000 4-bit keys 32 and 96 splits
 // took 20.4 and 34.2 us with four, 15.2 and 22.8 with 8, 14.9 and 22.3 with 12, more with 16, whose
-// registers the launch did not have.  join_kernel takes four: its waves are many (841 rows over up to 3000 f16 keys 10.9 us, 12.8 by 12).
+// registers the launch did not have (few_min_span has made 16 and 32 of them since: 13.1 and 18.7).  join_kernel takes four: its waves are many (841 rows over up to 3000 f16 keys 10.9 us, 12.8 by 12).
 constexpr int JOIN_DEEP = 16, JOIN_AHEAD = 4, JOIN_BATCH = 12;  // splits a lane, at most; splits whose outputs are read ahead
 constexpr int JOIN_THREADS = 256, JOIN_LANES = JOIN_THREADS / FEW_PAIRS, JOIN_SPLITS = JOIN_LANES * JOIN_DEEP;
 constexpr int JOIN_FLOATS = FEW_PAIRS * (JOIN_SPLITS + 1);  // of LDS
@@ -2047,7 +2047,8 @@ constexpr int TILE = 1, FEW = 2;
 // need little LDS: 48 rows over up to 8192 keys took 71 us with three waves (168 registers, none of
 // the loop's in memory), 76 with two and 98 with four, with registers in memory; heads
 // of 256 (half as many of them) 71 with two and 83 with one.  (With the small parts in idle columns and scales a lane
-// of a quad the 48 rows have come to 57 .. 62 us, 3.5 TB/s or more: half of the cycles are VALU issue, the rest the
+// of a quad the 48 rows have come to 58 us over the same keys again and again, which the 256 MB cache then holds, and 64 to
+// 65 over others in turn, 3.4 TB/s: half of the cycles are VALU issue, the rest the
 // first keys' three trips to memory and the join.)
 template <typename KV, int HD, int KIND>
 constexpr int waves_per_simd() {

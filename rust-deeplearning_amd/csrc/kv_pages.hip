@@ -159,9 +159,10 @@ __global__ __launch_bounds__(FORK_NT) void fork_lengths_kernel(ForkArgs a) {
 // ---- copy -------------------------------------------------------------------------------
 // A workgroup takes a piece of one head's page of K or V of one pool, threads
 // COPY_DEEP units of 8 values each (4-bit runs of the same type: 16 bytes), whose
-// loads are all on their way before the first store.  HBM bounds it: 32 children's last pages in
-// 32 layers (537 MB counted once per child, sources from L2 after the first) 77 us, 60 pages of 8 layers f16 to 4 bits 35 us,
-// back 25 (161 MB each).
+// loads are all on their way before the first store.  HBM bounds it: 32 copies of 4 pages in 32 layers (268 MB
+// written, 34 read and then 235 again from the caches) 77 us, 480 pages of 64 positions and 8 heads of 128, f16 to 4 bits 35 us,
+// back 25 (161 MB each).  A workgroup has 1024 units, the values of such a page's head; smaller ones leave threads without
+// any: as many bytes in pages of 32 positions take 51 and 28 us, in pages of 16 and heads of 64 151 and 83.
 constexpr int COPY_NT = 256, COPY_DEEP = 4, COPY_POOLS = 32;
 
 struct CopySide {

@@ -99,8 +99,9 @@ __device__ __forceinline__ void put(const PoolView& p, void* base, int64_t page,
 // ROWS rows at a time, whose loads are on their way together: slot and position,
 // then cos and sin, are two trips to memory one behind the other, and what is in
 // flight meanwhile bounds the rate, with the norm's 64-bit sums behind it.  4096 rows of 32 + 2 * 8
-// heads of 128 took 45 us one at a time, 40 by two (now 33, 5.5 TB/s; a large copy reaches
-// 5.1), 42 by four and 48 by eight, whose registers leave fewer waves.
+// heads of 128 took 45 us one at a time, 40 by two, 42 by four and 48 by eight, whose registers
+// leave fewer waves.  Now 33 where the 256 MB cache still holds the rows, three quarters of the cycles VALU issue; 42 with
+// other rows in turn, 4.4 TB/s of the 5.1 to 5.3 that a copy of 1 GiB reaches.
 // Few rows take one each, so that they spread over the CUs.  The first rows' loads stand before the loop and the next
 // ones' behind those of cos and sin: with all of a turn's in the turn the same took 49 us from cold caches, so 44, and
 // with 1536 .. 4096 workgroups that take several turns 46 to 56.

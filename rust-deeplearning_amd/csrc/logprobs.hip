@@ -19,17 +19,20 @@ namespace {
 // T = sum e^(x - M) (x - M), so that
 //   lse = M + log S,  entropy = lse - sum p x = log S - T / S;
 // and the range's largest values so far, the i-th in lane i as a 64-bit key of
-// value and place.  Values that pass the last of those are rare after the first
-// steps, so that a comparison a step is what the alternatives cost.  The waves of a
+// value and place.  A step without a value that passes the last of those costs a comparison; one
+// that does costs two passes over the step's registers, and each wave's range has some n log(range / n) of
+// them behind its first list: five alternatives take a sixth longer than one (a third, from the cache), more take a multiple.  The waves of a
 // workgroup join through LDS, the workgroups of a row (rows that are few are split, down to a
 // step a wave) through partial results that the last of them to arrive joins.
 // Few rows: latency.  16 rows of 32000, five alternatives: 10.5 us (8.7 with one alternative); one workgroup of 16 waves a
-// row took 16.3, the waves' lists then share one CU.  Many rows: HBM bounds it: 2000 rows of
-// 32003 take 44 us, 5.8 TB/s (a large copy reaches 5.1).
+// row took 16.3, the waves' lists then share one CU.  Many rows with one alternative: HBM bounds it: 2000 rows of
+// 32003 take 52 us, 4.9 TB/s, from memory, 44 where the 256 MB cache holds a part of them; with 5, 20 and 64
+// alternatives 61, 117 and 405, which those candidates and the lists' begin bound.
 constexpr int NT = 256, W = NT / 64, PER = 16, STEP = 64 * PER, TOP = 64;
 constexpr int WG_TARGET = 1024, MOST_PARTS = 64;
 // A list begins by counting (first_list), where that is faster than one by one: 16 rows of 32000 with 5,
-// 20 and 64 alternatives take 10.4, 12.8 and 71.7 us so, 10.5, 23.7 and 50.5 one by one.
+// 20 and 64 alternatives take 10.4, 12.8 and 71.7 us so, 10.5, 23.7 and 50.5 one by one; 2000 rows of 32003 with 5 and 20
+// 57 and 116 instead of 61 and 152.
 __host__ __device__ constexpr bool counted(int n) { return n > 4 && n <= 32; }
 constexpr float LOG2E = 1.44269504088896340736f;
 typedef float f4 __attribute__((ext_vector_type(4)));
