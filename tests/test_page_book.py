@@ -76,8 +76,8 @@ class Plain:
 def driver(tmp_path_factory):
     d = tmp_path_factory.mktemp("book")
     (d / "driver.cpp").write_text(DRIVER)
-    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=address,undefined", "-I", SRC,
-                    str(d / "driver.cpp"), "-o", str(d / "driver")], check=True)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-D_GLIBCXX_ASSERTIONS", "-I", SRC, str(d / "driver.cpp"),
+                    "-o", str(d / "driver")], check=True)
     return str(d / "driver")
 
 
